@@ -431,6 +431,83 @@ int tg_decode_attn_noalloc(const void* q, int64_t q_sb, int64_t q_sh,
                            void* out, int64_t o_sb, int64_t o_sh,
                            int B, int Hq, int Hkv, int D, float softmax_scale, void* stream);
 
+/*
+ * The 4-bit KV cache: K and V rows of head_dim 128 as 4-bit codes above a
+ * bf16 low, with a bf16 step, per group of 64 consecutive dims:
+ *   low   = min(x), scale = bf16((max/2 - min/2) / 7.5)  (0 below 2^-100)
+ *   code  = floor((x - low) / scale + 1/2), 0..15         (0 where scale is 0)
+ *   value = bf16(low + code * scale)
+ * A group with a NaN or an infinity, or with max - min past fp32's largest,
+ * reads back as NaN. 144 bytes per (slot, kv head) instead of 512. One buffer of tg_kv4_cache_bytes bytes, 16-byte
+ * aligned, holds K and V of one layer, (B, Hkv, capacity rounded up to 32
+ * slots); its inside is the library's own, 32-slot tiles of 4608 bytes. A
+ * slot's bytes are its own: writing one slot leaves the others as they were,
+ * and slots never written may hold anything. No counterpart in the reference.
+ */
+int tg_kv4_cache_bytes(int B, int Hkv, int64_t capacity, size_t* bytes);
+
+/* Quantises k and v, (B, count, Hkv, 128) bf16 with strides (k_sb, k_ss,
+ * k_sh, 1), into slots [start, start + count). Bases 16-byte aligned,
+ * strides multiples of 8 elements. count == 0 returns TG_OK. */
+int tg_kv4_write(const void* k, int64_t k_sb, int64_t k_ss, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_ss,
+                 int64_t v_sh, int B, int Hkv, int D, int64_t start, int64_t count, void* cache, int64_t capacity,
+                 void* stream);
+
+/* The values of slots [start, start + count) as bf16 k and v, (B, count,
+ * Hkv, 128) with strides (k_sb, k_ss, k_sh, 1); alignment as in tg_kv4_write. */
+int tg_kv4_read(const void* cache, int64_t capacity, int B, int Hkv, int D, int64_t start, int64_t count, void* k,
+                int64_t k_sb, int64_t k_ss, int64_t k_sh, void* v, int64_t v_sb, int64_t v_ss, int64_t v_sh,
+                void* stream);
+
+/* One decode token per row: every q and k head (head_dim 128) RMS-normalised
+ * with its norm weight and rotated (x*cos + rotate_half(x)*sin), in fp32 with
+ * one rounding to bf16; q goes to q_out (which may be q), k and v are
+ * quantised into slot *slot_dev (device int64) of the 4-bit cache. k and v
+ * are not changed. A slot outside [0, capacity) is not written. q / k / v:
+ * (rows, heads, 128) with row strides; cos / sin: (rows, 128) bf16, row stride
+ * ld_cs. Pointers 8-byte aligned, row strides multiples of 4.
+ * tg_qk_norm_rope_append for a 4-bit cache. */
+int tg_qk_norm_rope_append_kv4(const void* q, int64_t ld_q, int n_q_heads, const void* k, int64_t ld_k, int n_k_heads,
+                               const void* v, int64_t ld_v, int rows, const void* q_norm_w, const void* k_norm_w,
+                               const void* cos, const void* sin, int64_t ld_cs, int head_dim, float eps, void* q_out,
+                               int64_t ld_q_out, void* cache, int64_t capacity, const int64_t* slot_dev,
+                               void* stream);
+
+/* tg_decode_attn_ex over a 4-bit cache of `capacity` slots: the same
+ * operation on the values that the cache stands for, with the same bias,
+ * query scale, pad slots and device-side key count. A bias of -inf masks its
+ * key whatever the key holds; rows without any key give zeros. 1 to 8 query heads per kv head. workspace: device scratch of
+ * tg_decode_attn_kv4_workspace bytes (0: none), 16-byte aligned; calls
+ * sharing it must not overlap on the GPU. */
+int tg_decode_attn_kv4(const void* q, int64_t q_sb, int64_t q_sh, const float* q_scale, int64_t qs_sb,
+                       const void* cache, int64_t capacity, const float* bias, int64_t bias_sb, int64_t bias_sh,
+                       const int32_t* n_valid, int n_prefix, int n_keys, const int32_t* n_keys_dev, void* out,
+                       int64_t o_sb, int64_t o_sh, void* workspace, size_t workspace_bytes, int B, int Hq, int Hkv,
+                       int D, float softmax_scale, void* stream);
+int tg_decode_attn_kv4_workspace(int B, int Hq, int Hkv, int n_keys, size_t* bytes);
+
+/*
+ * Sampling of the next token from logits (B, V), dtype 0 = fp32 or 1 = bf16,
+ * row stride row_stride elements, V <= 2^19. Per row b, with device arrays
+ * of B entries:
+ *   d_i = x_i / T - x_max / T, w_i = exp(d_i); a NaN logit counts as -inf
+ *   in the order (x descending, index ascending): the first top_k, of these
+ *   the shortest prefix with mass >= top_p * (their mass), of these the ones
+ *   with w_i >= min_p;
+ *   token = the first index, by index, at which the running kept mass passes
+ *   u * (kept mass); logprob = d_token - log(kept mass).
+ * temperature T <= 0 (or NaN): the largest logit, lowest index on ties
+ * (logprob 0). top_k (nullable) <= 0, top_p (nullable) >= 1 and min_p
+ * (nullable) <= 0 are off; at least the largest logit is always kept. u in
+ * [0, 1]. A row of -inf or NaN alone gives token 0 and logprob NaN. Masses
+ * are summed exactly, so results do not depend on any order of summing.
+ * The reference decodes greedily (tokengate/e2e_gate/decode/gate_decode.py:
+ * 87-260); no counterpart there. B == 0 returns TG_OK.
+ */
+int tg_sample(const void* logits, int dtype, int64_t row_stride, int B, int V, const float* u,
+              const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p, int64_t* token,
+              float* logprob, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

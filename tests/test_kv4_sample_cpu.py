@@ -1,0 +1,81 @@
+"""Argument checks of the 4-bit cache and sampling entries at the C-ABI boundary, on CPU (nothing is launched)."""
+import ctypes
+
+import pytest
+import torch
+
+from tokengate_b200 import _lib, ops
+from tokengate_b200.kv4 import KV4Cache
+
+BAD, NO, ALIGN = _lib.TG_ERR_INVALID_ARGUMENT, _lib.TG_ERR_UNSUPPORTED, _lib.TG_ERR_ALIGNMENT
+
+
+def test_cache_bytes():
+    L, n = _lib.lib(), ctypes.c_size_t(7)
+    for cap, tiles in ((1, 1), (32, 1), (33, 2), (131072, 4096)):
+        assert L.tg_kv4_cache_bytes(3, 8, cap, ctypes.byref(n)) == 0 and n.value == 3 * 8 * tiles * 4608
+    assert L.tg_kv4_cache_bytes(3, 8, 0, ctypes.byref(n)) == BAD and n.value == 0
+    assert L.tg_kv4_cache_bytes(3, 8, 5, None) == BAD
+
+
+def _write(**over):
+    a = dict(k=4096, k_sb=0, k_ss=256, k_sh=128, v=8192, v_sb=0, v_ss=256, v_sh=128, B=1, Hkv=2, D=128, start=0,
+             count=5, cache=16384, capacity=8, stream=None)
+    a.update(over)
+    return list(a.values())
+
+
+def test_write_and_read_checks():
+    L = _lib.lib()
+    for over, st in ((dict(cache=None), BAD), (dict(k=None), BAD), (dict(D=64), NO), (dict(B=0), BAD), (dict(Hkv=0), BAD),
+                     (dict(start=-1), BAD), (dict(start=4), BAD), (dict(start=9, count=0), BAD), (dict(count=-1), BAD),
+                     (dict(start=2 ** 62), BAD), (dict(capacity=2 ** 31), BAD), (dict(k=4098), ALIGN), (dict(v_ss=260), ALIGN),
+                     (dict(cache=16392), ALIGN), (dict(count=0), 0)):
+        assert L.tg_kv4_write(*_write(**over)) == st, over
+    r = lambda *a: L.tg_kv4_read(*a)  # noqa: E731
+    assert r(16384, 8, 1, 2, 128, 4, 5, 4096, 0, 256, 128, 8192, 0, 256, 128, None) == BAD
+    assert r(16384, 8, 1, 2, 128, 0, 5, None, 0, 256, 128, 8192, 0, 256, 128, None) == BAD
+    assert r(16384, 8, 1, 2, 128, 8, 0, None, 0, 0, 0, None, 0, 0, 0, None) == 0
+
+
+def test_append_checks():
+    def call(**over):
+        a = dict(q=4096, ld_q=512, n_q=4, k=8192, ld_k=256, n_k=2, v=8192, ld_v=256, rows=1, qw=512, kw=512, cos=512,
+                 sin=512, ld_cs=128, D=128, eps=1e-6, q_out=4096, ld_qo=512, cache=16384, cap=8, slot=64, stream=None)
+        a.update(over)
+        return _lib.lib().tg_qk_norm_rope_append_kv4(*a.values())
+    for over, st in ((dict(q=None), BAD), (dict(slot=None), BAD), (dict(cache=None), BAD), (dict(D=96), NO), (dict(ld_q=500), BAD),
+                     (dict(ld_v=128), BAD), (dict(n_q=0), BAD), (dict(rows=-1), BAD), (dict(q=4100), ALIGN), (dict(ld_k=258), ALIGN),
+                     (dict(rows=0), 0)):
+        assert call(**over) == st, over
+
+
+def test_attention_checks():
+    def call(**over):
+        a = dict(q=4096, q_sb=0, q_sh=128, qs=None, qs_sb=0, cache=16384, cap=64, bias=None, b_sb=0, b_sh=0, n_valid=64,
+                 n_prefix=5, n_keys=6, nk=None, out=4096, o_sb=0, o_sh=128, ws=None, wsb=0, B=1, Hq=4, Hkv=2, D=128,
+                 scale=0.1, stream=None)
+        a.update(over)
+        return _lib.lib().tg_decode_attn_kv4(*a.values())
+    for over, st in ((dict(q=None), BAD), (dict(out=None), BAD), (dict(n_valid=None), BAD), (dict(cache=None), BAD), (dict(n_prefix=7), BAD),
+                     (dict(n_keys=0, n_prefix=0), BAD), (dict(n_keys=65), BAD), (dict(Hq=5), BAD), (dict(Hq=18), NO), (dict(D=64), NO),
+                     (dict(scale=0.0), BAD), (dict(scale=float("nan")), BAD), (dict(cache=16392), ALIGN), (dict(B=70000), BAD)):
+        assert call(**over) == st, over
+
+
+def test_sample_checks():
+    def call(**over):
+        a = dict(logits=4096, dtype=1, stride=100, B=2, V=100, u=64, t=64, k=None, p=None, m=None, token=64, lp=None, stream=None)
+        a.update(over)
+        return _lib.lib().tg_sample(*a.values())
+    for over, st in ((dict(logits=None), BAD), (dict(u=None), BAD), (dict(t=None), BAD), (dict(token=None), BAD), (dict(dtype=2), BAD),
+                     (dict(V=0), BAD), (dict(stride=99), BAD), (dict(B=-1), BAD), (dict(B=70000), BAD), (dict(V=2 ** 19 + 1, stride=2 ** 20), NO),
+                     (dict(logits=4097), ALIGN), (dict(dtype=0, logits=4098), ALIGN), (dict(B=0, logits=None), 0)):
+        assert call(**over) == st, over
+
+
+def test_no_cpu_path():
+    with pytest.raises(ValueError, match="CUDA"):
+        KV4Cache(1, 8, 2, device="cpu")
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.sample_tokens(torch.zeros(1, 8), torch.zeros(1))

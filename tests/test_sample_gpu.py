@@ -1,0 +1,211 @@
+"""Sampling on the B200 against a plain float64 restatement of its definition.
+
+The kept set and the running masses are computed in float64 from the row's
+fp32 scaled logits. A token is right when it is in the kept set and u times
+the kept mass lies in its interval of the running mass, within 2e-6 of the
+mass: the kernel's weights are fp32 exponentials (2^-22) of fp32 differences
+of magnitude below 32 (2^-20), and errors of the terms average out in sums.
+Boundaries of top-p are placed in the middle of a token's interval, so that
+no rounding can move them; logprob has the same 2e-6, plus fp32 rounding of
+values up to 32 (2^-19).
+"""
+import numpy as np
+import pytest
+import torch
+
+from tokengate_b200 import _lib, ops
+
+pytestmark = pytest.mark.gpu
+
+
+def weights(x, t):
+    z = (x.astype(np.float32) / np.float32(t)).astype(np.float32)
+    return np.exp((z - z.max()).astype(np.float64))
+
+
+def kept_set(x, t, k, p, m):
+    """Indices kept of one row, ascending, and every weight."""
+    x = np.where(np.isnan(x), -np.inf, x)
+    w = weights(x, t)
+    order = np.lexsort((np.arange(len(x)), -x.astype(np.float64)))
+    order = order[np.isfinite(x[order])]
+    if k > 0:
+        order = order[:k]
+    if p < 1:
+        cum = np.cumsum(w[order])
+        order = order[:int((cum < p * cum[-1]).sum()) + 1]
+    return np.sort(order[w[order] >= min(m, 1.0)]), w
+
+
+def check_rows(x, u, t, k, p, m, token, logprob):
+    for b in range(len(x)):
+        if t[b] <= 0:
+            assert token[b] == int(np.argmax(np.where(np.isnan(x[b]), -np.inf, x[b]))) and logprob[b] == 0.0, b
+            continue
+        keep, w = kept_set(x[b], t[b], k[b], p[b], m[b])
+        cum = np.cumsum(w[keep])
+        at = np.searchsorted(keep, token[b])
+        assert at < len(keep) and keep[at] == token[b], (b, token[b], len(keep))
+        goal, slack = u[b] * cum[-1], 2e-6 * cum[-1]
+        assert cum[at] - w[token[b]] - slack <= goal <= cum[at] + slack, (b, at, goal, cum[at], w[token[b]])
+        assert abs(logprob[b] - np.log(w[token[b]] / cum[-1])) <= 2e-6 + 2 ** -19 * 2, b
+
+
+def run(cuda, x, u, t, k=None, p=None, m=None):
+    B = len(x)
+    f = lambda v, dt: None if v is None else torch.as_tensor(np.broadcast_to(v, (B,)).copy(), dtype=dt, device=cuda)  # noqa: E731
+    tok, lp = ops.sample_tokens(x.to(cuda), f(u, torch.float32), f(t, torch.float32), top_k=f(k, torch.int32),
+                                top_p=f(p, torch.float32), min_p=f(m, torch.float32))
+    bc = lambda v, d: np.broadcast_to(d if v is None else v, (B,)).astype(np.float32)  # noqa: E731
+    check_rows(x.float().numpy(), bc(u, 0), bc(t, 1), np.broadcast_to(0 if k is None else k, (B,)), bc(p, 1), bc(m, 0),
+               tok.cpu().numpy(), lp.cpu().numpy())
+    return tok.cpu(), lp.cpu()
+
+
+def middle_p(x, t, k, n):
+    """A top-p whose boundary is the middle of the n-th kept token's interval."""
+    keep, w = kept_set(x, t, k, 1.0, 0.0)
+    o = keep[np.lexsort((keep, -x[keep].astype(np.float64)))]
+    cum = np.cumsum(w[o])
+    n = min(n, len(o) - 1)
+    return float((cum[n] - 0.5 * w[o[n]]) / cum[-1])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,V", [(1, 151936), (3, 1001), (2, 1), (5, 2), (1, 33), (20, 4097), (2, 32000), (70, 9000), (1, 300001)])
+def test_no_truncation_and_each_rule(cuda, dtype, B, V):
+    g = torch.Generator().manual_seed(V + B)
+    x = (torch.randn(B, V, generator=g) * 2.5).to(dtype)
+    u = torch.rand(B, generator=g).numpy()
+    t = 0.5 + torch.rand(B, generator=g).numpy()
+    run(cuda, x, u, t)
+    run(cuda, x, u, t, k=np.arange(B) % 60 + 1)
+    run(cuda, x, u, t, m=0.07)
+    xf = x.float().numpy()
+    for n in (0, 3, 200, V // 3):
+        run(cuda, x, u, t, p=np.array([middle_p(xf[b], t[b], 0, n) for b in range(B)], dtype=np.float32))
+    ks = np.array([5, 40, 1000])[np.arange(B) % 3]
+    run(cuda, x, u, t, k=ks, p=np.array([middle_p(xf[b], t[b], ks[b], ks[b] // 2) for b in range(B)], dtype=np.float32), m=0.001)
+
+
+@pytest.mark.parametrize("spread", [0.0, 1e-4, 0.02, 0.3, 8.0, 300.0])
+def test_flat_and_peaked(cuda, spread):
+    """All logits equal, all in one bucket, and ranges beyond the buckets."""
+    g = torch.Generator().manual_seed(11)
+    for dtype in (torch.bfloat16, torch.float32):
+        x = (torch.randn(4, 20000, generator=g) * spread - 3.0).to(dtype)
+        u = np.array([0.0, 0.25, 0.6, 0.999], dtype=np.float32)
+        xf = x.float().numpy()
+        run(cuda, x, u, 1.0)
+        run(cuda, x, u, 1.0, k=777)
+        run(cuda, x, u, 0.7, p=np.array([middle_p(xf[b], 0.7, 0, 9000 if spread < 1 else 5) for b in range(4)], dtype=np.float32))
+        run(cuda, x, u, 0.7, k=500, p=np.array([middle_p(xf[b], 0.7, 500, 250) for b in range(4)], dtype=np.float32))
+
+
+def test_ties_go_to_the_lowest_index(cuda):
+    x = torch.zeros(6, 5000)
+    x[:, 100::700] = 2.0                      # 7 ties at the top
+    k = np.array([1, 3, 7, 8, 9, 4999])
+    for u in (0.0, 0.5, 0.9999):
+        tok, _ = run(cuda, x, u, 1.0, k=k)
+        assert tok[0] == 100 and tok[1] in (100, 800, 1500)
+    # nine kept: the seven and the two lowest of the rest
+    tok, _ = run(cuda, x[:1], 0.0, 1.0, k=9)
+    assert tok[0] == 0
+    # greedy
+    tok, lp = run(cuda, x, 0.7, 0.0, k=50, p=0.2)
+    assert (tok == 100).all() and (lp == 0).all()
+
+
+def test_hard_logits(cuda):
+    inf, nan = float("inf"), float("nan")
+    x = torch.full((9, 1500), -inf)
+    x[0, 700] = -5.0                          # one token left
+    x[1, 3], x[1, 1499] = 1.0, 1.0
+    x[2] = torch.randn(1500)
+    x[2, 5] = nan
+    x[2, 6] = 30.0
+    x[4] = torch.finfo(torch.float32).min     # the type's lowest: finite, so uniform
+    x[5, 10] = x[5, 20] = inf                 # infinities share the mass
+    x[6, 0], x[6, 1] = 3e38, -3e38
+    x[7] = torch.linspace(-200, 0, 1500)      # a far tail
+    x[8] = nan
+    u = torch.full((9,), 0.75, device=cuda)
+    tok, lp = ops.sample_tokens(x.to(cuda), u, 1.0)
+    tok, lp = tok.cpu(), lp.cpu()
+    assert tok[0] == 700 and lp[0] == 0
+    assert tok[1] == 1499 and abs(lp[1] + np.log(2)) < 1e-6
+    assert tok[2] == 6
+    assert tok[3] == 0 and torch.isnan(lp[3]) and tok[8] == 0 and torch.isnan(lp[8])    # nothing to choose from
+    assert tok[4] == 1125 and abs(lp[4] + np.log(1500)) < 1e-5
+    assert tok[5] == 20 and abs(lp[5] + np.log(2)) < 1e-6
+    assert tok[6] == 0
+    for kw in (dict(top_k=100), dict(top_p=0.9), dict(min_p=0.3), dict(top_k=2, top_p=0.99), dict(temperature=1e-30)):
+        kw.setdefault("temperature", 1.0)
+        tk, l2 = ops.sample_tokens(x.to(cuda), u, **kw)
+        tk = tk.cpu()
+        assert tk[0] == 700 and tk[2] == 6 and tk[3] == 0 and tk[8] == 0 and tk[6] == 0, kw
+        assert torch.isnan(l2.cpu()[[3, 8]]).all()
+
+
+def test_edges_of_the_parameters(cuda):
+    g = torch.Generator().manual_seed(12)
+    x = torch.randn(3, 3000, generator=g) * 2
+    top = x.argmax(1)
+    for kw in (dict(top_p=0.0), dict(top_p=-1.0), dict(min_p=1.0), dict(min_p=2.0), dict(top_k=1), dict(temperature=-1.0),
+               dict(temperature=float("nan"))):
+        kw.setdefault("temperature", 1.0)
+        tok, lp = ops.sample_tokens(x.to(cuda), torch.full((3,), 0.9, device=cuda), **kw)
+        assert torch.equal(tok.cpu(), top) and (lp == 0).all(), kw
+    for u in (0.0, -1.0, float("nan")):       # the first kept index; u of 1 the last
+        tok, _ = ops.sample_tokens(x.to(cuda), torch.full((3,), u, device=cuda), 1.0, top_k=10)
+        assert torch.equal(tok.cpu(), x.topk(10).indices.min(1).values)
+    tok, _ = ops.sample_tokens(x.to(cuda), torch.ones(3, device=cuda), 1.0, top_k=10)
+    assert torch.equal(tok.cpu(), x.topk(10).indices.max(1).values)
+    same = [ops.sample_tokens(x.to(cuda), torch.full((3,), 0.3, device=cuda), 1.0, **kw)[0]
+            for kw in (dict(), dict(top_k=0), dict(top_k=-4), dict(top_k=3000), dict(top_k=10 ** 9), dict(top_p=1.0), dict(min_p=0.0))]
+    assert all(torch.equal(same[0], s) for s in same)
+
+
+def test_rows_with_a_stride_and_outputs_given(cuda):
+    g = torch.Generator().manual_seed(13)
+    big = (torch.randn(4, 2 * 1003, generator=g) * 2).bfloat16().to(cuda)
+    x = big[:, 5:1006]                         # rows that start off any vector boundary
+    u = torch.rand(4, generator=g).to(cuda)
+    token, lp = torch.empty(4, dtype=torch.int64, device=cuda), torch.empty(4, device=cuda)
+    a = ops.sample_tokens(x, u, 0.8, top_k=30, token=token, logprob=lp)
+    assert a[0] is token and a[1] is lp
+    b = ops.sample_tokens(x.contiguous(), u, 0.8, top_k=30)
+    assert torch.equal(token, b[0]) and torch.equal(lp, b[1])
+
+
+def test_frequencies(cuda):
+    """4096 draws of one row follow its distribution: chi-square over 20 tokens, far below its 1e-6 quantile."""
+    g = torch.Generator().manual_seed(14)
+    x = torch.randn(1, 500, generator=g) * 2
+    u = torch.rand(4096, generator=g)
+    tok, _ = ops.sample_tokens(x.expand(4096, -1).contiguous().to(cuda), u.to(cuda), 1.0, top_k=20)
+    keep, w = kept_set(x[0].numpy(), 1.0, 20, 1.0, 0.0)
+    want = 4096 * w[keep] / w[keep].sum()
+    seen = np.array([(tok.cpu().numpy() == i).sum() for i in keep])
+    assert seen.sum() == 4096 and ((seen - want) ** 2 / want).sum() < 70
+
+
+def test_refusals(cuda):
+    x, u = torch.zeros(2, 10, device=cuda), torch.zeros(2, device=cuda)
+    for bad in (x.half(), x[0], x.t(), x.cpu()):
+        with pytest.raises(ValueError):
+            ops.sample_tokens(bad, u)
+    with pytest.raises(ValueError):
+        ops.sample_tokens(x, None)
+    with pytest.raises(ValueError):
+        ops.sample_tokens(x, u[:1])
+    with pytest.raises(ValueError):
+        ops.sample_tokens(x, u, temperature=None)
+    with pytest.raises(ValueError):
+        ops.sample_tokens(x, u, top_k=torch.zeros(2, device=cuda))          # int32 wanted
+    with pytest.raises(ValueError):
+        ops.sample_tokens(x, u, token=torch.zeros(2, dtype=torch.int32, device=cuda))
+    with pytest.raises(_lib.TokenGateUnsupportedError):
+        ops.sample_tokens(torch.zeros(1, (1 << 19) + 1, device=cuda), u[:1])
+    assert ops.sample_tokens(x[:0], u[:0])[0].shape == (0,)

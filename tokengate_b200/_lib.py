@@ -102,6 +102,15 @@ _SIGNATURES = {
     "tg_decode_attn_workspace": [_I32, _I32, _I32, ctypes.POINTER(ctypes.c_size_t)],
     "tg_decode_attn_noalloc": [_P, _I64, _I64, _P, _I64, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64,
                                _I64, _P, _I32, _I32, _P, _I64, _I64, _I32, _I32, _I32, _I32, _F, _P],
+    "tg_kv4_cache_bytes": [_I32, _I32, _I64, ctypes.POINTER(ctypes.c_size_t)],
+    "tg_kv4_write": [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I32, _I32, _I32, _I64, _I64, _P, _I64, _P],
+    "tg_kv4_read": [_P, _I64, _I32, _I32, _I32, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P],
+    "tg_qk_norm_rope_append_kv4": [_P, _I64, _I32, _P, _I64, _I32, _P, _I64, _I32, _P, _P, _P, _P, _I64, _I32, _F,
+                                   _P, _I64, _P, _I64, _P, _P],
+    "tg_decode_attn_kv4": [_P, _I64, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _P, _I32, _I32, _P, _P, _I64, _I64,
+                           _P, ctypes.c_size_t, _I32, _I32, _I32, _I32, _F, _P],
+    "tg_decode_attn_kv4_workspace": [_I32, _I32, _I32, _I32, ctypes.POINTER(ctypes.c_size_t)],
+    "tg_sample": [_P, _I32, _I64, _I32, _I32, _P, _P, _P, _P, _P, _P, _P, _P],
 }
 EXPORTED = tuple(_SIGNATURES)
 

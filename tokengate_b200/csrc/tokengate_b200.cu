@@ -26,6 +26,8 @@
 #include "e2e_gate.cuh"
 #include "decode_attn.cuh"
 #include "gemv.cuh"
+#include "kv4_attn.cuh"
+#include "sample.cuh"
 
 // Bit flags set by kernels whose bounded waits gave up (see ptx.cuh).
 __device__ unsigned int g_tg_device_error = 0;
@@ -1302,6 +1304,285 @@ int tg_decode_attn_noalloc(const void* q, int64_t q_sb, int64_t q_sh, const floa
   return tg_decode_attn(q, q_sb, q_sh, q_scale, qs_sb, k, k_sb, k_ss, k_sh, v, v_sb, v_ss, v_sh, bias, bias_sb,
                         bias_sh, n_valid, n_prefix, n_keys, out, o_sb, o_sh, scratch, kNoAllocScratchBytes, B,
                         Hq, Hkv, D, softmax_scale, stream);
+}
+
+// ---- the 4-bit KV cache
+namespace {
+constexpr int64_t kKv4MaxSlots = (int64_t)1 << 30;
+int64_t kv4_tiles(int64_t capacity) { return (capacity + tg::kKv4Keys - 1) / tg::kKv4Keys; }
+
+int kv4_check(const char* what, const void* cache, int B, int Hkv, int D, int64_t capacity) {
+  if (cache == nullptr) return fail(TG_ERR_INVALID_ARGUMENT, "%s: cache must be non-NULL", what);
+  if (B < 1 || B > 65535 || Hkv < 1 || Hkv > 65535 || capacity < 1 || capacity > kKv4MaxSlots)
+    return fail(TG_ERR_INVALID_ARGUMENT, "%s: B=%d Hkv=%d capacity=%lld", what, B, Hkv, (long long)capacity);
+  if (D != 128) return fail(TG_ERR_UNSUPPORTED, "%s: head_dim %d not served (only 128)", what, D);
+  if (reinterpret_cast<uintptr_t>(cache) & 15) return fail(TG_ERR_ALIGNMENT, "%s: cache must be 16-byte aligned", what);
+  return TG_OK;
+}
+
+int kv4_rows(const char* what, bool write, const void* k, int64_t k_sb, int64_t k_ss, int64_t k_sh, const void* v,
+             int64_t v_sb, int64_t v_ss, int64_t v_sh, int B, int Hkv, int D, int64_t start, int64_t count,
+             void* cache, int64_t capacity, void* stream) {
+  int st = kv4_check(what, cache, B, Hkv, D, capacity);
+  if (st) return st;
+  if (start < 0 || count < 0 || start > capacity || count > capacity - start)
+    return fail(TG_ERR_INVALID_ARGUMENT, "%s: slots [%lld, %lld) outside the capacity %lld", what, (long long)start,
+                (long long)(start + count), (long long)capacity);
+  if (count == 0) return TG_OK;
+  if (k == nullptr || v == nullptr) return fail(TG_ERR_INVALID_ARGUMENT, "%s: k and v must be non-NULL", what);
+  if (B == 1) k_sb = v_sb = 0;  // the strides of a dim of one are not used
+  if (count == 1) k_ss = v_ss = 0;
+  if (Hkv == 1) k_sh = v_sh = 0;
+  if (((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) ||
+      ((k_sb | k_ss | k_sh | v_sb | v_ss | v_sh) & 7))
+    return fail(TG_ERR_ALIGNMENT, "%s: k and v 16-byte aligned with strides multiples of 8 elements", what);
+  tg::Kv4RowsParams p;
+  memset(&p, 0, sizeof(p));
+  if (write) {
+    p.k = static_cast<const __nv_bfloat16*>(k);
+    p.v = static_cast<const __nv_bfloat16*>(v);
+  } else {
+    p.k_out = static_cast<__nv_bfloat16*>(const_cast<void*>(k));
+    p.v_out = static_cast<__nv_bfloat16*>(const_cast<void*>(v));
+  }
+  p.k_sb = k_sb;
+  p.k_ss = k_ss;
+  p.k_sh = k_sh;
+  p.v_sb = v_sb;
+  p.v_ss = v_ss;
+  p.v_sh = v_sh;
+  p.cache = static_cast<uint8_t*>(cache);
+  p.c_sh = kv4_tiles(capacity) * tg::kKv4TileBytes;
+  p.c_sb = p.c_sh * Hkv;
+  p.start = (int)start;
+  p.count = (int)count;
+  p.Hkv = Hkv;
+  p.blk0 = (int)(start / 16);
+  p.n_blk = (int)((start + count + 15) / 16) - p.blk0;
+  p.items = (int64_t)B * p.n_blk * 2 * Hkv;
+  const int64_t blocks = resident_blocks((p.items + 7) / 8, 8);
+  cudaError_t e = launch_pdl(write ? tg::kv4_write_kernel : tg::kv4_read_kernel, dim3((unsigned)blocks), dim3(256), 0,
+                             static_cast<cudaStream_t>(stream), p);
+  if (e != cudaSuccess) return cuda_fail(e, what);
+  return TG_OK;
+}
+
+// Splits of a row's tiles over CTAs, and the tiles of one.
+void kv4_splits(int B, int Hkv, int n_keys, int* n_splits, int* per) {
+  const int tiles = (int)kv4_tiles(n_keys);
+  const int64_t want = ((int64_t)sm_count() * 3 + (int64_t)B * Hkv - 1) / ((int64_t)B * Hkv);
+  int64_t per_ = (tiles + want - 1) / want;
+  per_ = (per_ + tg::kKv4Warps - 1) / tg::kKv4Warps * tg::kKv4Warps;
+  *per = (int)per_;
+  *n_splits = (int)((tiles + per_ - 1) / per_);
+}
+}  // namespace
+
+int tg_kv4_cache_bytes(int B, int Hkv, int64_t capacity, size_t* bytes) {
+  if (bytes == nullptr) return fail(TG_ERR_INVALID_ARGUMENT, "kv4_cache_bytes: bytes must be non-NULL");
+  *bytes = 0;
+  if (B < 1 || Hkv < 1 || capacity < 1 || capacity > kKv4MaxSlots)
+    return fail(TG_ERR_INVALID_ARGUMENT, "kv4_cache_bytes: B=%d Hkv=%d capacity=%lld", B, Hkv, (long long)capacity);
+  *bytes = (size_t)B * Hkv * kv4_tiles(capacity) * tg::kKv4TileBytes;
+  return TG_OK;
+}
+
+int tg_kv4_write(const void* k, int64_t k_sb, int64_t k_ss, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_ss,
+                 int64_t v_sh, int B, int Hkv, int D, int64_t start, int64_t count, void* cache, int64_t capacity,
+                 void* stream) {
+  return kv4_rows("kv4_write", true, k, k_sb, k_ss, k_sh, v, v_sb, v_ss, v_sh, B, Hkv, D, start, count, cache,
+                  capacity, stream);
+}
+
+int tg_kv4_read(const void* cache, int64_t capacity, int B, int Hkv, int D, int64_t start, int64_t count, void* k,
+                int64_t k_sb, int64_t k_ss, int64_t k_sh, void* v, int64_t v_sb, int64_t v_ss, int64_t v_sh,
+                void* stream) {
+  return kv4_rows("kv4_read", false, k, k_sb, k_ss, k_sh, v, v_sb, v_ss, v_sh, B, Hkv, D, start, count,
+                  const_cast<void*>(cache), capacity, stream);
+}
+
+int tg_qk_norm_rope_append_kv4(const void* q, int64_t ld_q, int n_q_heads, const void* k, int64_t ld_k, int n_k_heads,
+                               const void* v, int64_t ld_v, int rows, const void* q_norm_w, const void* k_norm_w,
+                               const void* cos, const void* sin, int64_t ld_cs, int head_dim, float eps, void* q_out,
+                               int64_t ld_q_out, void* cache, int64_t capacity, const int64_t* slot_dev,
+                               void* stream) {
+  if (rows == 0) return TG_OK;
+  int st = kv4_check("qk_norm_rope_append_kv4", cache, rows, n_k_heads, head_dim, capacity);
+  if (st) return st;
+  if (q == nullptr || k == nullptr || v == nullptr || q_norm_w == nullptr || k_norm_w == nullptr || cos == nullptr ||
+      sin == nullptr || q_out == nullptr || slot_dev == nullptr)
+    return fail(TG_ERR_INVALID_ARGUMENT, "qk_norm_rope_append_kv4: NULL argument");
+  if (n_q_heads < 1 || n_q_heads > 65535 || ld_q < (int64_t)n_q_heads * 128 || ld_q_out < (int64_t)n_q_heads * 128 ||
+      ld_k < (int64_t)n_k_heads * 128 || ld_v < (int64_t)n_k_heads * 128 || ld_cs < 0)
+    return fail(TG_ERR_INVALID_ARGUMENT, "qk_norm_rope_append_kv4: row strides shorter than the heads");
+  const uintptr_t m = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+                      reinterpret_cast<uintptr_t>(q_norm_w) | reinterpret_cast<uintptr_t>(k_norm_w) |
+                      reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin) |
+                      reinterpret_cast<uintptr_t>(q_out);
+  if ((m & 7) || ((ld_q | ld_k | ld_v | ld_cs | ld_q_out) & 3))
+    return fail(TG_ERR_ALIGNMENT, "qk_norm_rope_append_kv4: pointers 8-byte aligned, strides multiples of 4 needed");
+  tg::Kv4AppendParams p;
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.k = static_cast<const __nv_bfloat16*>(k);
+  p.v = static_cast<const __nv_bfloat16*>(v);
+  p.q_out = static_cast<__nv_bfloat16*>(q_out);
+  p.ld_q = ld_q;
+  p.ld_k = ld_k;
+  p.ld_v = ld_v;
+  p.ld_qo = ld_q_out;
+  p.q_w = static_cast<const __nv_bfloat16*>(q_norm_w);
+  p.k_w = static_cast<const __nv_bfloat16*>(k_norm_w);
+  p.cos = static_cast<const __nv_bfloat16*>(cos);
+  p.sin = static_cast<const __nv_bfloat16*>(sin);
+  p.ld_cs = ld_cs;
+  p.cache = static_cast<uint8_t*>(cache);
+  p.c_sh = kv4_tiles(capacity) * tg::kKv4TileBytes;
+  p.c_sb = p.c_sh * n_k_heads;
+  p.slot = slot_dev;
+  p.slots = capacity;
+  p.rows = rows;
+  p.n_q = n_q_heads;
+  p.n_k = n_k_heads;
+  p.eps = eps;
+  const int64_t units = (int64_t)rows * (n_q_heads + 2 * n_k_heads);
+  constexpr int per = tg::kKv4AppendThreads / 16;
+  cudaError_t e = launch_pdl(tg::kv4_append_kernel, dim3((unsigned)((units + per - 1) / per)),
+                             dim3(tg::kKv4AppendThreads), 0, static_cast<cudaStream_t>(stream), p);
+  if (e != cudaSuccess) return cuda_fail(e, "qk_norm_rope_append_kv4 launch");
+  return TG_OK;
+}
+
+int tg_decode_attn_kv4_workspace(int B, int Hq, int Hkv, int n_keys, size_t* bytes) {
+  if (bytes == nullptr) return fail(TG_ERR_INVALID_ARGUMENT, "decode_attn_kv4_workspace: bytes must be non-NULL");
+  *bytes = 0;
+  if (B < 1 || Hq < 1 || Hkv < 1 || n_keys < 1)
+    return fail(TG_ERR_INVALID_ARGUMENT, "decode_attn_kv4_workspace: B=%d Hq=%d Hkv=%d n_keys=%d", B, Hq, Hkv, n_keys);
+  int ns, per;
+  kv4_splits(B, Hkv, n_keys, &ns, &per);
+  if (ns > 1) *bytes = (size_t)B * Hq * ns * tg::kKv4Part * sizeof(float);
+  return TG_OK;
+}
+
+int tg_decode_attn_kv4(const void* q, int64_t q_sb, int64_t q_sh, const float* q_scale, int64_t qs_sb,
+                       const void* cache, int64_t capacity, const float* bias, int64_t bias_sb, int64_t bias_sh,
+                       const int32_t* n_valid, int n_prefix, int n_keys, const int32_t* n_keys_dev, void* out,
+                       int64_t o_sb, int64_t o_sh, void* workspace, size_t workspace_bytes, int B, int Hq, int Hkv,
+                       int D, float softmax_scale, void* stream) {
+  int st = kv4_check("decode_attn_kv4", cache, B, Hkv, D, capacity);
+  if (st) return st;
+  if (q == nullptr || out == nullptr || n_valid == nullptr)
+    return fail(TG_ERR_INVALID_ARGUMENT, "decode_attn_kv4: q, out and n_valid must be non-NULL");
+  if (Hq < 1 || n_keys < 1 || n_prefix < 0 || n_prefix > n_keys || n_keys > capacity)
+    return fail(TG_ERR_INVALID_ARGUMENT, "decode_attn_kv4: Hq=%d n_prefix=%d n_keys=%d capacity=%lld", Hq, n_prefix,
+                n_keys, (long long)capacity);
+  if (Hq % Hkv != 0)
+    return fail(TG_ERR_INVALID_ARGUMENT, "decode_attn_kv4: query heads %d not a multiple of kv heads %d", Hq, Hkv);
+  if (Hq / Hkv > 8)
+    return fail(TG_ERR_UNSUPPORTED, "decode_attn_kv4: %d query heads per kv head (1 to 8 served)", Hq / Hkv);
+  if (!(softmax_scale > 0.f)) return fail(TG_ERR_INVALID_ARGUMENT, "decode_attn_kv4: softmax_scale must be > 0");
+  tg::Kv4AttnParams p;
+  kv4_splits(B, Hkv, n_keys, &p.n_splits, &p.tiles_per_split);
+  if (p.n_splits > 1) {
+    const size_t need = (size_t)B * Hq * p.n_splits * tg::kKv4Part * sizeof(float);
+    if (workspace == nullptr || workspace_bytes < need)
+      return fail(TG_ERR_INVALID_ARGUMENT, "decode_attn_kv4: workspace of %zu bytes, %zu needed", workspace_bytes,
+                  need);
+    if (reinterpret_cast<uintptr_t>(workspace) & 15)
+      return fail(TG_ERR_ALIGNMENT, "decode_attn_kv4: workspace must be 16-byte aligned");
+  }
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.q_sb = q_sb;
+  p.q_sh = q_sh;
+  p.q_scale = q_scale;
+  p.qs_sb = qs_sb;
+  p.cache = static_cast<const uint8_t*>(cache);
+  p.c_sh = kv4_tiles(capacity) * tg::kKv4TileBytes;
+  p.c_sb = p.c_sh * Hkv;
+  p.bias = bias;
+  p.bias_sb = bias_sb;
+  p.bias_sh = bias_sh;
+  p.n_valid = n_valid;
+  p.n_prefix = n_prefix;
+  p.n_keys = n_keys;
+  p.n_keys_dev = n_keys_dev;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.o_sb = o_sb;
+  p.o_sh = o_sh;
+  p.part = static_cast<float*>(workspace);
+  p.Hq = Hq;
+  p.Hkv = Hkv;
+  p.G = Hq / Hkv;
+  p.scale = softmax_scale;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = launch_pdl(tg::kv4_attn_kernel, dim3((unsigned)p.n_splits, (unsigned)Hkv, (unsigned)B),
+                             dim3(tg::kKv4AttnThreads), 0, s, p);
+  if (e != cudaSuccess) return cuda_fail(e, "decode_attn_kv4 launch");
+  if (p.n_splits > 1) {
+    e = launch_pdl(tg::kv4_combine_kernel, dim3((unsigned)Hq, (unsigned)B), dim3(128), 0, s, p);
+    if (e != cudaSuccess) return cuda_fail(e, "decode_attn_kv4 combine launch");
+  }
+  return TG_OK;
+}
+
+// ---- sampling
+namespace {
+bool g_smp_attr_set[2][kMaxDevices] = {};
+constexpr int kSmpMaxSmem = 227 * 1024;
+}  // namespace
+
+int tg_sample(const void* logits, int dtype, int64_t row_stride, int B, int V, const float* u,
+              const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p, int64_t* token,
+              float* logprob, void* stream) {
+  if (B == 0) return TG_OK;
+  if (logits == nullptr || u == nullptr || temperature == nullptr || token == nullptr)
+    return fail(TG_ERR_INVALID_ARGUMENT, "sample: logits, u, temperature and token must be non-NULL");
+  if (dtype != 0 && dtype != 1) return fail(TG_ERR_INVALID_ARGUMENT, "sample: dtype %d (0 = fp32, 1 = bf16)", dtype);
+  if (B < 1 || B > 65535 || V < 1 || (B > 1 && row_stride < V))
+    return fail(TG_ERR_INVALID_ARGUMENT, "sample: B=%d V=%d row_stride=%lld", B, V, (long long)row_stride);
+  if (V > tg::kSmpMaxV) return fail(TG_ERR_UNSUPPORTED, "sample: %d logits a row (at most %d)", V, tg::kSmpMaxV);
+  const int es = dtype ? 2 : 4;
+  if (reinterpret_cast<uintptr_t>(logits) & (es - 1)) return fail(TG_ERR_ALIGNMENT, "sample: logits misaligned");
+  int dev;
+  int st = current_device(&dev);
+  if (st) return st;
+  tg::SampleParams p;
+  p.logits = logits;
+  p.row_stride = row_stride;
+  p.V = V;
+  p.u = u;
+  p.temperature = temperature;
+  p.top_k = top_k;
+  p.top_p = top_p;
+  p.min_p = min_p;
+  p.token = token;
+  p.logprob = logprob;
+  int C = 1;
+  while (C < tg::kSmpMaxCluster && (int64_t)B * C * 2 <= sm_count() && V > C * 4096) C *= 2;
+  p.chunk = ((V + C - 1) / C + 127) / 128 * 128;
+  size_t smem = sizeof(tg::SmpShared) + (size_t)p.chunk * es;
+  p.in_smem = smem <= (size_t)kSmpMaxSmem;
+  if (!p.in_smem) smem = sizeof(tg::SmpShared);
+  cudaError_t e = dtype ? smem_limit_once(tg::sample_kernel<__nv_bfloat16>, kSmpMaxSmem, g_smp_attr_set[1], dev)
+                        : smem_limit_once(tg::sample_kernel<float>, kSmpMaxSmem, g_smp_attr_set[0], dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(sample smem)");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)C, (unsigned)B);
+  cfg.blockDim = dim3(tg::kSmpThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)C;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  e = dtype ? cudaLaunchKernelEx(&cfg, tg::sample_kernel<__nv_bfloat16>, p)
+            : cudaLaunchKernelEx(&cfg, tg::sample_kernel<float>, p);
+  if (e != cudaSuccess) return cuda_fail(e, "sample launch");
+  return TG_OK;
 }
 
 }  // extern "C"

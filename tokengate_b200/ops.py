@@ -14,6 +14,7 @@ import ctypes
 import torch
 
 from . import _lib
+from .kv4 import KV4Cache
 
 _LOG2E = 1.4426950408889634
 
@@ -694,3 +695,239 @@ def gemv(x: torch.Tensor, w: torch.Tensor, swiglu: bool = False, out: Optional[t
         _lib.check_launch(L.tg_gemv(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), out.data_ptr(), out.stride(0),
                              B, N, K, int(bool(swiglu)), _stream(x)))
     return out
+
+
+# ----------------------------------------------------------------- 4-bit KV cache
+def _kv4(cache: KV4Cache) -> KV4Cache:
+    if not isinstance(cache, KV4Cache):
+        raise TypeError(f"cache must be a KV4Cache, got {type(cache).__name__}")
+    return cache
+
+
+def _kv4_rows(name: str, t: torch.Tensor, cache: KV4Cache, n: Optional[int] = None) -> None:
+    _require_cuda(name, t, torch.bfloat16)
+    if t.dim() != 4 or t.shape[0] != cache.batch or t.shape[2] != cache.n_kv_heads or t.shape[3] != 128 \
+            or (n is not None and t.shape[1] != n):
+        raise ValueError(f"{name} must be ({cache.batch}, {'S' if n is None else n}, {cache.n_kv_heads}, 128), "
+                         f"got {tuple(t.shape)}")
+    if t.stride(3) != 1:
+        raise ValueError(f"{name} must have a contiguous last dim")
+    if t.device != cache.data.device:
+        raise ValueError(f"{name} and the cache must be on one device")
+
+
+def kv4_write(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, start: int = 0) -> None:
+    """Quantise k and v (B, S, Hkv, 128) bf16 into the cache's slots [start, start + S) (tg_kv4_write).
+
+    Any strides with a contiguous last dim, multiples of 8 elements (the K/V views of a fused
+    projection, say). Per group of 64 dims: low = min, scale = bf16((max - min) / 15), code =
+    floor((x - low) / scale + 1/2); a group with a NaN or an infinity (or a range past fp32's
+    largest) reads back as NaN."""
+    c = _kv4(cache)
+    _kv4_rows("k", k, c)
+    _kv4_rows("v", v, c, k.shape[1])
+    start, S = int(start), k.shape[1]
+    if start < 0 or start + S > c.capacity:
+        raise ValueError(f"slots [{start}, {start + S}) are outside the cache's capacity {c.capacity}")
+    if S == 0:
+        return
+    with _device_ctx(k):
+        _lib.check_launch(_lib.lib().tg_kv4_write(
+            k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], c.batch, c.n_kv_heads, 128, start, S,
+            c.data.data_ptr(), c.capacity, _stream(k)))
+
+
+def kv4_read(cache: KV4Cache, start: int = 0, n: Optional[int] = None, k_out: Optional[torch.Tensor] = None,
+             v_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The values of slots [start, start + n) as bf16 (k, v), each (B, n, Hkv, 128) (tg_kv4_read);
+    n None: up to the capacity. k_out / v_out: written instead of new tensors, any strides with a
+    contiguous last dim, multiples of 8 elements."""
+    c = _kv4(cache)
+    start = int(start)
+    n = c.capacity - start if n is None else int(n)
+    if start < 0 or n < 0 or start + n > c.capacity:
+        raise ValueError(f"slots [{start}, {start + n}) are outside the cache's capacity {c.capacity}")
+    outs = []
+    for name, t in (("k_out", k_out), ("v_out", v_out)):
+        if t is None:
+            t = torch.empty((c.batch, n, c.n_kv_heads, 128), dtype=torch.bfloat16, device=c.data.device)
+        else:
+            _kv4_rows(name, t, c, n)
+        outs.append(t)
+    k, v = outs
+    if n:
+        with _device_ctx(k):
+            _lib.check_launch(_lib.lib().tg_kv4_read(
+                c.data.data_ptr(), c.capacity, c.batch, c.n_kv_heads, 128, start, n, k.data_ptr(), *k.stride()[:3],
+                v.data_ptr(), *v.stride()[:3], _stream(k)))
+    return k, v
+
+
+def qk_norm_rope_append_kv4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm_w: torch.Tensor,
+                            k_norm_w: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, eps: float,
+                            cache: KV4Cache, slot: torch.Tensor, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """qk_norm_rope_append for a 4-bit cache (tg_qk_norm_rope_append_kv4): one decode token per row.
+
+    q (B, 1, Hq, 128), k / v (B, 1, Hkv, 128) with contiguous heads; cos / sin (B, 1, 128); slot: an
+    int64 (1,) device tensor (outside [0, capacity): nothing is written). q and k are normalised and
+    rotated in fp32 with one rounding to bf16; k and v are quantised into the slot and left unchanged.
+    Returns the finished q, (B, 1, Hq, 128) contiguous (or q_out, which may be q)."""
+    c = _kv4(cache)
+    dev = c.data.device
+    for nm, t in (("q", q), ("k", k), ("v", v)):
+        _require_cuda(nm, t, torch.bfloat16)
+        if t.dim() != 4 or t.shape[1] != 1 or t.shape[3] != 128 or t.stride(3) != 1 \
+                or (t.stride(2) != 128 and t.shape[2] > 1):
+            raise ValueError(f"{nm} must be (B, 1, heads, 128) with contiguous heads")
+    B, _, Hq, _ = q.shape
+    kv_shape = (c.batch, 1, c.n_kv_heads, 128)
+    if B != c.batch or k.shape != kv_shape or v.shape != kv_shape:
+        raise ValueError(f"k and v must be {kv_shape} and q have {c.batch} rows, got q {tuple(q.shape)} "
+                         f"k {tuple(k.shape)} v {tuple(v.shape)}")
+    for nm, t in (("cos", cos), ("sin", sin)):
+        _require_cuda(nm, t, torch.bfloat16)
+        if t.shape != (B, 1, 128) or t.stride(2) != 1:
+            raise ValueError(f"{nm} must be (B, 1, 128) with a contiguous last dim")
+    if cos.stride(0) != sin.stride(0):
+        raise ValueError("cos and sin must share strides")
+    for nm, t in (("q_norm_w", q_norm_w), ("k_norm_w", k_norm_w)):
+        _require_cuda(nm, t, torch.bfloat16)
+        if t.shape != (128,) or t.stride(0) != 1:
+            raise ValueError(f"{nm} must be a contiguous (128,) tensor")
+    _require_cuda("slot", slot, torch.int64)
+    if slot.numel() != 1:
+        raise ValueError("slot must be an int64 (1,) tensor")
+    if q_out is None:
+        q_out = torch.empty((B, 1, Hq, 128), dtype=torch.bfloat16, device=dev)
+    else:
+        _require_cuda("q_out", q_out, torch.bfloat16)
+        if q_out.shape != q.shape or q_out.stride(3) != 1 or (q_out.stride(2) != 128 and Hq > 1):
+            raise ValueError("q_out must have q's shape with contiguous heads")
+    if any(t.device != dev for t in (q, k, v, cos, sin, q_norm_w, k_norm_w, slot, q_out)):
+        raise ValueError("every tensor must be on the cache's device")
+    with _device_ctx(q):
+        _lib.check_launch(_lib.lib().tg_qk_norm_rope_append_kv4(
+            q.data_ptr(), q.stride(0), Hq, k.data_ptr(), k.stride(0), c.n_kv_heads, v.data_ptr(), v.stride(0), B,
+            q_norm_w.data_ptr(), k_norm_w.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.stride(0), 128, eps,
+            q_out.data_ptr(), q_out.stride(0), c.data.data_ptr(), c.capacity, slot.data_ptr(), _stream(q)))
+    return q_out
+
+
+def decode_attention_kv4(q: torch.Tensor, cache: KV4Cache, n_valid: torch.Tensor, n_prefix: int, n_keys: int,
+                         bias: Optional[torch.Tensor] = None, q_scale: Optional[torch.Tensor] = None,
+                         softmax_scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                         n_keys_dev: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """decode_attention over a 4-bit cache (tg_decode_attn_kv4): the same arguments, with the cache in
+    the place of k and v. q: (B, Hq, 128) bf16, Hq / Hkv from 1 to 8. A bias of -inf masks its key
+    whatever the key holds; a row without any key gives zeros. Returns (B, Hq, 128) bf16."""
+    c = _kv4(cache)
+    _require_cuda("q", q, torch.bfloat16)
+    if q.dim() != 3 or q.shape[0] != c.batch or q.shape[2] != 128 or q.stride(2) != 1:
+        raise ValueError(f"q must be ({c.batch}, Hq, 128) with a contiguous last dim, got {tuple(q.shape)}")
+    B, Hq, D = q.shape
+    dev = c.data.device
+    if not 0 <= n_prefix <= n_keys <= c.capacity:
+        raise ValueError(f"need 0 <= n_prefix ({n_prefix}) <= n_keys ({n_keys}) <= cache capacity ({c.capacity})")
+    _require_cuda("n_valid", n_valid, torch.int32)
+    if n_valid.numel() != B or not n_valid.is_contiguous():
+        raise ValueError("n_valid must be a contiguous (B,) int32 tensor")
+    if out is None:
+        out = torch.empty((B, Hq, D), dtype=torch.bfloat16, device=dev)
+    else:
+        _require_cuda("out", out, torch.bfloat16)
+        if out.shape != q.shape or out.stride(2) != 1:
+            raise ValueError("out must have q's shape with a contiguous last dim")
+    bias_ptr, bsb, bsh = None, 0, 0
+    if bias is not None:
+        _require_cuda("bias", bias, torch.float32)
+        bb = bias
+        while bb.dim() < 3:
+            bb = bb.unsqueeze(0)
+        if bb.dim() != 3 or bb.shape[2] < n_prefix or (bb.stride(2) != 1 and bb.shape[2] > 1) \
+                or bb.shape[0] not in (1, B) or bb.shape[1] not in (1, Hq):
+            raise ValueError(f"bias {tuple(bias.shape)} must broadcast to ({B}, {Hq}, >= {n_prefix}) "
+                             "with a contiguous last dim")
+        bsb = 0 if bb.shape[0] == 1 else bb.stride(0)
+        bsh = 0 if bb.shape[1] == 1 else bb.stride(1)
+        bias_ptr = bb.data_ptr()
+    qs_ptr, qsb = None, 0
+    if q_scale is not None:
+        _require_cuda("q_scale", q_scale, torch.float32)
+        if q_scale.shape != (B, Hq) or q_scale.stride(1) != 1:
+            raise ValueError(f"q_scale must be (B, Hq) = ({B}, {Hq}) with a contiguous last dim")
+        qs_ptr, qsb = q_scale.data_ptr(), q_scale.stride(0)
+    nk_ptr = None
+    if n_keys_dev is not None:
+        _require_cuda("n_keys_dev", n_keys_dev, torch.int32)
+        nk_ptr = n_keys_dev.data_ptr()
+    if any(t is not None and t.device != dev for t in (q, n_valid, out, bias, q_scale, n_keys_dev)):
+        raise ValueError("every tensor must be on the cache's device")
+    L = _lib.lib()
+    with _device_ctx(q):
+        nbytes = ctypes.c_size_t(0)
+        _lib.check(L.tg_decode_attn_kv4_workspace(B, Hq, c.n_kv_heads, n_keys, ctypes.byref(nbytes)))
+        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev) if nbytes.value else None
+        _lib.check_launch(L.tg_decode_attn_kv4(
+            q.data_ptr(), q.stride(0), q.stride(1), qs_ptr, qsb, c.data.data_ptr(), c.capacity,
+            bias_ptr, bsb, bsh, n_valid.data_ptr(), n_prefix, n_keys, nk_ptr,
+            out.data_ptr(), out.stride(0), out.stride(1), ws.data_ptr() if ws is not None else None, nbytes.value,
+            B, Hq, c.n_kv_heads, D, D ** -0.5 if softmax_scale is None else softmax_scale, _stream(q)))
+    return out
+
+
+# ----------------------------------------------------------------- sampling
+def _per_row(name: str, val, B: int, dtype: torch.dtype, device: torch.device) -> Optional[torch.Tensor]:
+    if val is None:
+        return None
+    if not isinstance(val, torch.Tensor):
+        return torch.full((B,), val, dtype=dtype, device=device)
+    _require_cuda(name, val, dtype)
+    if val.shape != (B,) or not val.is_contiguous() or val.device != device:
+        raise ValueError(f"{name} must be a number or a contiguous ({B},) tensor on the logits' device")
+    return val
+
+
+def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=None, top_p=None, min_p=None,
+                  token: Optional[torch.Tensor] = None,
+                  logprob: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Sample one token per row from logits (B, V), bf16 or fp32 (tg_sample).
+
+    u: fp32 (B,), a uniform number in [0, 1) per row. temperature, top_k, top_p, min_p: a number for
+    all rows or a (B,) device tensor (fp32, int32, fp32, fp32). temperature <= 0 is greedy; top_k
+    None or <= 0, top_p None or >= 1 and min_p None or <= 0 are off. Order: temperature, the top_k
+    largest, of these the shortest prefix with mass >= top_p, of these those at least min_p times as
+    likely as the largest; ties go to the lower index. The token is the first, by index, at which the
+    running kept mass passes u times the whole. A NaN logit counts as -inf; a row of nothing else
+    gives token 0 and logprob NaN. Returns (token int64 (B,), logprob fp32 (B,)), logprob under the
+    distribution sampled from. token / logprob: written instead of new tensors (logprob only if
+    given or allocated here)."""
+    if not isinstance(logits, torch.Tensor) or logits.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("logits must be an fp32 or bf16 tensor")
+    _require_cuda("logits", logits)
+    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError("logits must be (B, V) with a contiguous last dim")
+    B, V = logits.shape
+    dev = logits.device
+    u = _per_row("u", u, B, torch.float32, dev)
+    if u is None:
+        raise ValueError("u: one uniform number per row is needed")
+    t = _per_row("temperature", temperature, B, torch.float32, dev)
+    if t is None:
+        raise ValueError("temperature must be a number or a tensor")
+    k = _per_row("top_k", top_k, B, torch.int32, dev)
+    p = _per_row("top_p", top_p, B, torch.float32, dev)
+    m = _per_row("min_p", min_p, B, torch.float32, dev)
+    if token is None:
+        token = torch.empty(B, dtype=torch.int64, device=dev)
+    else:
+        _per_row("token", token, B, torch.int64, dev)
+    if logprob is None:
+        logprob = torch.empty(B, dtype=torch.float32, device=dev)
+    else:
+        _per_row("logprob", logprob, B, torch.float32, dev)
+    with _device_ctx(logits):
+        _lib.check_launch(_lib.lib().tg_sample(
+            logits.data_ptr(), 1 if logits.dtype == torch.bfloat16 else 0, logits.stride(0), B, V, u.data_ptr(),
+            t.data_ptr(), k.data_ptr() if k is not None else None, p.data_ptr() if p is not None else None,
+            m.data_ptr() if m is not None else None, token.data_ptr(), logprob.data_ptr(), _stream(logits)))
+    return token, logprob
