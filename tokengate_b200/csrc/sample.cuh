@@ -7,22 +7,25 @@
 //   mass of those k, then of these every w_i >= min_p (w = 1 is the largest);
 //   token = the first index, in index order, at which the running kept mass
 //   passes u times the kept mass; logprob = d_token - log(kept mass).
-// T <= 0 (or NaN) is greedy. Masses are sums of rint(w * 2^44) in 64-bit
-// integers: exact, so the token depends on no order of summing and every
-// block of a cluster takes the same decision (V <= 2^19 keeps them in range).
+// T <= 0 (or NaN) is greedy. Masses are sums of w * 2^44 in integers, exact, so
+// the token depends on no order of summing and every block of a cluster takes
+// the same decision (V <= 2^19 keeps them in 64 bits).
 //
-// A cluster of C blocks takes a row, each an index range of it, copied to its
-// shared memory where it fits. No sort: the k-th value (or the value at which
-// the mass reaches p) is found
-//   1. by a histogram over 2048 linear buckets of d, 1/64 wide (linear in the
-//      logit, so that logits spread over many buckets and shared-memory atomics
-//      seldom collide), counts for k and exp(d + bucket / 64) in fixed point
-//      for p, the latter only as a guess;
-//   2. exactly inside that bucket: the bucket's mass above and inside, and its
-//      smallest and largest key, in one pass (a wrong guess moves by a bucket);
-//      then 8-bit digits of the ordered key from the highest bit in which the
+// A cluster of C blocks takes a row, each an index range of it, whose weights
+// it computes once and keeps in shared memory (rows too long for that compute
+// them again in each pass). Bound by instructions and by the cluster's
+// barriers, not by memory: the row is read once. No sort: the k-th value (or
+// the value at which the mass reaches p) is found
+//   1. by a histogram over 2048 buckets of w, 64 to an octave (linear in w's
+//      bits: two instructions, and nearly linear in the logit, so that logits
+//      spread over many buckets and shared-memory atomics seldom collide):
+//      counts for k; for p the top 13 bits of the mantissas, as a guess only;
+//   2. exactly inside that bucket: one pass gives the mass above it and in it
+//      and its smallest and largest logit (a wrong guess moves by a bucket);
+//      then 8-bit digits of the ordered logit from the highest bit in which the
 //      two differ (none for bf16 logits, whose buckets hold one value).
-// The threshold is a key and a number of its ties, which go by index.
+// The threshold is a logit and a number of its ties, which go by index. Only
+// elements of the threshold's bucket are looked up in the row again.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -36,13 +39,12 @@ constexpr int kSmpWarps = kSmpThreads / 32;
 constexpr int kSmpBuckets = 2048;
 constexpr int kSmpMaxCluster = 8;
 constexpr int kSmpMaxV = 1 << 19;
-constexpr float kSmpMassOne = 17592186044416.f;  // 2^44
+constexpr double kSmpUnit = 1.0 / 17592186044416.0;  // 2^-44: a mass of 1
 
 struct SampleParams {
   const void* logits;
   int64_t row_stride;  // elements
-  int V, chunk;        // indices per block, a multiple of 128 (the last blocks may hold fewer or none)
-  int in_smem;         // the block's range is copied to shared memory
+  int V, chunk;        // indices per block, a multiple of kSmpThreads (the last blocks may hold fewer or none)
   const float* u;
   const float* temperature;
   const int32_t* top_k;   // nullable
@@ -52,18 +54,19 @@ struct SampleParams {
   float* logprob;         // nullable
 };
 
-struct SmpShared {
-  uint32_t cnt[kSmpBuckets];   // this block's histogram, then its slice's totals
+typedef unsigned long long smp_u64;
+
+struct alignas(16) SmpShared {
+  uint32_t cnt[kSmpBuckets];      // this block's histograms
   uint32_t mass[kSmpBuckets];
-  uint32_t tot_cnt[kSmpBuckets];  // the row's histogram, written by every block of the cluster
+  uint32_t tot_cnt[kSmpBuckets];  // the row's, written slice by slice by every block of the cluster
   float tot_mass[kSmpBuckets];
-  unsigned long long dig[2][256];  // digit histograms of a refinement, by pass parity
-  unsigned long long xch[8];       // what the other blocks read of this one
-  unsigned long long red[kSmpWarps][4];
-  float redf[kSmpWarps];
+  smp_u64 dig[2][256];            // digit histograms of a refinement, by pass parity
+  smp_u64 xch[2][4];              // what the other blocks read of this one, by turns
+  smp_u64 red[kSmpWarps][4];
   double scan[kSmpWarps];
   int pick;
-  unsigned long long pick_above;
+  smp_u64 pick_above;
 };
 
 __device__ __forceinline__ uint32_t smp_key(float x) {
@@ -77,120 +80,305 @@ __device__ __forceinline__ float smp_logit(float x) { return x == x ? x + 0.f : 
 __device__ __forceinline__ float smp_load(const float* p) { return smp_logit(*p); }
 __device__ __forceinline__ float smp_load(const __nv_bfloat16* p) { return smp_logit(__bfloat162float(*p)); }
 
-__device__ __forceinline__ float smp_d(float x, float xmax, float zmax, float t) {
-  if (x == xmax) return 0.f;
-  const float d = __fsub_rn(__fdiv_rn(x, t), zmax);
+struct SmpRow {
+  float xmax, zmax, t;
+};
+__device__ __forceinline__ float smp_d(float x, const SmpRow& r) {
+  if (x == r.xmax) return 0.f;
+  const float d = __fsub_rn(r.t == 1.f ? x : __fdiv_rn(x, r.t), r.zmax);
   return d <= 0.f ? d : -INFINITY;  // NaN: both quotients overflowed
 }
-__device__ __forceinline__ unsigned long long smp_mass(float w) { return (unsigned long long)rintf(w * kSmpMassOne); }
-__device__ __forceinline__ int smp_bucket(float d) { return min((int)(-d * 64.f), kSmpBuckets - 1); }
+__device__ __forceinline__ int smp_bucket(float w) {
+  return min(max((int)(0x3F7FFFFFu - __float_as_uint(w)) >> 17, 0), kSmpBuckets - 1);
+}
+// w * 2^44 rounded to an integer, w in [0, 1]: its 22 bits above 2^-22 and the
+// 22 below, each read off the mantissa of 2 + ...
+__device__ __forceinline__ void smp_add_mass(float w, uint32_t& hi, uint32_t& lo) {
+  const float t = __fadd_rz(w, 2.f);
+  const float rest = __fsub_rn(w, __fsub_rn(t, 2.f));
+  hi += __float_as_uint(t) - 0x40000000u;
+  lo += __float_as_uint(__fmaf_rn(rest, 4194304.f, 2.f)) - 0x40000000u;
+}
+__device__ __forceinline__ smp_u64 smp_mass(uint32_t hi, uint32_t lo) { return ((smp_u64)hi << 22) + lo; }
+__device__ __forceinline__ smp_u64 smp_mass(float w) {
+  uint32_t hi = 0, lo = 0;
+  smp_add_mass(w, hi, lo);
+  return smp_mass(hi, lo);
+}
 
-template <typename V>
-__device__ __forceinline__ V smp_warp_sum(V v) {
+__device__ __forceinline__ smp_u64 smp_warp_sum(smp_u64 v) {
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  return v;
+}
+__device__ __forceinline__ smp_u64 smp_warp_scan(smp_u64 v, int lane) {  // inclusive
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const smp_u64 a = __shfl_up_sync(0xffffffffu, v, off);
+    if (lane >= off) v += a;
+  }
   return v;
 }
 __device__ __forceinline__ uint32_t smp_warp_max(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
 __device__ __forceinline__ uint32_t smp_warp_min(uint32_t v) { return __reduce_min_sync(0xffffffffu, v); }
 
-// The row-wide facts every thread carries.
-struct SmpRow {
-  float xmax, zmax, t;
-};
+// One row's state in a block. HELD: sw holds the weights of the block's range.
+template <typename T, bool HELD>
+struct Smp {
+  SmpShared& s;
+  cooperative_groups::cluster_group cl;
+  const T* x;   // the block's range of the row
+  float* sw;
+  int C, rank, n, w0, w1, lane, warp;  // this warp's indices [w0, w1) of the range, contiguous: index order is warp order
+  SmpRow row;
+  int turn, parity;
 
-// The block's elements through `f(local index, logit)`.
-template <typename T, typename F>
-__device__ __forceinline__ void smp_each(const T* x, int n, F f) {
-  for (int i = threadIdx.x; i < n; i += kSmpThreads) f(i, smp_load(x + i));
-}
+  __device__ __forceinline__ void sync() {
+    if (C > 1) cl.sync(); else __syncthreads();
+  }
+  __device__ __forceinline__ float weight(int i) const {
+    if (HELD) return sw[i];
+    const float v = smp_load(x + i);
+    return expf(smp_d(v, row));
+  }
+  // sums a and b, minimum lo and maximum hi over the cluster, to every thread;
+  // mine[2]: this block's a and b, before[2]: those of the blocks of lower rank
+  __device__ void reduce(smp_u64& a, smp_u64& b, uint32_t& lo, uint32_t& hi, smp_u64* before = nullptr) {
+    a = smp_warp_sum(a);
+    b = smp_warp_sum(b);
+    lo = smp_warp_min(lo);
+    hi = smp_warp_max(hi);
+    if (lane == 0) {
+      s.red[warp][0] = a;
+      s.red[warp][1] = b;
+      s.red[warp][2] = lo;
+      s.red[warp][3] = hi;
+    }
+    __syncthreads();
+    smp_u64* o = s.xch[turn];
+    turn ^= 1;
+    if (warp == 0) {
+      a = smp_warp_sum(lane < kSmpWarps ? s.red[lane][0] : 0ull);
+      b = smp_warp_sum(lane < kSmpWarps ? s.red[lane][1] : 0ull);
+      lo = smp_warp_min(lane < kSmpWarps ? (uint32_t)s.red[lane][2] : 0xFFFFFFFFu);
+      hi = smp_warp_max(lane < kSmpWarps ? (uint32_t)s.red[lane][3] : 0u);
+      if (lane == 0) {
+        o[0] = a;
+        o[1] = b;
+        o[2] = lo;
+        o[3] = hi;
+      }
+    }
+    sync();
+    a = b = 0;
+    lo = 0xFFFFFFFFu;
+    hi = 0;
+    if (lane < C) {
+      const smp_u64* r = C > 1 ? cl.map_shared_rank(o, lane) : o;
+      a = r[0];
+      b = r[1];
+      lo = (uint32_t)r[2];
+      hi = (uint32_t)r[3];
+    }
+    if (before != nullptr) {
+      const smp_u64 sa = smp_warp_scan(a, lane) - a, sb = smp_warp_scan(b, lane) - b;
+      before[0] = __shfl_sync(0xffffffffu, sa, rank);
+      before[1] = __shfl_sync(0xffffffffu, sb, rank);
+    }
+    a = smp_warp_sum(a);
+    b = smp_warp_sum(b);
+    lo = smp_warp_min(lo);
+    hi = smp_warp_max(hi);
+  }
 
-// Exact selection inside bucket `bk`: finds the key T and the number r of its
-// ties to take so that the elements of the bucket above T, and r at T, are the
-// fewest whose count (BY_MASS: mass) reaches `need`. Returns also the mass and
-// the count above T inside the bucket.
-template <bool BY_MASS, typename T>
-__device__ void smp_refine(SmpShared& s, cooperative_groups::cluster_group cl, int C, const T* x, int n,
-                           const SmpRow& row, int bk, uint32_t lo_key, uint32_t hi_key, unsigned long long need,
-                           int& parity, uint32_t& key_out, unsigned long long& ties_out) {
-  // every key of the bucket lies in [lo_key, hi_key]
-  uint32_t prefix = 0, mask = 0;
-  if (lo_key == hi_key) {
-    prefix = lo_key;
-  } else {
-    const int top = 31 - __clz(lo_key ^ hi_key);
-    mask = top == 31 ? 0u : ~((2u << top) - 1u);
-    prefix = hi_key & mask;
-    for (int shift = max(top - 7, 0);; shift = max(shift - 8, 0)) {
-      unsigned long long* dig = s.dig[parity];
-      for (int i = threadIdx.x; i < 256; i += kSmpThreads) dig[i] = 0ull;
-      __syncthreads();
-      smp_each(x, n, [&](int, float v) {
-        const uint32_t k = smp_key(v);
-        if ((k & mask) != prefix || v == -INFINITY) return;
-        const float d = smp_d(v, row.xmax, row.zmax, row.t);
-        if (smp_bucket(d) != bk) return;
-        atomicAdd(&dig[(k >> shift) & 255u], BY_MASS ? smp_mass(expf(d)) : 1ull);
-      });
-      if (C > 1) cl.sync(); else __syncthreads();
-      // the cluster's digit totals in dig order, from the highest digit down, by warp 0 of every block
-      if (threadIdx.x < 32) {
-        unsigned long long v[8], sum = 0;
+  // The row's histograms from the blocks': each block sums a slice and hands it to all.
+  __device__ void merge_buckets(bool by_k, bool by_p) {
+    sync();
+    const int slice = kSmpBuckets / C;
+    for (int i = rank * slice + (int)threadIdx.x; i < (rank + 1) * slice; i += kSmpThreads) {
+      uint32_t a = 0;
+      float m = 0.f;
+      for (int c = 0; c < C; ++c) {
+        if (by_k) a += C > 1 ? cl.map_shared_rank(s.cnt, c)[i] : s.cnt[i];
+        if (by_p) m += (float)(C > 1 ? cl.map_shared_rank(s.mass, c)[i] : s.mass[i]);
+      }
+      m *= __uint_as_float((uint32_t)(127 - 13 - (i >> 6)) << 23);  // 2^-12 of the octave [2^-1-o, 2^-o)
+      for (int c = 0; c < C; ++c) {
+        if (by_k) (C > 1 ? cl.map_shared_rank(s.tot_cnt, c) : s.tot_cnt)[i] = a;
+        if (by_p) (C > 1 ? cl.map_shared_rank(s.tot_mass, c) : s.tot_mass)[i] = m;
+      }
+    }
+    sync();
+  }
+
+  // First bucket at which the running count / mass reaches `target` (the last if none does), and what is before it.
+  template <typename A>
+  __device__ int crossing(const A* tot, double target, double& above) {
+    constexpr int E = kSmpBuckets / kSmpThreads;
+    const int tid = threadIdx.x;
+    double v[E], run = 0.;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int dgt = 255 - (threadIdx.x * 8 + e);
-          v[e] = 0;
-          for (int c = 0; c < C; ++c) v[e] += C > 1 ? cl.map_shared_rank(dig, c)[dgt] : dig[dgt];
-          sum += v[e];
-        }
-        unsigned long long before = sum;
+    for (int e = 0; e < E; ++e) {
+      v[e] = (double)tot[E * tid + e];
+      run += v[e];
+    }
+    const double mine = run;
 #pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-          const unsigned long long a = __shfl_up_sync(0xffffffffu, before, off);
-          if ((int)threadIdx.x >= off) before += a;
-        }
-        before -= sum;
-        if (before < need && need <= before + sum) {
-          int e = 0;
-          while (need > before + v[e]) before += v[e++];
-          s.pick = 255 - (threadIdx.x * 8 + e);
-          s.pick_above = before;
+    for (int off = 1; off < 32; off <<= 1) {
+      const double a = __shfl_up_sync(0xffffffffu, run, off);
+      if (lane >= off) run += a;
+    }
+    if (lane == 31) s.scan[warp] = run;
+    if (tid == 0) s.pick = kSmpBuckets - 1;
+    __syncthreads();
+    double part = lane < kSmpWarps ? s.scan[lane] : 0.;  // the warps' sums, scanned by every warp
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const double a = __shfl_up_sync(0xffffffffu, part, off);
+      if (lane >= off) part += a;
+    }
+    const double before_warp = __shfl_sync(0xffffffffu, part, warp > 0 ? warp - 1 : 0);
+    double before = run - mine + (warp > 0 ? before_warp : 0.);
+    // (a thread just past the crossing may try too: the sums of masses round)
+    if (before <= target * (1. + 1e-9) && before + mine >= target) {
+      double at = before;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        at += v[e];
+        if (at >= target && v[e] > 0.) {
+          atomicMin(&s.pick, E * tid + e);
+          break;
         }
       }
-      __syncthreads();
-      const uint32_t dmask = shift + 8 >= 32 ? ~0u << shift : (255u << shift);
-      need -= s.pick_above;
-      prefix = (prefix & ~dmask) | ((uint32_t)s.pick << shift);
-      mask |= dmask;
-      parity ^= 1;
-      __syncthreads();
-      if (shift == 0) break;
+    }
+    __syncthreads();
+    const int bk = s.pick;
+    if (bk / E == tid) {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (e < bk % E) before += v[e];
+      s.scan[0] = before;
+    }
+    __syncthreads();
+    above = s.scan[0];
+    __syncthreads();
+    return bk;
+  }
+
+  // Of the elements in buckets up to `bk` (in `bk` itself only those of a logit above `floor_key`): the mass
+  // above bucket bk, the mass in it, and the range of its logits (hi 0: none).
+  __device__ void look(int bk, uint32_t floor_key, smp_u64& above, smp_u64& inside, uint32_t& lo, uint32_t& hi) {
+    uint32_t ah = 0, al = 0, ih = 0, il = 0;
+    lo = 0xFFFFFFFFu;
+    hi = 0;
+#pragma unroll 4
+    for (int i = w0 + lane; i < w1; i += 32) {
+      const float w = weight(i);
+      const int e = smp_bucket(w);
+      if (e < bk) {
+        smp_add_mass(w, ah, al);
+      } else if (e == bk && w > 0.f) {
+        const uint32_t k = smp_key(smp_load(x + i));
+        if (k > floor_key) {
+          smp_add_mass(w, ih, il);
+          lo = min(lo, k);
+          hi = max(hi, k);
+        }
+      }
+    }
+    above = smp_mass(ah, al);
+    inside = smp_mass(ih, il);
+    reduce(above, inside, lo, hi);
+  }
+
+  __device__ __forceinline__ smp_u64 mass_of_key(uint32_t key) const {
+    return smp_mass(expf(smp_d(smp_unkey(key), row)));
+  }
+
+  // Exact selection inside bucket `bk`, whose admitted logits span [lo_key, hi_key]: the key and the number of
+  // its ties such that the bucket's elements above the key, and those ties, are the fewest whose count
+  // (BY_MASS: mass) reaches `need`.
+  template <bool BY_MASS>
+  __device__ void refine(int bk, uint32_t lo_key, uint32_t hi_key, smp_u64 need, uint32_t& key, smp_u64& ties) {
+    uint32_t prefix = lo_key, mask = 0xFFFFFFFFu;
+    if (lo_key != hi_key) {
+      const int top = 31 - __clz(lo_key ^ hi_key);
+      mask = top == 31 ? 0u : ~((2u << top) - 1u);
+      prefix = hi_key & mask;
+      for (int shift = max(top - 7, 0);; shift = max(shift - 8, 0)) {
+        smp_u64* dig = s.dig[parity];
+        parity ^= 1;
+        if (threadIdx.x < 256) dig[threadIdx.x] = 0ull;
+        __syncthreads();
+        for (int i = w0 + lane; i < w1; i += 32) {
+          const float w = weight(i);
+          if (smp_bucket(w) != bk || w == 0.f) continue;
+          const uint32_t k = smp_key(smp_load(x + i));
+          if ((k & mask) == prefix) atomicAdd(&dig[(k >> shift) & 255u], BY_MASS ? smp_mass(w) : 1ull);
+        }
+        sync();
+        if (warp == 0) {  // the cluster's digits from the highest down, 8 to a lane
+          smp_u64 v[8], sum = 0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int dgt = 255 - (lane * 8 + e);
+            v[e] = 0;
+            for (int c = 0; c < C; ++c) v[e] += C > 1 ? cl.map_shared_rank(dig, c)[dgt] : dig[dgt];
+            sum += v[e];
+          }
+          smp_u64 before = smp_warp_scan(sum, lane) - sum;
+          if (before < need && need <= before + sum) {
+            int e = 0;
+#pragma unroll
+            for (int q = 0; q < 7; ++q)
+              if (e == q && need > before + v[q]) {
+                before += v[q];
+                ++e;
+              }
+            s.pick = 255 - (lane * 8 + e);
+            s.pick_above = before;
+          }
+        }
+        __syncthreads();
+        const uint32_t dmask = 255u << shift;
+        need -= s.pick_above;
+        prefix = (prefix & ~dmask) | ((uint32_t)s.pick << shift);
+        mask |= dmask;
+        __syncthreads();
+        if (shift == 0) break;
+      }
+    }
+    key = prefix;
+    ties = need;
+    if (BY_MASS) {
+      const smp_u64 w = mass_of_key(prefix);
+      ties = w == 0 ? 1ull : max((need + w - 1) / w, 1ull);
     }
   }
-  key_out = prefix;
-  if (BY_MASS) {
-    const unsigned long long w = smp_mass(expf(smp_d(smp_unkey(prefix), row.xmax, row.zmax, row.t)));
-    ties_out = w == 0 ? 1ull : (need + w - 1) / w;
-    if (ties_out == 0) ties_out = 1;
-  } else {
-    ties_out = need;
-  }
-}
+};
 
-template <typename T>
+template <typename T, bool HELD>
 __global__ void __launch_bounds__(kSmpThreads, 1) sample_kernel(const SampleParams p) {
-  namespace cg = cooperative_groups;
   extern __shared__ __align__(16) uint8_t smp_dyn[];
   SmpShared& s = *reinterpret_cast<SmpShared*>(smp_dyn);
-  T* held = reinterpret_cast<T*>(smp_dyn + sizeof(SmpShared));
-  cg::cluster_group cl = cg::this_cluster();
-  const int C = gridDim.x, rank = blockIdx.x, b = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int i0 = min(rank * p.chunk, p.V), n = min(p.chunk, p.V - i0);
-  const T* x = static_cast<const T*>(p.logits) + (int64_t)b * p.row_stride + i0;
-  auto sync_all = [&]() {
-    if (C > 1) cl.sync(); else __syncthreads();
-  };
+  const int b = blockIdx.y;
+  const int i0 = min((int)blockIdx.x * p.chunk, p.V), n = min(p.chunk, p.V - i0);
+  const int per = p.chunk / kSmpWarps;
+  Smp<T, HELD> c{s,
+                 cooperative_groups::this_cluster(),
+                 static_cast<const T*>(p.logits) + (int64_t)b * p.row_stride + i0,
+                 reinterpret_cast<float*>(smp_dyn + sizeof(SmpShared)),
+                 (int)gridDim.x,
+                 (int)blockIdx.x,
+                 n,
+                 min(warp * per, n),
+                 min((warp + 1) * per, n),
+                 lane,
+                 warp,
+                 {0.f, 0.f, 1.f},
+                 0,
+                 0};
   griddep_wait();
   griddep_launch_dependents();
 
@@ -201,326 +389,241 @@ __global__ void __launch_bounds__(kSmpThreads, 1) sample_kernel(const SamplePara
   if (greedy) top_k = 1u;
   const float top_p = p.top_p != nullptr && p.top_p[b] < 1.f ? fmaxf(p.top_p[b], 0.f) : 1.f;
   const float min_p = p.min_p != nullptr && p.min_p[b] > 0.f ? fminf(p.min_p[b], 1.f) : 0.f;
+  const float uu = p.u[b];
+  const bool by_k = top_k > 1u && top_k < (uint32_t)p.V, by_p = top_p < 1.f && top_k > 1u;
 
-  // ---- the largest logit
+  // ---- the largest logit; the range goes to shared memory as fp32
   uint32_t best = 0;
-  for (int i = tid; i < n; i += kSmpThreads) {
-    const T v = x[i];
-    if (p.in_smem) held[i] = v;
-    best = max(best, smp_key(smp_load(&v)));
-  }
-  if (p.in_smem) x = held;
-  best = smp_warp_max(best);
-  if (lane == 0) s.red[warp][0] = best;
-  __syncthreads();
-  if (warp == 0) {
-    best = smp_warp_max((uint32_t)s.red[lane][0]);
-    if (lane == 0) s.xch[0] = best;
-  }
-  sync_all();
-  for (int c = 0; c < C; ++c) best = max(c ? best : 0u, (uint32_t)(C > 1 ? *cl.map_shared_rank(&s.xch[0], c) : s.xch[0]));
-  SmpRow row;
-  row.xmax = smp_unkey(best);
-  row.t = t;
-  row.zmax = __fdiv_rn(row.xmax, t);
-  if (row.xmax == -INFINITY) {  // nothing to choose from (the same in every block of the cluster)
-    if (rank == 0 && tid == 0) {
-      p.token[b] = 0;
-      if (p.logprob != nullptr) p.logprob[b] = __uint_as_float(0x7FC00000u);
+  {
+    constexpr int VEC = 16 / sizeof(T);
+    int done = 0;
+    if ((reinterpret_cast<uintptr_t>(c.x) & 15) == 0) {
+      const uint4* xv = reinterpret_cast<const uint4*>(c.x);
+      const int nv = n / VEC;
+#pragma unroll 4
+      for (int i = tid; i < nv; i += kSmpThreads) {
+        const uint4 q = ld_nc_v4(xv + i);
+        const uint32_t wd[4] = {q.x, q.y, q.z, q.w};
+        float f[VEC];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (VEC == 4) {
+            f[e] = smp_logit(__uint_as_float(wd[e]));
+          } else {
+            f[2 * e % VEC] = smp_logit(__uint_as_float(wd[e] << 16));
+            f[(2 * e + 1) % VEC] = smp_logit(__uint_as_float(wd[e] & 0xFFFF0000u));
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) best = max(best, smp_key(f[e]));
+        if (HELD) {
+#pragma unroll
+          for (int e = 0; e < VEC / 4; ++e)
+            reinterpret_cast<float4*>(c.sw)[i * (VEC / 4) + e] =
+                make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
+        }
+      }
+      done = nv * VEC;
     }
-    sync_all();
+    for (int i = done + tid; i < n; i += kSmpThreads) {
+      const float v = smp_load(c.x + i);
+      if (HELD) c.sw[i] = v;
+      best = max(best, smp_key(v));
+    }
+  }
+  {
+    smp_u64 z0 = 0, z1 = 0;
+    uint32_t lo = 0;
+    c.reduce(z0, z1, lo, best);
+  }
+  c.row.xmax = smp_unkey(best);
+  c.row.t = t;
+  c.row.zmax = __fdiv_rn(c.row.xmax, t);
+  uint32_t thr = 0;      // kept: logits above key `thr` (0: below every finite one), and the first `ties` at it,
+  smp_u64 ties = 0;      // of weight >= min_p
+  smp_u64 my = 0, my_ties = 0, before[2] = {0, 0}, kept = 0;  // this warp's kept mass, without ties; lower blocks'
+
+  if (c.row.xmax == -INFINITY || top_k == 1u) {
+    // nothing to choose from, or the lowest index of the largest logit
+    uint32_t first = 0xFFFFFFFFu, top = 0;
+    for (int i = tid; i < n; i += kSmpThreads)
+      if ((HELD ? c.sw[i] : smp_load(c.x + i)) == c.row.xmax) {
+        first = i0 + i;
+        break;
+      }
+    c.reduce(my, my_ties, first, top);
+    if (c.rank == 0 && tid == 0) {
+      p.token[b] = first;
+      if (p.logprob != nullptr) p.logprob[b] = c.row.xmax == -INFINITY ? __uint_as_float(0x7FC00000u) : 0.f;
+    }
+    c.sync();  // no block leaves while another may read its shared memory
     return;
   }
 
-  // ---- the threshold: keys above `thr`, and the first `ties` at it
-  uint32_t thr = 0;  // key 0 is below every finite logit's
-  unsigned long long ties = 0;
-  const bool by_k = top_k > 1u && top_k < (uint32_t)p.V, by_p = top_p < 1.f && top_k > 1u;
-  if (top_k == 1u) {  // greedy, or a prefix of one: the lowest index of the largest value
-    thr = best;
-    ties = 1;
-  }
-  if (by_k || by_p) {
+  // ---- weights, their mass, and the histograms
+  const bool cut = by_k || by_p;
+  if (cut) {
     for (int i = tid; i < kSmpBuckets; i += kSmpThreads) s.cnt[i] = s.mass[i] = 0u;
     __syncthreads();
-    unsigned long long all = 0;  // exact mass, per thread
-    uint32_t far_n = 0;          // the last bucket gathers the far tail: counted apart
-    smp_each(x, n, [&](int, float v) {
-      if (v == -INFINITY) return;
-      const float d = smp_d(v, row.xmax, row.zmax, row.t);
-      const int bk = smp_bucket(d);
-      if (by_p) all += smp_mass(expf(d));
-      if (bk == kSmpBuckets - 1) {
-        ++far_n;
-        return;
-      }
-      atomicAdd(&s.cnt[bk], 1u);
-      if (by_p) atomicAdd(&s.mass[bk], (uint32_t)rintf(expf(fmaf((float)bk, 1.f / 64.f, d)) * 4096.f));
-    });
-    far_n = __reduce_add_sync(0xffffffffu, far_n);
-    if (lane == 0 && far_n) atomicAdd(&s.cnt[kSmpBuckets - 1], far_n);
-    all = smp_warp_sum(all);
-    if (lane == 0) s.red[warp][0] = all;
-    __syncthreads();
-    if (warp == 0) {
-      all = smp_warp_sum(s.red[lane][0]);
-      if (lane == 0) s.xch[1] = all;
-    }
-    sync_all();
-    // totals: each block sums its slice of the buckets and hands it to all
-    const int slice = kSmpBuckets / C;
-    for (int i = rank * slice + tid; i < (rank + 1) * slice; i += kSmpThreads) {
-      uint32_t a = 0;
-      float m = 0.f;
-      for (int c = 0; c < C; ++c) {
-        a += C > 1 ? cl.map_shared_rank(s.cnt, c)[i] : s.cnt[i];
-        m += (float)(C > 1 ? cl.map_shared_rank(s.mass, c)[i] : s.mass[i]);
-      }
-      m *= expf((float)i * (-1.f / 64.f)) * (1.f / 4096.f);
-      for (int c = 0; c < C; ++c) {
-        (C > 1 ? cl.map_shared_rank(s.tot_cnt, c) : s.tot_cnt)[i] = a;
-        (C > 1 ? cl.map_shared_rank(s.tot_mass, c) : s.tot_mass)[i] = m;
-      }
-    }
-    unsigned long long total = 0;
-    for (int c = 0; c < C; ++c) total += C > 1 ? *cl.map_shared_rank(&s.xch[1], c) : s.xch[1];
-    sync_all();
-    int parity = 0;
-
-    // first bucket at which the running count / mass reaches `target`
-    auto crossing = [&](bool by_mass, double target, double& above) {
-      const double a0 = by_mass ? (double)s.tot_mass[2 * tid] : (double)s.tot_cnt[2 * tid];
-      const double a1 = by_mass ? (double)s.tot_mass[2 * tid + 1] : (double)s.tot_cnt[2 * tid + 1];
-      double run = a0 + a1;
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const double a = __shfl_up_sync(0xffffffffu, run, off);
-        if (lane >= off) run += a;
-      }
-      if (lane == 31) s.scan[warp] = run;
-      if (tid == 0) s.pick = kSmpBuckets - 1;
-      __syncthreads();
-      double before = run - a0 - a1;
-      for (int w = 0; w < warp; ++w) before += s.scan[w];
-      if (before + a0 >= target && a0 > 0.) atomicMin(&s.pick, 2 * tid);
-      else if (before + a0 + a1 >= target && a1 > 0.) atomicMin(&s.pick, 2 * tid + 1);
-      __syncthreads();
-      const int bk = s.pick;
-      if (2 * tid == bk || 2 * tid + 1 == bk) s.scan[0] = bk == 2 * tid ? before : before + a0;
-      __syncthreads();
-      above = s.scan[0];
-      __syncthreads();
-      return bk;
-    };
-    // of the elements that the threshold so far admits: mass above bucket bk, mass in it, its keys' range
-    auto look = [&](int bk, bool limited, uint32_t tk, unsigned long long& above, unsigned long long& inside,
-                    uint32_t& lo, uint32_t& hi) {
-      unsigned long long a = 0, m = 0;
-      uint32_t kl = 0xFFFFFFFFu, kh = 0;
-      smp_each(x, n, [&](int, float v) {
-        if (v == -INFINITY) return;
-        const uint32_t k = smp_key(v);
-        if (limited && k <= tk) return;
-        const float d = smp_d(v, row.xmax, row.zmax, row.t);
-        const int e = smp_bucket(d);
-        if (e > bk) return;
-        const unsigned long long w = smp_mass(expf(d));
-        if (e < bk) {
-          a += w;
+  }
+  {
+    uint32_t hi = 0, lo = 0, far = 0;
+#pragma unroll 4
+    for (int i = c.w0 + lane; i < c.w1; i += 32) {
+      const float w = expf(smp_d(HELD ? c.sw[i] : smp_load(c.x + i), c.row));
+      if (HELD) c.sw[i] = w;
+      if (!cut) {
+        if (w >= min_p) smp_add_mass(w, hi, lo);
+      } else if (w > 0.f) {
+        if (!by_k) smp_add_mass(w, hi, lo);
+        const int e = smp_bucket(w);
+        if (e == kSmpBuckets - 1) {
+          ++far;  // the far tail shares the last bucket: counted apart, its mass left out of the guess
         } else {
-          m += w;
-          kl = min(kl, k);
-          kh = max(kh, k);
-        }
-      });
-      a = smp_warp_sum(a);
-      m = smp_warp_sum(m);
-      kl = smp_warp_min(kl);
-      kh = smp_warp_max(kh);
-      if (lane == 0) {
-        s.red[warp][0] = a;
-        s.red[warp][1] = m;
-        s.red[warp][2] = kl;
-        s.red[warp][3] = kh;
-      }
-      __syncthreads();
-      // xch[2..5] are rewritten by a later look only after another cluster barrier (parity)
-      unsigned long long* xo = &s.xch[2];
-      if (warp == 0) {
-        a = smp_warp_sum(s.red[lane][0]);
-        m = smp_warp_sum(s.red[lane][1]);
-        kl = smp_warp_min((uint32_t)s.red[lane][2]);
-        kh = smp_warp_max((uint32_t)s.red[lane][3]);
-        if (lane == 0) {
-          xo[0] = a;
-          xo[1] = m;
-          xo[2] = kl;
-          xo[3] = kh;
+          if (by_k) atomicAdd(&s.cnt[e], 1u);
+          if (by_p)
+            atomicAdd(&s.mass[e], w == 1.f ? 8192u : ((__float_as_uint(w) & 0x7FFFFFu) | 0x800000u) >> 11);
         }
       }
-      sync_all();
-      above = inside = 0;
-      lo = 0xFFFFFFFFu;
-      hi = 0;
-      for (int c = 0; c < C; ++c) {
-        const unsigned long long* o = C > 1 ? cl.map_shared_rank(xo, c) : xo;
-        above += o[0];
-        inside += o[1];
-        lo = min(lo, (uint32_t)o[2]);
-        hi = max(hi, (uint32_t)o[3]);
+    }
+    my = smp_mass(hi, lo);
+    if (cut) {
+      far = __reduce_add_sync(0xffffffffu, far);
+      if (lane == 0 && far) {
+        atomicAdd(&s.cnt[kSmpBuckets - 1], far);
+        atomicAdd(&s.mass[kSmpBuckets - 1], 1u);  // there is something
       }
-      sync_all();  // before anyone writes xch again
-    };
-
-    unsigned long long kept = total;  // mass of the top-k set
+    }
+  }
+  if (cut) {
+    smp_u64 total = my, above = 0, inside = 0;
+    uint32_t lo = 0, hi = 0;
     double above_n;
+    if (by_k) __syncthreads(); else c.reduce(total, inside, lo, hi);
+    c.merge_buckets(by_k, by_p);
     if (by_k) {
-      const int bk = crossing(false, (double)top_k, above_n);
-      unsigned long long above, inside;
-      uint32_t lo, hi;
-      look(bk, false, 0u, above, inside, lo, hi);
+      const int bk = c.crossing(s.tot_cnt, (double)top_k, above_n);
+      c.look(bk, 0u, above, inside, lo, hi);
+      total = above + inside;
       if (hi != 0u) {
-        const uint32_t in_bucket = s.tot_cnt[bk];
-        const unsigned long long need = (unsigned long long)top_k - (unsigned long long)above_n;
-        if (need >= in_bucket) {  // the whole bucket (or fewer finite logits than k)
+        const smp_u64 need = (smp_u64)top_k - (smp_u64)above_n;
+        if (need >= s.tot_cnt[bk]) {  // the whole bucket, or fewer logits than k
           thr = lo - 1u;
-          ties = 0;
-          kept = above + inside;
         } else {
-          smp_refine<false>(s, cl, C, x, n, row, bk, lo, hi, need, parity, thr, ties);
+          c.template refine<false>(bk, lo, hi, need, thr, ties);
           if (by_p) {
-            unsigned long long a2, m2;
-            uint32_t l2, h2;
-            look(bk, true, thr, a2, m2, l2, h2);
-            kept = a2 + m2 + ties * smp_mass(expf(smp_d(smp_unkey(thr), row.xmax, row.zmax, row.t)));
+            if (lo != hi) c.look(bk, thr, above, inside, lo, hi); else inside = 0;
+            total = above + inside + ties * c.mass_of_key(thr);
           }
         }
       }
     }
     if (by_p) {
-      const double goal = (double)top_p * (double)kept;
-      unsigned long long need = (unsigned long long)ceil(goal);
-      if (need < 1) need = 1;
-      int bp = crossing(true, goal * (1.0 / (double)kSmpMassOne), above_n);
+      const double goal = (double)top_p * (double)total;
+      const smp_u64 need = max((smp_u64)ceil(goal), 1ull);
+      const int bt = thr != 0u ? smp_bucket(expf(smp_d(smp_unkey(thr), c.row))) : kSmpBuckets - 1;
+      int bp = min(c.crossing(s.tot_mass, goal * kSmpUnit, above_n), bt);
       // exact: move the guess until the mass above bucket bp is short of `need` and the mass with it is not
-      unsigned long long above = 0, inside = 0;
-      uint32_t lo, hi;
-      bool beyond = false;  // the boundary lies among the top-k threshold's own ties
       for (;;) {
-        look(bp, by_k && thr != 0u, thr, above, inside, lo, hi);
+        c.look(bp, bp == bt ? thr : 0u, above, inside, lo, hi);
         if (above >= need && bp > 0) {
-          do --bp; while (bp > 0 && s.tot_cnt[bp] == 0u);
-        } else if (above + inside < need && bp < kSmpBuckets - 1) {
-          int nb = bp + 1;
-          while (nb < kSmpBuckets && s.tot_cnt[nb] == 0u) ++nb;
-          if (nb == kSmpBuckets) {
-            beyond = true;
-            break;
-          }
-          bp = nb;
+          do --bp; while (bp > 0 && s.tot_mass[bp] == 0.f);
+        } else if (above + inside < need && bp < bt) {
+          do ++bp; while (bp < bt && s.tot_mass[bp] == 0.f);
         } else {
-          beyond = above + inside < need;
           break;
         }
       }
-      if (beyond) {
-        // everything above the top-k threshold is in; some of its ties are still needed
-        if (by_k && thr != 0u && ties > 0) {
-          const unsigned long long w = smp_mass(expf(smp_d(smp_unkey(thr), row.xmax, row.zmax, row.t)));
-          const unsigned long long left = need - (above + inside);
-          const unsigned long long r = w == 0 ? ties : (left + w - 1) / w;
-          ties = r < ties ? r : ties;
-        }
+      if (above + inside < need) {
+        // everything above the top-k threshold is in, and some of its ties
+        const smp_u64 w = thr != 0u ? c.mass_of_key(thr) : 0ull, left = need - (above + inside);
+        if (w != 0) ties = min(ties, (left + w - 1) / w);
       } else {
-        // the digit passes see the whole bucket; above the top-k threshold the order is the same
-        smp_refine<true>(s, cl, C, x, n, row, bp, lo, hi, need - above, parity, thr, ties);
+        // the digit passes see the whole bucket; above the top-k threshold its order is the same
+        c.template refine<true>(bp, lo, hi, need - above, thr, ties);
       }
     }
   }
 
-  // ---- the kept mass, by 128-index pieces, then the token
-  auto admitted = [&](float v, float& d, float& w) {  // 0: no, 1: above the threshold, 2: a tie
-    if (v == -INFINITY) return 0;
-    const uint32_t k = smp_key(v);
-    if (k < thr || (k == thr && ties == 0)) return 0;
-    d = smp_d(v, row.xmax, row.zmax, row.t);
-    w = expf(d);
-    if (!(w >= min_p)) return 0;
-    return k > thr ? 1 : 2;
+  // ---- the kept mass by warp and block
+  const float w_thr = thr != 0u ? expf(smp_d(smp_unkey(thr), c.row)) : 0.f;
+  const int bt = thr != 0u ? smp_bucket(w_thr) : kSmpBuckets;
+  auto admitted = [&](int i, float w) {  // 0: no, 1: above the threshold, 2: a tie
+    if (!(w >= min_p) || w == 0.f) return 0;
+    const int e = smp_bucket(w);
+    if (e != bt) return e < bt ? 1 : 0;
+    const uint32_t k = smp_key(smp_load(c.x + i));
+    return k > thr ? 1 : (k == thr && ties != 0) ? 2 : 0;
   };
-  unsigned long long mass = 0;
-  uint32_t n_tie = 0;
-  smp_each(x, n, [&](int, float v) {
-    float d, w;
-    const int a = admitted(v, d, w);
-    if (a == 1) mass += smp_mass(w);
-    if (a == 2) ++n_tie;
-  });
-  mass = smp_warp_sum(mass);
-  n_tie = __reduce_add_sync(0xffffffffu, n_tie);
-  if (lane == 0) {
-    s.red[warp][0] = mass;
-    s.red[warp][1] = n_tie;
-  }
-  __syncthreads();
-  if (warp == 0) {
-    mass = smp_warp_sum(s.red[lane][0]);
-    const unsigned long long nt = smp_warp_sum(s.red[lane][1]);
-    if (lane == 0) {
-      s.xch[6] = mass;
-      s.xch[7] = nt;
+  if (cut) {
+    uint32_t hi = 0, lo = 0, nt = 0;
+#pragma unroll 4
+    for (int i = c.w0 + lane; i < c.w1; i += 32) {
+      const float w = c.weight(i);
+      const int a = admitted(i, w);
+      if (a == 1) smp_add_mass(w, hi, lo);
+      if (a == 2) ++nt;
     }
+    my = smp_mass(hi, lo);
+    my_ties = nt;
   }
-  sync_all();
-  const unsigned long long w_tie =
-      thr != 0u ? smp_mass(expf(smp_d(smp_unkey(thr), row.xmax, row.zmax, row.t))) : 0ull;
-  unsigned long long kept = 0, before = 0, tie_before = 0, own = 0, tie_run = 0;
-  for (int c = 0; c < C; ++c) {
-    const unsigned long long* o = C > 1 ? cl.map_shared_rank(&s.xch[6], c) : &s.xch[6];
-    const unsigned long long tk = o[1] < ties - tie_run ? o[1] : ties - tie_run;
-    const unsigned long long here = o[0] + tk * w_tie;
-    if (c == rank) {
-      before = kept;
-      tie_before = tie_run;
-      own = here;
-    }
-    kept += here;
-    tie_run += tk;
+  smp_u64 all_ties = my_ties;
+  kept = my;
+  {
+    uint32_t lo = 0, hi = 0;
+    c.reduce(kept, all_ties, lo, hi, before);
   }
-  // first index with running mass > u * kept; u >= 1 (or its rounding) takes the last kept token
-  const float uu = p.u[b];
-  const double goal_f = (double)fminf(fmaxf(uu, 0.f), 1.f) * (double)kept;
-  unsigned long long goal = (unsigned long long)floor(goal_f);
+  // s.red[w][0 .. 1] still holds the block's warps' masses and ties
+  const smp_u64 w_tie = smp_mass(w_thr);
+  auto with_ties = [&](smp_u64 m, smp_u64 nt) { return m + min(nt, ties) * w_tie; };
+  kept = with_ties(kept, all_ties);
+  // first index with running mass > u * kept; u of 1 or more takes the last kept token
+  smp_u64 goal = (smp_u64)floor((double)fminf(fmaxf(uu, 0.f), 1.f) * (double)kept);
   if (goal >= kept) goal = kept - 1;
-  if (kept > 0 && goal >= before && goal < before + own && warp == 0) {
-    // warp 0 walks its block's range; `run` is the kept mass before the piece
-    unsigned long long run = before, tr = tie_before;
-    for (int base = 0; base < n; base += 32) {
-      const int i = base + lane;
-      float d = 0.f, w = 0.f;
-      const int a = i < n ? admitted(smp_load(x + i), d, w) : 0;
-      const uint32_t tm = __ballot_sync(0xffffffffu, a == 2);
-      const unsigned long long tie_rank = tr + __popc(tm & ((1u << lane) - 1u));
-      unsigned long long mine = a == 1 || (a == 2 && tie_rank < ties) ? smp_mass(w) : 0ull;
-      unsigned long long inc = mine;
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const unsigned long long y = __shfl_up_sync(0xffffffffu, inc, off);
-        if (lane >= off) inc += y;
+  {
+    const smp_u64 wm = lane < kSmpWarps ? s.red[lane][0] : 0ull, wt = lane < kSmpWarps ? s.red[lane][1] : 0ull;
+    const smp_u64 em = before[0] + smp_warp_scan(wm, lane), et = before[1] + smp_warp_scan(wt, lane);
+    const smp_u64 m0 = __shfl_sync(0xffffffffu, em - wm, warp), t0 = __shfl_sync(0xffffffffu, et - wt, warp);
+    const smp_u64 m1 = __shfl_sync(0xffffffffu, em, warp), t1 = __shfl_sync(0xffffffffu, et, warp);
+    if (goal >= with_ties(m0, t0) && goal < with_ties(m1, t1)) {
+      // this warp holds the token: its lanes sum a contiguous run each, then all walk the run that holds it
+      const int run = (c.w1 - c.w0 + 31) >> 5;
+      const int r0 = min(c.w0 + lane * run, c.w1), r1 = min(r0 + run, c.w1);
+      uint32_t hi = 0, lo = 0, nt = 0;
+      for (int i = r0; i < r1; ++i) {
+        const float w = c.weight(i);
+        const int a = admitted(i, w);
+        if (a == 1) smp_add_mass(w, hi, lo);
+        if (a == 2) ++nt;
       }
-      const uint32_t hit = __ballot_sync(0xffffffffu, run + inc > goal);
-      if (hit) {
-        if (lane == __ffs(hit) - 1) {
-          p.token[b] = i0 + i;
-          if (p.logprob != nullptr) p.logprob[b] = d - logf((float)((double)kept * (1.0 / (double)kSmpMassOne)));
+      const smp_u64 rm = smp_mass(hi, lo), rt = nt;
+      const smp_u64 im = m0 + smp_warp_scan(rm, lane), it = t0 + smp_warp_scan(rt, lane);
+      const uint32_t hit = __ballot_sync(0xffffffffu, with_ties(im, it) > goal);
+      const int src = __ffs(hit) - 1;
+      smp_u64 fm = __shfl_sync(0xffffffffu, im - rm, src), ft = __shfl_sync(0xffffffffu, it - rt, src);
+      const int j0 = __shfl_sync(0xffffffffu, r0, src), j1 = __shfl_sync(0xffffffffu, r1, src);
+      for (int base = j0; base < j1; base += 32) {
+        const int i = base + lane;
+        const float w = i < j1 ? c.weight(i) : 0.f;
+        const int a = i < j1 ? admitted(i, w) : 0;
+        const smp_u64 sm = fm + smp_warp_scan(a == 1 ? smp_mass(w) : 0ull, lane);
+        const uint32_t tm = __ballot_sync(0xffffffffu, a == 2);
+        const smp_u64 st = ft + __popc(tm & (0xFFFFFFFFu >> (31 - lane)));
+        const uint32_t found = __ballot_sync(0xffffffffu, with_ties(sm, st) > goal);
+        if (found) {
+          if (lane == __ffs(found) - 1) {
+            p.token[b] = i0 + i;
+            if (p.logprob != nullptr)
+              p.logprob[b] = smp_d(smp_load(c.x + i), c.row) - logf((float)((double)kept * kSmpUnit));
+          }
+          break;
         }
-        break;
+        fm = __shfl_sync(0xffffffffu, sm, 31);
+        ft += __popc(tm);
       }
-      run += __shfl_sync(0xffffffffu, inc, 31);
-      tr += __popc(tm);
     }
   }
-  sync_all();  // no block leaves while another may read its shared memory
+  c.sync();  // no block leaves while another may read its shared memory
 }
 
 }  // namespace tg

@@ -1526,7 +1526,7 @@ int tg_decode_attn_kv4(const void* q, int64_t q_sb, int64_t q_sh, const float* q
 
 // ---- sampling
 namespace {
-bool g_smp_attr_set[2][kMaxDevices] = {};
+bool g_smp_attr_set[4][kMaxDevices] = {};  // per dtype and whether the weights are held
 constexpr int kSmpMaxSmem = 227 * 1024;
 }  // namespace
 
@@ -1540,8 +1540,7 @@ int tg_sample(const void* logits, int dtype, int64_t row_stride, int B, int V, c
   if (B < 1 || B > 65535 || V < 1 || (B > 1 && row_stride < V))
     return fail(TG_ERR_INVALID_ARGUMENT, "sample: B=%d V=%d row_stride=%lld", B, V, (long long)row_stride);
   if (V > tg::kSmpMaxV) return fail(TG_ERR_UNSUPPORTED, "sample: %d logits a row (at most %d)", V, tg::kSmpMaxV);
-  const int es = dtype ? 2 : 4;
-  if (reinterpret_cast<uintptr_t>(logits) & (es - 1)) return fail(TG_ERR_ALIGNMENT, "sample: logits misaligned");
+  if (reinterpret_cast<uintptr_t>(logits) & (dtype ? 1 : 3)) return fail(TG_ERR_ALIGNMENT, "sample: logits misaligned");
   int dev;
   int st = current_device(&dev);
   if (st) return st;
@@ -1556,19 +1555,23 @@ int tg_sample(const void* logits, int dtype, int64_t row_stride, int B, int V, c
   p.min_p = min_p;
   p.token = token;
   p.logprob = logprob;
+  // blocks of a cluster: as many as keep one block per SM busy, at least as many as hold the weights
   int C = 1;
-  while (C < tg::kSmpMaxCluster && (int64_t)B * C * 2 <= sm_count() && V > C * 4096) C *= 2;
-  p.chunk = ((V + C - 1) / C + 127) / 128 * 128;
-  size_t smem = sizeof(tg::SmpShared) + (size_t)p.chunk * es;
-  p.in_smem = smem <= (size_t)kSmpMaxSmem;
-  if (!p.in_smem) smem = sizeof(tg::SmpShared);
-  cudaError_t e = dtype ? smem_limit_once(tg::sample_kernel<__nv_bfloat16>, kSmpMaxSmem, g_smp_attr_set[1], dev)
-                        : smem_limit_once(tg::sample_kernel<float>, kSmpMaxSmem, g_smp_attr_set[0], dev);
+  auto chunk_of = [&](int c) { return (V + c * tg::kSmpThreads - 1) / (c * tg::kSmpThreads) * tg::kSmpThreads; };
+  auto smem_of = [&](int c) { return sizeof(tg::SmpShared) + (size_t)chunk_of(c) * sizeof(float); };
+  while (C < tg::kSmpMaxCluster &&
+         (((int64_t)B * C * 2 <= sm_count() && V > C * 4096) || smem_of(C) > (size_t)kSmpMaxSmem))
+    C *= 2;
+  p.chunk = chunk_of(C);
+  const bool held = smem_of(C) <= (size_t)kSmpMaxSmem;
+  auto kern = dtype ? (held ? tg::sample_kernel<__nv_bfloat16, true> : tg::sample_kernel<__nv_bfloat16, false>)
+                    : (held ? tg::sample_kernel<float, true> : tg::sample_kernel<float, false>);
+  cudaError_t e = smem_limit_once(kern, kSmpMaxSmem, g_smp_attr_set[2 * dtype + held], dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(sample smem)");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)C, (unsigned)B);
   cfg.blockDim = dim3(tg::kSmpThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = held ? smem_of(C) : sizeof(tg::SmpShared);
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1579,8 +1582,7 @@ int tg_sample(const void* logits, int dtype, int64_t row_stride, int B, int V, c
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  e = dtype ? cudaLaunchKernelEx(&cfg, tg::sample_kernel<__nv_bfloat16>, p)
-            : cudaLaunchKernelEx(&cfg, tg::sample_kernel<float>, p);
+  e = cudaLaunchKernelEx(&cfg, kern, p);
   if (e != cudaSuccess) return cuda_fail(e, "sample launch");
   return TG_OK;
 }
