@@ -16,16 +16,21 @@
 // them again in each pass). Bound by instructions and by the cluster's
 // barriers, not by memory: the row is read once. No sort: the k-th value (or
 // the value at which the mass reaches p) is found
-//   1. by a histogram over 2048 buckets of w, 64 to an octave (linear in w's
+//   1. by a histogram over 1024 buckets of w, 32 to an octave (linear in w's
 //      bits: two instructions, and nearly linear in the logit, so that logits
 //      spread over many buckets and shared-memory atomics seldom collide):
-//      counts for k; for p the top 13 bits of the mantissas, as a guess only;
-//   2. exactly inside that bucket: one pass gives the mass above it and in it
-//      and its smallest and largest logit (a wrong guess moves by a bucket);
-//      then 8-bit digits of the ordered logit from the highest bit in which the
-//      two differ (none for bf16 logits, whose buckets hold one value).
+//      counts for k; for p the top 12 bits of the mantissas, as a guess only.
+//      Each block owns a slice of the row's and hands it to the others;
+//   2. exactly inside that bucket: one pass gives the mass above it and in it,
+//      its smallest and largest logit and the list of its logits (a wrong guess
+//      moves by a bucket); then 8-bit digits of the ordered logit from the
+//      highest bit in which the two differ (none for bf16 logits, whose buckets
+//      hold one or two values), every block on a copy of all lists, so without
+//      a cluster barrier (lists too long for that: over the row again).
 // The threshold is a logit and a number of its ties, which go by index. Only
-// elements of the threshold's bucket are looked up in the row again.
+// elements of the threshold's bucket are looked up in the row again. Blocks
+// write to one another's shared memory and read their own: a remote load costs
+// the reader its latency, and sixteen blocks reading one word queue up.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -34,10 +39,12 @@
 
 namespace tg {
 
-constexpr int kSmpThreads = 1024;
+constexpr int kSmpThreads = 512;
 constexpr int kSmpWarps = kSmpThreads / 32;
-constexpr int kSmpBuckets = 2048;
-constexpr int kSmpMaxCluster = 8;
+constexpr int kSmpBuckets = 1024;
+constexpr int kSmpList = 1024;      // logits of one bucket that a block can list
+constexpr int kSmpAllLists = 2048;  // and the cluster
+constexpr int kSmpMaxCluster = 16;   // above 8: opt-in
 constexpr int kSmpMaxV = 1 << 19;
 constexpr double kSmpUnit = 1.0 / 17592186044416.0;  // 2^-44: a mass of 1
 
@@ -57,16 +64,17 @@ struct SampleParams {
 typedef unsigned long long smp_u64;
 
 struct alignas(16) SmpShared {
-  uint32_t cnt[kSmpBuckets];      // this block's histograms
-  uint32_t mass[kSmpBuckets];
-  uint32_t tot_cnt[kSmpBuckets];  // the row's, written slice by slice by every block of the cluster
-  float tot_mass[kSmpBuckets];
+  uint32_t own[2][kSmpBuckets];   // this block's histograms (counts, masses); then lists of a bucket's logits, by turns
+  uint32_t tot[2][kSmpBuckets];   // the row's histograms
+  uint32_t all[kSmpAllLists];     // this block's slices of the row's histograms; then the blocks' lists together
+  uint32_t at[kSmpList];          // where in the block's range the listed logits are
   smp_u64 dig[2][256];            // digit histograms of a refinement, by pass parity
-  smp_u64 xch[2][4];              // what the other blocks read of this one, by turns
+  smp_u64 xch[2][kSmpMaxCluster][4];  // what each block of the cluster has sent, by turns
   smp_u64 red[kSmpWarps][4];
   double scan[kSmpWarps];
-  int pick;
   smp_u64 pick_above;
+  int pick;
+  uint32_t n_list;
 };
 
 __device__ __forceinline__ uint32_t smp_key(float x) {
@@ -80,16 +88,30 @@ __device__ __forceinline__ float smp_logit(float x) { return x == x ? x + 0.f : 
 __device__ __forceinline__ float smp_load(const float* p) { return smp_logit(*p); }
 __device__ __forceinline__ float smp_load(const __nv_bfloat16* p) { return smp_logit(__bfloat162float(*p)); }
 
+// x / T as x * (1/T) with 1/T held as a sum of two floats (N. Brisebarre and
+// J.-M. Muller, "Correctly rounded multiplication by arbitrary precision
+// constants", 2008): x * high + RN(x * low) in one fma is within 2^-47 of the
+// quotient before its rounding, a division's cost without a division. Outside
+// the range in which the low part is a normal number, the division itself.
 struct SmpRow {
-  float xmax, zmax, t;
+  float xmax, zmax, t, rh, rl;
+  bool by_product;
+  __device__ __forceinline__ void set_t(float tt) {
+    t = tt;
+    by_product = t > 8.6736174e-19f && t < 1.1529215e18f;  // 2^-60, 2^60
+    rh = __frcp_rn(t);
+    rl = __fdiv_rn(__fmaf_rn(-t, rh, 1.f), t);
+  }
+  __device__ __forceinline__ float over_t(float x) const {
+    return by_product ? __fmaf_rn(x, rh, __fmul_rn(x, rl)) : __fdiv_rn(x, t);
+  }
 };
 __device__ __forceinline__ float smp_d(float x, const SmpRow& r) {
-  if (x == r.xmax) return 0.f;
-  const float d = __fsub_rn(r.t == 1.f ? x : __fdiv_rn(x, r.t), r.zmax);
-  return d <= 0.f ? d : -INFINITY;  // NaN: both quotients overflowed
+  const float d = __fsub_rn(r.over_t(x), r.zmax);
+  return x == r.xmax ? 0.f : d <= 0.f ? d : -INFINITY;  // NaN: both quotients overflowed
 }
 __device__ __forceinline__ int smp_bucket(float w) {
-  return min(max((int)(0x3F7FFFFFu - __float_as_uint(w)) >> 17, 0), kSmpBuckets - 1);
+  return min(max((int)(0x3F7FFFFFu - __float_as_uint(w)) >> 18, 0), kSmpBuckets - 1);
 }
 // w * 2^44 rounded to an integer, w in [0, 1]: its 22 bits above 2^-22 and the
 // 22 below, each read off the mantissa of 2 + ...
@@ -126,7 +148,6 @@ __device__ __forceinline__ uint32_t smp_warp_min(uint32_t v) { return __reduce_m
 template <typename T, bool HELD>
 struct Smp {
   SmpShared& s;
-  cooperative_groups::cluster_group cl;
   const T* x;   // the block's range of the row
   float* sw;
   int C, rank, n, w0, w1, lane, warp;  // this warp's indices [w0, w1) of the range, contiguous: index order is warp order
@@ -134,16 +155,25 @@ struct Smp {
   int turn, parity;
 
   __device__ __forceinline__ void sync() {
-    if (C > 1) cl.sync(); else __syncthreads();
+    if (C > 1) {
+      __syncwarp();  // the cluster barrier wants whole warps
+      cluster_sync_all();
+    } else {
+      __syncthreads();
+    }
+  }
+  template <typename V>
+  __device__ __forceinline__ V* remote(V* p, int r) const {
+    return C > 1 ? cooperative_groups::this_cluster().map_shared_rank(p, r) : p;
   }
   __device__ __forceinline__ float weight(int i) const {
     if (HELD) return sw[i];
-    const float v = smp_load(x + i);
-    return expf(smp_d(v, row));
+    return expf(smp_d(smp_load(x + i), row));
   }
-  // sums a and b, minimum lo and maximum hi over the cluster, to every thread;
-  // mine[2]: this block's a and b, before[2]: those of the blocks of lower rank
-  __device__ void reduce(smp_u64& a, smp_u64& b, uint32_t& lo, uint32_t& hi, smp_u64* before = nullptr) {
+  // To every thread: the sums of a and b, the minimum lo, the maximum hi and the sum of cnt (one value per block)
+  // over the cluster; before[2]: a and b of the blocks of lower rank. s.red[w][0 .. 1] keeps a and b of warp w.
+  __device__ __forceinline__ void reduce(smp_u64& a, smp_u64& b, uint32_t& lo, uint32_t& hi, uint32_t& cnt,
+                                         smp_u64* before) {
     a = smp_warp_sum(a);
     b = smp_warp_sum(b);
     lo = smp_warp_min(lo);
@@ -155,30 +185,32 @@ struct Smp {
       s.red[warp][3] = hi;
     }
     __syncthreads();
-    smp_u64* o = s.xch[turn];
+    smp_u64(*o)[4] = s.xch[turn];
     turn ^= 1;
     if (warp == 0) {
-      a = smp_warp_sum(lane < kSmpWarps ? s.red[lane][0] : 0ull);
-      b = smp_warp_sum(lane < kSmpWarps ? s.red[lane][1] : 0ull);
-      lo = smp_warp_min(lane < kSmpWarps ? (uint32_t)s.red[lane][2] : 0xFFFFFFFFu);
-      hi = smp_warp_max(lane < kSmpWarps ? (uint32_t)s.red[lane][3] : 0u);
-      if (lane == 0) {
-        o[0] = a;
-        o[1] = b;
-        o[2] = lo;
-        o[3] = hi;
+      const bool in = lane < kSmpWarps;
+      a = smp_warp_sum(in ? s.red[lane][0] : 0ull);
+      b = smp_warp_sum(in ? s.red[lane][1] : 0ull);
+      lo = smp_warp_min(in ? (uint32_t)s.red[lane][2] : 0xFFFFFFFFu);
+      hi = smp_warp_max(in ? (uint32_t)s.red[lane][3] : 0u);
+      if (lane < C) {
+        smp_u64* to = remote(o[rank], lane);
+        to[0] = a;
+        to[1] = b;
+        to[2] = lo | (smp_u64)hi << 32;
+        to[3] = s.n_list;
       }
     }
     sync();
     a = b = 0;
     lo = 0xFFFFFFFFu;
-    hi = 0;
+    hi = cnt = 0;
     if (lane < C) {
-      const smp_u64* r = C > 1 ? cl.map_shared_rank(o, lane) : o;
-      a = r[0];
-      b = r[1];
-      lo = (uint32_t)r[2];
-      hi = (uint32_t)r[3];
+      a = o[lane][0];
+      b = o[lane][1];
+      lo = (uint32_t)o[lane][2];
+      hi = (uint32_t)(o[lane][2] >> 32);
+      cnt = (uint32_t)o[lane][3];
     }
     if (before != nullptr) {
       const smp_u64 sa = smp_warp_scan(a, lane) - a, sb = smp_warp_scan(b, lane) - b;
@@ -189,37 +221,44 @@ struct Smp {
     b = smp_warp_sum(b);
     lo = smp_warp_min(lo);
     hi = smp_warp_max(hi);
+    if (__any_sync(0xffffffffu, cnt > kSmpList)) cnt = kSmpAllLists;  // some block's list ran over
+    cnt = __reduce_add_sync(0xffffffffu, cnt);
   }
 
-  // The row's histograms from the blocks': each block sums a slice and hands it to all.
-  __device__ void merge_buckets(bool by_k, bool by_p) {
-    sync();
+  // The row's histogram `which` (0: counts, 1: masses) into every block's s.tot: each block's goes to the owners of
+  // its slices, and from there to all. In two steps, with a cluster barrier after each.
+  __device__ __forceinline__ void merge_to_owner(int which) {
     const int slice = kSmpBuckets / C;
-    for (int i = rank * slice + (int)threadIdx.x; i < (rank + 1) * slice; i += kSmpThreads) {
-      uint32_t a = 0;
-      float m = 0.f;
-      for (int c = 0; c < C; ++c) {
-        if (by_k) a += C > 1 ? cl.map_shared_rank(s.cnt, c)[i] : s.cnt[i];
-        if (by_p) m += (float)(C > 1 ? cl.map_shared_rank(s.mass, c)[i] : s.mass[i]);
-      }
-      m *= __uint_as_float((uint32_t)(127 - 13 - (i >> 6)) << 23);  // 2^-12 of the octave [2^-1-o, 2^-o)
-      for (int c = 0; c < C; ++c) {
-        if (by_k) (C > 1 ? cl.map_shared_rank(s.tot_cnt, c) : s.tot_cnt)[i] = a;
-        if (by_p) (C > 1 ? cl.map_shared_rank(s.tot_mass, c) : s.tot_mass)[i] = m;
+    for (int i = threadIdx.x; i < kSmpBuckets; i += kSmpThreads) {
+      const uint32_t v = s.own[which][i];
+      if (C == 1) {
+        s.tot[which][i] = v;
+      } else if (v != 0u) {
+        atomicAdd(remote(s.all, i / slice) + which * (kSmpAllLists / 2) + i % slice, v);
       }
     }
-    sync();
+  }
+  __device__ __forceinline__ void merge_to_all(int which) {
+    const int slice = kSmpBuckets / C;
+    for (int i = threadIdx.x; i < kSmpBuckets / 4; i += kSmpThreads) {  // 4 buckets to one block
+      const int to = i / (slice / 4), j = i % (slice / 4);
+      *(reinterpret_cast<uint4*>(remote(s.tot[which], to) + rank * slice) + j) =
+          *(reinterpret_cast<const uint4*>(s.all + which * (kSmpAllLists / 2)) + j);
+    }
   }
 
   // First bucket at which the running count / mass reaches `target` (the last if none does), and what is before it.
-  template <typename A>
-  __device__ int crossing(const A* tot, double target, double& above) {
+  template <bool BY_MASS>
+  __device__ __forceinline__ int crossing(double target, double& above) {
     constexpr int E = kSmpBuckets / kSmpThreads;
     const int tid = threadIdx.x;
+    const uint32_t* tot = s.tot[BY_MASS ? 1 : 0];
     double v[E], run = 0.;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      v[e] = (double)tot[E * tid + e];
+      const int i = E * tid + e;
+      v[e] = (double)tot[i];
+      if (BY_MASS) v[e] *= __longlong_as_double((long long)(1023 - 12 - (i >> 5)) << 52);  // units of [2^-1-o, 2^-o)
       run += v[e];
     }
     const double mine = run;
@@ -266,11 +305,16 @@ struct Smp {
   }
 
   // Of the elements in buckets up to `bk` (in `bk` itself only those of a logit above `floor_key`): the mass
-  // above bucket bk, the mass in it, and the range of its logits (hi 0: none).
-  __device__ void look(int bk, uint32_t floor_key, smp_u64& above, smp_u64& inside, uint32_t& lo, uint32_t& hi) {
+  // above bucket bk, the mass in it, the range of its logits (hi 0: none). Each block lists its logits of the bucket
+  // (0 for those not above floor_key), `cnt` in all.
+  __device__ __forceinline__ void look(int bk, uint32_t floor_key, smp_u64& above, smp_u64& inside, uint32_t& lo,
+                                       uint32_t& hi, uint32_t& cnt) {
     uint32_t ah = 0, al = 0, ih = 0, il = 0;
+    uint32_t* list = s.own[turn];
     lo = 0xFFFFFFFFu;
     hi = 0;
+    if (threadIdx.x == 0) s.n_list = 0u;
+    __syncthreads();
 #pragma unroll 4
     for (int i = w0 + lane; i < w1; i += 32) {
       const float w = weight(i);
@@ -278,52 +322,90 @@ struct Smp {
       if (e < bk) {
         smp_add_mass(w, ah, al);
       } else if (e == bk && w > 0.f) {
-        const uint32_t k = smp_key(smp_load(x + i));
-        if (k > floor_key) {
-          smp_add_mass(w, ih, il);
-          lo = min(lo, k);
-          hi = max(hi, k);
-        }
+        const uint32_t j = atomicAdd(&s.n_list, 1u);
+        if (j < kSmpList) s.at[j] = i;
+      }
+    }
+    __syncthreads();
+    const uint32_t m = s.n_list;
+    auto take = [&](int i) {
+      const uint32_t k = smp_key(smp_load(x + i));
+      if (k <= floor_key) return 0u;
+      smp_add_mass(weight(i), ih, il);
+      lo = min(lo, k);
+      hi = max(hi, k);
+      return k;
+    };
+    if (m <= kSmpList) {
+      for (uint32_t j = threadIdx.x; j < m; j += kSmpThreads) list[j] = take(s.at[j]);
+    } else {
+      for (int i = w0 + lane; i < w1; i += 32) {
+        const float w = weight(i);
+        if (smp_bucket(w) == bk && w > 0.f) take(i);
       }
     }
     above = smp_mass(ah, al);
     inside = smp_mass(ih, il);
-    reduce(above, inside, lo, hi);
+    reduce(above, inside, lo, hi, cnt, nullptr);
   }
 
   __device__ __forceinline__ smp_u64 mass_of_key(uint32_t key) const {
     return smp_mass(expf(smp_d(smp_unkey(key), row)));
   }
 
-  // Exact selection inside bucket `bk`, whose admitted logits span [lo_key, hi_key]: the key and the number of
-  // its ties such that the bucket's elements above the key, and those ties, are the fewest whose count
-  // (BY_MASS: mass) reaches `need`.
+  // Exact selection inside bucket `bk`, whose admitted logits span [lo_key, hi_key] and were listed by the last
+  // look() (`cnt` of them): the key and the number of its ties such that the bucket's elements above the key, and
+  // those ties, are the fewest whose count (BY_MASS: mass) reaches `need`.
   template <bool BY_MASS>
-  __device__ void refine(int bk, uint32_t lo_key, uint32_t hi_key, smp_u64 need, uint32_t& key, smp_u64& ties) {
+  __device__ __forceinline__ void refine(int bk, uint32_t lo_key, uint32_t hi_key, uint32_t cnt, smp_u64 need,
+                                      uint32_t& key, smp_u64& ties) {
     uint32_t prefix = lo_key, mask = 0xFFFFFFFFu;
     if (lo_key != hi_key) {
+      const bool listed = cnt <= kSmpAllLists - 1;
+      if (listed) {
+        uint32_t base = 0;
+        for (int c = 0; c < C; ++c) {
+          const uint32_t m = (uint32_t)s.xch[turn ^ 1][c][3];  // as the last reduce() left it
+          const uint32_t* from = remote(s.own[turn ^ 1], c);
+          for (uint32_t i = threadIdx.x; i < m; i += kSmpThreads) s.all[base + i] = from[i];
+          base += m;
+        }
+      }
       const int top = 31 - __clz(lo_key ^ hi_key);
       mask = top == 31 ? 0u : ~((2u << top) - 1u);
       prefix = hi_key & mask;
       for (int shift = max(top - 7, 0);; shift = max(shift - 8, 0)) {
         smp_u64* dig = s.dig[parity];
         parity ^= 1;
-        if (threadIdx.x < 256) dig[threadIdx.x] = 0ull;
+        for (int i = threadIdx.x; i < 256; i += kSmpThreads) dig[i] = 0ull;
         __syncthreads();
-        for (int i = w0 + lane; i < w1; i += 32) {
-          const float w = weight(i);
-          if (smp_bucket(w) != bk || w == 0.f) continue;
-          const uint32_t k = smp_key(smp_load(x + i));
-          if ((k & mask) == prefix) atomicAdd(&dig[(k >> shift) & 255u], BY_MASS ? smp_mass(w) : 1ull);
+        if (listed) {
+          for (uint32_t i = threadIdx.x; i < cnt; i += kSmpThreads) {
+            const uint32_t k = s.all[i];
+            if (k != 0u && (k & mask) == prefix)
+              atomicAdd(&dig[(k >> shift) & 255u], BY_MASS ? mass_of_key(k) : 1ull);
+          }
+          __syncthreads();
+        } else {
+          for (int i = w0 + lane; i < w1; i += 32) {
+            const float w = weight(i);
+            if (smp_bucket(w) != bk || w == 0.f) continue;
+            const uint32_t k = smp_key(smp_load(x + i));
+            if ((k & mask) == prefix) atomicAdd(&dig[(k >> shift) & 255u], BY_MASS ? smp_mass(w) : 1ull);
+          }
+          sync();
         }
-        sync();
-        if (warp == 0) {  // the cluster's digits from the highest down, 8 to a lane
+        if (warp == 0) {  // the digits from the highest down, 8 to a lane
           smp_u64 v[8], sum = 0;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const int dgt = 255 - (lane * 8 + e);
             v[e] = 0;
-            for (int c = 0; c < C; ++c) v[e] += C > 1 ? cl.map_shared_rank(dig, c)[dgt] : dig[dgt];
+            if (listed) {
+              v[e] = dig[dgt];
+            } else {
+              for (int c = 0; c < C; ++c) v[e] += remote(dig, c)[dgt];
+            }
             sum += v[e];
           }
           smp_u64 before = smp_warp_scan(sum, lane) - sum;
@@ -358,7 +440,7 @@ struct Smp {
 };
 
 template <typename T, bool HELD>
-__global__ void __launch_bounds__(kSmpThreads, 1) sample_kernel(const SampleParams p) {
+__global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SampleParams p) {
   extern __shared__ __align__(16) uint8_t smp_dyn[];
   SmpShared& s = *reinterpret_cast<SmpShared*>(smp_dyn);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -366,7 +448,6 @@ __global__ void __launch_bounds__(kSmpThreads, 1) sample_kernel(const SamplePara
   const int i0 = min((int)blockIdx.x * p.chunk, p.V), n = min(p.chunk, p.V - i0);
   const int per = p.chunk / kSmpWarps;
   Smp<T, HELD> c{s,
-                 cooperative_groups::this_cluster(),
                  static_cast<const T*>(p.logits) + (int64_t)b * p.row_stride + i0,
                  reinterpret_cast<float*>(smp_dyn + sizeof(SmpShared)),
                  (int)gridDim.x,
@@ -376,7 +457,7 @@ __global__ void __launch_bounds__(kSmpThreads, 1) sample_kernel(const SamplePara
                  min((warp + 1) * per, n),
                  lane,
                  warp,
-                 {0.f, 0.f, 1.f},
+                 {},
                  0,
                  0};
   griddep_wait();
@@ -391,6 +472,10 @@ __global__ void __launch_bounds__(kSmpThreads, 1) sample_kernel(const SamplePara
   const float min_p = p.min_p != nullptr && p.min_p[b] > 0.f ? fminf(p.min_p[b], 1.f) : 0.f;
   const float uu = p.u[b];
   const bool by_k = top_k > 1u && top_k < (uint32_t)p.V, by_p = top_p < 1.f && top_k > 1u;
+
+  for (int i = tid; i < kSmpBuckets; i += kSmpThreads) s.own[0][i] = s.own[1][i] = 0u;
+  for (int i = tid; i < kSmpAllLists; i += kSmpThreads) s.all[i] = 0u;
+  if (tid == 0) s.n_list = 0u;
 
   // ---- the largest logit; the range goes to shared memory as fp32
   uint32_t best = 0;
@@ -433,39 +518,34 @@ __global__ void __launch_bounds__(kSmpThreads, 1) sample_kernel(const SamplePara
   }
   {
     smp_u64 z0 = 0, z1 = 0;
-    uint32_t lo = 0;
-    c.reduce(z0, z1, lo, best);
+    uint32_t lo = 0, cnt;
+    c.reduce(z0, z1, lo, best, cnt, nullptr);
   }
   c.row.xmax = smp_unkey(best);
-  c.row.t = t;
-  c.row.zmax = __fdiv_rn(c.row.xmax, t);
+  c.row.set_t(t);
+  c.row.zmax = c.row.over_t(c.row.xmax);
   uint32_t thr = 0;      // kept: logits above key `thr` (0: below every finite one), and the first `ties` at it,
   smp_u64 ties = 0;      // of weight >= min_p
   smp_u64 my = 0, my_ties = 0, before[2] = {0, 0}, kept = 0;  // this warp's kept mass, without ties; lower blocks'
 
   if (c.row.xmax == -INFINITY || top_k == 1u) {
     // nothing to choose from, or the lowest index of the largest logit
-    uint32_t first = 0xFFFFFFFFu, top = 0;
+    uint32_t first = 0xFFFFFFFFu, top = 0, cnt;
     for (int i = tid; i < n; i += kSmpThreads)
       if ((HELD ? c.sw[i] : smp_load(c.x + i)) == c.row.xmax) {
         first = i0 + i;
         break;
       }
-    c.reduce(my, my_ties, first, top);
+    c.reduce(my, my_ties, first, top, cnt, nullptr);
     if (c.rank == 0 && tid == 0) {
       p.token[b] = first;
       if (p.logprob != nullptr) p.logprob[b] = c.row.xmax == -INFINITY ? __uint_as_float(0x7FC00000u) : 0.f;
     }
-    c.sync();  // no block leaves while another may read its shared memory
     return;
   }
 
   // ---- weights, their mass, and the histograms
   const bool cut = by_k || by_p;
-  if (cut) {
-    for (int i = tid; i < kSmpBuckets; i += kSmpThreads) s.cnt[i] = s.mass[i] = 0u;
-    __syncthreads();
-  }
   {
     uint32_t hi = 0, lo = 0, far = 0;
 #pragma unroll 4
@@ -480,9 +560,9 @@ __global__ void __launch_bounds__(kSmpThreads, 1) sample_kernel(const SamplePara
         if (e == kSmpBuckets - 1) {
           ++far;  // the far tail shares the last bucket: counted apart, its mass left out of the guess
         } else {
-          if (by_k) atomicAdd(&s.cnt[e], 1u);
+          if (by_k) atomicAdd(&s.own[0][e], 1u);
           if (by_p)
-            atomicAdd(&s.mass[e], w == 1.f ? 8192u : ((__float_as_uint(w) & 0x7FFFFFu) | 0x800000u) >> 11);
+            atomicAdd(&s.own[1][e], w == 1.f ? 4096u : ((__float_as_uint(w) & 0x7FFFFFu) | 0x800000u) >> 12);
         }
       }
     }
@@ -490,29 +570,37 @@ __global__ void __launch_bounds__(kSmpThreads, 1) sample_kernel(const SamplePara
     if (cut) {
       far = __reduce_add_sync(0xffffffffu, far);
       if (lane == 0 && far) {
-        atomicAdd(&s.cnt[kSmpBuckets - 1], far);
-        atomicAdd(&s.mass[kSmpBuckets - 1], 1u);  // there is something
+        atomicAdd(&s.own[0][kSmpBuckets - 1], far);
+        atomicAdd(&s.own[1][kSmpBuckets - 1], 1u);  // there is something
       }
     }
   }
+  bool listed = min_p == 0.f;
   if (cut) {
     smp_u64 total = my, above = 0, inside = 0;
-    uint32_t lo = 0, hi = 0;
+    uint32_t lo = 0, hi = 0, cnt;
     double above_n;
-    if (by_k) __syncthreads(); else c.reduce(total, inside, lo, hi);
-    c.merge_buckets(by_k, by_p);
+    __syncthreads();
+    if (by_k) c.merge_to_owner(0);
+    if (by_p) c.merge_to_owner(1);
+    if (c.C > 1) {
+      c.sync();
+      if (by_k) c.merge_to_all(0);
+      if (by_p) c.merge_to_all(1);
+    }
+    c.reduce(total, inside, lo, hi, cnt, nullptr);
     if (by_k) {
-      const int bk = c.crossing(s.tot_cnt, (double)top_k, above_n);
-      c.look(bk, 0u, above, inside, lo, hi);
+      const int bk = c.template crossing<false>((double)top_k, above_n);
+      c.look(bk, 0u, above, inside, lo, hi, cnt);
       total = above + inside;
       if (hi != 0u) {
         const smp_u64 need = (smp_u64)top_k - (smp_u64)above_n;
-        if (need >= s.tot_cnt[bk]) {  // the whole bucket, or fewer logits than k
+        if (need >= s.tot[0][bk]) {  // the whole bucket, or fewer logits than k
           thr = lo - 1u;
         } else {
-          c.template refine<false>(bk, lo, hi, need, thr, ties);
+          c.template refine<false>(bk, lo, hi, cnt, need, thr, ties);
           if (by_p) {
-            if (lo != hi) c.look(bk, thr, above, inside, lo, hi); else inside = 0;
+            if (lo != hi) c.look(bk, thr, above, inside, lo, hi, cnt); else inside = 0;
             total = above + inside + ties * c.mass_of_key(thr);
           }
         }
@@ -522,14 +610,14 @@ __global__ void __launch_bounds__(kSmpThreads, 1) sample_kernel(const SamplePara
       const double goal = (double)top_p * (double)total;
       const smp_u64 need = max((smp_u64)ceil(goal), 1ull);
       const int bt = thr != 0u ? smp_bucket(expf(smp_d(smp_unkey(thr), c.row))) : kSmpBuckets - 1;
-      int bp = min(c.crossing(s.tot_mass, goal * kSmpUnit, above_n), bt);
+      int bp = min(c.template crossing<true>(goal * kSmpUnit, above_n), bt);
       // exact: move the guess until the mass above bucket bp is short of `need` and the mass with it is not
       for (;;) {
-        c.look(bp, bp == bt ? thr : 0u, above, inside, lo, hi);
+        c.look(bp, bp == bt ? thr : 0u, above, inside, lo, hi, cnt);
         if (above >= need && bp > 0) {
-          do --bp; while (bp > 0 && s.tot_mass[bp] == 0.f);
+          do --bp; while (bp > 0 && s.tot[1][bp] == 0u);
         } else if (above + inside < need && bp < bt) {
-          do ++bp; while (bp < bt && s.tot_mass[bp] == 0.f);
+          do ++bp; while (bp < bt && s.tot[1][bp] == 0u);
         } else {
           break;
         }
@@ -538,9 +626,10 @@ __global__ void __launch_bounds__(kSmpThreads, 1) sample_kernel(const SamplePara
         // everything above the top-k threshold is in, and some of its ties
         const smp_u64 w = thr != 0u ? c.mass_of_key(thr) : 0ull, left = need - (above + inside);
         if (w != 0) ties = min(ties, (left + w - 1) / w);
+        listed = false;  // the last look() left the ties out
       } else {
-        // the digit passes see the whole bucket; above the top-k threshold its order is the same
-        c.template refine<true>(bp, lo, hi, need - above, thr, ties);
+        // (digit passes over the row see the whole bucket; above the top-k threshold its order is the same)
+        c.template refine<true>(bp, lo, hi, cnt, need - above, thr, ties);
       }
     }
   }
@@ -555,9 +644,23 @@ __global__ void __launch_bounds__(kSmpThreads, 1) sample_kernel(const SamplePara
     const uint32_t k = smp_key(smp_load(c.x + i));
     return k > thr ? 1 : (k == thr && ties != 0) ? 2 : 0;
   };
-  if (cut) {
+  if (cut && listed && s.n_list <= kSmpList) {
+    // what the last look() found: s.red[w][0] is the mass that warp w has above the bucket
+    if (lane == 0) s.red[warp][1] = 0ull;
+    __syncthreads();
+    const uint32_t* list = s.own[c.turn ^ 1];
+    for (uint32_t j = tid; j < s.n_list; j += kSmpThreads) {
+      const int i = s.at[j];
+      if (list[j] > thr) atomicAdd(&s.red[i / per][0], smp_mass(c.weight(i)));
+      else if (list[j] == thr && ties != 0) atomicAdd(&s.red[i / per][1], 1ull);
+    }
+    __syncthreads();
+    my = lane == 0 ? s.red[warp][0] : 0ull;
+    my_ties = lane == 0 ? s.red[warp][1] : 0ull;
+    __syncwarp();
+  } else if (cut) {
     uint32_t hi = 0, lo = 0, nt = 0;
-#pragma unroll 4
+#pragma unroll 2
     for (int i = c.w0 + lane; i < c.w1; i += 32) {
       const float w = c.weight(i);
       const int a = admitted(i, w);
@@ -570,8 +673,8 @@ __global__ void __launch_bounds__(kSmpThreads, 1) sample_kernel(const SamplePara
   smp_u64 all_ties = my_ties;
   kept = my;
   {
-    uint32_t lo = 0, hi = 0;
-    c.reduce(kept, all_ties, lo, hi, before);
+    uint32_t lo = 0, hi = 0, cnt;
+    c.reduce(kept, all_ties, lo, hi, cnt, before);
   }
   // s.red[w][0 .. 1] still holds the block's warps' masses and ties
   const smp_u64 w_tie = smp_mass(w_thr);
@@ -623,7 +726,6 @@ __global__ void __launch_bounds__(kSmpThreads, 1) sample_kernel(const SamplePara
       }
     }
   }
-  c.sync();  // no block leaves while another may read its shared memory
 }
 
 }  // namespace tg

@@ -1555,19 +1555,22 @@ int tg_sample(const void* logits, int dtype, int64_t row_stride, int B, int V, c
   p.min_p = min_p;
   p.token = token;
   p.logprob = logprob;
-  // blocks of a cluster: as many as keep one block per SM busy, at least as many as hold the weights
+  // blocks of a cluster: as many as half fill the GPU (one row of 151936: 16 blocks 23 us, 8 blocks 30 us), and as
+  // many as let two blocks share an SM's memory (64 fp32 rows of 151936: 8 blocks 94 us, 4 blocks 114 us)
   int C = 1;
   auto chunk_of = [&](int c) { return (V + c * tg::kSmpThreads - 1) / (c * tg::kSmpThreads) * tg::kSmpThreads; };
   auto smem_of = [&](int c) { return sizeof(tg::SmpShared) + (size_t)chunk_of(c) * sizeof(float); };
   while (C < tg::kSmpMaxCluster &&
-         (((int64_t)B * C * 2 <= sm_count() && V > C * 4096) || smem_of(C) > (size_t)kSmpMaxSmem))
+         (((int64_t)B * C * 2 <= sm_count() && V > C * 4096) || smem_of(C) > (size_t)kSmpMaxSmem / 2 - 1024))
     C *= 2;
   p.chunk = chunk_of(C);
   const bool held = smem_of(C) <= (size_t)kSmpMaxSmem;
   auto kern = dtype ? (held ? tg::sample_kernel<__nv_bfloat16, true> : tg::sample_kernel<__nv_bfloat16, false>)
                     : (held ? tg::sample_kernel<float, true> : tg::sample_kernel<float, false>);
   cudaError_t e = smem_limit_once(kern, kSmpMaxSmem, g_smp_attr_set[2 * dtype + held], dev);
-  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(sample smem)");
+  if (e == cudaSuccess && C > 8)
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(sample)");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)C, (unsigned)B);
   cfg.blockDim = dim3(tg::kSmpThreads);
