@@ -476,7 +476,8 @@ int tg_qk_norm_rope_append_kv4(const void* q, int64_t ld_q, int n_q_heads, const
 /* tg_decode_attn_ex over a 4-bit cache of `capacity` slots: the same
  * operation on the values that the cache stands for, with the same bias,
  * query scale, pad slots and device-side key count. A bias of -inf masks its
- * key whatever the key holds; rows without any key give zeros. 1 to 8 query heads per kv head. workspace: device scratch of
+ * key whatever the key holds; rows without any key give zeros. 1 to 8 query
+ * heads per kv head. workspace: device scratch of
  * tg_decode_attn_kv4_workspace bytes (0: none), 16-byte aligned; calls
  * sharing it must not overlap on the GPU. */
 int tg_decode_attn_kv4(const void* q, int64_t q_sb, int64_t q_sh, const float* q_scale, int64_t qs_sb,

@@ -3,34 +3,46 @@
 //   out = softmax_j( softmax_scale * (q' . k_j) + m_j ) V
 // with k_j, v_j the values that the codes stand for, low + code * scale.
 //
-// Everything rests on writing a value as z + s * (code - 8), z = low + 8 s:
-//   q . k = sum over the row's two groups of  s * (q . (code - 8)) + z * sum(q)
-//   sum_j p_j v_j = (sum_j (p_j s_j) (code_j - 8)) + sum_j p_j z_j     per group
-// so the tensor cores multiply by the small integers code - 8, exact in fp16,
-// and the scales and lows enter in fp32 outside the products. K is the A
-// operand (16 keys x 16 dims, m16n8k16) against the heads of one kv head as the
-// 8 columns; V^T is A (16 dims x 16 keys) against the probabilities. A nibble
-// pair becomes two fp16 integers with one LOP3 (or into the mantissa of 1024)
-// and one HADD2 / HFMA2.
-//   q': scaled by a power of two per head (largest |q| in [256, 512)) so that
-//       bf16 fits fp16; exact down to 2^-22 of the largest, 2^-33 of it below.
+// Per group of 64 dims a value is low + s * code, so
+//   q . k         = sum over the row's two groups of  s * (q . code) + low * sum(q)
+//   sum_j p_j v_j = sum_j (p_j s_j) code_j + sum_j p_j low_j
+// and the tensor cores multiply by the small integers themselves, exact in
+// fp16; scales and lows enter in fp32 outside the products. K is the A operand
+// (16 keys x 16 dims, m16n8k16) against the heads of one kv head as the 8
+// columns; V^T is A (16 dims x 16 keys) against the probabilities. A pair of
+// nibbles, masked, IS a pair of fp16 numbers: below 2^11 fp16's bits are linear
+// (subnormals and the first binade), so the nibble at bit 0 reads code * 2^-24
+// and the one at bit 4 code * 2^-20: five logic instructions unpack eight codes.
+// The factors 2^-24 and 2^-20 go into q' (K: each nibble meets its own dim) and
+// into the final sums (V: each nibble is a row of the accumulators).
+//   q': scaled by a power of two per head (largest |q| in [2^12, 2^13)) so that
+//       bf16 fits fp16; exact down to 2^-22 of the largest (the sixteenth that
+//       meets the upper nibbles too), 2^-33 of it below.
 //   p s: fp16 (11 bits), the one rounding of the products' operands; p is
-//       relative to a running maximum that may lag by kKv4Lag, s to a running
-//       power of two, so neither leaves fp16's range.
+//       relative to a running maximum that may lag, s to a running power of
+//       two, so neither leaves fp16's range (maximum and power move together,
+//       in a branch that the first tiles take and later ones hardly ever).
 // Scores, maxima, sums and the accumulators are fp32.
+//
+// The cache is read once, at 144 bytes per key: every warp streams its own
+// tiles through a ring of three in shared memory (one bulk copy of 4608 bytes
+// each, no barrier between warps). What bounds it is the instructions per tile
+// as much as the bytes: see kv4_tile.
 #pragma once
 
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
 #include "kv4.cuh"
 
 namespace tg {
 
-constexpr int kKv4Warps = 4;
-constexpr int kKv4AttnThreads = 32 * kKv4Warps;
-constexpr int kKv4Part = 4 + 128;     // m, l, 2 pad, O[128] per (row, head, split)
-constexpr float kKv4Lag = 4.f;        // a score may pass the running maximum by this (natural units)
+constexpr unsigned int ERR_KV4 = 1u << 15;  // bit of the device error word
+constexpr int kKv4Stages = 3;
+constexpr int kKv4MaxWarps = 12;
+constexpr int kKv4MaxCluster = 16;
 constexpr float kKv4Head = 4.f;       // p = 2^(4 + ...): small p stay normal in fp16
+constexpr float kLog2e = 1.4426950408889634f;
 
 struct Kv4AttnParams {
   const __nv_bfloat16* q;
@@ -46,34 +58,45 @@ struct Kv4AttnParams {
   const int32_t* n_keys_dev;
   __nv_bfloat16* out;
   int64_t o_sb, o_sh;
-  float* part;           // [B][Hq][n_splits][kKv4Part]
-  int Hq, Hkv, G, n_splits, tiles_per_split;
+  float* part;           // nullable: [row][head][block][kKv4Part] instead of a merge in a cluster
+  int G, Hq;
   float scale;
+  unsigned int* err;
 };
+constexpr int kKv4Part = 4 + 128;  // m, l, 2 pad, O[128]
+
+struct alignas(16) Kv4AttnShared {
+  __half q[8][128];
+  float mul[8];
+  float m[kKv4MaxWarps][8], l[kKv4MaxWarps][8];
+  float got_o[8 * 128];                           // [rank][slice]: this block's slice of the blocks' sums
+  float got_m[kKv4MaxCluster][8], got_l[kKv4MaxCluster][8];
+  uint64_t full[kKv4MaxWarps][kKv4Stages];
+};
+constexpr int kKv4Ring = (sizeof(Kv4AttnShared) + 127) / 128 * 128;  // byte offset of the warps' rings
+constexpr int kv4_attn_smem(int warps) { return kKv4Ring + warps * kKv4Stages * kKv4TileBytes; }
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                               uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
   uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 
-// The 8 codes of a word minus 8, as fp16 pairs (nibble j, nibble j + 4).
+// The 8 codes of a word as fp16 pairs (nibble j, nibble j + 4): j even * 2^-24, j odd * 2^-20.
 __device__ __forceinline__ void kv4_unpack(uint32_t w, uint32_t (&o)[4]) {
-  const __half2 c1032 = __float2half2_rn(-1032.f), c72 = __float2half2_rn(-72.f), r16 = __float2half2_rn(0.0625f);
   const uint32_t w8 = w >> 8;
-  o[0] = h2_bits(__hadd2(bits_h2((w & 0x000F000Fu) | 0x64006400u), c1032));         // 1024 + n - 1032
-  o[1] = h2_bits(__hfma2(bits_h2((w & 0x00F000F0u) | 0x64006400u), r16, c72));      // (1024 + 16 n) / 16 - 72
-  o[2] = h2_bits(__hadd2(bits_h2((w8 & 0x000F000Fu) | 0x64006400u), c1032));
-  o[3] = h2_bits(__hfma2(bits_h2((w8 & 0x00F000F0u) | 0x64006400u), r16, c72));
+  o[0] = w & 0x000F000Fu;
+  o[1] = w & 0x00F000F0u;
+  o[2] = w8 & 0x000F000Fu;
+  o[3] = w8 & 0x00F000F0u;
 }
 __device__ __forceinline__ float kv4_scale(uint32_t param) { return __uint_as_float(param << 16); }
 __device__ __forceinline__ float kv4_low(uint32_t param) { return __uint_as_float(param & 0xFFFF0000u); }
@@ -89,46 +112,216 @@ __device__ __forceinline__ float warp_sum_rows(float v) {
   return v;
 }
 
-struct Kv4Tile {
-  uint4 k[2][2], v[2][2];
-  uint2 kp[4], vp[4];
+// A warp's running softmax over its tiles, for the heads 2 t and 2 t + 1 of
+// lane (g, t). Without a bias the scores are in log2 units; with one they stay
+// in natural units, where a bias of the type's lowest value does not overflow.
+struct Kv4State {
+  uint32_t qf[8][2];    // B fragments of q'
+  float qs[2][2];       // sum(q') per group and head
+  float mul[2];
+  float m[2], l[2], zs[2][2];  // running maximum, sum p, sum p * low per group
+  float acc[8][4];             // sum (p s) code, times 2^-24 (rows g) or 2^-20 (rows g + 8)
+  float eref, einv;            // the power of two that s is relative to
 };
 
-__device__ __forceinline__ void kv4_load_tile(const uint8_t* tile, int lane, Kv4Tile& x) {
+// One tile of 32 keys from shared memory. ALL: every key is attended.
+template <bool BIAS, bool ALL>
+__device__ __forceinline__ void kv4_tile(Kv4State& st, const uint8_t* tile, int j0, int n_keys, int nv, int n_prefix,
+                                         const float* bias0, const float* bias1, int lane) {
   const int g = lane >> 2, t = lane & 3;
+  uint2 vp[4];
+  float sc[8], bj[8];
+  bool row_ok[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int key = j0 + 8 * r + g;
+    row_ok[r] = ALL || (key < n_keys && (key < nv || key >= n_prefix));
+    if (BIAS) {
+      const bool has = row_ok[r] && key < n_prefix;
+      bj[2 * r] = has && bias0 != nullptr ? __ldg(bias0 + key) : 0.f;
+      bj[2 * r + 1] = has && bias1 != nullptr ? __ldg(bias1 + key) : 0.f;
+    }
+    vp[r] = *reinterpret_cast<const uint2*>(tile + kKv4Vp + (8 * r + g) * 8);
+    if (!row_ok[r]) vp[r] = make_uint2(0u, 0u);  // whatever a masked slot holds
+  }
+  // ---- scores: sc[2 r + j] of key 8 r + g and head 2 t + j
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
+    float c[2][4];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      x.k[s][r] = ld_nc_v4(reinterpret_cast<const uint4*>(tile + (16 * s + 8 * r + g) * 64 + t * 16));
-      x.v[s][r] = ld_nc_v4(reinterpret_cast<const uint4*>(tile + kKv4V + s * 1024 + r * 512 + lane * 16));
-      x.kp[2 * s + r] = *reinterpret_cast<const uint2*>(tile + kKv4Kp + (16 * s + 8 * r + g) * 8);
-      x.vp[2 * s + r] = *reinterpret_cast<const uint2*>(tile + kKv4Vp + (16 * s + 8 * r + g) * 8);
+    for (int gr = 0; gr < 2; ++gr)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c[gr][e] = 0.f;
+    const uint4 x0 = *reinterpret_cast<const uint4*>(tile + (16 * s + g) * 64 + t * 16);
+    const uint4 x1 = *reinterpret_cast<const uint4*>(tile + (16 * s + 8 + g) * 64 + t * 16);
+    const uint32_t w0[4] = {x0.x, x0.y, x0.z, x0.w}, w1[4] = {x1.x, x1.y, x1.z, x1.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t a[4], d[4];
+      kv4_unpack(w0[i], a);
+      kv4_unpack(w1[i], d);
+      mma_f16_16816(c[i >> 1], a[0], d[0], a[1], d[1], st.qf[2 * i][0], st.qf[2 * i][1]);
+      mma_f16_16816(c[i >> 1], a[2], d[2], a[3], d[3], st.qf[2 * i + 1][0], st.qf[2 * i + 1][1]);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = 2 * s + h;
+      const uint2 kp = *reinterpret_cast<const uint2*>(tile + kKv4Kp + (8 * r + g) * 8);
+      const float s0 = kv4_scale(kp.x) * 16777216.f, s1 = kv4_scale(kp.y) * 16777216.f;  // 2^24: the codes' units
+      const float z0 = kv4_low(kp.x), z1 = kv4_low(kp.y);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float v = z0 * st.qs[0][j];
+        v = fmaf(z1, st.qs[1][j], v);
+        v = fmaf(s0, c[0][2 * h + j], v);
+        v = fmaf(s1, c[1][2 * h + j], v);
+        v = BIAS ? fmaf(v, st.mul[j], bj[2 * r + j]) : v * st.mul[j];
+        // -inf in the bias is a mask, whatever the key holds
+        sc[2 * r + j] = !row_ok[r] || (BIAS && bj[2 * r + j] == -INFINITY) ? -INFINITY : v;
+      }
+    }
+  }
+  // ---- move the running maximum / power of two when a score or a step outgrows them
+  float sn[8], smax = 0.f, top[2];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    sn[2 * r] = kv4_scale(vp[r].x) * st.einv;
+    sn[2 * r + 1] = kv4_scale(vp[r].y) * st.einv;
+    smax = fmax3(smax, sn[2 * r], sn[2 * r + 1]);
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) top[j] = fmaxf(fmax3(sc[j], sc[2 + j], sc[4 + j]), sc[6 + j]);
+  constexpr float kLag = BIAS ? 4.f : 4.f * kLog2e;
+  const bool grow = top[0] > st.m[0] + kLag || top[1] > st.m[1] + kLag || smax > 16.f;
+  if (__any_sync(0xffffffffu, grow)) {
+    float sraw = 0.f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sraw = fmax3(sraw, kv4_scale(vp[r].x), kv4_scale(vp[r].y));
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) sraw = fmaxf(sraw, __shfl_xor_sync(0xffffffffu, sraw, off));
+    // a power of two above the largest step, at most 2^126
+    const uint32_t eb = min((__float_as_uint(sraw) >> 23) + 1u, 253u);
+    const float enew = fmaxf(st.eref, __uint_as_float(eb << 23));
+    const float beta = st.eref / enew;
+    st.eref = enew;
+    st.einv = 1.f / enew;
+    float al[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float mn = fmaxf(st.m[j], warp_max_rows(top[j]));
+      al[j] = mn == -INFINITY ? 1.f : ex2_approx((st.m[j] - mn) * (BIAS ? kLog2e : 1.f));
+      st.m[j] = mn;
+      st.l[j] *= al[j];
+      st.zs[0][j] *= al[j];
+      st.zs[1][j] *= al[j];
+    }
+#pragma unroll
+    for (int w = 0; w < 8; ++w)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) st.acc[w][e] *= al[e & 1] * beta;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      sn[2 * r] = kv4_scale(vp[r].x) * st.einv;
+      sn[2 * r + 1] = kv4_scale(vp[r].y) * st.einv;
+    }
+  }
+  // ---- p, its sums, and P V
+  const float off[2] = {kKv4Head - st.m[0], kKv4Head - st.m[1]};
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    uint32_t pf[2][2];  // B fragments per group
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = 2 * s + h;
+      float p[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float v = sc[2 * r + j];
+        const float e = BIAS ? ex2_approx(fmaf(v - st.m[j], kLog2e, kKv4Head)) : ex2_approx(v + off[j]);
+        p[j] = (BIAS || !ALL) && v == -INFINITY ? 0.f : e;
+        st.l[j] += p[j];
+      }
+#pragma unroll
+      for (int gr = 0; gr < 2; ++gr) {
+        const float z = kv4_low(gr ? vp[r].y : vp[r].x), sg = sn[2 * r + gr];
+        float u0 = p[0] * sg, u1 = p[1] * sg;
+        if (BIAS) {  // a masked key may hold NaN
+          st.zs[gr][0] = p[0] == 0.f ? st.zs[gr][0] : fmaf(p[0], z, st.zs[gr][0]);
+          u0 = p[0] == 0.f ? 0.f : u0;
+          st.zs[gr][1] = p[1] == 0.f ? st.zs[gr][1] : fmaf(p[1], z, st.zs[gr][1]);
+          u1 = p[1] == 0.f ? 0.f : u1;
+        } else {
+          st.zs[gr][0] = fmaf(p[0], z, st.zs[gr][0]);
+          st.zs[gr][1] = fmaf(p[1], z, st.zs[gr][1]);
+        }
+        pf[gr][h] = movmatrix_trans(h2_bits(__floats2half2_rn(u0, u1)));
+      }
+    }
+#pragma unroll
+    for (int gr = 0; gr < 2; ++gr) {
+      const uint4 x = *reinterpret_cast<const uint4*>(tile + kKv4V + s * 1024 + gr * 512 + lane * 16);
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t a[4];
+        kv4_unpack(w[i], a);
+        mma_f16_16816(st.acc[4 * gr + i], a[0], a[1], a[2], a[3], pf[gr][0], pf[gr][1]);
+      }
     }
   }
 }
 
-// A CTA takes one kv head of one row and a run of tiles, its warps every
-// kKv4Warps-th tile of it; each warp keeps its own running softmax, the CTA
-// merges them in shared memory. One split writes the output, more write
-// (m, l, O) records that kv4_combine_kernel merges.
-__global__ void __launch_bounds__(kKv4AttnThreads) kv4_attn_kernel(const Kv4AttnParams p) {
-  __shared__ float sq[8][128];
-  __shared__ float s_mul[8];
-  __shared__ float s_m[kKv4Warps][8], s_l[kKv4Warps][8];
-  __shared__ float s_o[kKv4Warps][8][128];
-
+// C blocks take one kv head of one row (grid (C, Hkv, B)): the tiles that hold
+// attended keys, evenly in order to the blocks and in turn to a block's warps.
+// Each warp keeps its own running softmax; warps merge in shared memory. The
+// blocks merge in one of two ways: as a cluster, sending each other their
+// slices of the output (one barrier, no second launch, no workspace), or
+// through records that kv4_combine_kernel merges (any number of blocks, so
+// every SM can take part: clusters of 16 leave a quarter of them idle).
+template <bool BIAS>
+__global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv4AttnParams p) {
+  extern __shared__ __align__(128) uint8_t kv4_smem[];
+  Kv4AttnShared& sh = *reinterpret_cast<Kv4AttnShared*>(kv4_smem);
+  const int W = blockDim.x >> 5, C = gridDim.x, rank = blockIdx.x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+  const int kvh = blockIdx.y, b = blockIdx.z;
+  uint8_t* ring = kv4_smem + kKv4Ring + warp * kKv4Stages * kKv4TileBytes;
+  const uint32_t ring_s = smem_u32(ring), full_s = smem_u32(sh.full[warp]);
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < kKv4Stages; ++i) mbar_init(full_s + 8 * i, 1);
+    fence_mbar_init();
+  }
+  __syncwarp();
+  const bool clustered = C > 1 && p.part == nullptr;
+  if (clustered) cluster_arrive();
   griddep_wait();
   griddep_launch_dependents();
   const int n_keys = p.n_keys_dev != nullptr ? min(__ldg(p.n_keys_dev), p.n_keys) : p.n_keys;
-  const int nv = __ldg(p.n_valid + b);
+  const int nv = min(max(__ldg(p.n_valid + b), 0), p.n_prefix);
   const uint8_t* base = p.cache + (int64_t)b * p.c_sb + (int64_t)kvh * p.c_sh;
 
+  // tiles with attended keys: [0, na) and from tb on
+  const int tiles = (n_keys + kKv4Keys - 1) / kKv4Keys;
+  const int na = min((nv + kKv4Keys - 1) / kKv4Keys, tiles), tb = max(p.n_prefix / kKv4Keys, na);
+  const int n = na + max(tiles - tb, 0);
+  const int v0 = (int)((int64_t)n * rank / C), v1 = (int)((int64_t)n * (rank + 1) / C);
+  const int mine = v1 - v0 > warp ? (v1 - v0 - warp + W - 1) / W : 0;  // this warp's tiles
+  auto tile_of = [&](int i) {
+    const int v = v0 + warp + i * W;
+    return v < na ? v : v - na + tb;
+  };
+  auto fetch = [&](int i) {
+    const int s = i % kKv4Stages;
+    mbar_arrive_expect_tx(full_s + 8 * s, kKv4TileBytes);
+    bulk_load(ring_s + s * kKv4TileBytes, base + (int64_t)tile_of(i) * kKv4TileBytes, kKv4TileBytes, full_s + 8 * s);
+  };
+  if (lane == 0)
+    for (int i = 0; i < min(mine, kKv4Stages); ++i) fetch(i);
+
   // the heads' q', scaled by a power of two
-  for (int h = warp; h < 8; h += kKv4Warps) {
+  for (int h = warp; h < 8; h += W) {
     float v[4] = {0.f, 0.f, 0.f, 0.f}, mx = 0.f;
     if (h < p.G) {
       const int hq = kvh * p.G + h;
@@ -143,232 +336,194 @@ __global__ void __launch_bounds__(kKv4AttnThreads) kv4_attn_kernel(const Kv4Attn
     }
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-    // 2^(8 - exponent), inside fp32's normal range on both sides
-    const int ex = min(max((int)(__float_as_uint(mx) >> 23) - 127 - 8, -126), 126);
+    // 2^(12 - exponent), inside fp32's normal range on both sides
+    const int ex = min(max((int)(__float_as_uint(mx) >> 23) - 127 - 12, -126), 126);
     const float down = __uint_as_float((uint32_t)(127 - ex) << 23);
-    if (lane == 0) s_mul[h] = __uint_as_float((uint32_t)(127 + ex) << 23) * p.scale;
+    if (lane == 0) sh.mul[h] = __uint_as_float((uint32_t)(127 + ex) << 23) * p.scale * (BIAS ? 1.f : kLog2e);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sq[h][lane + 32 * e] = __half2float(__float2half_rn(v[e] * down));
+    for (int e = 0; e < 4; ++e) sh.q[h][lane + 32 * e] = __float2half_rn(v[e] * down);
   }
   __syncthreads();
-  // B fragments: MMA (i, 0): nibbles (0, 4), (1, 5) of word i; (i, 1): (2, 6), (3, 7)
-  uint32_t qf[8][2];
+  Kv4State st;
+  // MMA (i, 0): nibbles (0, 4), (1, 5) of word i; (i, 1): (2, 6), (3, 7)
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int d = 32 * i + 8 * t + u;
-      qf[2 * i + (u >> 1)][u & 1] = h2_bits(__floats2half2_rn(sq[g][d], sq[g][d + 4]));
+      __half2 f = __halves2half2(sh.q[g][d], sh.q[g][d + 4]);
+      if (u & 1) f = __hmul2(f, __float2half2_rn(0.0625f));  // its nibbles read 16 times as large
+      st.qf[2 * i + (u >> 1)][u & 1] = h2_bits(f);
     }
   }
-  float qsum[2][2], mul[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    mul[j] = s_mul[2 * t + j];
+    st.mul[j] = sh.mul[2 * t + j];
+    st.m[j] = -INFINITY;
+    st.l[j] = st.zs[0][j] = st.zs[1][j] = 0.f;
 #pragma unroll
     for (int gr = 0; gr < 2; ++gr) {
       float a = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) a += sq[2 * t + j][64 * gr + 8 * g + e];
-      qsum[gr][j] = warp_sum_rows(a);
+      for (int e = 0; e < 8; ++e) a += __half2float(sh.q[2 * t + j][64 * gr + 8 * g + e]);
+      st.qs[gr][j] = warp_sum_rows(a);
     }
   }
-
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, zs[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
-  float acc[8][4];
 #pragma unroll
   for (int w = 0; w < 8; ++w)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[w][e] = 0.f;
-  float eref = 1.17549435e-38f, einv = 8.507059173e37f;  // 2^-126, 2^126
-
-  const int t0 = split * p.tiles_per_split;
-  const int t1 = min(t0 + p.tiles_per_split, (n_keys + kKv4Keys - 1) / kKv4Keys);
-  for (int tile = t0 + warp; tile < t1; tile += kKv4Warps) {
-    const int j0 = tile * kKv4Keys;
-    if (j0 >= nv && j0 + kKv4Keys <= p.n_prefix) continue;  // pad slots only
-    Kv4Tile x;
-    kv4_load_tile(base + (int64_t)tile * kKv4TileBytes, lane, x);
-    // ---- scores: sc[4 * s + 2 * r + j] of key 16 s + 8 r + g and head 2 t + j
-    float sc[8];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      float c[2][4];
-#pragma unroll
-      for (int gr = 0; gr < 2; ++gr)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c[gr][e] = 0.f;
-      const uint32_t w0[4] = {x.k[s][0].x, x.k[s][0].y, x.k[s][0].z, x.k[s][0].w};
-      const uint32_t w1[4] = {x.k[s][1].x, x.k[s][1].y, x.k[s][1].z, x.k[s][1].w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t a[4], d[4];
-        kv4_unpack(w0[i], a);
-        kv4_unpack(w1[i], d);
-        mma_f16_16816(c[i >> 1], a[0], d[0], a[1], d[1], qf[2 * i][0], qf[2 * i][1]);
-        mma_f16_16816(c[i >> 1], a[2], d[2], a[3], d[3], qf[2 * i + 1][0], qf[2 * i + 1][1]);
-      }
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const uint2 kp = x.kp[2 * s + r];
-        const float s0 = kv4_scale(kp.x), s1 = kv4_scale(kp.y);
-        const float z0 = fmaf(8.f, s0, kv4_low(kp.x)), z1 = fmaf(8.f, s1, kv4_low(kp.y));
-        const int key = j0 + 16 * s + 8 * r + g;
-        const bool valid = key < n_keys && (key < nv || key >= p.n_prefix);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float v = s0 * c[0][2 * r + j];
-          v = fmaf(s1, c[1][2 * r + j], v);
-          v = fmaf(z0, qsum[0][j], v);
-          v = fmaf(z1, qsum[1][j], v);
-          v *= mul[j];
-          bool seen = valid;
-          if (p.bias != nullptr && key < p.n_prefix && 2 * t + j < p.G && valid) {
-            const float bj = __ldg(p.bias + (int64_t)b * p.bias_sb + (int64_t)(kvh * p.G + 2 * t + j) * p.bias_sh + key);
-            v += bj;
-            seen = bj != -INFINITY;  // a mask, whatever the key holds
-          }
-          sc[4 * s + 2 * r + j] = seen ? v : -INFINITY;
-        }
-      }
-    }
-    // ---- move the running maximum / power of two when a score or a step outgrows them
-    float smax = 0.f;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int key = j0 + 8 * r + g;
-      if (key < n_keys && (key < nv || key >= p.n_prefix)) smax = fmaxf(smax, fmaxf(kv4_scale(x.vp[r].x), kv4_scale(x.vp[r].y)));
-    }
-    float top[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) top[j] = fmaxf(fmaxf(sc[j], sc[2 + j]), fmaxf(sc[4 + j], sc[6 + j]));
-    const bool grow = top[0] > m[0] + kKv4Lag || top[1] > m[1] + kKv4Lag || smax * einv > 16.f;
-    if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-      for (int off = 16; off >= 1; off >>= 1) smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, off));
-      // a power of two >= smax, at most 2^126
-      const uint32_t eb = min((__float_as_uint(smax) >> 23) + 1u, 253u);
-      const float enew = fmaxf(eref, __uint_as_float(max(eb, 1u) << 23));
-      const float beta = eref / enew;
-      eref = enew;
-      einv = 1.f / enew;
-      float al[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float mn = fmaxf(m[j], warp_max_rows(top[j]));
-        al[j] = mn == -INFINITY ? 1.f : ex2_approx((m[j] - mn) * 1.4426950408889634f);
-        m[j] = mn;
-        l[j] *= al[j];
-        zs[0][j] *= al[j];
-        zs[1][j] *= al[j];
-      }
-#pragma unroll
-      for (int w = 0; w < 8; ++w)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[w][e] *= al[e & 1] * beta;
-    }
-    // ---- p, its sums, and P V
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      uint32_t pf[2][2];  // B fragments per group
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const uint2 vp = x.vp[2 * s + r];
-        float pr[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float v = sc[4 * s + 2 * r + j];
-          pr[j] = v == -INFINITY ? 0.f : ex2_approx(fmaf(v - m[j], 1.4426950408889634f, kKv4Head));
-          l[j] += pr[j];
-        }
-        const bool any = sc[4 * s + 2 * r] != -INFINITY || sc[4 * s + 2 * r + 1] != -INFINITY;
-#pragma unroll
-        for (int gr = 0; gr < 2; ++gr) {
-          const uint32_t pm = gr ? vp.y : vp.x;
-          const float sv = any ? kv4_scale(pm) : 0.f, z = any ? fmaf(8.f, kv4_scale(pm), kv4_low(pm)) : 0.f;
-          zs[gr][0] = fmaf(pr[0], z, zs[gr][0]);
-          zs[gr][1] = fmaf(pr[1], z, zs[gr][1]);
-          const float sn = sv * einv;
-          pf[gr][r] = movmatrix_trans(h2_bits(__floats2half2_rn(pr[0] * sn, pr[1] * sn)));
-        }
-      }
-#pragma unroll
-      for (int hv = 0; hv < 2; ++hv) {
-        const uint32_t w[4] = {x.v[s][hv].x, x.v[s][hv].y, x.v[s][hv].z, x.v[s][hv].w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t a[4];
-          kv4_unpack(w[i], a);
-          mma_f16_16816(acc[4 * hv + i], a[0], a[1], a[2], a[3], pf[hv][0], pf[hv][1]);
-        }
-      }
-    }
+    for (int e = 0; e < 4; ++e) st.acc[w][e] = 0.f;
+  st.eref = 1.17549435e-38f;  // 2^-126
+  st.einv = 8.507059173e37f;
+  const float *bias0 = nullptr, *bias1 = nullptr;
+  if (BIAS) {
+    const float* bp = p.bias + (int64_t)b * p.bias_sb + (int64_t)(kvh * p.G + 2 * t) * p.bias_sh;
+    if (2 * t < p.G) bias0 = bp;
+    if (2 * t + 1 < p.G) bias1 = bp + p.bias_sh;
   }
 
-  // ---- merge the warps
+  bool ok = true;
+  for (int i = 0, s = 0, ph = 0; i < mine; ++i) {
+    if (!mbar_wait(full_s + 8 * s, ph, p.err, ERR_KV4)) {
+      ok = false;
+      break;
+    }
+    const int j0 = tile_of(i) * kKv4Keys;
+    const uint8_t* tile = ring + s * kKv4TileBytes;
+    if (j0 + kKv4Keys <= n_keys && (j0 + kKv4Keys <= nv || j0 >= p.n_prefix))
+      kv4_tile<BIAS, true>(st, tile, j0, n_keys, nv, p.n_prefix, bias0, bias1, lane);
+    else
+      kv4_tile<BIAS, false>(st, tile, j0, n_keys, nv, p.n_prefix, bias0, bias1, lane);
+    __syncwarp();
+    if (lane == 0 && i + kKv4Stages < mine) fetch(i + kKv4Stages);
+    if (++s == kKv4Stages) {
+      s = 0;
+      ph ^= 1;
+    }
+  }
+  if (!ok)  // a copy never came: give those in flight their time before the shared memory goes
+    for (int s = 0; s < kKv4Stages; ++s) mbar_wait(full_s + 8 * s, 0, p.err, ERR_KV4);
+
+  // ---- merge the warps: their sums into the rings' memory
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    l[j] = warp_sum_rows(l[j]);
-    zs[0][j] = warp_sum_rows(zs[0][j]);
-    zs[1][j] = warp_sum_rows(zs[1][j]);
+    st.l[j] = warp_sum_rows(st.l[j]);
+    st.zs[0][j] = warp_sum_rows(st.zs[0][j]);
+    st.zs[1][j] = warp_sum_rows(st.zs[1][j]);
     if (g == 0) {
-      s_m[warp][2 * t + j] = m[j];
-      s_l[warp][2 * t + j] = l[j];
+      sh.m[warp][2 * t + j] = st.m[j];
+      sh.l[warp][2 * t + j] = st.l[j];
     }
   }
+  __syncwarp();
+  float* so = reinterpret_cast<float*>(ring);  // [8][128] of this warp
 #pragma unroll
   for (int w = 0; w < 8; ++w)
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      s_o[warp][2 * t + (e & 1)][16 * w + g + 8 * (e >> 1)] = fmaf(acc[w][e], eref, zs[w >> 2][e & 1]);
+      so[(2 * t + (e & 1)) * 128 + 16 * w + g + 8 * (e >> 1)] =
+          fmaf(st.acc[w][e] * (e < 2 ? 16777216.f : 1048576.f), st.eref, st.zs[w >> 2][e & 1]);
+  if (clustered) cluster_wait();  // every block has started
   __syncthreads();
-  for (int idx = threadIdx.x; idx < p.G * 128; idx += kKv4AttnThreads) {
-    const int h = idx >> 7, d = idx & 127;
-    float mt = s_m[0][h];
-#pragma unroll
-    for (int w = 1; w < kKv4Warps; ++w) mt = fmaxf(mt, s_m[w][h]);
+  const float* all_o = reinterpret_cast<const float*>(kv4_smem + kKv4Ring);
+  constexpr float kUnit = BIAS ? kLog2e : 1.f;  // of m
+  const int slice = p.G * 128 / C;
+  for (int idx = threadIdx.x; idx < p.G * 128; idx += blockDim.x) {
+    const int h = idx >> 7;
+    float mt = sh.m[0][h];
+    for (int w = 1; w < W; ++w) mt = fmaxf(mt, sh.m[w][h]);
     float o = 0.f, lt = 0.f;
-#pragma unroll
-    for (int w = 0; w < kKv4Warps; ++w) {
-      const float lw = s_l[w][h];
+    for (int w = 0; w < W; ++w) {
+      const float lw = sh.l[w][h];
       if (lw != 0.f) {  // 0: the warp saw no key (a NaN sum stays in)
-        const float f = ex2_approx((s_m[w][h] - mt) * 1.4426950408889634f);
-        o = fmaf(f, s_o[w][h][d], o);
+        const float f = ex2_approx((sh.m[w][h] - mt) * kUnit);
+        o = fmaf(f, all_o[w * (kKv4Stages * kKv4TileBytes / 4) + idx], o);
         lt = fmaf(f, lw, lt);
       }
     }
-    const int hq = kvh * p.G + h;
-    if (p.n_splits == 1) {
-      p.out[(int64_t)b * p.o_sb + (int64_t)hq * p.o_sh + d] = __float2bfloat16_rn(lt == 0.f ? 0.f : o / lt);
-    } else {
-      float* rec = p.part + (((int64_t)b * p.Hq + hq) * p.n_splits + split) * kKv4Part;
-      rec[4 + d] = o;
-      if (d == 0) {
+    if (C == 1) {
+      p.out[(int64_t)b * p.o_sb + (int64_t)(kvh * p.G + h) * p.o_sh + (idx & 127)] =
+          __float2bfloat16_rn(lt == 0.f ? 0.f : o / lt);
+    } else if (!clustered) {
+      float* rec = p.part + (((int64_t)b * p.Hq + kvh * p.G + h) * C + rank) * kKv4Part;
+      rec[4 + (idx & 127)] = o;
+      if ((idx & 127) == 0) {
         rec[0] = mt;
         rec[1] = lt;
       }
+    } else {
+      cooperative_groups::cluster_group cl = cooperative_groups::this_cluster();
+      cl.map_shared_rank(sh.got_o, idx / slice)[rank * slice + idx % slice] = o;
+      if ((idx & 127) < C) {
+        cl.map_shared_rank(&sh.got_m[rank][h], idx & 127)[0] = mt;
+        cl.map_shared_rank(&sh.got_l[rank][h], idx & 127)[0] = lt;
+      }
     }
+  }
+  if (!clustered) return;
+  __syncwarp();
+  cluster_sync_all();
+  for (int i = threadIdx.x; i < slice; i += blockDim.x) {
+    const int idx = rank * slice + i, h = idx >> 7;
+    float mt = sh.got_m[0][h];
+    for (int c = 1; c < C; ++c) mt = fmaxf(mt, sh.got_m[c][h]);
+    float o = 0.f, lt = 0.f;
+    for (int c = 0; c < C; ++c) {
+      const float lw = sh.got_l[c][h];
+      if (lw != 0.f) {
+        const float f = ex2_approx((sh.got_m[c][h] - mt) * kUnit);
+        o = fmaf(f, sh.got_o[c * slice + i], o);
+        lt = fmaf(f, lw, lt);
+      }
+    }
+    p.out[(int64_t)b * p.o_sb + (int64_t)(kvh * p.G + h) * p.o_sh + (idx & 127)] =
+        __float2bfloat16_rn(lt == 0.f ? 0.f : o / lt);
   }
 }
 
-// Merges the splits' (m, l, O) of one (row, head): 128 threads, one dim each.
-__global__ void __launch_bounds__(128) kv4_combine_kernel(const Kv4AttnParams p) {
+// Merges the blocks' records of one (row, head): 8 warps take every 8th record
+// (lane: dims 4 l .. 4 l + 3, 16-byte loads), then merge through shared memory.
+constexpr int kKv4CombineWarps = 8;
+__global__ void __launch_bounds__(32 * kKv4CombineWarps) kv4_combine_kernel(const Kv4AttnParams p, int C) {
+  __shared__ float s_l[kKv4CombineWarps];
+  __shared__ float s_o[kKv4CombineWarps][128];
   griddep_wait();
   griddep_launch_dependents();
-  const int h = blockIdx.x, b = blockIdx.y, d = threadIdx.x;
-  const float* rec = p.part + ((int64_t)b * p.Hq + h) * p.n_splits * kKv4Part;
+  const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float* rec = p.part + ((int64_t)b * p.Hq + h) * C * kKv4Part;
+  const float unit = p.bias != nullptr ? kLog2e : 1.f;  // of m
   float m = -INFINITY;
-  for (int c = 0; c < p.n_splits; ++c) m = fmaxf(m, rec[(int64_t)c * kKv4Part]);
-  float o = 0.f, l = 0.f;
-  for (int c = 0; c < p.n_splits; ++c) {
+  for (int c = lane; c < C; c += 32) m = fmaxf(m, rec[(int64_t)c * kKv4Part]);
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+#pragma unroll 4
+  for (int c = warp; c < C; c += kKv4CombineWarps) {
     const float* r = rec + (int64_t)c * kKv4Part;
-    if (r[1] != 0.f) {  // 0: the split saw no key (a NaN sum stays in)
-      const float f = ex2_approx((r[0] - m) * 1.4426950408889634f);
-      o = fmaf(f, r[4 + d], o);
-      l = fmaf(f, r[1], l);
+    const float4 v = *reinterpret_cast<const float4*>(r + 4 + 4 * lane);
+    const float lc = r[1];
+    if (lc != 0.f) {  // 0: the block saw no key (a NaN sum stays in)
+      const float f = ex2_approx((r[0] - m) * unit);
+      l = fmaf(f, lc, l);
+      o.x = fmaf(f, v.x, o.x);
+      o.y = fmaf(f, v.y, o.y);
+      o.z = fmaf(f, v.z, o.z);
+      o.w = fmaf(f, v.w, o.w);
     }
   }
-  p.out[(int64_t)b * p.o_sb + (int64_t)h * p.o_sh + d] = __float2bfloat16_rn(l == 0.f ? 0.f : o / l);
+  *reinterpret_cast<float4*>(&s_o[warp][4 * lane]) = o;
+  if (lane == 0) s_l[warp] = l;
+  __syncthreads();
+  if (threadIdx.x < 128) {
+    float ot = 0.f, lt = 0.f;
+#pragma unroll
+    for (int w = 0; w < kKv4CombineWarps; ++w) {
+      ot += s_o[w][threadIdx.x];
+      lt += s_l[w];
+    }
+    p.out[(int64_t)b * p.o_sb + (int64_t)h * p.o_sh + threadIdx.x] = __float2bfloat16_rn(lt == 0.f ? 0.f : ot / lt);
+  }
 }
 
 }  // namespace tg

@@ -385,6 +385,10 @@ __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n"
                "barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
+// the same in two steps, with work of one's own between them (a block's first
+// access to another's shared memory has to come after both have started)
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory"); }
 // arrive on an mbarrier of either CTA (shared::cluster address) with the
 // default semantics (release at CTA scope): for handing TMEM contents to the
 // pair's MMA issuer, ordered by tcgen05.fence::before_thread_sync

@@ -460,6 +460,7 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SamplePara
                  {},
                  0,
                  0};
+  if (c.C > 1) cluster_arrive();
   griddep_wait();
   griddep_launch_dependents();
 
@@ -519,6 +520,8 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SamplePara
   {
     smp_u64 z0 = 0, z1 = 0;
     uint32_t lo = 0, cnt;
+    __syncwarp();
+    if (c.C > 1) cluster_wait();  // every block has started
     c.reduce(z0, z1, lo, best, cnt, nullptr);
   }
   c.row.xmax = smp_unkey(best);

@@ -199,6 +199,26 @@ cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t sme
   return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
+// The same for a kernel whose clusters are C blocks along x.
+template <typename P>
+cudaError_t launch_cluster(void (*kern)(P), dim3 grid, dim3 block, size_t smem, cudaStream_t s, int C, const P& p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)C;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kern, p);
+}
+
 constexpr int kGemvMaxSmem = 200 * 1024;  // the rows of x in shared memory: BT * K * 2 bytes at most
 
 // One gemv launch: the kernel's shared-memory limit is raised once per device
@@ -1367,15 +1387,30 @@ int kv4_rows(const char* what, bool write, const void* k, int64_t k_sb, int64_t 
   return TG_OK;
 }
 
-// Splits of a row's tiles over CTAs, and the tiles of one.
-void kv4_splits(int B, int Hkv, int n_keys, int* n_splits, int* per) {
-  const int tiles = (int)kv4_tiles(n_keys);
-  const int64_t want = ((int64_t)sm_count() * 3 + (int64_t)B * Hkv - 1) / ((int64_t)B * Hkv);
-  int64_t per_ = (tiles + want - 1) / want;
-  per_ = (per_ + tg::kKv4Warps - 1) / tg::kKv4Warps * tg::kKv4Warps;
-  *per = (int)per_;
-  *n_splits = (int)((tiles + per_ - 1) / per_);
+// Blocks that share one kv head of one row, warps of a block, and whether the
+// blocks are a cluster or leave records to kv4_combine_kernel.
+struct Kv4Shape {
+  int blocks, warps;
+  bool cluster;
+};
+Kv4Shape kv4_shape(int B, int Hkv, int n_keys) {
+  const int64_t rows = (int64_t)B * Hkv, tiles = kv4_tiles(n_keys);
+  const int sms = sm_count();
+  Kv4Shape s = {1, tg::kKv4MaxWarps, true};
+  if (tiles <= 192 && rows * 2 <= sms) {
+    while (s.blocks < 8 && rows * s.blocks * 2 <= sms && tiles > s.blocks) s.blocks *= 2;
+  } else if (rows * 2 <= sms) {
+    s.cluster = false;
+    s.blocks = (int)(sms / rows);
+  }
+  const int64_t per = (tiles + s.blocks - 1) / s.blocks;
+  if (per < s.warps) s.warps = (int)per;
+  return s;
 }
+size_t kv4_part_bytes(int B, int Hq, const Kv4Shape& s) {
+  return s.cluster || s.blocks == 1 ? 0 : (size_t)B * Hq * s.blocks * tg::kKv4Part * sizeof(float);
+}
+bool g_kv4_attr_set[2][kMaxDevices] = {};
 }  // namespace
 
 int tg_kv4_cache_bytes(int B, int Hkv, int64_t capacity, size_t* bytes) {
@@ -1457,9 +1492,7 @@ int tg_decode_attn_kv4_workspace(int B, int Hq, int Hkv, int n_keys, size_t* byt
   *bytes = 0;
   if (B < 1 || Hq < 1 || Hkv < 1 || n_keys < 1)
     return fail(TG_ERR_INVALID_ARGUMENT, "decode_attn_kv4_workspace: B=%d Hq=%d Hkv=%d n_keys=%d", B, Hq, Hkv, n_keys);
-  int ns, per;
-  kv4_splits(B, Hkv, n_keys, &ns, &per);
-  if (ns > 1) *bytes = (size_t)B * Hq * ns * tg::kKv4Part * sizeof(float);
+  *bytes = kv4_part_bytes(B, Hq, kv4_shape(B, Hkv, n_keys));
   return TG_OK;
 }
 
@@ -1481,15 +1514,6 @@ int tg_decode_attn_kv4(const void* q, int64_t q_sb, int64_t q_sh, const float* q
     return fail(TG_ERR_UNSUPPORTED, "decode_attn_kv4: %d query heads per kv head (1 to 8 served)", Hq / Hkv);
   if (!(softmax_scale > 0.f)) return fail(TG_ERR_INVALID_ARGUMENT, "decode_attn_kv4: softmax_scale must be > 0");
   tg::Kv4AttnParams p;
-  kv4_splits(B, Hkv, n_keys, &p.n_splits, &p.tiles_per_split);
-  if (p.n_splits > 1) {
-    const size_t need = (size_t)B * Hq * p.n_splits * tg::kKv4Part * sizeof(float);
-    if (workspace == nullptr || workspace_bytes < need)
-      return fail(TG_ERR_INVALID_ARGUMENT, "decode_attn_kv4: workspace of %zu bytes, %zu needed", workspace_bytes,
-                  need);
-    if (reinterpret_cast<uintptr_t>(workspace) & 15)
-      return fail(TG_ERR_ALIGNMENT, "decode_attn_kv4: workspace must be 16-byte aligned");
-  }
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.q_sb = q_sb;
   p.q_sh = q_sh;
@@ -1508,17 +1532,35 @@ int tg_decode_attn_kv4(const void* q, int64_t q_sb, int64_t q_sh, const float* q
   p.out = static_cast<__nv_bfloat16*>(out);
   p.o_sb = o_sb;
   p.o_sh = o_sh;
-  p.part = static_cast<float*>(workspace);
-  p.Hq = Hq;
-  p.Hkv = Hkv;
   p.G = Hq / Hkv;
   p.scale = softmax_scale;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  cudaError_t e = launch_pdl(tg::kv4_attn_kernel, dim3((unsigned)p.n_splits, (unsigned)Hkv, (unsigned)B),
-                             dim3(tg::kKv4AttnThreads), 0, s, p);
+  if ((st = device_error_ptr(&p.err))) return st;
+  int dev;
+  if ((st = current_device(&dev))) return st;
+  const Kv4Shape shape = kv4_shape(B, Hkv, n_keys);
+  const size_t need = kv4_part_bytes(B, Hq, shape);
+  if (need > 0) {
+    if (workspace == nullptr || workspace_bytes < need)
+      return fail(TG_ERR_INVALID_ARGUMENT, "decode_attn_kv4: workspace of %zu bytes, %zu needed", workspace_bytes,
+                  need);
+    if (reinterpret_cast<uintptr_t>(workspace) & 15)
+      return fail(TG_ERR_ALIGNMENT, "decode_attn_kv4: workspace must be 16-byte aligned");
+  }
+  p.part = need > 0 ? static_cast<float*>(workspace) : nullptr;
+  p.Hq = Hq;
+  auto kern = bias != nullptr ? tg::kv4_attn_kernel<true> : tg::kv4_attn_kernel<false>;
+  bool(&flags)[kMaxDevices] = g_kv4_attr_set[bias != nullptr];
+  cudaError_t e = cudaSuccess;
+  if (!flags[dev]) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) e = smem_limit_once(kern, tg::kv4_attn_smem(tg::kKv4MaxWarps), flags, dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(decode_attn_kv4)");
+  const dim3 grid((unsigned)shape.blocks, (unsigned)Hkv, (unsigned)B), block(32u * shape.warps);
+  e = launch_cluster(kern, grid, block, tg::kv4_attn_smem(shape.warps), static_cast<cudaStream_t>(stream),
+                     shape.cluster ? shape.blocks : 1, p);
   if (e != cudaSuccess) return cuda_fail(e, "decode_attn_kv4 launch");
-  if (p.n_splits > 1) {
-    e = launch_pdl(tg::kv4_combine_kernel, dim3((unsigned)Hq, (unsigned)B), dim3(128), 0, s, p);
+  if (need > 0) {
+    e = launch_pdl(tg::kv4_combine_kernel, dim3((unsigned)Hq, (unsigned)B), dim3(32 * tg::kKv4CombineWarps), 0,
+                   static_cast<cudaStream_t>(stream), p, shape.blocks);
     if (e != cudaSuccess) return cuda_fail(e, "decode_attn_kv4 combine launch");
   }
   return TG_OK;
@@ -1567,25 +1609,13 @@ int tg_sample(const void* logits, int dtype, int64_t row_stride, int B, int V, c
   const bool held = smem_of(C) <= (size_t)kSmpMaxSmem;
   auto kern = dtype ? (held ? tg::sample_kernel<__nv_bfloat16, true> : tg::sample_kernel<__nv_bfloat16, false>)
                     : (held ? tg::sample_kernel<float, true> : tg::sample_kernel<float, false>);
-  cudaError_t e = smem_limit_once(kern, kSmpMaxSmem, g_smp_attr_set[2 * dtype + held], dev);
-  if (e == cudaSuccess && C > 8)
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  bool(&flags)[kMaxDevices] = g_smp_attr_set[2 * dtype + held];
+  cudaError_t e = cudaSuccess;
+  if (!flags[dev]) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) e = smem_limit_once(kern, kSmpMaxSmem, flags, dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(sample)");
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)C, (unsigned)B);
-  cfg.blockDim = dim3(tg::kSmpThreads);
-  cfg.dynamicSmemBytes = held ? smem_of(C) : sizeof(tg::SmpShared);
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = (unsigned)C;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  e = cudaLaunchKernelEx(&cfg, kern, p);
+  e = launch_cluster(kern, dim3((unsigned)C, (unsigned)B), dim3(tg::kSmpThreads),
+                     held ? smem_of(C) : sizeof(tg::SmpShared), static_cast<cudaStream_t>(stream), C, p);
   if (e != cudaSuccess) return cuda_fail(e, "sample launch");
   return TG_OK;
 }

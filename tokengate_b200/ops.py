@@ -10,6 +10,7 @@ from typing import Optional, Sequence, Tuple
 
 import contextlib
 import ctypes
+import functools
 
 import torch
 
@@ -813,6 +814,13 @@ def qk_norm_rope_append_kv4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q
     return q_out
 
 
+@functools.lru_cache(maxsize=4096)
+def _kv4_workspace(B: int, Hq: int, Hkv: int, n_keys: int) -> int:
+    nbytes = ctypes.c_size_t(0)
+    _lib.check(_lib.lib().tg_decode_attn_kv4_workspace(B, Hq, Hkv, n_keys, ctypes.byref(nbytes)))
+    return nbytes.value
+
+
 def decode_attention_kv4(q: torch.Tensor, cache: KV4Cache, n_valid: torch.Tensor, n_prefix: int, n_keys: int,
                          bias: Optional[torch.Tensor] = None, q_scale: Optional[torch.Tensor] = None,
                          softmax_scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
@@ -864,13 +872,12 @@ def decode_attention_kv4(q: torch.Tensor, cache: KV4Cache, n_valid: torch.Tensor
         raise ValueError("every tensor must be on the cache's device")
     L = _lib.lib()
     with _device_ctx(q):
-        nbytes = ctypes.c_size_t(0)
-        _lib.check(L.tg_decode_attn_kv4_workspace(B, Hq, c.n_kv_heads, n_keys, ctypes.byref(nbytes)))
-        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev) if nbytes.value else None
+        nbytes = _kv4_workspace(B, Hq, c.n_kv_heads, n_keys)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         _lib.check_launch(L.tg_decode_attn_kv4(
             q.data_ptr(), q.stride(0), q.stride(1), qs_ptr, qsb, c.data.data_ptr(), c.capacity,
             bias_ptr, bsb, bsh, n_valid.data_ptr(), n_prefix, n_keys, nk_ptr,
-            out.data_ptr(), out.stride(0), out.stride(1), ws.data_ptr() if ws is not None else None, nbytes.value,
+            out.data_ptr(), out.stride(0), out.stride(1), ws.data_ptr() if ws is not None else None, nbytes,
             B, Hq, c.n_kv_heads, D, D ** -0.5 if softmax_scale is None else softmax_scale, _stream(q)))
     return out
 
