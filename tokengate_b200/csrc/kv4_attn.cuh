@@ -58,8 +58,9 @@ struct Kv4AttnParams {
   const int32_t* n_keys_dev;
   __nv_bfloat16* out;
   int64_t o_sb, o_sh;
-  float* part;           // nullable: [row][head][block][kKv4Part] instead of a merge in a cluster
-  int G, Hq;
+  float* part;           // nullable: records [Hq][parts + B][kKv4Part] instead of a merge in a cluster
+  int parts;             // blocks per kv head that fill the GPU, shared among the batch rows
+  int B, G, Hq;
   float scale;
   unsigned int* err;
 };
@@ -69,7 +70,7 @@ struct alignas(16) Kv4AttnShared {
   __half q[8][128];
   float mul[8];
   float m[kKv4MaxWarps][8], l[kKv4MaxWarps][8];
-  float got_o[8 * 128];                           // [rank][slice]: this block's slice of the blocks' sums
+  float got_o[8 * 128 + kKv4MaxCluster];          // [rank][slice]: this block's slice of the blocks' sums
   float got_m[kKv4MaxCluster][8], got_l[kKv4MaxCluster][8];
   uint64_t full[kKv4MaxWarps][kKv4Stages];
 };
@@ -110,6 +111,68 @@ __device__ __forceinline__ float warp_sum_rows(float v) {
 #pragma unroll
   for (int off = 4; off <= 16; off <<= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
   return v;
+}
+
+// The lane's four values of a head's q, (B, heads, 128) bf16 with any alignment.
+__device__ __forceinline__ uint2 kv4_load_q(const __nv_bfloat16* qp, int lane) {
+  if ((reinterpret_cast<uintptr_t>(qp) & 7) == 0) return *(reinterpret_cast<const uint2*>(qp) + lane);
+  const uint16_t* u = reinterpret_cast<const uint16_t*>(qp) + 4 * lane;
+  return make_uint2(u[0] | (uint32_t)u[1] << 16, u[2] | (uint32_t)u[3] << 16);
+}
+
+// Tiles with attended keys of a row: [0, na) and from tb on, n in all.
+struct Kv4Span {
+  int na, tb, n;
+};
+__device__ __forceinline__ Kv4Span kv4_span(int n_valid, int n_prefix, int n_keys) {
+  const int tiles = (n_keys + kKv4Keys - 1) / kKv4Keys;
+  const int nv = min(max(n_valid, 0), n_prefix);
+  Kv4Span r;
+  r.na = min((nv + kKv4Keys - 1) / kKv4Keys, tiles);
+  r.tb = max(n_prefix / kKv4Keys, r.na);
+  r.n = r.na + max(tiles - r.tb, 0);
+  return r;
+}
+
+// How the `parts` blocks of a kv head are shared among the batch rows: by the
+// tiles that each has (rows of unlike length keep every SM as busy), at least
+// one to a row that has any. Of the row b for which pick(b, first, count) is
+// true, with its blocks [first, first + count): b, first and count to the whole
+// warp (b = -1: none). The counts' sum is below parts + B. Every warp computes
+// it for itself, 32 rows at a time.
+template <typename Pick>
+__device__ __forceinline__ void kv4_share(const Kv4AttnParams& p, int n_keys, int lane, Pick pick, int& b, int& first,
+                                          int& count) {
+  auto tiles_of = [&](int r) { return r < p.B ? kv4_span(__ldg(p.n_valid + r), p.n_prefix, n_keys).n : 0; };
+  int n = tiles_of(lane);
+  float total = (float)__reduce_add_sync(0xffffffffu, (unsigned)n);
+  for (int b0 = 32; b0 < p.B; b0 += 32) total += (float)__reduce_add_sync(0xffffffffu, (unsigned)tiles_of(b0 + lane));
+  // a share rounded down of all blocks, or rounded up of all but one per row: whichever is more (the same fp32
+  // roundings wherever it is computed)
+  const float down = __fdiv_rn((float)p.parts, total), up = __fdiv_rn((float)max(p.parts - p.B, 0), total);
+  b = -1;
+  first = count = 0;
+  int run = 0;
+  for (int b0 = 0; b0 < p.B && b < 0; b0 += 32) {
+    if (b0 > 0) n = tiles_of(b0 + lane);
+    const int c = n == 0 ? 0
+                         : max(max((int)floorf(__fmul_rn((float)n, down) + 1e-3f), (int)ceilf(__fmul_rn((float)n, up) - 1e-3f)), 1);
+    int end = c;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int a = __shfl_up_sync(0xffffffffu, end, off);
+      if (lane >= off) end += a;
+    }
+    end += run;
+    const uint32_t hit = __ballot_sync(0xffffffffu, b0 + lane < p.B && pick(b0 + lane, end - c, c));
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      b = b0 + src;
+      first = __shfl_sync(0xffffffffu, end - c, src);
+      count = __shfl_sync(0xffffffffu, c, src);
+    }
+    run = __shfl_sync(0xffffffffu, end, 31);
+  }
 }
 
 // A warp's running softmax over its tiles, for the heads 2 t and 2 t + 1 of
@@ -271,21 +334,23 @@ __device__ __forceinline__ void kv4_tile(Kv4State& st, const uint8_t* tile, int 
   }
 }
 
-// C blocks take one kv head of one row (grid (C, Hkv, B)): the tiles that hold
-// attended keys, evenly in order to the blocks and in turn to a block's warps.
-// Each warp keeps its own running softmax; warps merge in shared memory. The
-// blocks merge in one of two ways: as a cluster, sending each other their
-// slices of the output (one barrier, no second launch, no workspace), or
-// through records that kv4_combine_kernel merges (any number of blocks, so
-// every SM can take part: clusters of 16 leave a quarter of them idle).
+// C blocks take one kv head of one row: the tiles that hold attended keys,
+// evenly in order to the blocks and in turn to a block's warps. Each warp keeps
+// its own running softmax; warps merge in shared memory. The blocks merge in
+// one of two ways: as a cluster (grid (C, Hkv, B)), sending each other their
+// slices of the output (one barrier, no second launch, no workspace), or, grid
+// (parts + B, Hkv), C by kv4_share, through records that kv4_combine_kernel
+// merges (so every SM can take part: clusters of 16 leave a quarter of them
+// idle).
 template <bool BIAS>
 __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv4AttnParams p) {
   extern __shared__ __align__(128) uint8_t kv4_smem[];
   Kv4AttnShared& sh = *reinterpret_cast<Kv4AttnShared*>(kv4_smem);
-  const int W = blockDim.x >> 5, C = gridDim.x, rank = blockIdx.x;
+  const int W = blockDim.x >> 5;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const int kvh = blockIdx.y, b = blockIdx.z;
+  const int kvh = blockIdx.y;
+  int b = blockIdx.z, C = gridDim.x, rank = blockIdx.x;
   uint8_t* ring = kv4_smem + kKv4Ring + warp * kKv4Stages * kKv4TileBytes;
   const uint32_t ring_s = smem_u32(ring), full_s = smem_u32(sh.full[warp]);
   if (lane == 0) {
@@ -294,23 +359,37 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
     fence_mbar_init();
   }
   __syncwarp();
-  const bool clustered = C > 1 && p.part == nullptr;
+  const bool clustered = p.part == nullptr && C > 1;
   if (clustered) cluster_arrive();
   griddep_wait();
   griddep_launch_dependents();
   const int n_keys = p.n_keys_dev != nullptr ? min(__ldg(p.n_keys_dev), p.n_keys) : p.n_keys;
-  const int nv = min(max(__ldg(p.n_valid + b), 0), p.n_prefix);
+  if (p.part != nullptr) {
+    int first;
+    kv4_share(p, n_keys, lane, [&](int, int f, int c) { return (int)blockIdx.x >= f && (int)blockIdx.x < f + c; }, b,
+              first, C);
+    if (b < 0) return;
+    rank = blockIdx.x - first;
+  }
+  // the counts and the heads' q (warp w: heads w, w + W, ..) wait for one another's latency only
+  const int nv_raw = __ldg(p.n_valid + b);
+  uint2 q_raw = make_uint2(0u, 0u);
+  float q_mul = 1.f;
+  if (warp < p.G) {
+    const int hq = kvh * p.G + warp;
+    const __nv_bfloat16* qp = p.q + (int64_t)b * p.q_sb + (int64_t)hq * p.q_sh;
+    q_raw = kv4_load_q(qp, lane);
+    if (p.q_scale != nullptr) q_mul = p.q_scale[(int64_t)b * p.qs_sb + hq];
+  }
+  const int nv = min(max(nv_raw, 0), p.n_prefix);
   const uint8_t* base = p.cache + (int64_t)b * p.c_sb + (int64_t)kvh * p.c_sh;
-
-  // tiles with attended keys: [0, na) and from tb on
-  const int tiles = (n_keys + kKv4Keys - 1) / kKv4Keys;
-  const int na = min((nv + kKv4Keys - 1) / kKv4Keys, tiles), tb = max(p.n_prefix / kKv4Keys, na);
-  const int n = na + max(tiles - tb, 0);
+  const Kv4Span span = kv4_span(nv_raw, p.n_prefix, n_keys);
+  const int n = span.n;
   const int v0 = (int)((int64_t)n * rank / C), v1 = (int)((int64_t)n * (rank + 1) / C);
   const int mine = v1 - v0 > warp ? (v1 - v0 - warp + W - 1) / W : 0;  // this warp's tiles
   auto tile_of = [&](int i) {
     const int v = v0 + warp + i * W;
-    return v < na ? v : v - na + tb;
+    return v < span.na ? v : v - span.na + span.tb;
   };
   auto fetch = [&](int i) {
     const int s = i % kKv4Stages;
@@ -322,17 +401,18 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
 
   // the heads' q', scaled by a power of two
   for (int h = warp; h < 8; h += W) {
-    float v[4] = {0.f, 0.f, 0.f, 0.f}, mx = 0.f;
-    if (h < p.G) {
+    if (h != warp && h < p.G) {
       const int hq = kvh * p.G + h;
-      const __nv_bfloat16* qp = p.q + (int64_t)b * p.q_sb + (int64_t)hq * p.q_sh;
-      const float qs = p.q_scale != nullptr ? round_bf16(p.q_scale[(int64_t)b * p.qs_sb + hq]) : 1.f;
+      q_raw = kv4_load_q(p.q + (int64_t)b * p.q_sb + (int64_t)hq * p.q_sh, lane);
+      if (p.q_scale != nullptr) q_mul = p.q_scale[(int64_t)b * p.qs_sb + hq];
+    }
+    float v[4] = {bf16_lo(q_raw.x), bf16_hi(q_raw.x), bf16_lo(q_raw.y), bf16_hi(q_raw.y)}, mx = 0.f;
+    const float qs = round_bf16(q_mul);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[e] = __bfloat162float(qp[lane + 32 * e]);
-        if (p.q_scale != nullptr) v[e] = round_bf16(v[e] * qs);
-        mx = fmaxf(mx, fabsf(v[e]));
-      }
+    for (int e = 0; e < 4; ++e) {
+      if (p.q_scale != nullptr) v[e] = round_bf16(v[e] * qs);
+      if (h >= p.G) v[e] = 0.f;
+      mx = fmaxf(mx, fabsf(v[e]));
     }
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
@@ -340,20 +420,21 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
     const int ex = min(max((int)(__float_as_uint(mx) >> 23) - 127 - 12, -126), 126);
     const float down = __uint_as_float((uint32_t)(127 - ex) << 23);
     if (lane == 0) sh.mul[h] = __uint_as_float((uint32_t)(127 + ex) << 23) * p.scale * (BIAS ? 1.f : kLog2e);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sh.q[h][lane + 32 * e] = __float2half_rn(v[e] * down);
+    const __half2 a = __floats2half2_rn(v[0] * down, v[1] * down), c = __floats2half2_rn(v[2] * down, v[3] * down);
+    *reinterpret_cast<uint2*>(&sh.q[h][4 * lane]) = make_uint2(h2_bits(a), h2_bits(c));
   }
   __syncthreads();
   Kv4State st;
   // MMA (i, 0): nibbles (0, 4), (1, 5) of word i; (i, 1): (2, 6), (3, 7)
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
+    const uint4 x = *reinterpret_cast<const uint4*>(&sh.q[g][32 * i + 8 * t]);  // 8 dims
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int d = 32 * i + 8 * t + u;
-      __half2 f = __halves2half2(sh.q[g][d], sh.q[g][d + 4]);
-      if (u & 1) f = __hmul2(f, __float2half2_rn(0.0625f));  // its nibbles read 16 times as large
-      st.qf[2 * i + (u >> 1)][u & 1] = h2_bits(f);
+      uint32_t f = __byte_perm(w[u >> 1], w[2 + (u >> 1)], u & 1 ? 0x7632 : 0x5410);  // dims u, u + 4
+      if (u & 1) f = h2_bits(__hmul2(bits_h2(f), __float2half2_rn(0.0625f)));  // its nibbles read 16 times as large
+      st.qf[2 * i + (u >> 1)][u & 1] = f;
     }
   }
 #pragma unroll
@@ -363,9 +444,14 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
     st.l[j] = st.zs[0][j] = st.zs[1][j] = 0.f;
 #pragma unroll
     for (int gr = 0; gr < 2; ++gr) {
+      const uint4 x = *reinterpret_cast<const uint4*>(&sh.q[2 * t + j][64 * gr + 8 * g]);
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
       float a = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) a += __half2float(sh.q[2 * t + j][64 * gr + 8 * g + e]);
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = __half22float2(bits_h2(w[e]));
+        a += f.x + f.y;
+      }
       st.qs[gr][j] = warp_sum_rows(a);
     }
   }
@@ -427,17 +513,18 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
   __syncthreads();
   const float* all_o = reinterpret_cast<const float*>(kv4_smem + kKv4Ring);
   constexpr float kUnit = BIAS ? kLog2e : 1.f;  // of m
-  const int slice = p.G * 128 / C;
+  const int slice = (p.G * 128 + C - 1) / C;
   for (int idx = threadIdx.x; idx < p.G * 128; idx += blockDim.x) {
     const int h = idx >> 7;
     float mt = sh.m[0][h];
     for (int w = 1; w < W; ++w) mt = fmaxf(mt, sh.m[w][h]);
     float o = 0.f, lt = 0.f;
+#pragma unroll 4
     for (int w = 0; w < W; ++w) {
-      const float lw = sh.l[w][h];
+      const float lw = sh.l[w][h], ow = all_o[w * (kKv4Stages * kKv4TileBytes / 4) + idx];
       if (lw != 0.f) {  // 0: the warp saw no key (a NaN sum stays in)
         const float f = ex2_approx((sh.m[w][h] - mt) * kUnit);
-        o = fmaf(f, all_o[w * (kKv4Stages * kKv4TileBytes / 4) + idx], o);
+        o = fmaf(f, ow, o);
         lt = fmaf(f, lw, lt);
       }
     }
@@ -445,7 +532,7 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
       p.out[(int64_t)b * p.o_sb + (int64_t)(kvh * p.G + h) * p.o_sh + (idx & 127)] =
           __float2bfloat16_rn(lt == 0.f ? 0.f : o / lt);
     } else if (!clustered) {
-      float* rec = p.part + (((int64_t)b * p.Hq + kvh * p.G + h) * C + rank) * kKv4Part;
+      float* rec = p.part + ((int64_t)(kvh * p.G + h) * gridDim.x + blockIdx.x) * kKv4Part;
       rec[4 + (idx & 127)] = o;
       if ((idx & 127) == 0) {
         rec[0] = mt;
@@ -465,6 +552,7 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
   cluster_sync_all();
   for (int i = threadIdx.x; i < slice; i += blockDim.x) {
     const int idx = rank * slice + i, h = idx >> 7;
+    if (idx >= p.G * 128) break;
     float mt = sh.got_m[0][h];
     for (int c = 1; c < C; ++c) mt = fmaxf(mt, sh.got_m[c][h]);
     float o = 0.f, lt = 0.f;
@@ -482,45 +570,73 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
 }
 
 // Merges the blocks' records of one (row, head): 8 warps take every 8th record
-// (lane: dims 4 l .. 4 l + 3, 16-byte loads), then merge through shared memory.
+// (lane: dims 4 l .. 4 l + 3, 16-byte loads), four at a time with every load
+// before any arithmetic, then merge through shared memory.
 constexpr int kKv4CombineWarps = 8;
-__global__ void __launch_bounds__(32 * kKv4CombineWarps) kv4_combine_kernel(const Kv4AttnParams p, int C) {
-  __shared__ float s_l[kKv4CombineWarps];
+__global__ void __launch_bounds__(32 * kKv4CombineWarps) kv4_combine_kernel(const Kv4AttnParams p) {
+  __shared__ float s_m[kKv4CombineWarps], s_l[kKv4CombineWarps];
   __shared__ float s_o[kKv4CombineWarps][128];
   griddep_wait();
   griddep_launch_dependents();
   const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const float* rec = p.part + ((int64_t)b * p.Hq + h) * C * kKv4Part;
+  const int n_keys = p.n_keys_dev != nullptr ? min(__ldg(p.n_keys_dev), p.n_keys) : p.n_keys;
+  int found, first, C;
+  kv4_share(p, n_keys, lane, [&](int r, int, int) { return r == b; }, found, first, C);
+  if (C == 1) return;  // its one block has written the output
+  const float* rec = p.part + ((int64_t)h * (p.parts + p.B) + first) * kKv4Part;
   const float unit = p.bias != nullptr ? kLog2e : 1.f;  // of m
-  float m = -INFINITY;
-  for (int c = lane; c < C; c += 32) m = fmaxf(m, rec[(int64_t)c * kKv4Part]);
-#pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+  float m = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.f;
-#pragma unroll 4
-  for (int c = warp; c < C; c += kKv4CombineWarps) {
-    const float* r = rec + (int64_t)c * kKv4Part;
-    const float4 v = *reinterpret_cast<const float4*>(r + 4 + 4 * lane);
-    const float lc = r[1];
-    if (lc != 0.f) {  // 0: the block saw no key (a NaN sum stays in)
-      const float f = ex2_approx((r[0] - m) * unit);
-      l = fmaf(f, lc, l);
-      o.x = fmaf(f, v.x, o.x);
-      o.y = fmaf(f, v.y, o.y);
-      o.z = fmaf(f, v.z, o.z);
-      o.w = fmaf(f, v.w, o.w);
+  for (int c0 = warp; c0 < C; c0 += 4 * kKv4CombineWarps) {
+    float4 v[4];
+    float2 ml[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int c = c0 + k * kKv4CombineWarps;
+      ml[k] = make_float2(-INFINITY, 0.f);
+      if (c < C) {
+        const float* r = rec + (int64_t)c * kKv4Part;
+        ml[k] = *reinterpret_cast<const float2*>(r);
+        v[k] = *reinterpret_cast<const float4*>(r + 4 + 4 * lane);
+      }
+    }
+    const float mn = fmaxf(fmax3(m, ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x));
+    const float back = l == 0.f ? 0.f : ex2_approx((m - mn) * unit);
+    m = mn;
+    l *= back;
+    o.x *= back;
+    o.y *= back;
+    o.z *= back;
+    o.w *= back;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (ml[k].y != 0.f) {  // 0: the block saw no key (a NaN sum stays in)
+        const float f = ex2_approx((ml[k].x - m) * unit);
+        l = fmaf(f, ml[k].y, l);
+        o.x = fmaf(f, v[k].x, o.x);
+        o.y = fmaf(f, v[k].y, o.y);
+        o.z = fmaf(f, v[k].z, o.z);
+        o.w = fmaf(f, v[k].w, o.w);
+      }
     }
   }
+  if (lane == 0) {
+    s_m[warp] = m;
+    s_l[warp] = l;
+  }
   *reinterpret_cast<float4*>(&s_o[warp][4 * lane]) = o;
-  if (lane == 0) s_l[warp] = l;
   __syncthreads();
   if (threadIdx.x < 128) {
-    float ot = 0.f, lt = 0.f;
+    float mt = s_m[0], ot = 0.f, lt = 0.f;
+#pragma unroll
+    for (int w = 1; w < kKv4CombineWarps; ++w) mt = fmaxf(mt, s_m[w]);
 #pragma unroll
     for (int w = 0; w < kKv4CombineWarps; ++w) {
-      ot += s_o[w][threadIdx.x];
-      lt += s_l[w];
+      if (s_l[w] != 0.f) {
+        const float f = ex2_approx((s_m[w] - mt) * unit);
+        ot = fmaf(f, s_o[w][threadIdx.x], ot);
+        lt = fmaf(f, s_l[w], lt);
+      }
     }
     p.out[(int64_t)b * p.o_sb + (int64_t)h * p.o_sh + threadIdx.x] = __float2bfloat16_rn(lt == 0.f ? 0.f : ot / lt);
   }

@@ -1387,28 +1387,30 @@ int kv4_rows(const char* what, bool write, const void* k, int64_t k_sb, int64_t 
   return TG_OK;
 }
 
-// Blocks that share one kv head of one row, warps of a block, and whether the
-// blocks are a cluster or leave records to kv4_combine_kernel.
+// Warps of a block, and the blocks: of a cluster per kv head and row, or (parts
+// > 0) the blocks per kv head that the rows share.
 struct Kv4Shape {
-  int blocks, warps;
-  bool cluster;
+  int warps, cluster, parts;
 };
 Kv4Shape kv4_shape(int B, int Hkv, int n_keys) {
   const int64_t rows = (int64_t)B * Hkv, tiles = kv4_tiles(n_keys);
   const int sms = sm_count();
-  Kv4Shape s = {1, tg::kKv4MaxWarps, true};
+  Kv4Shape s = {tg::kKv4MaxWarps, 1, 0};
   if (tiles <= 192 && rows * 2 <= sms) {
-    while (s.blocks < 8 && rows * s.blocks * 2 <= sms && tiles > s.blocks) s.blocks *= 2;
+    // short caches, where a second launch costs more than idle SMs
+    while (s.cluster < 8 && rows * s.cluster * 2 <= sms && tiles > s.cluster) s.cluster *= 2;
+    const int64_t per = (tiles + s.cluster - 1) / s.cluster;
+    if (per < s.warps) s.warps = (int)per;
   } else if (rows * 2 <= sms) {
-    s.cluster = false;
-    s.blocks = (int)(sms / rows);
+    s.parts = sms / Hkv;          // one block of 12 warps per SM
+  } else {
+    s.warps = 4;                  // many rows: three blocks of 4 warps per SM
+    s.parts = 3 * sms / Hkv > 0 ? 3 * sms / Hkv : 1;
   }
-  const int64_t per = (tiles + s.blocks - 1) / s.blocks;
-  if (per < s.warps) s.warps = (int)per;
   return s;
 }
 size_t kv4_part_bytes(int B, int Hq, const Kv4Shape& s) {
-  return s.cluster || s.blocks == 1 ? 0 : (size_t)B * Hq * s.blocks * tg::kKv4Part * sizeof(float);
+  return s.parts == 0 ? 0 : (size_t)Hq * (s.parts + B) * tg::kKv4Part * sizeof(float);
 }
 bool g_kv4_attr_set[2][kMaxDevices] = {};
 }  // namespace
@@ -1547,6 +1549,8 @@ int tg_decode_attn_kv4(const void* q, int64_t q_sb, int64_t q_sh, const float* q
       return fail(TG_ERR_ALIGNMENT, "decode_attn_kv4: workspace must be 16-byte aligned");
   }
   p.part = need > 0 ? static_cast<float*>(workspace) : nullptr;
+  p.parts = shape.parts;
+  p.B = B;
   p.Hq = Hq;
   auto kern = bias != nullptr ? tg::kv4_attn_kernel<true> : tg::kv4_attn_kernel<false>;
   bool(&flags)[kMaxDevices] = g_kv4_attr_set[bias != nullptr];
@@ -1554,13 +1558,14 @@ int tg_decode_attn_kv4(const void* q, int64_t q_sb, int64_t q_sh, const float* q
   if (!flags[dev]) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e == cudaSuccess) e = smem_limit_once(kern, tg::kv4_attn_smem(tg::kKv4MaxWarps), flags, dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(decode_attn_kv4)");
-  const dim3 grid((unsigned)shape.blocks, (unsigned)Hkv, (unsigned)B), block(32u * shape.warps);
+  const dim3 grid((unsigned)(need > 0 ? shape.parts + B : shape.cluster), (unsigned)Hkv, (unsigned)(need > 0 ? 1 : B));
+  const dim3 block(32u * shape.warps);
   e = launch_cluster(kern, grid, block, tg::kv4_attn_smem(shape.warps), static_cast<cudaStream_t>(stream),
-                     shape.cluster ? shape.blocks : 1, p);
+                     shape.cluster, p);
   if (e != cudaSuccess) return cuda_fail(e, "decode_attn_kv4 launch");
   if (need > 0) {
     e = launch_pdl(tg::kv4_combine_kernel, dim3((unsigned)Hq, (unsigned)B), dim3(32 * tg::kKv4CombineWarps), 0,
-                   static_cast<cudaStream_t>(stream), p, shape.blocks);
+                   static_cast<cudaStream_t>(stream), p);
     if (e != cudaSuccess) return cuda_fail(e, "decode_attn_kv4 combine launch");
   }
   return TG_OK;
