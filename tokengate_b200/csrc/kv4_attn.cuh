@@ -25,7 +25,7 @@
 // Scores, maxima, sums and the accumulators are fp32.
 //
 // The cache is read once, at 144 bytes per key: every warp streams its own
-// tiles through a ring of three in shared memory (one bulk copy of 4608 bytes
+// tiles through a ring of two or three in shared memory (one bulk copy of 4608 bytes
 // each, no barrier between warps). What bounds it is the instructions per tile
 // as much as the bytes: see kv4_tile.
 #pragma once
@@ -38,8 +38,8 @@
 namespace tg {
 
 constexpr unsigned int ERR_KV4 = 1u << 15;  // bit of the device error word
-constexpr int kKv4Stages = 3;
-constexpr int kKv4MaxWarps = 12;
+constexpr int kKv4Stages = 3;          // ring tiles per warp, at most
+constexpr int kKv4MaxWarps = 16;
 constexpr int kKv4MaxCluster = 16;
 constexpr float kKv4Head = 4.f;       // p = 2^(4 + ...): small p stay normal in fp16
 constexpr float kLog2e = 1.4426950408889634f;
@@ -60,7 +60,7 @@ struct Kv4AttnParams {
   int64_t o_sb, o_sh;
   float* part;           // nullable: records [Hq][parts + B][kKv4Part] instead of a merge in a cluster
   int parts;             // blocks per kv head that fill the GPU, shared among the batch rows
-  int B, G, Hq;
+  int B, G, Hq, stages;
   float scale;
   unsigned int* err;
 };
@@ -75,13 +75,19 @@ struct alignas(16) Kv4AttnShared {
   uint64_t full[kKv4MaxWarps][kKv4Stages];
 };
 constexpr int kKv4Ring = (sizeof(Kv4AttnShared) + 127) / 128 * 128;  // byte offset of the warps' rings
-constexpr int kv4_attn_smem(int warps) { return kKv4Ring + warps * kKv4Stages * kKv4TileBytes; }
+constexpr int kv4_attn_smem(int warps, int stages) { return kKv4Ring + warps * stages * kKv4TileBytes; }
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                               uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16_16816_zero(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                   uint32_t b0, uint32_t b1) {  // the same from zero
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
   uint32_t d;
@@ -143,6 +149,12 @@ __device__ __forceinline__ Kv4Span kv4_span(int n_valid, int n_prefix, int n_key
 template <typename Pick>
 __device__ __forceinline__ void kv4_share(const Kv4AttnParams& p, int n_keys, int lane, Pick pick, int& b, int& first,
                                           int& count) {
+  if (p.B == 1) {  // nothing to share, so nothing to wait for
+    b = pick(0, 0, p.parts) ? 0 : -1;
+    first = 0;
+    count = p.parts;
+    return;
+  }
   auto tiles_of = [&](int r) { return r < p.B ? kv4_span(__ldg(p.n_valid + r), p.n_prefix, n_keys).n : 0; };
   int n = tiles_of(lane);
   float total = (float)__reduce_add_sync(0xffffffffu, (unsigned)n);
@@ -175,12 +187,17 @@ __device__ __forceinline__ void kv4_share(const Kv4AttnParams& p, int n_keys, in
   }
 }
 
-// A warp's running softmax over its tiles, for the heads 2 t and 2 t + 1 of
-// lane (g, t). Without a bias the scores are in log2 units; with one they stay
-// in natural units, where a bias of the type's lowest value does not overflow.
+// A warp's running softmax over its tiles. The 8 columns of the products are
+// 8 independent softmaxes, lane (g, t) having columns 2 t and 2 t + 1:
+//   PAIR (up to 4 query heads per kv head): column 4 s + h is head h over the
+//         16-key halves s of the tiles, so no lane works on an empty column
+//         (480 -> 400 instructions a tile) and the two are merged at the end;
+//   else: column h is head h.
+// Without a bias the scores are in log2 units; with one they stay in natural
+// units, where a bias of the type's lowest value does not overflow.
 struct Kv4State {
   uint32_t qf[8][2];    // B fragments of q'
-  float qs[2][2];       // sum(q') per group and head
+  float qs[2][2];       // sum(q') per group and column
   float mul[2];
   float m[2], l[2], zs[2][2];  // running maximum, sum p, sum p * low per group
   float acc[8][4];             // sum (p s) code, times 2^-24 (rows g) or 2^-20 (rows g + 8)
@@ -188,33 +205,31 @@ struct Kv4State {
 };
 
 // One tile of 32 keys from shared memory. ALL: every key is attended.
-template <bool BIAS, bool ALL>
+template <bool BIAS, bool PAIR, bool ALL>
 __device__ __forceinline__ void kv4_tile(Kv4State& st, const uint8_t* tile, int j0, int n_keys, int nv, int n_prefix,
                                          const float* bias0, const float* bias1, int lane) {
+  constexpr int R = PAIR ? 2 : 4;  // key rows of a lane: row0 + 8 r
   const int g = lane >> 2, t = lane & 3;
-  uint2 vp[4];
-  float sc[8], bj[8];
-  bool row_ok[4];
+  const int row0 = PAIR ? 16 * (t >> 1) + g : g;
+  uint2 vp[R];
+  float sc[R][2], bj[R][2];
+  bool row_ok[R];
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int key = j0 + 8 * r + g;
+  for (int r = 0; r < R; ++r) {
+    const int key = j0 + row0 + 8 * r;
     row_ok[r] = ALL || (key < n_keys && (key < nv || key >= n_prefix));
     if (BIAS) {
       const bool has = row_ok[r] && key < n_prefix;
-      bj[2 * r] = has && bias0 != nullptr ? __ldg(bias0 + key) : 0.f;
-      bj[2 * r + 1] = has && bias1 != nullptr ? __ldg(bias1 + key) : 0.f;
+      bj[r][0] = has && bias0 != nullptr ? __ldg(bias0 + key) : 0.f;
+      bj[r][1] = has && bias1 != nullptr ? __ldg(bias1 + key) : 0.f;
     }
-    vp[r] = *reinterpret_cast<const uint2*>(tile + kKv4Vp + (8 * r + g) * 8);
+    vp[r] = *reinterpret_cast<const uint2*>(tile + kKv4Vp + (row0 + 8 * r) * 8);
     if (!row_ok[r]) vp[r] = make_uint2(0u, 0u);  // whatever a masked slot holds
   }
-  // ---- scores: sc[2 r + j] of key 8 r + g and head 2 t + j
+  // ---- q' . code of the two 16-key halves, by group
+  float c[2][2][4];
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
-    float c[2][4];
-#pragma unroll
-    for (int gr = 0; gr < 2; ++gr)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) c[gr][e] = 0.f;
     const uint4 x0 = *reinterpret_cast<const uint4*>(tile + (16 * s + g) * 64 + t * 16);
     const uint4 x1 = *reinterpret_cast<const uint4*>(tile + (16 * s + 8 + g) * 64 + t * 16);
     const uint32_t w0[4] = {x0.x, x0.y, x0.z, x0.w}, w1[4] = {x1.x, x1.y, x1.z, x1.w};
@@ -223,43 +238,52 @@ __device__ __forceinline__ void kv4_tile(Kv4State& st, const uint8_t* tile, int 
       uint32_t a[4], d[4];
       kv4_unpack(w0[i], a);
       kv4_unpack(w1[i], d);
-      mma_f16_16816(c[i >> 1], a[0], d[0], a[1], d[1], st.qf[2 * i][0], st.qf[2 * i][1]);
-      mma_f16_16816(c[i >> 1], a[2], d[2], a[3], d[3], st.qf[2 * i + 1][0], st.qf[2 * i + 1][1]);
+      if ((i & 1) == 0)
+        mma_f16_16816_zero(c[s][i >> 1], a[0], d[0], a[1], d[1], st.qf[2 * i][0], st.qf[2 * i][1]);
+      else
+        mma_f16_16816(c[s][i >> 1], a[0], d[0], a[1], d[1], st.qf[2 * i][0], st.qf[2 * i][1]);
+      mma_f16_16816(c[s][i >> 1], a[2], d[2], a[3], d[3], st.qf[2 * i + 1][0], st.qf[2 * i + 1][1]);
     }
+  }
+  // ---- scores
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = 2 * s + h;
-      const uint2 kp = *reinterpret_cast<const uint2*>(tile + kKv4Kp + (8 * r + g) * 8);
-      const float s0 = kv4_scale(kp.x) * 16777216.f, s1 = kv4_scale(kp.y) * 16777216.f;  // 2^24: the codes' units
-      const float z0 = kv4_low(kp.x), z1 = kv4_low(kp.y);
+  for (int r = 0; r < R; ++r) {
+    const uint2 kp = *reinterpret_cast<const uint2*>(tile + kKv4Kp + (row0 + 8 * r) * 8);
+    const float s0 = kv4_scale(kp.x) * 16777216.f, s1 = kv4_scale(kp.y) * 16777216.f;  // 2^24: the codes' units
+    const float z0 = kv4_low(kp.x), z1 = kv4_low(kp.y);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float v = z0 * st.qs[0][j];
-        v = fmaf(z1, st.qs[1][j], v);
-        v = fmaf(s0, c[0][2 * h + j], v);
-        v = fmaf(s1, c[1][2 * h + j], v);
-        v = BIAS ? fmaf(v, st.mul[j], bj[2 * r + j]) : v * st.mul[j];
-        // -inf in the bias is a mask, whatever the key holds
-        sc[2 * r + j] = !row_ok[r] || (BIAS && bj[2 * r + j] == -INFINITY) ? -INFINITY : v;
-      }
+    for (int j = 0; j < 2; ++j) {
+      const int e = 2 * (r & 1) + j;
+      const float c0 = PAIR ? (t < 2 ? c[0][0][e] : c[1][0][e]) : c[r >> 1][0][e];
+      const float c1 = PAIR ? (t < 2 ? c[0][1][e] : c[1][1][e]) : c[r >> 1][1][e];
+      float v = z0 * st.qs[0][j];
+      v = fmaf(z1, st.qs[1][j], v);
+      v = fmaf(s0, c0, v);
+      v = fmaf(s1, c1, v);
+      v = BIAS ? fmaf(v, st.mul[j], bj[r][j]) : v * st.mul[j];
+      // -inf in the bias is a mask, whatever the key holds
+      sc[r][j] = !row_ok[r] || (BIAS && bj[r][j] == -INFINITY) ? -INFINITY : v;
     }
   }
   // ---- move the running maximum / power of two when a score or a step outgrows them
-  float sn[8], smax = 0.f, top[2];
+  float sn[R][2], smax = 0.f, top[2];
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    sn[2 * r] = kv4_scale(vp[r].x) * st.einv;
-    sn[2 * r + 1] = kv4_scale(vp[r].y) * st.einv;
-    smax = fmax3(smax, sn[2 * r], sn[2 * r + 1]);
+  for (int r = 0; r < R; ++r) {
+    sn[r][0] = kv4_scale(vp[r].x) * st.einv;
+    sn[r][1] = kv4_scale(vp[r].y) * st.einv;
+    smax = fmax3(smax, sn[r][0], sn[r][1]);
   }
 #pragma unroll
-  for (int j = 0; j < 2; ++j) top[j] = fmaxf(fmax3(sc[j], sc[2 + j], sc[4 + j]), sc[6 + j]);
+  for (int j = 0; j < 2; ++j) {
+    top[j] = fmaxf(sc[0][j], sc[1][j]);
+    if (!PAIR) top[j] = fmax3(top[j], sc[R - 2][j], sc[R - 1][j]);
+  }
   constexpr float kLag = BIAS ? 4.f : 4.f * kLog2e;
   const bool grow = top[0] > st.m[0] + kLag || top[1] > st.m[1] + kLag || smax > 16.f;
   if (__any_sync(0xffffffffu, grow)) {
     float sraw = 0.f;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) sraw = fmax3(sraw, kv4_scale(vp[r].x), kv4_scale(vp[r].y));
+    for (int r = 0; r < R; ++r) sraw = fmax3(sraw, kv4_scale(vp[r].x), kv4_scale(vp[r].y));
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) sraw = fmaxf(sraw, __shfl_xor_sync(0xffffffffu, sraw, off));
     // a power of two above the largest step, at most 2^126
@@ -283,52 +307,52 @@ __device__ __forceinline__ void kv4_tile(Kv4State& st, const uint8_t* tile, int 
 #pragma unroll
       for (int e = 0; e < 4; ++e) st.acc[w][e] *= al[e & 1] * beta;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      sn[2 * r] = kv4_scale(vp[r].x) * st.einv;
-      sn[2 * r + 1] = kv4_scale(vp[r].y) * st.einv;
+    for (int r = 0; r < R; ++r) {
+      sn[r][0] = kv4_scale(vp[r].x) * st.einv;
+      sn[r][1] = kv4_scale(vp[r].y) * st.einv;
     }
   }
-  // ---- p, its sums, and P V
+  // ---- p and its sums; p s as B fragments (two key rows to a register)
   const float off[2] = {kKv4Head - st.m[0], kKv4Head - st.m[1]};
+  uint32_t pf[2][R];
 #pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    uint32_t pf[2][2];  // B fragments per group
+  for (int r = 0; r < R; ++r) {
+    float p[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = 2 * s + h;
-      float p[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float v = sc[2 * r + j];
-        const float e = BIAS ? ex2_approx(fmaf(v - st.m[j], kLog2e, kKv4Head)) : ex2_approx(v + off[j]);
-        p[j] = (BIAS || !ALL) && v == -INFINITY ? 0.f : e;
-        st.l[j] += p[j];
-      }
-#pragma unroll
-      for (int gr = 0; gr < 2; ++gr) {
-        const float z = kv4_low(gr ? vp[r].y : vp[r].x), sg = sn[2 * r + gr];
-        float u0 = p[0] * sg, u1 = p[1] * sg;
-        if (BIAS) {  // a masked key may hold NaN
-          st.zs[gr][0] = p[0] == 0.f ? st.zs[gr][0] : fmaf(p[0], z, st.zs[gr][0]);
-          u0 = p[0] == 0.f ? 0.f : u0;
-          st.zs[gr][1] = p[1] == 0.f ? st.zs[gr][1] : fmaf(p[1], z, st.zs[gr][1]);
-          u1 = p[1] == 0.f ? 0.f : u1;
-        } else {
-          st.zs[gr][0] = fmaf(p[0], z, st.zs[gr][0]);
-          st.zs[gr][1] = fmaf(p[1], z, st.zs[gr][1]);
-        }
-        pf[gr][h] = movmatrix_trans(h2_bits(__floats2half2_rn(u0, u1)));
-      }
+    for (int j = 0; j < 2; ++j) {
+      const float v = sc[r][j];
+      const float e = BIAS ? ex2_approx(fmaf(v - st.m[j], kLog2e, kKv4Head)) : ex2_approx(v + off[j]);
+      p[j] = (BIAS || !ALL) && v == -INFINITY ? 0.f : e;
+      st.l[j] += p[j];
     }
 #pragma unroll
     for (int gr = 0; gr < 2; ++gr) {
+      const float z = kv4_low(gr ? vp[r].y : vp[r].x);
+      float u[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float zn = fmaf(p[j], z, st.zs[gr][j]);
+        u[j] = p[j] * sn[r][gr];
+        st.zs[gr][j] = BIAS && p[j] == 0.f ? st.zs[gr][j] : zn;  // a key that the bias masks may hold NaN
+        if (BIAS && p[j] == 0.f) u[j] = 0.f;
+      }
+      pf[gr][r] = movmatrix_trans(h2_bits(__floats2half2_rn(u[0], u[1])));
+    }
+  }
+  // ---- P V
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const uint32_t own = (g >> 2) == s ? 0xFFFFFFFFu : 0u;  // PAIR: this half's columns
+#pragma unroll
+    for (int gr = 0; gr < 2; ++gr) {
+      const uint32_t b0 = PAIR ? pf[gr][0] & own : pf[gr][(2 * s) % R], b1 = PAIR ? pf[gr][1] & own : pf[gr][(2 * s + 1) % R];
       const uint4 x = *reinterpret_cast<const uint4*>(tile + kKv4V + s * 1024 + gr * 512 + lane * 16);
       const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint32_t a[4];
         kv4_unpack(w[i], a);
-        mma_f16_16816(st.acc[4 * gr + i], a[0], a[1], a[2], a[3], pf[gr][0], pf[gr][1]);
+        mma_f16_16816(st.acc[4 * gr + i], a[0], a[1], a[2], a[3], b0, b1);
       }
     }
   }
@@ -342,7 +366,7 @@ __device__ __forceinline__ void kv4_tile(Kv4State& st, const uint8_t* tile, int 
 // (parts + B, Hkv), C by kv4_share, through records that kv4_combine_kernel
 // merges (so every SM can take part: clusters of 16 leave a quarter of them
 // idle).
-template <bool BIAS>
+template <bool BIAS, bool PAIR>
 __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv4AttnParams p) {
   extern __shared__ __align__(128) uint8_t kv4_smem[];
   Kv4AttnShared& sh = *reinterpret_cast<Kv4AttnShared*>(kv4_smem);
@@ -351,7 +375,8 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
   const int g = lane >> 2, t = lane & 3;
   const int kvh = blockIdx.y;
   int b = blockIdx.z, C = gridDim.x, rank = blockIdx.x;
-  uint8_t* ring = kv4_smem + kKv4Ring + warp * kKv4Stages * kKv4TileBytes;
+  const int S = p.stages;
+  uint8_t* ring = kv4_smem + kKv4Ring + warp * S * kKv4TileBytes;
   const uint32_t ring_s = smem_u32(ring), full_s = smem_u32(sh.full[warp]);
   if (lane == 0) {
 #pragma unroll
@@ -391,13 +416,12 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
     const int v = v0 + warp + i * W;
     return v < span.na ? v : v - span.na + span.tb;
   };
-  auto fetch = [&](int i) {
-    const int s = i % kKv4Stages;
+  auto fetch = [&](int i, int s) {
     mbar_arrive_expect_tx(full_s + 8 * s, kKv4TileBytes);
     bulk_load(ring_s + s * kKv4TileBytes, base + (int64_t)tile_of(i) * kKv4TileBytes, kKv4TileBytes, full_s + 8 * s);
   };
   if (lane == 0)
-    for (int i = 0; i < min(mine, kKv4Stages); ++i) fetch(i);
+    for (int i = 0; i < min(mine, S); ++i) fetch(i, i);
 
   // the heads' q', scaled by a power of two
   for (int h = warp; h < 8; h += W) {
@@ -428,7 +452,7 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
   // MMA (i, 0): nibbles (0, 4), (1, 5) of word i; (i, 1): (2, 6), (3, 7)
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint4 x = *reinterpret_cast<const uint4*>(&sh.q[g][32 * i + 8 * t]);  // 8 dims
+    const uint4 x = *reinterpret_cast<const uint4*>(&sh.q[PAIR ? g & 3 : g][32 * i + 8 * t]);  // 8 dims
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -437,14 +461,15 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
       st.qf[2 * i + (u >> 1)][u & 1] = f;
     }
   }
+  const int h0 = PAIR ? 2 * (t & 1) : 2 * t;  // head of column 2 t
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    st.mul[j] = sh.mul[2 * t + j];
+    st.mul[j] = sh.mul[h0 + j];
     st.m[j] = -INFINITY;
     st.l[j] = st.zs[0][j] = st.zs[1][j] = 0.f;
 #pragma unroll
     for (int gr = 0; gr < 2; ++gr) {
-      const uint4 x = *reinterpret_cast<const uint4*>(&sh.q[2 * t + j][64 * gr + 8 * g]);
+      const uint4 x = *reinterpret_cast<const uint4*>(&sh.q[h0 + j][64 * gr + 8 * g]);
       const uint32_t w[4] = {x.x, x.y, x.z, x.w};
       float a = 0.f;
 #pragma unroll
@@ -463,9 +488,9 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
   st.einv = 8.507059173e37f;
   const float *bias0 = nullptr, *bias1 = nullptr;
   if (BIAS) {
-    const float* bp = p.bias + (int64_t)b * p.bias_sb + (int64_t)(kvh * p.G + 2 * t) * p.bias_sh;
-    if (2 * t < p.G) bias0 = bp;
-    if (2 * t + 1 < p.G) bias1 = bp + p.bias_sh;
+    const float* bp = p.bias + (int64_t)b * p.bias_sb + (int64_t)(kvh * p.G + h0) * p.bias_sh;
+    if (h0 < p.G) bias0 = bp;
+    if (h0 + 1 < p.G) bias1 = bp + p.bias_sh;
   }
 
   bool ok = true;
@@ -477,18 +502,18 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
     const int j0 = tile_of(i) * kKv4Keys;
     const uint8_t* tile = ring + s * kKv4TileBytes;
     if (j0 + kKv4Keys <= n_keys && (j0 + kKv4Keys <= nv || j0 >= p.n_prefix))
-      kv4_tile<BIAS, true>(st, tile, j0, n_keys, nv, p.n_prefix, bias0, bias1, lane);
+      kv4_tile<BIAS, PAIR, true>(st, tile, j0, n_keys, nv, p.n_prefix, bias0, bias1, lane);
     else
-      kv4_tile<BIAS, false>(st, tile, j0, n_keys, nv, p.n_prefix, bias0, bias1, lane);
+      kv4_tile<BIAS, PAIR, false>(st, tile, j0, n_keys, nv, p.n_prefix, bias0, bias1, lane);
     __syncwarp();
-    if (lane == 0 && i + kKv4Stages < mine) fetch(i + kKv4Stages);
-    if (++s == kKv4Stages) {
+    if (lane == 0 && i + S < mine) fetch(i + S, s);
+    if (++s == S) {
       s = 0;
       ph ^= 1;
     }
   }
   if (!ok)  // a copy never came: give those in flight their time before the shared memory goes
-    for (int s = 0; s < kKv4Stages; ++s) mbar_wait(full_s + 8 * s, 0, p.err, ERR_KV4);
+    for (int s = 0; s < S; ++s) mbar_wait(full_s + 8 * s, 0, p.err, ERR_KV4);
 
   // ---- merge the warps: their sums into the rings' memory
 #pragma unroll
@@ -516,16 +541,22 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
   const int slice = (p.G * 128 + C - 1) / C;
   for (int idx = threadIdx.x; idx < p.G * 128; idx += blockDim.x) {
     const int h = idx >> 7;
-    float mt = sh.m[0][h];
-    for (int w = 1; w < W; ++w) mt = fmaxf(mt, sh.m[w][h]);
+    constexpr int K = PAIR ? 2 : 1;  // columns of a head, 4 apart
+    float mt = -INFINITY;
+    for (int w = 0; w < W; ++w)
+#pragma unroll
+      for (int k = 0; k < K; ++k) mt = fmaxf(mt, sh.m[w][h + 4 * k]);
     float o = 0.f, lt = 0.f;
 #pragma unroll 4
     for (int w = 0; w < W; ++w) {
-      const float lw = sh.l[w][h], ow = all_o[w * (kKv4Stages * kKv4TileBytes / 4) + idx];
-      if (lw != 0.f) {  // 0: the warp saw no key (a NaN sum stays in)
-        const float f = ex2_approx((sh.m[w][h] - mt) * kUnit);
-        o = fmaf(f, ow, o);
-        lt = fmaf(f, lw, lt);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const float lw = sh.l[w][h + 4 * k], ow = all_o[w * (S * kKv4TileBytes / 4) + 512 * k + idx];
+        if (lw != 0.f) {  // 0: the column saw no key (a NaN sum stays in)
+          const float f = ex2_approx((sh.m[w][h + 4 * k] - mt) * kUnit);
+          o = fmaf(f, ow, o);
+          lt = fmaf(f, lw, lt);
+        }
       }
     }
     if (C == 1) {

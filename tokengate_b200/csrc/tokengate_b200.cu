@@ -1390,21 +1390,22 @@ int kv4_rows(const char* what, bool write, const void* k, int64_t k_sb, int64_t 
 // Warps of a block, and the blocks: of a cluster per kv head and row, or (parts
 // > 0) the blocks per kv head that the rows share.
 struct Kv4Shape {
-  int warps, cluster, parts;
+  int warps, stages, cluster, parts;
 };
 Kv4Shape kv4_shape(int B, int Hkv, int n_keys) {
   const int64_t rows = (int64_t)B * Hkv, tiles = kv4_tiles(n_keys);
   const int sms = sm_count();
-  Kv4Shape s = {tg::kKv4MaxWarps, 1, 0};
+  Kv4Shape s = {tg::kKv4MaxWarps, 2, 1, 0};
   if (tiles <= 192 && rows * 2 <= sms) {
     // short caches, where a second launch costs more than idle SMs
     while (s.cluster < 8 && rows * s.cluster * 2 <= sms && tiles > s.cluster) s.cluster *= 2;
     const int64_t per = (tiles + s.cluster - 1) / s.cluster;
     if (per < s.warps) s.warps = (int)per;
   } else if (rows * 2 <= sms) {
-    s.parts = sms / Hkv;          // one block of 12 warps per SM
+    s.parts = sms / Hkv;          // one block of 16 warps per SM (16 rows of 131081: 55 us, 12 warps of 3 tiles 57)
   } else {
-    s.warps = 4;                  // many rows: three blocks of 4 warps per SM
+    s.warps = 4;                  // many rows: three blocks of 4 warps per SM, and with fewer warps more tiles in flight
+    s.stages = 3;
     s.parts = 3 * sms / Hkv > 0 ? 3 * sms / Hkv : 1;
   }
   return s;
@@ -1412,7 +1413,7 @@ Kv4Shape kv4_shape(int B, int Hkv, int n_keys) {
 size_t kv4_part_bytes(int B, int Hq, const Kv4Shape& s) {
   return s.parts == 0 ? 0 : (size_t)Hq * (s.parts + B) * tg::kKv4Part * sizeof(float);
 }
-bool g_kv4_attr_set[2][kMaxDevices] = {};
+bool g_kv4_attr_set[4][kMaxDevices] = {};
 }  // namespace
 
 int tg_kv4_cache_bytes(int B, int Hkv, int64_t capacity, size_t* bytes) {
@@ -1550,17 +1551,20 @@ int tg_decode_attn_kv4(const void* q, int64_t q_sb, int64_t q_sh, const float* q
   }
   p.part = need > 0 ? static_cast<float*>(workspace) : nullptr;
   p.parts = shape.parts;
+  p.stages = shape.stages;
   p.B = B;
   p.Hq = Hq;
-  auto kern = bias != nullptr ? tg::kv4_attn_kernel<true> : tg::kv4_attn_kernel<false>;
-  bool(&flags)[kMaxDevices] = g_kv4_attr_set[bias != nullptr];
+  const bool pair = p.G <= 4;
+  auto kern = bias != nullptr ? (pair ? tg::kv4_attn_kernel<true, true> : tg::kv4_attn_kernel<true, false>)
+                              : (pair ? tg::kv4_attn_kernel<false, true> : tg::kv4_attn_kernel<false, false>);
+  bool(&flags)[kMaxDevices] = g_kv4_attr_set[2 * (bias != nullptr) + pair];
   cudaError_t e = cudaSuccess;
   if (!flags[dev]) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e == cudaSuccess) e = smem_limit_once(kern, tg::kv4_attn_smem(tg::kKv4MaxWarps), flags, dev);
+  if (e == cudaSuccess) e = smem_limit_once(kern, tg::kv4_attn_smem(tg::kKv4MaxWarps, 2), flags, dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(decode_attn_kv4)");
   const dim3 grid((unsigned)(need > 0 ? shape.parts + B : shape.cluster), (unsigned)Hkv, (unsigned)(need > 0 ? 1 : B));
   const dim3 block(32u * shape.warps);
-  e = launch_cluster(kern, grid, block, tg::kv4_attn_smem(shape.warps), static_cast<cudaStream_t>(stream),
+  e = launch_cluster(kern, grid, block, tg::kv4_attn_smem(shape.warps, shape.stages), static_cast<cudaStream_t>(stream),
                      shape.cluster, p);
   if (e != cudaSuccess) return cuda_fail(e, "decode_attn_kv4 launch");
   if (need > 0) {

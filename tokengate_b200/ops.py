@@ -699,22 +699,40 @@ def gemv(x: torch.Tensor, w: torch.Tensor, swiglu: bool = False, out: Optional[t
 
 
 # ----------------------------------------------------------------- 4-bit KV cache
+# These wrappers run once per layer and decode step, where the host's time is
+# the step's: they ask each tensor for what they need once, and read the
+# current stream and device without making Python objects of them.
+def _on(name: str, t: torch.Tensor, dtype: torch.dtype, index: int) -> None:
+    """t is a CUDA tensor of `dtype` on device `index`."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != index:
+        _require_cuda(name, t, dtype)
+        raise ValueError(f"{name} must be on cuda:{index}, got {t.device}")
+
+
+def _launch(index: int, fn, *args) -> None:
+    """fn(*args, stream) on device `index`, on its current stream."""
+    if torch._C._cuda_getDevice() == index:
+        _lib.check_launch(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+    else:
+        with torch.cuda.device(index):
+            _lib.check_launch(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+
+
 def _kv4(cache: KV4Cache) -> KV4Cache:
     if not isinstance(cache, KV4Cache):
         raise TypeError(f"cache must be a KV4Cache, got {type(cache).__name__}")
     return cache
 
 
-def _kv4_rows(name: str, t: torch.Tensor, cache: KV4Cache, n: Optional[int] = None) -> None:
-    _require_cuda(name, t, torch.bfloat16)
-    if t.dim() != 4 or t.shape[0] != cache.batch or t.shape[2] != cache.n_kv_heads or t.shape[3] != 128 \
-            or (n is not None and t.shape[1] != n):
-        raise ValueError(f"{name} must be ({cache.batch}, {'S' if n is None else n}, {cache.n_kv_heads}, 128), "
-                         f"got {tuple(t.shape)}")
-    if t.stride(3) != 1:
+def _kv4_rows(name: str, t: torch.Tensor, c: KV4Cache, n: int) -> Tuple[int, int, int]:
+    """The batch, slot and head strides of a (B, n, Hkv, 128) tensor."""
+    _on(name, t, torch.bfloat16, c.index)
+    if t.shape != (c.batch, n, c.n_kv_heads, 128):
+        raise ValueError(f"{name} must be ({c.batch}, {n}, {c.n_kv_heads}, 128), got {tuple(t.shape)}")
+    sb, ss, sh, sd = t.stride()
+    if sd != 1:
         raise ValueError(f"{name} must have a contiguous last dim")
-    if t.device != cache.data.device:
-        raise ValueError(f"{name} and the cache must be on one device")
+    return sb, ss, sh
 
 
 def kv4_write(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, start: int = 0) -> None:
@@ -725,17 +743,15 @@ def kv4_write(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, start: int = 0)
     floor((x - low) / scale + 1/2); a group with a NaN or an infinity (or a range past fp32's
     largest) reads back as NaN."""
     c = _kv4(cache)
-    _kv4_rows("k", k, c)
-    _kv4_rows("v", v, c, k.shape[1])
-    start, S = int(start), k.shape[1]
+    if not isinstance(k, torch.Tensor) or k.dim() != 4:
+        raise ValueError("k must be a 4-D (B, S, Hkv, 128) tensor")
+    S = k.shape[1]
+    ks, vs = _kv4_rows("k", k, c, S), _kv4_rows("v", v, c, S)
     if start < 0 or start + S > c.capacity:
         raise ValueError(f"slots [{start}, {start + S}) are outside the cache's capacity {c.capacity}")
-    if S == 0:
-        return
-    with _device_ctx(k):
-        _lib.check_launch(_lib.lib().tg_kv4_write(
-            k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], c.batch, c.n_kv_heads, 128, start, S,
-            c.data.data_ptr(), c.capacity, _stream(k)))
+    if S:
+        _launch(c.index, _lib.lib().tg_kv4_write, k.data_ptr(), *ks, v.data_ptr(), *vs, c.batch, c.n_kv_heads, 128,
+                start, S, c.ptr, c.capacity)
 
 
 def kv4_read(cache: KV4Cache, start: int = 0, n: Optional[int] = None, k_out: Optional[torch.Tensor] = None,
@@ -744,24 +760,30 @@ def kv4_read(cache: KV4Cache, start: int = 0, n: Optional[int] = None, k_out: Op
     n None: up to the capacity. k_out / v_out: written instead of new tensors, any strides with a
     contiguous last dim, multiples of 8 elements."""
     c = _kv4(cache)
-    start = int(start)
-    n = c.capacity - start if n is None else int(n)
+    n = c.capacity - start if n is None else n
     if start < 0 or n < 0 or start + n > c.capacity:
         raise ValueError(f"slots [{start}, {start + n}) are outside the cache's capacity {c.capacity}")
-    outs = []
-    for name, t in (("k_out", k_out), ("v_out", v_out)):
-        if t is None:
-            t = torch.empty((c.batch, n, c.n_kv_heads, 128), dtype=torch.bfloat16, device=c.data.device)
-        else:
-            _kv4_rows(name, t, c, n)
-        outs.append(t)
-    k, v = outs
+    if k_out is None:
+        k_out = torch.empty((c.batch, n, c.n_kv_heads, 128), dtype=torch.bfloat16, device=c.data.device)
+    if v_out is None:
+        v_out = torch.empty_like(k_out, memory_format=torch.contiguous_format)
+    ks, vs = _kv4_rows("k_out", k_out, c, n), _kv4_rows("v_out", v_out, c, n)
     if n:
-        with _device_ctx(k):
-            _lib.check_launch(_lib.lib().tg_kv4_read(
-                c.data.data_ptr(), c.capacity, c.batch, c.n_kv_heads, 128, start, n, k.data_ptr(), *k.stride()[:3],
-                v.data_ptr(), *v.stride()[:3], _stream(k)))
-    return k, v
+        _launch(c.index, _lib.lib().tg_kv4_read, c.ptr, c.capacity, c.batch, c.n_kv_heads, 128, start, n,
+                k_out.data_ptr(), *ks, v_out.data_ptr(), *vs)
+    return k_out, v_out
+
+
+def _token_heads(name: str, t: torch.Tensor, B: int, heads: Optional[int], index: int) -> int:
+    """The row stride of a (B, 1, heads, 128) tensor with contiguous heads."""
+    _on(name, t, torch.bfloat16, index)
+    if t.dim() != 4 or t.shape[0] != B or t.shape[1] != 1 or t.shape[3] != 128 \
+            or (heads is not None and t.shape[2] != heads):
+        raise ValueError(f"{name} must be ({B}, 1, {'heads' if heads is None else heads}, 128), got {tuple(t.shape)}")
+    sb, _, sh, sd = t.stride()
+    if sd != 1 or (sh != 128 and t.shape[2] > 1):
+        raise ValueError(f"{name} must have contiguous heads")
+    return sb
 
 
 def qk_norm_rope_append_kv4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm_w: torch.Tensor,
@@ -774,43 +796,30 @@ def qk_norm_rope_append_kv4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q
     rotated in fp32 with one rounding to bf16; k and v are quantised into the slot and left unchanged.
     Returns the finished q, (B, 1, Hq, 128) contiguous (or q_out, which may be q)."""
     c = _kv4(cache)
-    dev = c.data.device
-    for nm, t in (("q", q), ("k", k), ("v", v)):
-        _require_cuda(nm, t, torch.bfloat16)
-        if t.dim() != 4 or t.shape[1] != 1 or t.shape[3] != 128 or t.stride(3) != 1 \
-                or (t.stride(2) != 128 and t.shape[2] > 1):
-            raise ValueError(f"{nm} must be (B, 1, heads, 128) with contiguous heads")
-    B, _, Hq, _ = q.shape
-    kv_shape = (c.batch, 1, c.n_kv_heads, 128)
-    if B != c.batch or k.shape != kv_shape or v.shape != kv_shape:
-        raise ValueError(f"k and v must be {kv_shape} and q have {c.batch} rows, got q {tuple(q.shape)} "
-                         f"k {tuple(k.shape)} v {tuple(v.shape)}")
+    B, dev = c.batch, c.index
+    ld_q = _token_heads("q", q, B, None, dev)
+    ld_k, ld_v = _token_heads("k", k, B, c.n_kv_heads, dev), _token_heads("v", v, B, c.n_kv_heads, dev)
     for nm, t in (("cos", cos), ("sin", sin)):
-        _require_cuda(nm, t, torch.bfloat16)
+        _on(nm, t, torch.bfloat16, dev)
         if t.shape != (B, 1, 128) or t.stride(2) != 1:
-            raise ValueError(f"{nm} must be (B, 1, 128) with a contiguous last dim")
-    if cos.stride(0) != sin.stride(0):
+            raise ValueError(f"{nm} must be ({B}, 1, 128) with a contiguous last dim")
+    ld_cs = cos.stride(0)
+    if sin.stride(0) != ld_cs:
         raise ValueError("cos and sin must share strides")
     for nm, t in (("q_norm_w", q_norm_w), ("k_norm_w", k_norm_w)):
-        _require_cuda(nm, t, torch.bfloat16)
-        if t.shape != (128,) or t.stride(0) != 1:
+        _on(nm, t, torch.bfloat16, dev)
+        if t.shape != (128,) or not t.is_contiguous():
             raise ValueError(f"{nm} must be a contiguous (128,) tensor")
-    _require_cuda("slot", slot, torch.int64)
+    _on("slot", slot, torch.int64, dev)
     if slot.numel() != 1:
         raise ValueError("slot must be an int64 (1,) tensor")
+    Hq = q.shape[2]
     if q_out is None:
-        q_out = torch.empty((B, 1, Hq, 128), dtype=torch.bfloat16, device=dev)
-    else:
-        _require_cuda("q_out", q_out, torch.bfloat16)
-        if q_out.shape != q.shape or q_out.stride(3) != 1 or (q_out.stride(2) != 128 and Hq > 1):
-            raise ValueError("q_out must have q's shape with contiguous heads")
-    if any(t.device != dev for t in (q, k, v, cos, sin, q_norm_w, k_norm_w, slot, q_out)):
-        raise ValueError("every tensor must be on the cache's device")
-    with _device_ctx(q):
-        _lib.check_launch(_lib.lib().tg_qk_norm_rope_append_kv4(
-            q.data_ptr(), q.stride(0), Hq, k.data_ptr(), k.stride(0), c.n_kv_heads, v.data_ptr(), v.stride(0), B,
-            q_norm_w.data_ptr(), k_norm_w.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.stride(0), 128, eps,
-            q_out.data_ptr(), q_out.stride(0), c.data.data_ptr(), c.capacity, slot.data_ptr(), _stream(q)))
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    ld_qo = _token_heads("q_out", q_out, B, Hq, dev)
+    _launch(dev, _lib.lib().tg_qk_norm_rope_append_kv4, q.data_ptr(), ld_q, Hq, k.data_ptr(), ld_k, c.n_kv_heads,
+            v.data_ptr(), ld_v, B, q_norm_w.data_ptr(), k_norm_w.data_ptr(), cos.data_ptr(), sin.data_ptr(), ld_cs,
+            128, eps, q_out.data_ptr(), ld_qo, c.ptr, c.capacity, slot.data_ptr())
     return q_out
 
 
@@ -829,68 +838,67 @@ def decode_attention_kv4(q: torch.Tensor, cache: KV4Cache, n_valid: torch.Tensor
     the place of k and v. q: (B, Hq, 128) bf16, Hq / Hkv from 1 to 8. A bias of -inf masks its key
     whatever the key holds; a row without any key gives zeros. Returns (B, Hq, 128) bf16."""
     c = _kv4(cache)
-    _require_cuda("q", q, torch.bfloat16)
-    if q.dim() != 3 or q.shape[0] != c.batch or q.shape[2] != 128 or q.stride(2) != 1:
-        raise ValueError(f"q must be ({c.batch}, Hq, 128) with a contiguous last dim, got {tuple(q.shape)}")
-    B, Hq, D = q.shape
-    dev = c.data.device
+    B, dev = c.batch, c.index
+    _on("q", q, torch.bfloat16, dev)
+    if q.dim() != 3 or q.shape[0] != B or q.shape[2] != 128:
+        raise ValueError(f"q must be ({B}, Hq, 128), got {tuple(q.shape)}")
+    Hq = q.shape[1]
+    q_sb, q_sh, q_sd = q.stride()
+    if q_sd != 1:
+        raise ValueError("q must have a contiguous last dim")
     if not 0 <= n_prefix <= n_keys <= c.capacity:
         raise ValueError(f"need 0 <= n_prefix ({n_prefix}) <= n_keys ({n_keys}) <= cache capacity ({c.capacity})")
-    _require_cuda("n_valid", n_valid, torch.int32)
+    _on("n_valid", n_valid, torch.int32, dev)
     if n_valid.numel() != B or not n_valid.is_contiguous():
         raise ValueError("n_valid must be a contiguous (B,) int32 tensor")
     if out is None:
-        out = torch.empty((B, Hq, D), dtype=torch.bfloat16, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        o_sb, o_sh = Hq * 128, 128
     else:
-        _require_cuda("out", out, torch.bfloat16)
+        _on("out", out, torch.bfloat16, dev)
         if out.shape != q.shape or out.stride(2) != 1:
             raise ValueError("out must have q's shape with a contiguous last dim")
-    bias_ptr, bsb, bsh = None, 0, 0
+        o_sb, o_sh = out.stride(0), out.stride(1)
+    bias_ptr = qs_ptr = nk_ptr = None
+    bsb = bsh = qsb = 0
     if bias is not None:
-        _require_cuda("bias", bias, torch.float32)
+        _on("bias", bias, torch.float32, dev)
         bb = bias
         while bb.dim() < 3:
             bb = bb.unsqueeze(0)
-        if bb.dim() != 3 or bb.shape[2] < n_prefix or (bb.stride(2) != 1 and bb.shape[2] > 1) \
-                or bb.shape[0] not in (1, B) or bb.shape[1] not in (1, Hq):
+        (b0, b1, b2), (s0, s1, s2) = bb.shape, bb.stride()
+        if b2 < n_prefix or (s2 != 1 and b2 > 1) or (b0 != 1 and b0 != B) or (b1 != 1 and b1 != Hq):
             raise ValueError(f"bias {tuple(bias.shape)} must broadcast to ({B}, {Hq}, >= {n_prefix}) "
                              "with a contiguous last dim")
-        bsb = 0 if bb.shape[0] == 1 else bb.stride(0)
-        bsh = 0 if bb.shape[1] == 1 else bb.stride(1)
+        bsb, bsh = 0 if b0 == 1 else s0, 0 if b1 == 1 else s1
         bias_ptr = bb.data_ptr()
-    qs_ptr, qsb = None, 0
     if q_scale is not None:
-        _require_cuda("q_scale", q_scale, torch.float32)
-        if q_scale.shape != (B, Hq) or q_scale.stride(1) != 1:
+        _on("q_scale", q_scale, torch.float32, dev)
+        if q_scale.shape != (B, Hq) or (q_scale.stride(1) != 1 and Hq > 1):
             raise ValueError(f"q_scale must be (B, Hq) = ({B}, {Hq}) with a contiguous last dim")
         qs_ptr, qsb = q_scale.data_ptr(), q_scale.stride(0)
-    nk_ptr = None
     if n_keys_dev is not None:
-        _require_cuda("n_keys_dev", n_keys_dev, torch.int32)
+        _on("n_keys_dev", n_keys_dev, torch.int32, dev)
         nk_ptr = n_keys_dev.data_ptr()
-    if any(t is not None and t.device != dev for t in (q, n_valid, out, bias, q_scale, n_keys_dev)):
-        raise ValueError("every tensor must be on the cache's device")
-    L = _lib.lib()
-    with _device_ctx(q):
-        nbytes = _kv4_workspace(B, Hq, c.n_kv_heads, n_keys)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        _lib.check_launch(L.tg_decode_attn_kv4(
-            q.data_ptr(), q.stride(0), q.stride(1), qs_ptr, qsb, c.data.data_ptr(), c.capacity,
-            bias_ptr, bsb, bsh, n_valid.data_ptr(), n_prefix, n_keys, nk_ptr,
-            out.data_ptr(), out.stride(0), out.stride(1), ws.data_ptr() if ws is not None else None, nbytes,
-            B, Hq, c.n_kv_heads, D, D ** -0.5 if softmax_scale is None else softmax_scale, _stream(q)))
+    ws, ws_ptr, nbytes = None, None, _kv4_workspace(B, Hq, c.n_kv_heads, n_keys)
+    if nbytes:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        ws_ptr = ws.data_ptr()
+    _launch(dev, _lib.lib().tg_decode_attn_kv4, q.data_ptr(), q_sb, q_sh, qs_ptr, qsb, c.ptr, c.capacity, bias_ptr,
+            bsb, bsh, n_valid.data_ptr(), n_prefix, n_keys, nk_ptr, out.data_ptr(), o_sb, o_sh, ws_ptr, nbytes, B, Hq,
+            c.n_kv_heads, 128, 128 ** -0.5 if softmax_scale is None else softmax_scale)
     return out
 
 
 # ----------------------------------------------------------------- sampling
-def _per_row(name: str, val, B: int, dtype: torch.dtype, device: torch.device) -> Optional[torch.Tensor]:
+def _per_row(name: str, val, B: int, dtype: torch.dtype, index: int) -> Optional[torch.Tensor]:
     if val is None:
         return None
     if not isinstance(val, torch.Tensor):
-        return torch.full((B,), val, dtype=dtype, device=device)
-    _require_cuda(name, val, dtype)
-    if val.shape != (B,) or not val.is_contiguous() or val.device != device:
-        raise ValueError(f"{name} must be a number or a contiguous ({B},) tensor on the logits' device")
+        return torch.full((B,), val, dtype=dtype, device=torch.device("cuda", index))
+    _on(name, val, dtype, index)
+    if val.shape != (B,) or not val.is_contiguous():
+        raise ValueError(f"{name} must be a number or a contiguous ({B},) tensor")
     return val
 
 
@@ -906,35 +914,28 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     likely as the largest; ties go to the lower index. The token is the first, by index, at which the
     running kept mass passes u times the whole. A NaN logit counts as -inf; a row of nothing else
     gives token 0 and logprob NaN. Returns (token int64 (B,), logprob fp32 (B,)), logprob under the
-    distribution sampled from. token / logprob: written instead of new tensors (logprob only if
-    given or allocated here)."""
-    if not isinstance(logits, torch.Tensor) or logits.dtype not in (torch.float32, torch.bfloat16):
+    distribution sampled from. token / logprob: written instead of new tensors."""
+    if not isinstance(logits, torch.Tensor) or (logits.dtype is not torch.float32 and logits.dtype is not torch.bfloat16):
         raise ValueError("logits must be an fp32 or bf16 tensor")
-    _require_cuda("logits", logits)
-    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
-        raise ValueError("logits must be (B, V) with a contiguous last dim")
+    dev = logits.get_device()
+    if dev < 0:
+        _require_cuda("logits", logits)
+    if logits.dim() != 2:
+        raise ValueError("logits must be (B, V)")
     B, V = logits.shape
-    dev = logits.device
+    ld, sd = logits.stride()
+    if sd != 1 and V > 1:
+        raise ValueError("logits must have a contiguous last dim")
     u = _per_row("u", u, B, torch.float32, dev)
-    if u is None:
-        raise ValueError("u: one uniform number per row is needed")
     t = _per_row("temperature", temperature, B, torch.float32, dev)
-    if t is None:
-        raise ValueError("temperature must be a number or a tensor")
+    if u is None or t is None:
+        raise ValueError("u and temperature must be a number or a tensor")
     k = _per_row("top_k", top_k, B, torch.int32, dev)
     p = _per_row("top_p", top_p, B, torch.float32, dev)
     m = _per_row("min_p", min_p, B, torch.float32, dev)
-    if token is None:
-        token = torch.empty(B, dtype=torch.int64, device=dev)
-    else:
-        _per_row("token", token, B, torch.int64, dev)
-    if logprob is None:
-        logprob = torch.empty(B, dtype=torch.float32, device=dev)
-    else:
-        _per_row("logprob", logprob, B, torch.float32, dev)
-    with _device_ctx(logits):
-        _lib.check_launch(_lib.lib().tg_sample(
-            logits.data_ptr(), 1 if logits.dtype == torch.bfloat16 else 0, logits.stride(0), B, V, u.data_ptr(),
-            t.data_ptr(), k.data_ptr() if k is not None else None, p.data_ptr() if p is not None else None,
-            m.data_ptr() if m is not None else None, token.data_ptr(), logprob.data_ptr(), _stream(logits)))
+    token = torch.empty_like(u, dtype=torch.int64) if token is None else _per_row("token", token, B, torch.int64, dev)
+    logprob = torch.empty_like(u) if logprob is None else _per_row("logprob", logprob, B, torch.float32, dev)
+    _launch(dev, _lib.lib().tg_sample, logits.data_ptr(), 1 if logits.dtype is torch.bfloat16 else 0, ld, B, V,
+            u.data_ptr(), t.data_ptr(), None if k is None else k.data_ptr(), None if p is None else p.data_ptr(),
+            None if m is None else m.data_ptr(), token.data_ptr(), logprob.data_ptr())
     return token, logprob
