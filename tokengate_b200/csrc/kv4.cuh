@@ -41,7 +41,7 @@ constexpr int kKv4Vp = 4352;
 
 struct Kv4Group {
   float low, inv;
-  uint32_t param;  // scale | low << 16
+  uint32_t param;  // scale | low << 16; a NaN scale above a low of 0 for a group that cannot be held
   bool bad;
 };
 
@@ -66,12 +66,15 @@ __device__ __forceinline__ uint32_t kv4_code_bits(float x, const Kv4Group& gp) {
   const float u = __fadd_rn(__fmul_rn(__fsub_rn(x, gp.low), gp.inv), 0.5f);
   return __float_as_uint(__fadd_rz(u, 8388608.f));
 }
+// the same for two values: 2^23 + codes, as bits
+__device__ __forceinline__ uint2 kv4_code_bits2(uint32_t pair, float neg_low, float inv) {
+  float2 v = make_float2(bf16_lo(pair), bf16_hi(pair));
+  v = __fmul2_rn(__fadd2_rn(v, make_float2(neg_low, neg_low)), make_float2(inv, inv));
+  v = __fadd2_rz(__fadd2_rn(v, make_float2(0.5f, 0.5f)), make_float2(8388608.f, 8388608.f));
+  return make_uint2(__float_as_uint(v.x), __float_as_uint(v.y));
+}
 constexpr uint32_t kKv4Bias8 = 0u - 0x4B000000u * 0x11111111u;  // minus the biases of 8 codes 4 bits apart
 constexpr uint32_t kKv4Bias4 = 0u - 0x4B000000u * 0x01010101u;  // of 4 codes 8 bits apart
-
-__device__ __forceinline__ float kv4_value(uint32_t code, uint32_t param) {
-  return fmaf((float)code, __uint_as_float(param << 16), __uint_as_float(param & 0xFFFF0000u));
-}
 
 // byte of a V key inside its 16-key block's words, and its fragment column t
 __device__ __forceinline__ int kv4_v_byte(int kb) { return ((kb & 1) << 1) | (kb >> 3); }
@@ -86,8 +89,8 @@ struct Kv4RowsParams {
   uint8_t* cache;              // (B, Hkv, tiles, 4608)
   int64_t c_sb, c_sh;          // cache strides (bytes)
   int start, count;            // slots [start, start + count)
-  int Hkv, blk0, n_blk;        // 16-key blocks that the slots touch, from block blk0
-  int64_t items;               // B * n_blk * 2 * Hkv
+  int Hkv, blk0;               // 16-key blocks that the slots touch start at block blk0
+  unsigned items;              // warps of a batch row: blocks * 2 * Hkv
 };
 
 // (max, -min) of 8 bf16 values, as a bf16 pair; NaN propagates
@@ -118,87 +121,112 @@ __device__ __forceinline__ __nv_bfloat162 shfl_xor_bf162(__nv_bfloat162 v, int o
 // 32-byte sectors. Consecutive warps take consecutive heads of the same keys
 // (adjacent in the source). Rows outside [start, start + count) are neither
 // read nor written; a word that mixes both is written byte by byte.
+// Bound by instructions before memory, so: the extrema of a lane's 8 rows are
+// reduced and scattered in one exchange (lane c % 8 ends up with row c % 8's,
+// 7 shuffles instead of 24) and a row's step and reciprocal are computed by that
+// lane alone; codes come two at a time (packed fp32). 22 instructions a value
+// (59 us for 32768 keys of 8 heads, 2.9 TB/s) became 8.
 __global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4RowsParams p) {
   griddep_wait();
   griddep_launch_dependents();
   const int lane = threadIdx.x & 31, c = lane & 15;
-  const int64_t n_warps = ((int64_t)gridDim.x * blockDim.x) >> 5;
-  for (int64_t item = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5; item < p.items; item += n_warps) {
-    const int h = (int)(item % p.Hkv);
-    int64_t rest = item / p.Hkv;
-    const int half = (int)(rest & 1);
-    rest >>= 1;
-    const int blk = p.blk0 + (int)(rest % p.n_blk);
-    const int64_t b = rest / p.n_blk;
-    const int t = 2 * half + (lane >> 4);
-    const __nv_bfloat16* kb = p.k + b * p.k_sb + (int64_t)h * p.k_sh + 8 * c;
-    const __nv_bfloat16* vb = p.v + b * p.v_sb + (int64_t)h * p.v_sh + 8 * c;
-    uint8_t* tile = p.cache + b * p.c_sb + (int64_t)h * p.c_sh + (int64_t)(blk >> 1) * kKv4TileBytes;
-    const int row0 = (blk & 1) * 16;
-    uint4 x[2][4];
-    bool in[4];
+  const unsigned item = blockIdx.x * 8u + (threadIdx.x >> 5);
+  if (item >= p.items) return;
+  const unsigned rest = item / (unsigned)p.Hkv;
+  const int h = (int)(item - rest * (unsigned)p.Hkv), blk = p.blk0 + (int)(rest >> 1);
+  const int t = 2 * (int)(rest & 1u) + (lane >> 4);
+  const int64_t b = blockIdx.y;
+  // row of key 2 t + {0, 8, 1, 9} in the source
+  const int r0 = blk * 16 + 2 * t - p.start;
+  const __nv_bfloat16* kb = p.k + b * p.k_sb + (int64_t)h * p.k_sh + (int64_t)r0 * p.k_ss + 8 * c;
+  const __nv_bfloat16* vb = p.v + b * p.v_sb + (int64_t)h * p.v_sh + (int64_t)r0 * p.v_ss + 8 * c;
+  uint8_t* tile = p.cache + b * p.c_sb + (int64_t)h * p.c_sh + (int64_t)(blk >> 1) * kKv4TileBytes;
+  const int row0 = (blk & 1) * 16 + 2 * t;
+  uint4 x[8];  // K then V
+  bool in[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t r = (int64_t)blk * 16 + 2 * t + (j >> 1) + 8 * (j & 1) - p.start;
-      in[j] = r >= 0 && r < p.count;
-      x[0][j] = x[1][j] = make_uint4(0u, 0u, 0u, 0u);
-      if (in[j]) {
-        x[0][j] = ld_nc_v4(reinterpret_cast<const uint4*>(kb + r * p.k_ss));
-        x[1][j] = ld_nc_v4(reinterpret_cast<const uint4*>(vb + r * p.v_ss));
-      }
+  for (int j = 0; j < 4; ++j) {
+    const int dr = (j >> 1) + 8 * (j & 1);
+    in[j] = (unsigned)(r0 + dr) < (unsigned)p.count;
+    x[j] = x[4 + j] = make_uint4(0u, 0u, 0u, 0u);
+    if (in[j]) {
+      x[j] = ld_nc_v4(reinterpret_cast<const uint4*>(kb + dr * p.k_ss));
+      x[4 + j] = ld_nc_v4(reinterpret_cast<const uint4*>(vb + dr * p.v_ss));
     }
-    uint32_t acc[8];  // V: byte j of word g = the code of key j at this lane's dim g
+  }
+  // ---- extrema of the 8 rows: rows split over the lanes as the lanes are merged
+  __nv_bfloat162 mm[8];
 #pragma unroll
-    for (int g = 0; g < 8; ++g) acc[g] = 0u;
+  for (int r = 0; r < 8; ++r) mm[r] = kv4_minmax8(x[r]);
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
+  for (int off = 4; off >= 1; off >>= 1) {
+    const bool up = (c & off) != 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        __nv_bfloat162 mm = kv4_minmax8(x[kv][j]);
-#pragma unroll
-        for (int off = 1; off <= 4; off <<= 1) mm = __hmax2_nan(mm, shfl_xor_bf162(mm, off));
-        const Kv4Group gp = kv4_group(__low2float(mm), __high2float(mm));
-        const uint32_t w[4] = {x[kv][j].x, x[kv][j].y, x[kv][j].z, x[kv][j].w};
-        const int row = row0 + 2 * t + (j >> 1) + 8 * (j & 1);
-        if (in[j] && (c & 7) == 0)
-          *reinterpret_cast<uint32_t*>(tile + (kv ? kKv4Vp : kKv4Kp) + row * 8 + (c >> 3) * 4) = gp.param;
-        if (kv == 0) {
-          uint32_t word = kKv4Bias8;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            word += kv4_code_bits(bf16_lo(w[e]), gp) << (8 * e);
-            word += kv4_code_bits(bf16_hi(w[e]), gp) << (8 * e + 4);
-          }
-          if (in[j])
-            *reinterpret_cast<uint32_t*>(tile + row * 64 + (c & 3) * 16 + (c >> 2) * 4) = gp.bad ? 0u : word;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t lo = kv4_code_bits(bf16_lo(w[e]), gp) - 0x4B000000u;
-            const uint32_t hi = kv4_code_bits(bf16_hi(w[e]), gp) - 0x4B000000u;
-            acc[2 * e] += gp.bad ? 0u : lo << (8 * j);
-            acc[2 * e + 1] += gp.bad ? 0u : hi << (8 * j);
-          }
-        }
-      }
+    for (int r = 0; r < off; ++r) {
+      const __nv_bfloat162 give = up ? mm[r] : mm[r + off], keep = up ? mm[r + off] : mm[r];
+      mm[r] = __hmax2_nan(keep, shfl_xor_bf162(give, off));
     }
-    // lanes c (even: low nibbles) and c + 1 (high nibbles) make the 8 words of
-    // their 16 dims: the even lane words g = 0..3, the odd one 4..7
-    const int odd = c & 1, wd = c >> 1;
-    uint8_t* vt = tile + kKv4V + (blk & 1) * 1024 + (wd >> 2) * 512 + t * 16 + (wd & 3) * 4;
+  }
+  const Kv4Group own = kv4_group(__low2float(mm[0]), __high2float(mm[0]));  // of row c % 8
+  {
+    const int j = c & 3, row = row0 + (j >> 1) + 8 * (j & 1);
+    if (j == 0 ? in[0] : j == 1 ? in[1] : j == 2 ? in[2] : in[3])
+      *reinterpret_cast<uint32_t*>(tile + ((c & 4) ? kKv4Vp : kKv4Kp) + row * 8 + (c >> 3) * 4) = own.param;
+  }
+  float neg_low[8], inv[8];
+  const bool any_bad = __any_sync(0xffffffffu, own.bad);
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const uint32_t give = odd ? acc[g] : acc[4 + g], mine = odd ? acc[4 + g] : acc[g];
-      const uint32_t got = __shfl_xor_sync(0xffffffffu, give, 1);
-      const uint32_t word = odd ? (mine << 4) | got : mine | (got << 4);
-      uint8_t* at = vt + (4 * odd + g) * 64;
-      if (in[0] && in[1] && in[2] && in[3]) {
-        *reinterpret_cast<uint32_t*>(at) = word;
-      } else {
+  for (int r = 0; r < 8; ++r) {
+    const int src = (lane & 24) | r;
+    neg_low[r] = -__shfl_sync(0xffffffffu, own.low, src);
+    inv[r] = __shfl_sync(0xffffffffu, own.inv, src);
+    if (any_bad && __shfl_sync(0xffffffffu, own.bad, src)) x[r] = make_uint4(0u, 0u, 0u, 0u);  // codes of 0
+  }
+  // ---- K: the lane's 8 codes are one word of the row
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (in[j]) at[j] = (uint8_t)(word >> (8 * j));
-      }
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+    uint32_t word = kKv4Bias8;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint2 n = kv4_code_bits2(w[e], neg_low[j], inv[j]);
+      word += n.x << (8 * e);
+      word += n.y << (8 * e + 4);
+    }
+    const int row = row0 + (j >> 1) + 8 * (j & 1);
+    if (in[j]) *reinterpret_cast<uint32_t*>(tile + row * 64 + (c & 3) * 16 + (c >> 2) * 4) = word;
+  }
+  // ---- V: byte j of word g = the code of key j at this lane's dim g
+  uint32_t acc[8];
+#pragma unroll
+  for (int g = 0; g < 8; ++g) acc[g] = kKv4Bias4;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t w[4] = {x[4 + j].x, x[4 + j].y, x[4 + j].z, x[4 + j].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint2 n = kv4_code_bits2(w[e], neg_low[4 + j], inv[4 + j]);
+      acc[2 * e] += n.x << (8 * j);
+      acc[2 * e + 1] += n.y << (8 * j);
+    }
+  }
+  // lanes c (even: low nibbles) and c + 1 (high nibbles) make the 8 words of
+  // their 16 dims: the even lane words g = 0..3, the odd one 4..7
+  const int odd = c & 1, wd = c >> 1;
+  uint8_t* vt = tile + kKv4V + (blk & 1) * 1024 + (wd >> 2) * 512 + t * 16 + (wd & 3) * 4;
+  const bool whole = in[0] && in[1] && in[2] && in[3];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const uint32_t give = odd ? acc[g] : acc[4 + g], mine = odd ? acc[4 + g] : acc[g];
+    const uint32_t got = __shfl_xor_sync(0xffffffffu, give, 1);
+    const uint32_t word = odd ? (mine << 4) | got : mine | (got << 4);
+    uint8_t* at = vt + (4 * odd + g) * 64;
+    if (whole) {
+      *reinterpret_cast<uint32_t*>(at) = word;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (in[j]) at[j] = (uint8_t)(word >> (8 * j));
     }
   }
 }
@@ -208,54 +236,60 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4RowsParams p) {
   griddep_wait();
   griddep_launch_dependents();
   const int lane = threadIdx.x & 31, c = lane & 15;
-  const int64_t n_warps = ((int64_t)gridDim.x * blockDim.x) >> 5;
-  for (int64_t item = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5; item < p.items; item += n_warps) {
-    const int h = (int)(item % p.Hkv);
-    int64_t rest = item / p.Hkv;
-    const int half = (int)(rest & 1);
-    rest >>= 1;
-    const int blk = p.blk0 + (int)(rest % p.n_blk);
-    const int64_t b = rest / p.n_blk;
-    const int t = 2 * half + (lane >> 4);
-    const uint8_t* tile = p.cache + b * p.c_sb + (int64_t)h * p.c_sh + (int64_t)(blk >> 1) * kKv4TileBytes;
-    const int row0 = (blk & 1) * 16;
-    const int odd = c & 1, wd = c >> 1;
-    uint32_t kw[4], kp[4], vp[4], vw[4];
+  const unsigned item = blockIdx.x * 8u + (threadIdx.x >> 5);
+  if (item >= p.items) return;
+  const unsigned rest = item / (unsigned)p.Hkv;
+  const int h = (int)(item - rest * (unsigned)p.Hkv), blk = p.blk0 + (int)(rest >> 1);
+  const int t = 2 * (int)(rest & 1u) + (lane >> 4);
+  const int64_t b = blockIdx.y;
+  const uint8_t* tile = p.cache + b * p.c_sb + (int64_t)h * p.c_sh + (int64_t)(blk >> 1) * kKv4TileBytes;
+  const int row0 = (blk & 1) * 16 + 2 * t;
+  const int odd = c & 1, wd = c >> 1;
+  uint32_t kw[4], kp[4], vp[4], vw[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {  // a tile is allocated whole: rows past the range are read, not returned
-      const int row = row0 + 2 * t + (j >> 1) + 8 * (j & 1);
-      kw[j] = *reinterpret_cast<const uint32_t*>(tile + row * 64 + (c & 3) * 16 + (c >> 2) * 4);
-      kp[j] = *reinterpret_cast<const uint32_t*>(tile + kKv4Kp + row * 8 + (c >> 3) * 4);
-      vp[j] = *reinterpret_cast<const uint32_t*>(tile + kKv4Vp + row * 8 + (c >> 3) * 4);
-      vw[j] = *reinterpret_cast<const uint32_t*>(tile + kKv4V + (blk & 1) * 1024 + (wd >> 2) * 512 +
-                                                 ((4 * odd + j) * 4 + t) * 16 + (wd & 3) * 4);
+  for (int j = 0; j < 4; ++j) {  // a tile is allocated whole: rows past the range are read, not returned
+    const int row = row0 + (j >> 1) + 8 * (j & 1);
+    kw[j] = *reinterpret_cast<const uint32_t*>(tile + row * 64 + (c & 3) * 16 + (c >> 2) * 4);
+    kp[j] = *reinterpret_cast<const uint32_t*>(tile + kKv4Kp + row * 8 + (c >> 3) * 4);
+    vp[j] = *reinterpret_cast<const uint32_t*>(tile + kKv4Vp + row * 8 + (c >> 3) * 4);
+    vw[j] = *reinterpret_cast<const uint32_t*>(tile + kKv4V + (blk & 1) * 1024 + (wd >> 2) * 512 +
+                                               ((4 * odd + j) * 4 + t) * 16 + (wd & 3) * 4);
+  }
+  uint32_t acc[8];  // byte j of word g = the code of key j at this lane's dim g
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    // my words are g' = 4 odd + g, the partner's the other four; I keep my nibble of all eight
+    const uint32_t got = __shfl_xor_sync(0xffffffffu, vw[g], 1);
+    const uint32_t a = odd ? got : vw[g], d = odd ? vw[g] : got;
+    acc[g] = (a >> (4 * odd)) & 0x0F0F0F0Fu;
+    acc[4 + g] = (d >> (4 * odd)) & 0x0F0F0F0Fu;
+  }
+  const int r0 = blk * 16 + 2 * t - p.start;
+  __nv_bfloat16* kb = p.k_out + b * p.k_sb + (int64_t)h * p.k_sh + (int64_t)r0 * p.k_ss + 8 * c;
+  __nv_bfloat16* vb = p.v_out + b * p.v_sb + (int64_t)h * p.v_sh + (int64_t)r0 * p.v_ss + 8 * c;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int dr = (j >> 1) + 8 * (j & 1);
+    if ((unsigned)(r0 + dr) >= (unsigned)p.count) continue;
+    const float ks = __uint_as_float(kp[j] << 16), kl = __uint_as_float(kp[j] & 0xFFFF0000u);
+    const float vs = __uint_as_float(vp[j] << 16), vl = __uint_as_float(vp[j] & 0xFFFF0000u);
+    const float2 ks2 = make_float2(ks, ks), kl2 = make_float2(kl, kl), vs2 = make_float2(vs, vs), vl2 = make_float2(vl, vl);
+    const uint32_t even = kw[j] & 0x0F0F0F0Fu, high = (kw[j] >> 4) & 0x0F0F0F0Fu;  // dims 2 e, 2 e + 1
+    uint32_t ok[4], ov[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      // prmt: bytes 0..3 of the codes, 4..7 of 0x4B000000 (7: the exponent, 4: zero)
+      float2 v = make_float2(__uint_as_float(__byte_perm(even, 0x4B000000u, 0x7440 + e)),
+                             __uint_as_float(__byte_perm(high, 0x4B000000u, 0x7440 + e)));
+      v = __ffma2_rn(__fadd2_rn(v, make_float2(-8388608.f, -8388608.f)), ks2, kl2);
+      ok[e] = pack_bf16x2(v.x, v.y);
+      v = make_float2(__uint_as_float(__byte_perm(acc[2 * e], 0x4B000000u, 0x7440 + j)),
+                      __uint_as_float(__byte_perm(acc[2 * e + 1], 0x4B000000u, 0x7440 + j)));
+      v = __ffma2_rn(__fadd2_rn(v, make_float2(-8388608.f, -8388608.f)), vs2, vl2);
+      ov[e] = pack_bf16x2(v.x, v.y);
     }
-    uint32_t acc[8];
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      // my words are g' = 4 odd + g, the partner's the other four; I keep my
-      // nibble of all eight
-      const uint32_t got = __shfl_xor_sync(0xffffffffu, vw[g], 1);
-      const uint32_t a = odd ? got : vw[g], d = odd ? vw[g] : got;
-      acc[g] = (a >> (4 * odd)) & 0x0F0F0F0Fu;
-      acc[4 + g] = (d >> (4 * odd)) & 0x0F0F0F0Fu;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t r = (int64_t)blk * 16 + 2 * t + (j >> 1) + 8 * (j & 1) - p.start;
-      if (r < 0 || r >= p.count) continue;
-      uint32_t ok[4], ov[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        ok[e] = pack_bf16x2(kv4_value((kw[j] >> (8 * e)) & 15u, kp[j]), kv4_value((kw[j] >> (8 * e + 4)) & 15u, kp[j]));
-        ov[e] = pack_bf16x2(kv4_value((acc[2 * e] >> (8 * j)) & 15u, vp[j]),
-                            kv4_value((acc[2 * e + 1] >> (8 * j)) & 15u, vp[j]));
-      }
-      *reinterpret_cast<uint4*>(p.k_out + b * p.k_sb + r * p.k_ss + (int64_t)h * p.k_sh + 8 * c) =
-          make_uint4(ok[0], ok[1], ok[2], ok[3]);
-      *reinterpret_cast<uint4*>(p.v_out + b * p.v_sb + r * p.v_ss + (int64_t)h * p.v_sh + 8 * c) =
-          make_uint4(ov[0], ov[1], ov[2], ov[3]);
-    }
+    *reinterpret_cast<uint4*>(kb + dr * p.k_ss) = make_uint4(ok[0], ok[1], ok[2], ok[3]);
+    *reinterpret_cast<uint4*>(vb + dr * p.v_ss) = make_uint4(ov[0], ov[1], ov[2], ov[3]);
   }
 }
 

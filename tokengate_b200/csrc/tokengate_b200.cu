@@ -1349,6 +1349,8 @@ int kv4_rows(const char* what, bool write, const void* k, int64_t k_sb, int64_t 
     return fail(TG_ERR_INVALID_ARGUMENT, "%s: slots [%lld, %lld) outside the capacity %lld", what, (long long)start,
                 (long long)(start + count), (long long)capacity);
   if (count == 0) return TG_OK;
+  if (((start + count + 15) / 16 - start / 16) * 2 * Hkv > (int64_t)UINT32_MAX)
+    return fail(TG_ERR_UNSUPPORTED, "%s: %lld slots of %d heads in one call", what, (long long)count, Hkv);
   if (k == nullptr || v == nullptr) return fail(TG_ERR_INVALID_ARGUMENT, "%s: k and v must be non-NULL", what);
   if (B == 1) k_sb = v_sb = 0;  // the strides of a dim of one are not used
   if (count == 1) k_ss = v_ss = 0;
@@ -1378,11 +1380,9 @@ int kv4_rows(const char* what, bool write, const void* k, int64_t k_sb, int64_t 
   p.count = (int)count;
   p.Hkv = Hkv;
   p.blk0 = (int)(start / 16);
-  p.n_blk = (int)((start + count + 15) / 16) - p.blk0;
-  p.items = (int64_t)B * p.n_blk * 2 * Hkv;
-  const int64_t blocks = resident_blocks((p.items + 7) / 8, 8);
-  cudaError_t e = launch_pdl(write ? tg::kv4_write_kernel : tg::kv4_read_kernel, dim3((unsigned)blocks), dim3(256), 0,
-                             static_cast<cudaStream_t>(stream), p);
+  p.items = (unsigned)(((start + count + 15) / 16 - p.blk0) * 2 * Hkv);
+  cudaError_t e = launch_pdl(write ? tg::kv4_write_kernel : tg::kv4_read_kernel,
+                             dim3((p.items + 7) / 8, (unsigned)B), dim3(256), 0, static_cast<cudaStream_t>(stream), p);
   if (e != cudaSuccess) return cuda_fail(e, what);
   return TG_OK;
 }
