@@ -1,4 +1,4 @@
-"""Gated generation: the prefill, then greedy decode over the gated KV cache.
+"""Gated generation: the prefill, then decode over the gated KV cache.
 
 Mirrors the reference's one generation implementation, generate_batch
 (tokengate/e2e_gate/decode/gate_decode.py:87-260), with its decode-side
@@ -26,6 +26,12 @@ contracts:
 Each decode step runs the fused layer ops (residual add + RMSNorm, one
 [q; k; v] projection, q/k RMSNorm + RoPE, the tg_decode_attn kernel over
 the cache, o projection, SwiGLU MLP) and the head.
+
+Beyond the reference, which decodes greedily over a bf16 cache: kv_bits=4
+keeps the decode cache in 4 bits (kv4.KV4Cache: 144 bytes per slot and KV
+head instead of 512; the prefill's K/V are quantised into it, the step's
+k and v as they are appended, and attention runs on the codes), and a
+Sampling draws the tokens (tg_sample) instead of the argmax.
 """
 import time
 from dataclasses import dataclass
@@ -35,6 +41,7 @@ import torch
 import torch.nn.functional as F
 
 from . import ops
+from .kv4 import KV4Cache
 from .layers import fused_weights
 from .prefill import prefill_batch_for_decode
 
@@ -49,6 +56,40 @@ class GateGenerateResult:
     prefill_s: float
     decode_s: float
     steps: int                  # decode steps run (batch-wide)
+    logprobs: Optional[List[List[float]]] = None  # of token_ids, under the distributions sampled from
+
+
+@dataclass
+class Sampling:
+    """How tokens are drawn (ops.sample_tokens): each setting one number, or one per request.
+
+    temperature <= 0 is greedy; top_k None or <= 0, top_p None or >= 1 and min_p None or <= 0 are
+    off. generator: a torch.Generator on the model's device for the uniform numbers (None: torch's
+    own). One number per request and step is drawn, all of them before the first step."""
+    temperature: Union[float, Sequence[float]] = 1.0
+    top_k: Union[None, int, Sequence[int]] = None
+    top_p: Union[None, float, Sequence[float]] = None
+    min_p: Union[None, float, Sequence[float]] = None
+    generator: Optional[torch.Generator] = None
+
+    def on(self, B: int, device) -> dict:
+        """The (B,) device tensors of the settings, as ops.sample_tokens takes them."""
+        out = {}
+        for name, dtype in (("temperature", torch.float32), ("top_k", torch.int32), ("top_p", torch.float32),
+                            ("min_p", torch.float32)):
+            val = getattr(self, name)
+            if val is None:
+                if name == "temperature":
+                    raise ValueError("temperature must be a number or one per request")
+                out[name] = None
+                continue
+            t = torch.as_tensor(val, dtype=dtype, device="cpu")
+            if t.dim() > 1 or (t.dim() == 1 and t.shape[0] != B):
+                raise ValueError(f"{name}: one value, or one for each of the {B} requests, got shape {tuple(t.shape)}")
+            if t.is_floating_point() and bool(torch.isnan(t).any()):
+                raise ValueError(f"{name} must not be NaN")
+            out[name] = t.expand(B).contiguous().to(device)
+        return out
 
 
 def _sync(device) -> None:
@@ -93,6 +134,20 @@ class _DecodeCache:
             self.width.append(W)
 
 
+class _DecodeCacheKV4:
+    """The same in 4 bits: the prefill's prefix quantised to the front, decode tokens appended after it."""
+
+    def __init__(self, cache, n_layers: int, extra: int):
+        self.kv, self.width = [], []
+        for i in range(n_layers):
+            k, v = cache.layers[i].k_tok, cache.layers[i].v_tok
+            B, W, Hkv, _ = k.shape
+            c = KV4Cache(B, W + extra, Hkv, device=k.device)
+            ops.kv4_write(c, k, v)
+            self.kv.append(c)
+            self.width.append(W)
+
+
 @torch.no_grad()
 def generate_batch(model, gate, prompt_ids_list: Sequence, article_starts: Sequence[int],
                    article_ends: Sequence[int], gate_layer: int, max_kept_prefill_tokens,
@@ -100,8 +155,9 @@ def generate_batch(model, gate, prompt_ids_list: Sequence, article_starts: Seque
                    phase2_form: bool = True, prune_below_gate: bool = False,
                    streamer=None, forced_tokens: Optional[torch.Tensor] = None,
                    logits_out: Optional[list] = None, use_graph: bool = True,
-                   use_gemv: bool = True) -> GateGenerateResult:
-    """Gated prefill + greedy decode of up to max_new_tokens tokens per row.
+                   use_gemv: bool = True, sampling: Optional[Sampling] = None,
+                   kv_bits: int = 16) -> GateGenerateResult:
+    """Gated prefill + decode of up to max_new_tokens tokens per row.
 
     forced_tokens: (B, max_new_tokens - 1) ids fed to the decode steps in
     place of the previous step's argmax (teacher forcing, to score a given
@@ -110,9 +166,14 @@ def generate_batch(model, gate, prompt_ids_list: Sequence, article_starts: Seque
     use_graph: replay the decode step as one CUDA graph after the first
     (eager) step — the state a step reads (token, position, append slot, key
     count) lives in device buffers the step itself advances; use_gemv: the
-    decode projections on the tg_gemv kernel (False: cuBLAS)."""
+    decode projections on the tg_gemv kernel (False: cuBLAS);
+    sampling: draw the tokens as it says (None: the argmax of each step) and
+    return their log-probabilities;
+    kv_bits: 16 for a bf16 decode cache, 4 for a 4-bit one."""
     if max_new_tokens < 1:
         raise ValueError("max_new_tokens must be positive")
+    if kv_bits not in (4, 16):
+        raise ValueError(f"kv_bits={kv_bits}: 16 (bf16) or 4")
     device = next(model.parameters()).device
     inner = model.model
     n_layers = len(inner.layers)
@@ -125,6 +186,13 @@ def generate_batch(model, gate, prompt_ids_list: Sequence, article_starts: Seque
     _sync(device)
     prefill_s = time.perf_counter() - t0
     B = first.shape[0]
+    lps = []
+    if sampling is not None:
+        draw = sampling.on(B, device)
+        u_all = torch.rand((max_new_tokens, B), dtype=torch.float32, device=device, generator=sampling.generator)
+        tok, lp = ops.sample_tokens(st["logits"], u_all[0], **draw)
+        first = tok.view(B, 1)
+        lps.append(lp)
     if streamer is not None:
         streamer.put(first.detach().cpu())
     gen = [first]
@@ -133,7 +201,7 @@ def generate_batch(model, gate, prompt_ids_list: Sequence, article_starts: Seque
     if max_new_tokens > 1:
         fw = fused_weights(model)
         lens = st["lens"]
-        dc = _DecodeCache(cache, n_layers, max_new_tokens - 1)
+        dc = (_DecodeCacheKV4 if kv_bits == 4 else _DecodeCache)(cache, n_layers, max_new_tokens - 1)
         del cache
         n_kept_dev = torch.tensor(n_kepts, dtype=torch.int32, device=device)
         valid_below = n_kept_dev if prune_below_gate else torch.tensor(lens, dtype=torch.int32, device=device)
@@ -173,6 +241,7 @@ def generate_batch(model, gate, prompt_ids_list: Sequence, article_starts: Seque
         rot = torch.stack((cos_t, sin_t), dim=2)                                                 # (B, extra, 2, D)
         qs_cur = torch.empty_like(qs_all[0]) if qs_all is not None else None
         lg_buf = torch.empty((B, model.lm_head.weight.shape[0]), dtype=torch.float32, device=device)
+        lp_buf = torch.empty(B, dtype=torch.float32, device=device)
 
         def step_body():
             h = inner.embed_tokens(cur)                                               # (B, 1, H)
@@ -187,24 +256,31 @@ def generate_batch(model, gate, prompt_ids_list: Sequence, article_starts: Seque
                 q = qkv[:, :, :nq]
                 k = qkv[:, :, nq:nq + nkv]
                 v = qkv[:, :, nq + nkv:]
-                ops.qk_norm_rope_append(q, k, v, lw.q_norm_w, lw.k_norm_w, cos, sin, lw.qk_eps,
-                                        dc.k[i], dc.v[i], slot_b if below else slot_2)
-                W = dc.width[i]
-                if below:
-                    a = ops.decode_attention(q[:, 0], dc.k[i], dc.v[i], valid_below, W, W + extra,
-                                             n_keys_dev=nk_b)
+                W, li = dc.width[i], i - gate_layer - 1
+                slot, nk = (slot_b, nk_b) if below else (slot_2, nk_2)
+                valid = valid_below if below else n_kept_dev
+                kw = dict(n_keys_dev=nk)
+                if not below:
+                    kw.update(bias=bias[li], q_scale=qs_cur[li] if qs_cur is not None else None)
+                if kv_bits == 4:
+                    q = ops.qk_norm_rope_append_kv4(q, k, v, lw.q_norm_w, lw.k_norm_w, cos, sin, lw.qk_eps,
+                                                    dc.kv[i], slot)
+                    a = ops.decode_attention_kv4(q[:, 0], dc.kv[i], valid, W, W + extra, **kw)
                 else:
-                    li = i - gate_layer - 1
-                    a = ops.decode_attention(q[:, 0], dc.k[i], dc.v[i], n_kept_dev, W, W + extra,
-                                             bias=bias[li], q_scale=qs_cur[li] if qs_cur is not None else None,
-                                             n_keys_dev=nk_2)
+                    ops.qk_norm_rope_append(q, k, v, lw.q_norm_w, lw.k_norm_w, cos, sin, lw.qk_eps,
+                                            dc.k[i], dc.v[i], slot)
+                    a = ops.decode_attention(q[:, 0], dc.k[i], dc.v[i], valid, W, W + extra, **kw)
                 o = _proj(a.view(B, 1, nq * D), lw.wo, gemv=use_gemv)
                 h, x2 = ops.add_rmsnorm(h, o, lw.post_w, lw.eps, h_out=h)
                 delta = _proj(_proj(x2, lw.wgu, swiglu=True, gemv=use_gemv), lw.wdown, gemv=use_gemv)
             _, hn = ops.add_rmsnorm(h, delta, inner.norm.weight, float(inner.norm.variance_epsilon))
             lg = _proj(hn, model.lm_head.weight, gemv=use_gemv)[:, -1]
             lg_buf.copy_(lg)
-            cur.copy_(lg.argmax(-1, keepdim=True))
+            if sampling is not None:     # the step after step_idx draws with the next row of numbers
+                ops.sample_tokens(lg, u_all.index_select(0, step_idx + 1).view(B), token=cur.view(B), logprob=lp_buf,
+                                  **draw)
+            else:
+                cur.copy_(lg.argmax(-1, keepdim=True))
             ctr.add_(1)
             nkc.add_(1)
 
@@ -235,6 +311,8 @@ def generate_batch(model, gate, prompt_ids_list: Sequence, article_starts: Seque
             if streamer is not None:
                 streamer.put(nxt.detach().cpu())
             gen.append(nxt)
+            if sampling is not None:
+                lps.append(lp_buf.clone())
             steps += 1
         del graph
     _sync(device)
@@ -242,7 +320,9 @@ def generate_batch(model, gate, prompt_ids_list: Sequence, article_starts: Seque
     if streamer is not None:
         streamer.end()
     allg = torch.cat(gen, dim=1).cpu().tolist()
-    token_ids, n_gen = [], []
+    token_ids, n_gen, logprobs = [], [], None
+    if lps:
+        logprobs = torch.stack(lps, dim=1).cpu().tolist()
     for row in allg:
         if eos_token_id is not None and eos_token_id in row:
             end = row.index(eos_token_id)
@@ -251,4 +331,7 @@ def generate_batch(model, gate, prompt_ids_list: Sequence, article_starts: Seque
         else:
             token_ids.append(row)
             n_gen.append(len(row))
-    return GateGenerateResult(token_ids, n_gen, list(n_kepts), kept_pos, list(K_cl), prefill_s, decode_s, steps)
+    if logprobs is not None:
+        logprobs = [row[:len(t)] for row, t in zip(logprobs, token_ids)]
+    return GateGenerateResult(token_ids, n_gen, list(n_kepts), kept_pos, list(K_cl), prefill_s, decode_s, steps,
+                              logprobs)

@@ -8,7 +8,8 @@ helpers (tokengate/e2e_gate/gate_module/gate_forward.py:664-689):
   * generate runs the gated prefill on the B200 kernels and, for
     max_new_tokens > 1 (default 20, as the reference), greedy decoding over
     the gated KV cache (decode.generate_batch), returning a GenerateOutput
-    with the reference's fields;
+    with the reference's fields; a temperature samples the tokens instead,
+    and kv_bits=4 keeps the decode cache in 4 bits;
   * load_model takes a gate .pt, or a local run directory in which the
     newest-stage gate wins (swa_gate_*.pt > gate_final.pt > gate_step*.pt,
     tokengate/inference.py:38-59). Both gate kinds load: the linear
@@ -118,6 +119,7 @@ class GenerateOutput:
     prefill_s: float
     decode_s: float
     token_ids: List[List[int]]
+    logprobs: Optional[List[List[float]]] = None   # of token_ids, when they were sampled
 
 
 class TokenGateModel:
@@ -139,8 +141,9 @@ class TokenGateModel:
 
     def generate(self, ids: Union[List[int], List[List[int]]], tokenizer=None, *,
                  max_new_tokens: int = 20, max_kept_prefill_tokens: Optional[int] = None,
-                 streamer=None) -> GenerateOutput:
-        """Gated prefill + greedy decode (tokengate/inference.py:90-134).
+                 streamer=None, temperature=None, top_k=None, top_p=None, min_p=None,
+                 generator: Optional[torch.Generator] = None, kv_bits: int = 16) -> GenerateOutput:
+        """Gated prefill + decode (tokengate/inference.py:90-134), greedy unless a temperature is given.
 
         ids : one sequence or a batch (lists, int tensors or arrays), each with
             the state sentinels (ValueError otherwise).
@@ -150,7 +153,16 @@ class TokenGateModel:
         max_kept_prefill_tokens : K, the state tokens kept into the cache;
             None keeps all.
         streamer : optional put(cpu_ids (B, 1)) / end() receiver.
+        temperature, top_k, top_p, min_p : sample the tokens (decode.Sampling: a
+            number each, or one per sequence); temperature None: greedy, and
+            the others must be None too.
+        generator : a torch.Generator on the model's device for the sampling.
+        kv_bits : 16, or 4 for a decode cache in 4 bits.
         """
+        if temperature is None and not (top_k is None and top_p is None and min_p is None and generator is None):
+            raise ValueError("top_k, top_p, min_p and generator need a temperature")
+        if kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits={kv_bits}: 16 (bf16) or 4")
         if max_new_tokens < 1:
             raise ValueError("max_new_tokens must be positive")
         if torch.is_tensor(ids) or isinstance(ids, np.ndarray):
@@ -163,12 +175,14 @@ class TokenGateModel:
         starts = [s[1] for s in split]
         ends = [s[2] for s in split]
         k = _NO_PRUNING if max_kept_prefill_tokens is None else max_kept_prefill_tokens
-        if max_new_tokens > 1:
-            # gated prefill + greedy decode over the gated KV cache (decode.generate_batch)
-            from .decode import generate_batch
+        if max_new_tokens > 1 or temperature is not None:
+            # gated prefill + decode over the gated KV cache (decode.generate_batch)
+            from .decode import Sampling, generate_batch
+            sampling = None if temperature is None else Sampling(temperature, top_k, top_p, min_p, generator)
             eos = getattr(tokenizer, "eos_token_id", None) if tokenizer is not None else None
             r = generate_batch(self.model, self.gate, clean, starts, ends, self.gate_layer, k,
-                               max_new_tokens, eos_token_id=eos, streamer=streamer)
+                               max_new_tokens, eos_token_id=eos, streamer=streamer, sampling=sampling,
+                               kv_bits=kv_bits)
             answers = []
             for toks, n in zip(r.token_ids, r.n_gen):
                 answers.append(_strip_thinking(tokenizer.decode(toks[:n], skip_special_tokens=True))
@@ -177,7 +191,8 @@ class TokenGateModel:
             kept_pos = [kept_host[b, :n].tolist() for b, n in enumerate(r.n_kepts)]
             return GenerateOutput(answers=answers, n_kept=list(r.n_kepts),
                                   n_state=[e - s for s, e in zip(starts, ends)], kept_pos=kept_pos,
-                                  prefill_s=r.prefill_s, decode_s=r.decode_s, token_ids=r.token_ids)
+                                  prefill_s=r.prefill_s, decode_s=r.decode_s, token_ids=r.token_ids,
+                                  logprobs=r.logprobs)
         torch.cuda.synchronize(dev)
         t0 = time.perf_counter()
         first, _cache, kept, n_kepts, _kc = self.prefill(clean, starts, ends, k)

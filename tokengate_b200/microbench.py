@@ -11,6 +11,7 @@
     python -m tokengate_b200.microbench gemv [--n 12288] [--hidden 2048] [--batch 1]
     python -m tokengate_b200.microbench gemvchain [--layers 26] [--hidden 2048] [--inter 6144] [--batch 1]
     python -m tokengate_b200.microbench generate [--seq 32768] [--k 2000] [--batch 1] [--new 64] [--gate linear|e2e] [--proj gemv|cublas]
+                                                    [--kv-bits 16|4] [--temperature 0.8]
 
 Prints one JSON line per run with the CUDA-event time per launch and the
 algorithmic FLOPs or bytes of one launch (attention: 4*B*Hq*D*S(S+1)/2, also
@@ -23,7 +24,8 @@ written; decode: the K and V rows of the n_keys cached tokens + q, bias
 row and output, timed as 20 launches in one CUDA graph so the host launch
 path is not what is measured). generate: the gated generation of the
 Qwen3-1.7B-shape model (random init) — prefill seconds
-and decode milliseconds per token.
+and decode milliseconds per token, with the decode cache in bf16 or 4 bits
+and greedy or (a temperature above 0) sampled with top-k 50 and top-p 0.9.
 """
 import argparse
 import json
@@ -247,6 +249,8 @@ def main(argv=None):
     ap.add_argument("--new", type=int, default=64)
     ap.add_argument("--gate", default="linear", choices=("linear", "e2e"))
     ap.add_argument("--proj", default="gemv", choices=("gemv", "cublas"))
+    ap.add_argument("--kv-bits", type=int, default=16, choices=(16, 4))
+    ap.add_argument("--temperature", type=float, default=0.0)
     ap.add_argument("--inter", type=int, default=6144)
     ap.add_argument("--layers", type=int, default=26)
     ap.add_argument("--seq", type=int, default=32768)
@@ -360,8 +364,9 @@ def main(argv=None):
         res.update(layers=NL, hidden=H, inter=I, ms=ms, us_per_layer=ms * 1e3 / NL, mbytes=byts / 1e6,
                    gbs=byts / ms / 1e6, l2_resident_us_per_layer=ms_l2 * 1e3)
     elif a.kernel == "generate":
-        from .decode import generate_batch
+        from .decode import Sampling, generate_batch
         from .inference import load_model
+        sampling = Sampling(a.temperature, top_k=50, top_p=0.9) if a.temperature > 0 else None
         tm = load_model(base_model="qwen3-1.7b", gate_layer=1, gate_attn="b200", device=dev, seed=0,
                         gate="e2e" if a.gate == "e2e" else None)
         vocab = tm.model.config.vocab_size
@@ -369,11 +374,12 @@ def main(argv=None):
         prompts = [torch.randint(0, vocab, (S,), generator=gh) for _ in range(B)]
         st0, st1 = 512, S - 256
         run = lambda n: generate_batch(tm.model, tm.gate, prompts, [st0] * B, [st1] * B, 1, a.k, n,
-                                       use_gemv=a.proj == "gemv")
+                                       use_gemv=a.proj == "gemv", kv_bits=a.kv_bits, sampling=sampling)
         run(4)
         run(a.new)
         r = run(a.new)
-        res.update(seq=S, k=a.k, gate=a.gate, proj=a.proj, new=a.new, prefill_ms=r.prefill_s * 1e3,
+        res.update(seq=S, k=a.k, gate=a.gate, proj=a.proj, kv_bits=a.kv_bits, temperature=a.temperature,
+                   new=a.new, prefill_ms=r.prefill_s * 1e3,
                    decode_ms_per_token=r.decode_s * 1e3 / max(r.steps, 1),
                    decode_tokens_per_s=B * r.steps / r.decode_s if r.steps else None)
     elif a.kernel == "attn":

@@ -160,8 +160,8 @@ def prefill_batch_for_decode(model: torch.nn.Module, gate, prompt_ids_list: Sequ
     prefill (the reference reads the same values from the layers' bias /
     scale attributes, qwen3_flex_attention.py:978-1057): 'bias', one fp32
     (B, H|1, max_n_kept) Phase-2 key bias per layer above the gate;
-    'gamma', the (L', H) fp32 scaled-softmax gains or None; 'lens'. Fused
-    path only."""
+    'gamma', the (L', H) fp32 scaled-softmax gains or None; 'lens'; 'logits',
+    the (B, vocab) logits of the first token. Fused path only."""
     B = len(prompt_ids_list)
     if B < 1:
         raise ValueError("empty batch")
@@ -356,7 +356,10 @@ def prefill_batch_for_decode(model: torch.nn.Module, gate, prompt_ids_list: Sequ
         decode_state["lens"] = lens
 
     # ---- head
-    first_tokens = model.lm_head(hs_last).argmax(-1, keepdim=True)
+    logits = model.lm_head(hs_last)
+    first_tokens = logits.argmax(-1, keepdim=True)
+    if decode_state is not None:
+        decode_state["logits"] = logits
     if n_alloc != max_n_kept:
         for i in range(gate_layer + 1, n_layers):
             lc = cache.layers[i]
