@@ -92,23 +92,29 @@ __device__ __forceinline__ float smp_load(const __nv_bfloat16* p) { return smp_l
 // J.-M. Muller, "Correctly rounded multiplication by arbitrary precision
 // constants", 2008): x * high + RN(x * low) in one fma is within 2^-47 of the
 // quotient before its rounding, a division's cost without a division. Outside
-// the range in which the low part is a normal number, the division itself.
+// the range in which the low part is a normal number, and for rows whose
+// maximum is huge or infinite, the division itself.
 struct SmpRow {
   float xmax, zmax, t, rh, rl;
-  bool by_product;
-  __device__ __forceinline__ void set_t(float tt) {
+  bool plain;  // the usual row: a finite maximum, and quotients as products
+  __device__ __forceinline__ void set(float x, float tt) {
+    xmax = x;
     t = tt;
-    by_product = t > 8.6736174e-19f && t < 1.1529215e18f;  // 2^-60, 2^60
     rh = __frcp_rn(t);
     rl = __fdiv_rn(__fmaf_rn(-t, rh, 1.f), t);
+    plain = t > 8.6736174e-19f && t < 1.1529215e18f && fabsf(x) < 1e18f;  // 2^-60 < T < 2^60
+    zmax = plain ? product(x) : __fdiv_rn(x, t);
   }
-  __device__ __forceinline__ float over_t(float x) const {
-    return by_product ? __fmaf_rn(x, rh, __fmul_rn(x, rl)) : __fdiv_rn(x, t);
-  }
+  __device__ __forceinline__ float product(float x) const { return __fmaf_rn(x, rh, __fmul_rn(x, rl)); }
 };
 __device__ __forceinline__ float smp_d(float x, const SmpRow& r) {
-  const float d = __fsub_rn(r.over_t(x), r.zmax);
-  return x == r.xmax ? 0.f : d <= 0.f ? d : -INFINITY;  // NaN: both quotients overflowed
+  float d;
+  if (r.plain) {
+    d = __fsub_rn(r.product(x), r.zmax);
+  } else {
+    d = x == r.xmax ? 0.f : __fsub_rn(__fdiv_rn(x, r.t), r.zmax);
+  }
+  return d <= 0.f ? d : -INFINITY;  // NaN: a NaN logit, -inf times 0, or quotients that both overflowed
 }
 __device__ __forceinline__ int smp_bucket(float w) {
   return min(max((int)(0x3F7FFFFFu - __float_as_uint(w)) >> 18, 0), kSmpBuckets - 1);
@@ -128,10 +134,12 @@ __device__ __forceinline__ smp_u64 smp_mass(float w) {
   return smp_mass(hi, lo);
 }
 
+// sum over the warp: 24-bit pieces (32 of them stay below 2^32), one reduction instruction each
 __device__ __forceinline__ smp_u64 smp_warp_sum(smp_u64 v) {
-#pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-  return v;
+  const uint32_t a = __reduce_add_sync(0xffffffffu, (uint32_t)v & 0xFFFFFFu);
+  const uint32_t b = __reduce_add_sync(0xffffffffu, (uint32_t)(v >> 24) & 0xFFFFFFu);
+  const uint32_t c = __reduce_add_sync(0xffffffffu, (uint32_t)(v >> 48));
+  return a + ((smp_u64)b << 24) + ((smp_u64)c << 48);
 }
 __device__ __forceinline__ smp_u64 smp_warp_scan(smp_u64 v, int lane) {  // inclusive
 #pragma unroll
@@ -478,8 +486,8 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SamplePara
   for (int i = tid; i < kSmpAllLists; i += kSmpThreads) s.all[i] = 0u;
   if (tid == 0) s.n_list = 0u;
 
-  // ---- the largest logit; the range goes to shared memory as fp32
-  uint32_t best = 0;
+  // ---- the largest logit; the range goes to shared memory as fp32 (a NaN as it is: it gets no weight below)
+  float top = -INFINITY;
   {
     constexpr int VEC = 16 / sizeof(T);
     int done = 0;
@@ -494,14 +502,14 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SamplePara
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if (VEC == 4) {
-            f[e] = smp_logit(__uint_as_float(wd[e]));
+            f[e] = __uint_as_float(wd[e]);
           } else {
-            f[2 * e % VEC] = smp_logit(__uint_as_float(wd[e] << 16));
-            f[(2 * e + 1) % VEC] = smp_logit(__uint_as_float(wd[e] & 0xFFFF0000u));
+            f[2 * e % VEC] = __uint_as_float(wd[e] << 16);
+            f[(2 * e + 1) % VEC] = __uint_as_float(wd[e] & 0xFFFF0000u);
           }
         }
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) best = max(best, smp_key(f[e]));
+        for (int e = 0; e < VEC; e += 2) top = fmax3(top, f[e], f[e + 1]);
         if (HELD) {
 #pragma unroll
           for (int e = 0; e < VEC / 4; ++e)
@@ -514,9 +522,10 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SamplePara
     for (int i = done + tid; i < n; i += kSmpThreads) {
       const float v = smp_load(c.x + i);
       if (HELD) c.sw[i] = v;
-      best = max(best, smp_key(v));
+      top = fmaxf(top, v);
     }
   }
+  uint32_t best = smp_key(smp_logit(top));
   {
     smp_u64 z0 = 0, z1 = 0;
     uint32_t lo = 0, cnt;
@@ -524,24 +533,22 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SamplePara
     if (c.C > 1) cluster_wait();  // every block has started
     c.reduce(z0, z1, lo, best, cnt, nullptr);
   }
-  c.row.xmax = smp_unkey(best);
-  c.row.set_t(t);
-  c.row.zmax = c.row.over_t(c.row.xmax);
+  c.row.set(smp_unkey(best), t);
   uint32_t thr = 0;      // kept: logits above key `thr` (0: below every finite one), and the first `ties` at it,
   smp_u64 ties = 0;      // of weight >= min_p
   smp_u64 my = 0, my_ties = 0, before[2] = {0, 0}, kept = 0;  // this warp's kept mass, without ties; lower blocks'
 
   if (c.row.xmax == -INFINITY || top_k == 1u) {
     // nothing to choose from, or the lowest index of the largest logit
-    uint32_t first = 0xFFFFFFFFu, top = 0, cnt;
+    uint32_t first = 0xFFFFFFFFu, none = 0, cnt;
     for (int i = tid; i < n; i += kSmpThreads)
       if ((HELD ? c.sw[i] : smp_load(c.x + i)) == c.row.xmax) {
         first = i0 + i;
         break;
       }
-    c.reduce(my, my_ties, first, top, cnt, nullptr);
+    c.reduce(my, my_ties, first, none, cnt, nullptr);
     if (c.rank == 0 && tid == 0) {
-      p.token[b] = first;
+      p.token[b] = first == 0xFFFFFFFFu ? 0 : first;  // (NaN alone equals nothing)
       if (p.logprob != nullptr) p.logprob[b] = c.row.xmax == -INFINITY ? __uint_as_float(0x7FC00000u) : 0.f;
     }
     return;
