@@ -509,6 +509,23 @@ int tg_sample(const void* logits, int dtype, int64_t row_stride, int B, int V, c
               const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p, int64_t* token,
               float* logprob, void* stream);
 
+/*
+ * The entries of the 4-bit cache and of sampling with their arguments in one
+ * array, in the order of their declarations without the stream: integers,
+ * sizes and pointers as int64, floats as the bits of a double; the stream
+ * apart. For callers whose foreign-function interface charges by the argument
+ * (Python's ctypes: 0.1 us each, two fifths of such a call). n: the number of
+ * args, checked.
+ */
+typedef enum {
+  TG_CALL_KV4_WRITE = 0,
+  TG_CALL_KV4_READ = 1,
+  TG_CALL_QK_NORM_ROPE_APPEND_KV4 = 2,
+  TG_CALL_DECODE_ATTN_KV4 = 3,
+  TG_CALL_SAMPLE = 4
+} tg_call_entry;
+int tg_call(int entry, const int64_t* args, int n, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

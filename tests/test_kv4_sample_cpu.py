@@ -74,6 +74,38 @@ def test_sample_checks():
         assert call(**over) == st, over
 
 
+def test_packed_calls_are_the_calls():
+    """tg_call with the arguments in one array: the same checks, its own for the entry and the count, and
+    values outside an int's range refused instead of cut."""
+    import struct
+    L = _lib.lib()
+    names = ["tg_kv4_write", "tg_kv4_read", "tg_qk_norm_rope_append_kv4", "tg_decode_attn_kv4", "tg_sample"]
+    calls = [_lib.kv4_write, _lib.kv4_read, _lib.qk_norm_rope_append_kv4, _lib.decode_attn_kv4, _lib.sample]
+    floats = [[], [], [15], [23], []]
+    for e, (name, call) in enumerate(zip(names, calls)):
+        sig = _lib._SIGNATURES[name]
+        assert (call._entry, call._n) == (e, len(sig) - 1)
+        assert [i for i, t in enumerate(sig) if t is ctypes.c_float] == floats[e]
+        zeros = bytes(8 * call._n)
+        n = call._n
+        # empty sizes do nothing, all else of zeros is refused
+        assert L.tg_call(e, zeros, n, None) == (0 if name in ("tg_sample", "tg_qk_norm_rope_append_kv4") else BAD)
+        assert L.tg_call(e, zeros, n - 1, None) == BAD and b"takes" in L.tg_last_error()
+        assert L.tg_call(e, None, n, None) == BAD
+    assert L.tg_call(5, bytes(96), 12, None) == BAD and L.tg_call(-1, bytes(96), 12, None) == BAD
+    # logits dtype stride B V u t k p m token lp
+    ok = [4096, 1, 100, 2, 100, 64, 64, 0, 0, 0, 64, 0]
+    for i, v, st in ((3, 70000, BAD), (3, 2 ** 32 + 1, BAD), (4, 2 ** 33, BAD), (4, 2 ** 19 + 1, BAD), (0, 4097, ALIGN), (1, 2, BAD)):
+        a = list(ok)
+        a[i] = v
+        assert L.tg_call(4, struct.pack("<12q", *a), 12, None) == st, (i, v)
+    w = _write(D=64)[:-1]
+    assert L.tg_call(0, struct.pack("<15q", *w), 15, None) == NO
+    assert L.tg_call(0, struct.pack("<15q", *_write(start=4)[:-1]), 15, None) == BAD
+    a = [4096, 0, 128, 0, 0, 16384, 64, 0, 0, 0, 64, 5, 6, 0, 4096, 0, 128, 0, 0, 1, 4, 2, 128, float("nan")]
+    assert L.tg_call(3, struct.pack("<23qd", *a), 24, None) == BAD and b"softmax_scale" in L.tg_last_error()
+
+
 def test_no_cpu_path():
     with pytest.raises(ValueError, match="CUDA"):
         KV4Cache(1, 8, 2, device="cpu")

@@ -7,7 +7,10 @@ command, mirroring the reference loader's loud failure
 """
 import ctypes
 import os
+import struct
 import threading
+
+import torch
 
 from .build import LIB_PATH
 
@@ -111,6 +114,7 @@ _SIGNATURES = {
                            _P, ctypes.c_size_t, _I32, _I32, _I32, _I32, _F, _P],
     "tg_decode_attn_kv4_workspace": [_I32, _I32, _I32, _I32, ctypes.POINTER(ctypes.c_size_t)],
     "tg_sample": [_P, _I32, _I64, _I32, _I32, _P, _P, _P, _P, _P, _P, _P, _P],
+    "tg_call": [_I32, ctypes.c_char_p, _I32, _P],
 }
 EXPORTED = tuple(_SIGNATURES)
 
@@ -169,6 +173,36 @@ def check_launch(status: int) -> None:
     global LAUNCH_CALLS
     LAUNCH_CALLS += 1
     check(status)
+
+
+class Call:
+    """An entry of the library called through tg_call: its arguments (without the stream) packed into
+    one array, for the calls of a decode step, where ctypes' cost per argument would show. `fmt`: a
+    struct format of 8-byte items, q for integers and pointers (0 for NULL), d for floats."""
+
+    def __init__(self, entry: int, fmt: str):
+        self._entry, self._n = entry, len(fmt)
+        self._pack = struct.Struct("<" + fmt).pack
+
+    def __call__(self, index: int, *args) -> None:
+        """Launch on device `index`, on its current stream."""
+        global LAUNCH_CALLS
+        packed = self._pack(*args)
+        if torch._C._cuda_getDevice() == index:
+            status = lib().tg_call(self._entry, packed, self._n, torch._C._cuda_getCurrentRawStream(index))
+        else:
+            with torch.cuda.device(index):
+                status = lib().tg_call(self._entry, packed, self._n, torch._C._cuda_getCurrentRawStream(index))
+        LAUNCH_CALLS += 1
+        if status != TG_OK:
+            check(status)
+
+
+kv4_write = Call(0, "qqqqqqqqqqqqqqq")
+kv4_read = Call(1, "qqqqqqqqqqqqqqq")
+qk_norm_rope_append_kv4 = Call(2, "qqqqqqqqqqqqqqqdqqqqq")
+decode_attn_kv4 = Call(3, "qqqqqqqqqqqqqqqqqqqqqqqd")
+sample = Call(4, "qqqqqqqqqqqq")
 
 
 def device_error(stream_handle: int = 0, clear: bool = False) -> int:

@@ -1629,4 +1629,53 @@ int tg_sample(const void* logits, int dtype, int64_t row_stride, int B, int V, c
   return TG_OK;
 }
 
+// ---- the same with the arguments in one array
+namespace {
+struct CallArgs {
+  const int64_t* a;
+  void* ptr(int i) const { return reinterpret_cast<void*>(static_cast<uintptr_t>(a[i])); }
+  const float* fp(int i) const { return static_cast<const float*>(ptr(i)); }
+  const int32_t* ip(int i) const { return static_cast<const int32_t*>(ptr(i)); }
+  int i32(int i) const {  // out of an int's range: a value that every entry refuses
+    return a[i] < INT32_MIN || a[i] > INT32_MAX ? INT32_MIN : (int)a[i];
+  }
+  float f(int i) const {
+    double d;
+    memcpy(&d, a + i, sizeof(d));
+    return (float)d;
+  }
+};
+}  // namespace
+
+int tg_call(int entry, const int64_t* args, int n, void* stream) {
+  constexpr int kArgs[] = {15, 15, 21, 24, 12};
+  if (args == nullptr) return fail(TG_ERR_INVALID_ARGUMENT, "call: args must be non-NULL");
+  if (entry < 0 || entry >= (int)(sizeof(kArgs) / sizeof(kArgs[0])))
+    return fail(TG_ERR_INVALID_ARGUMENT, "call: no entry %d", entry);
+  if (n != kArgs[entry]) return fail(TG_ERR_INVALID_ARGUMENT, "call: entry %d takes %d args, got %d", entry, kArgs[entry], n);
+  const CallArgs c{args};
+  const int64_t* a = args;
+  switch (entry) {
+    case TG_CALL_KV4_WRITE:
+      return tg_kv4_write(c.ptr(0), a[1], a[2], a[3], c.ptr(4), a[5], a[6], a[7], c.i32(8), c.i32(9), c.i32(10), a[11],
+                          a[12], c.ptr(13), a[14], stream);
+    case TG_CALL_KV4_READ:
+      return tg_kv4_read(c.ptr(0), a[1], c.i32(2), c.i32(3), c.i32(4), a[5], a[6], c.ptr(7), a[8], a[9], a[10],
+                         c.ptr(11), a[12], a[13], a[14], stream);
+    case TG_CALL_QK_NORM_ROPE_APPEND_KV4:
+      return tg_qk_norm_rope_append_kv4(c.ptr(0), a[1], c.i32(2), c.ptr(3), a[4], c.i32(5), c.ptr(6), a[7], c.i32(8),
+                                        c.ptr(9), c.ptr(10), c.ptr(11), c.ptr(12), a[13], c.i32(14), c.f(15),
+                                        c.ptr(16), a[17], c.ptr(18), a[19], static_cast<const int64_t*>(c.ptr(20)), stream);
+    case TG_CALL_DECODE_ATTN_KV4:
+      return tg_decode_attn_kv4(c.ptr(0), a[1], a[2], c.fp(3), a[4], c.ptr(5), a[6],
+                                c.fp(7), a[8], a[9], c.ip(10), c.i32(11), c.i32(12),
+                                c.ip(13), c.ptr(14), a[15], a[16], c.ptr(17), (size_t)a[18], c.i32(19),
+                                c.i32(20), c.i32(21), c.i32(22), c.f(23), stream);
+    default:
+      return tg_sample(c.ptr(0), c.i32(1), a[2], c.i32(3), c.i32(4), c.fp(5), c.fp(6),
+                       c.ip(7), c.fp(8), c.fp(9), static_cast<int64_t*>(c.ptr(10)),
+                       static_cast<float*>(c.ptr(11)), stream);
+  }
+}
+
 }  // extern "C"

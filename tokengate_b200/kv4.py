@@ -17,7 +17,7 @@ TILE_BYTES = 4608
 class KV4Cache:
     """`capacity` slots of `batch` rows with `n_kv_heads` KV heads, on a CUDA device."""
 
-    __slots__ = ("data", "batch", "capacity", "n_kv_heads", "ptr", "index")
+    __slots__ = ("data", "batch", "capacity", "n_kv_heads", "ptr", "index", "bf16")
 
     def __init__(self, batch: int, capacity: int, n_kv_heads: int, device="cuda"):
         if batch < 1 or capacity < 1 or n_kv_heads < 1:
@@ -28,6 +28,7 @@ class KV4Cache:
         if not self.data.is_cuda:
             raise ValueError(f"a KV4Cache lives on a CUDA device (the B200 kernels have no CPU path), got {self.data.device}")
         self.ptr, self.index = self.data.data_ptr(), self.data.get_device()     # what every call asks for
+        self.bf16 = torch.empty(0, dtype=torch.bfloat16, device=self.data.device)   # makes the outputs (new_empty)
 
     @property
     def device(self) -> torch.device:

@@ -700,22 +700,13 @@ def gemv(x: torch.Tensor, w: torch.Tensor, swiglu: bool = False, out: Optional[t
 
 # ----------------------------------------------------------------- 4-bit KV cache
 # These wrappers run once per layer and decode step, where the host's time is
-# the step's: they ask each tensor for what they need once, and read the
-# current stream and device without making Python objects of them.
+# the step's: they ask each tensor for what they need once, and call the
+# library through one packed argument (_lib.Call).
 def _on(name: str, t: torch.Tensor, dtype: torch.dtype, index: int) -> None:
     """t is a CUDA tensor of `dtype` on device `index`."""
     if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != index:
         _require_cuda(name, t, dtype)
         raise ValueError(f"{name} must be on cuda:{index}, got {t.device}")
-
-
-def _launch(index: int, fn, *args) -> None:
-    """fn(*args, stream) on device `index`, on its current stream."""
-    if torch._C._cuda_getDevice() == index:
-        _lib.check_launch(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
-    else:
-        with torch.cuda.device(index):
-            _lib.check_launch(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
 
 
 def _kv4(cache: KV4Cache) -> KV4Cache:
@@ -750,8 +741,8 @@ def kv4_write(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, start: int = 0)
     if start < 0 or start + S > c.capacity:
         raise ValueError(f"slots [{start}, {start + S}) are outside the cache's capacity {c.capacity}")
     if S:
-        _launch(c.index, _lib.lib().tg_kv4_write, k.data_ptr(), *ks, v.data_ptr(), *vs, c.batch, c.n_kv_heads, 128,
-                start, S, c.ptr, c.capacity)
+        _lib.kv4_write(c.index, k.data_ptr(), *ks, v.data_ptr(), *vs, c.batch, c.n_kv_heads, 128, start, S, c.ptr,
+                       c.capacity)
 
 
 def kv4_read(cache: KV4Cache, start: int = 0, n: Optional[int] = None, k_out: Optional[torch.Tensor] = None,
@@ -763,14 +754,18 @@ def kv4_read(cache: KV4Cache, start: int = 0, n: Optional[int] = None, k_out: Op
     n = c.capacity - start if n is None else n
     if start < 0 or n < 0 or start + n > c.capacity:
         raise ValueError(f"slots [{start}, {start + n}) are outside the cache's capacity {c.capacity}")
-    if k_out is None:
-        k_out = torch.empty((c.batch, n, c.n_kv_heads, 128), dtype=torch.bfloat16, device=c.data.device)
-    if v_out is None:
-        v_out = torch.empty_like(k_out, memory_format=torch.contiguous_format)
-    ks, vs = _kv4_rows("k_out", k_out, c, n), _kv4_rows("v_out", v_out, c, n)
+    H = c.n_kv_heads
+    if k_out is None and v_out is None:
+        k_out = c.bf16.new_empty((c.batch, n, H, 128))
+        v_out = torch.empty_like(k_out)
+        ks = vs = (n * H * 128, H * 128, 128)
+    else:
+        k_out = c.bf16.new_empty((c.batch, n, H, 128)) if k_out is None else k_out
+        v_out = c.bf16.new_empty((c.batch, n, H, 128)) if v_out is None else v_out
+        ks, vs = _kv4_rows("k_out", k_out, c, n), _kv4_rows("v_out", v_out, c, n)
     if n:
-        _launch(c.index, _lib.lib().tg_kv4_read, c.ptr, c.capacity, c.batch, c.n_kv_heads, 128, start, n,
-                k_out.data_ptr(), *ks, v_out.data_ptr(), *vs)
+        _lib.kv4_read(c.index, c.ptr, c.capacity, c.batch, H, 128, start, n, k_out.data_ptr(), *ks, v_out.data_ptr(),
+                      *vs)
     return k_out, v_out
 
 
@@ -799,13 +794,14 @@ def qk_norm_rope_append_kv4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q
     B, dev = c.batch, c.index
     ld_q = _token_heads("q", q, B, None, dev)
     ld_k, ld_v = _token_heads("k", k, B, c.n_kv_heads, dev), _token_heads("v", v, B, c.n_kv_heads, dev)
+    row = (B, 1, 128)
     for nm, t in (("cos", cos), ("sin", sin)):
         _on(nm, t, torch.bfloat16, dev)
-        if t.shape != (B, 1, 128) or t.stride(2) != 1:
-            raise ValueError(f"{nm} must be ({B}, 1, 128) with a contiguous last dim")
-    ld_cs = cos.stride(0)
-    if sin.stride(0) != ld_cs:
-        raise ValueError("cos and sin must share strides")
+        if t.shape != row:
+            raise ValueError(f"{nm} must be ({B}, 1, 128), got {tuple(t.shape)}")
+    ld_cs, _, cd = cos.stride()
+    if cd != 1 or sin.stride() != cos.stride():
+        raise ValueError("cos and sin must share strides and have a contiguous last dim")
     for nm, t in (("q_norm_w", q_norm_w), ("k_norm_w", k_norm_w)):
         _on(nm, t, torch.bfloat16, dev)
         if t.shape != (128,) or not t.is_contiguous():
@@ -815,11 +811,12 @@ def qk_norm_rope_append_kv4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q
         raise ValueError("slot must be an int64 (1,) tensor")
     Hq = q.shape[2]
     if q_out is None:
-        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    ld_qo = _token_heads("q_out", q_out, B, Hq, dev)
-    _launch(dev, _lib.lib().tg_qk_norm_rope_append_kv4, q.data_ptr(), ld_q, Hq, k.data_ptr(), ld_k, c.n_kv_heads,
-            v.data_ptr(), ld_v, B, q_norm_w.data_ptr(), k_norm_w.data_ptr(), cos.data_ptr(), sin.data_ptr(), ld_cs,
-            128, eps, q_out.data_ptr(), ld_qo, c.ptr, c.capacity, slot.data_ptr())
+        q_out, ld_qo = c.bf16.new_empty((B, 1, Hq, 128)), Hq * 128
+    else:
+        ld_qo = _token_heads("q_out", q_out, B, Hq, dev)
+    _lib.qk_norm_rope_append_kv4(dev, q.data_ptr(), ld_q, Hq, k.data_ptr(), ld_k, c.n_kv_heads, v.data_ptr(), ld_v, B,
+                                 q_norm_w.data_ptr(), k_norm_w.data_ptr(), cos.data_ptr(), sin.data_ptr(), ld_cs, 128,
+                                 eps, q_out.data_ptr(), ld_qo, c.ptr, c.capacity, slot.data_ptr())
     return q_out
 
 
@@ -852,26 +849,24 @@ def decode_attention_kv4(q: torch.Tensor, cache: KV4Cache, n_valid: torch.Tensor
     if n_valid.numel() != B or not n_valid.is_contiguous():
         raise ValueError("n_valid must be a contiguous (B,) int32 tensor")
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        o_sb, o_sh = Hq * 128, 128
+        out, o_sb, o_sh = c.bf16.new_empty((B, Hq, 128)), Hq * 128, 128
     else:
         _on("out", out, torch.bfloat16, dev)
         if out.shape != q.shape or out.stride(2) != 1:
             raise ValueError("out must have q's shape with a contiguous last dim")
         o_sb, o_sh = out.stride(0), out.stride(1)
-    bias_ptr = qs_ptr = nk_ptr = None
-    bsb = bsh = qsb = 0
+    bias_ptr = qs_ptr = nk_ptr = bsb = bsh = qsb = 0
     if bias is not None:
         _on("bias", bias, torch.float32, dev)
-        bb = bias
-        while bb.dim() < 3:
-            bb = bb.unsqueeze(0)
-        (b0, b1, b2), (s0, s1, s2) = bb.shape, bb.stride()
+        shape, strides = (1, 1, *bias.shape)[-3:], (0, 0, *bias.stride())[-3:]
+        if bias.dim() > 3:
+            raise ValueError(f"bias {tuple(bias.shape)} must broadcast to ({B}, {Hq}, >= {n_prefix})")
+        (b0, b1, b2), (s0, s1, s2) = shape, strides
         if b2 < n_prefix or (s2 != 1 and b2 > 1) or (b0 != 1 and b0 != B) or (b1 != 1 and b1 != Hq):
             raise ValueError(f"bias {tuple(bias.shape)} must broadcast to ({B}, {Hq}, >= {n_prefix}) "
                              "with a contiguous last dim")
         bsb, bsh = 0 if b0 == 1 else s0, 0 if b1 == 1 else s1
-        bias_ptr = bb.data_ptr()
+        bias_ptr = bias.data_ptr()
     if q_scale is not None:
         _on("q_scale", q_scale, torch.float32, dev)
         if q_scale.shape != (B, Hq) or (q_scale.stride(1) != 1 and Hq > 1):
@@ -880,13 +875,13 @@ def decode_attention_kv4(q: torch.Tensor, cache: KV4Cache, n_valid: torch.Tensor
     if n_keys_dev is not None:
         _on("n_keys_dev", n_keys_dev, torch.int32, dev)
         nk_ptr = n_keys_dev.data_ptr()
-    ws, ws_ptr, nbytes = None, None, _kv4_workspace(B, Hq, c.n_kv_heads, n_keys)
+    ws, ws_ptr, nbytes = None, 0, _kv4_workspace(B, Hq, c.n_kv_heads, n_keys)
     if nbytes:
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        ws = c.data.new_empty(nbytes)
         ws_ptr = ws.data_ptr()
-    _launch(dev, _lib.lib().tg_decode_attn_kv4, q.data_ptr(), q_sb, q_sh, qs_ptr, qsb, c.ptr, c.capacity, bias_ptr,
-            bsb, bsh, n_valid.data_ptr(), n_prefix, n_keys, nk_ptr, out.data_ptr(), o_sb, o_sh, ws_ptr, nbytes, B, Hq,
-            c.n_kv_heads, 128, 128 ** -0.5 if softmax_scale is None else softmax_scale)
+    _lib.decode_attn_kv4(dev, q.data_ptr(), q_sb, q_sh, qs_ptr, qsb, c.ptr, c.capacity, bias_ptr, bsb, bsh,
+                         n_valid.data_ptr(), n_prefix, n_keys, nk_ptr, out.data_ptr(), o_sb, o_sh, ws_ptr, nbytes, B,
+                         Hq, c.n_kv_heads, 128, 128 ** -0.5 if softmax_scale is None else softmax_scale)
     return out
 
 
@@ -935,7 +930,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     m = _per_row("min_p", min_p, B, torch.float32, dev)
     token = torch.empty_like(u, dtype=torch.int64) if token is None else _per_row("token", token, B, torch.int64, dev)
     logprob = torch.empty_like(u) if logprob is None else _per_row("logprob", logprob, B, torch.float32, dev)
-    _launch(dev, _lib.lib().tg_sample, logits.data_ptr(), 1 if logits.dtype is torch.bfloat16 else 0, ld, B, V,
-            u.data_ptr(), t.data_ptr(), None if k is None else k.data_ptr(), None if p is None else p.data_ptr(),
-            None if m is None else m.data_ptr(), token.data_ptr(), logprob.data_ptr())
+    _lib.sample(dev, logits.data_ptr(), 1 if logits.dtype is torch.bfloat16 else 0, ld, B, V, u.data_ptr(),
+                t.data_ptr(), 0 if k is None else k.data_ptr(), 0 if p is None else p.data_ptr(),
+                0 if m is None else m.data_ptr(), token.data_ptr(), logprob.data_ptr())
     return token, logprob
