@@ -27,6 +27,9 @@
 //      highest bit in which the two differ (none for bf16 logits, whose buckets
 //      hold one or two values), every block on a copy of all lists, so without
 //      a cluster barrier (lists too long for that: over the row again).
+// Where no more than 256 logits reach down to the k-th's bucket, they go to one
+// block, which orders them by counting and finishes alone (one row of 151936,
+// k = 50, p = 0.9: 22 -> 14 us).
 // The threshold is a logit and a number of its ties, which go by index. Only
 // elements of the threshold's bucket are looked up in the row again. Blocks
 // write to one another's shared memory and read their own: a remote load costs
@@ -44,6 +47,7 @@ constexpr int kSmpWarps = kSmpThreads / 32;
 constexpr int kSmpBuckets = 1024;
 constexpr int kSmpList = 1024;      // logits of one bucket that a block can list
 constexpr int kSmpAllLists = 2048;  // and the cluster
+constexpr int kSmpFew = 256;        // logits that one block orders by counting
 constexpr int kSmpMaxCluster = 16;   // above 8: opt-in
 constexpr int kSmpMaxV = 1 << 19;
 constexpr double kSmpUnit = 1.0 / 17592186044416.0;  // 2^-44: a mass of 1
@@ -66,7 +70,13 @@ typedef unsigned long long smp_u64;
 struct alignas(16) SmpShared {
   uint32_t own[2][kSmpBuckets];   // this block's histograms (counts, masses); then lists of a bucket's logits, by turns
   uint32_t tot[2][kSmpBuckets];   // the row's histograms
-  uint32_t all[kSmpAllLists];     // this block's slices of the row's histograms; then the blocks' lists together
+  union {
+    uint32_t all[kSmpAllLists];   // this block's slices of the row's histograms; then the blocks' lists together
+    struct {                      // or, in block 0, the few logits down to the k-th's bucket
+      smp_u64 few_ord[kSmpFew];   // ordered logit above the index's complement: the order of the row, descending
+      smp_u64 few_mass[kSmpFew];
+    };
+  };
   uint32_t at[kSmpList];          // where in the block's range the listed logits are
   smp_u64 dig[2][256];            // digit histograms of a refinement, by pass parity
   smp_u64 xch[2][kSmpMaxCluster][4];  // what each block of the cluster has sent, by turns
@@ -74,7 +84,7 @@ struct alignas(16) SmpShared {
   double scan[kSmpWarps];
   smp_u64 pick_above;
   int pick;
-  uint32_t n_list;
+  uint32_t n_list, n_few;
 };
 
 __device__ __forceinline__ uint32_t smp_key(float x) {
@@ -361,6 +371,79 @@ struct Smp {
     return smp_mass(expf(smp_d(smp_unkey(key), row)));
   }
 
+  // The row's token from the elements in buckets up to `bk`, kSmpFew at most, of which the k largest and the rest of
+  // the rules are taken: every block sends its own to block 0, and that one compares each with all.
+  __device__ __forceinline__ void few(const SampleParams& p, int b, int i0, int bk, uint32_t top_k, float top_p,
+                                      float min_p, float u) {
+    const int tid = threadIdx.x;
+    if (tid == 0) s.n_list = 0u;
+    __syncthreads();
+#pragma unroll 4
+    for (int i = w0 + lane; i < w1; i += 32) {
+      const float w = weight(i);
+      if (smp_bucket(w) <= bk && w > 0.f) s.at[atomicAdd(&s.n_list, 1u)] = i;
+    }
+    __syncthreads();
+    const uint32_t own = s.n_list;
+    if (tid == 0) s.pick = (int)atomicAdd(remote(&s.n_few, 0), own);
+    __syncthreads();
+    for (uint32_t j = tid; j < own; j += kSmpThreads) {
+      const int i = s.at[j];
+      remote(s.few_ord, 0)[s.pick + j] = (smp_u64)smp_key(smp_load(x + i)) << 32 | ~(uint32_t)(i0 + i);
+    }
+    sync();
+    if (rank != 0) return;
+    const int m = (int)s.n_few;
+    smp_u64 ord = 0, mass = 0;
+    float d = 0.f, w = 0.f;
+    if (tid < m) {
+      ord = s.few_ord[tid];
+      d = smp_d(smp_unkey((uint32_t)(ord >> 32)), row);
+      w = expf(d);
+      mass = smp_mass(w);
+      s.few_mass[tid] = mass;
+    }
+    const uint32_t at = ~(uint32_t)ord;
+    __syncthreads();
+    // how many, and what mass, come before in the order (no branches: every load independent of the last)
+    uint32_t place = 0;
+    smp_u64 ahead = 0;
+    if (warp * 32 < m) {
+#pragma unroll 8
+      for (int j = 0; j < m; ++j) {
+        const bool first = s.few_ord[j] > ord;
+        place += first;
+        ahead += first ? s.few_mass[j] : 0ull;
+      }
+    }
+    bool in = tid < m && place < top_k;
+    auto total = [&](smp_u64 v) {  // over the block
+      v = smp_warp_sum(v);
+      if (lane == 0) s.red[warp][0] = v;
+      __syncthreads();
+      v = smp_warp_sum(lane < kSmpWarps ? s.red[lane][0] : 0ull);
+      __syncthreads();
+      return v;
+    };
+    const smp_u64 of_k = total(in ? mass : 0ull);
+    if (top_p < 1.f) in = in && ahead < max((smp_u64)ceil((double)top_p * (double)of_k), 1ull);
+    in = in && w >= min_p;
+    const smp_u64 kept = total(in ? mass : 0ull);
+    if (tid < m) s.few_mass[tid] = in ? mass : 0ull;
+    __syncthreads();
+    smp_u64 goal = (smp_u64)floor((double)fminf(fmaxf(u, 0.f), 1.f) * (double)kept);
+    if (goal >= kept) goal = kept - 1;
+    if (warp * 32 < m) {
+      smp_u64 before = 0;  // by index
+#pragma unroll 8
+      for (int j = 0; j < m; ++j) before += (uint32_t)~(uint32_t)s.few_ord[j] < at ? s.few_mass[j] : 0ull;
+      if (in && goal >= before && goal < before + mass) {
+        p.token[b] = at;
+        if (p.logprob != nullptr) p.logprob[b] = d - logf((float)((double)kept * kSmpUnit));
+      }
+    }
+  }
+
   // Exact selection inside bucket `bk`, whose admitted logits span [lo_key, hi_key] and were listed by the last
   // look() (`cnt` of them): the key and the number of its ties such that the bucket's elements above the key, and
   // those ties, are the fewest whose count (BY_MASS: mass) reaches `need`.
@@ -484,7 +567,7 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SamplePara
 
   for (int i = tid; i < kSmpBuckets; i += kSmpThreads) s.own[0][i] = s.own[1][i] = 0u;
   for (int i = tid; i < kSmpAllLists; i += kSmpThreads) s.all[i] = 0u;
-  if (tid == 0) s.n_list = 0u;
+  if (tid == 0) s.n_list = s.n_few = 0u;
 
   // ---- the largest logit; the range goes to shared memory as fp32 (a NaN as it is: it gets no weight below)
   float top = -INFINITY;
@@ -601,6 +684,10 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SamplePara
     c.reduce(total, inside, lo, hi, cnt, nullptr);
     if (by_k) {
       const int bk = c.template crossing<false>((double)top_k, above_n);
+      if ((uint32_t)above_n + s.tot[0][bk] <= kSmpFew) {  // (the same in every block)
+        c.few(p, b, i0, bk, top_k, top_p, min_p, uu);
+        return;
+      }
       c.look(bk, 0u, above, inside, lo, hi, cnt);
       total = above + inside;
       if (hi != 0u) {
