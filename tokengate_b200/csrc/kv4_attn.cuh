@@ -40,7 +40,8 @@ namespace tg {
 constexpr unsigned int ERR_KV4 = 1u << 15;  // bit of the device error word
 constexpr int kKv4Stages = 3;          // ring tiles per warp, at most
 constexpr int kKv4MaxWarps = 16;
-constexpr int kKv4MaxCluster = 16;
+constexpr int kKv4MaxCluster = 8;
+constexpr int kKv4OStride = 132;       // of a head's sums in shared memory: the four lanes of a row on different banks
 constexpr float kKv4Head = 4.f;       // p = 2^(4 + ...): small p stay normal in fp16
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -69,8 +70,9 @@ constexpr int kKv4Part = 4 + 128;  // m, l, 2 pad, O[128]
 struct alignas(16) Kv4AttnShared {
   __half q[8][128];
   float mul[8];
-  float m[kKv4MaxWarps][8], l[kKv4MaxWarps][8];
-  float got_o[8 * 128 + kKv4MaxCluster];          // [rank][slice]: this block's slice of the blocks' sums
+  float m[kKv4MaxWarps][8], l[kKv4MaxWarps][8];   // of the warps' columns; m becomes their factors of the merge
+  float head_m[8], head_l[8];
+  float got_o[8 * 128];                           // [rank][slice]: this block's slice of the blocks' sums
   float got_m[kKv4MaxCluster][8], got_l[kKv4MaxCluster][8];
   uint64_t full[kKv4MaxWarps][kKv4Stages];
 };
@@ -184,6 +186,21 @@ __device__ __forceinline__ void kv4_share(const Kv4AttnParams& p, int n_keys, in
       count = __shfl_sync(0xffffffffu, c, src);
     }
     run = __shfl_sync(0xffffffffu, end, 31);
+  }
+}
+
+// Four dims of an output row (any alignment), normalised; no key: zeros.
+__device__ __forceinline__ void kv4_store_out(__nv_bfloat16* at, float4 o, float l) {
+  const float r = l == 0.f ? 0.f : 1.f / l;
+  const uint32_t a = pack_bf16x2(o.x * r, o.y * r), b = pack_bf16x2(o.z * r, o.w * r);
+  if ((reinterpret_cast<uintptr_t>(at) & 7) == 0) {
+    *reinterpret_cast<uint2*>(at) = make_uint2(a, b);
+  } else {
+    uint16_t* u = reinterpret_cast<uint16_t*>(at);
+    u[0] = (uint16_t)a;
+    u[1] = (uint16_t)(a >> 16);
+    u[2] = (uint16_t)b;
+    u[3] = (uint16_t)(b >> 16);
   }
 }
 
@@ -527,54 +544,65 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
     }
   }
   __syncwarp();
-  float* so = reinterpret_cast<float*>(ring);  // [8][128] of this warp
+  float* so = reinterpret_cast<float*>(ring);  // [8][kKv4OStride] of this warp
 #pragma unroll
   for (int w = 0; w < 8; ++w)
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      so[(2 * t + (e & 1)) * 128 + 16 * w + g + 8 * (e >> 1)] =
+      so[(2 * t + (e & 1)) * kKv4OStride + 16 * w + g + 8 * (e >> 1)] =
           fmaf(st.acc[w][e] * (e < 2 ? 16777216.f : 1048576.f), st.eref, st.zs[w >> 2][e & 1]);
   if (clustered) cluster_wait();  // every block has started
   __syncthreads();
-  const float* all_o = reinterpret_cast<const float*>(kv4_smem + kKv4Ring);
   constexpr float kUnit = BIAS ? kLog2e : 1.f;  // of m
-  const int slice = (p.G * 128 + C - 1) / C;
-  for (int idx = threadIdx.x; idx < p.G * 128; idx += blockDim.x) {
-    const int h = idx >> 7;
-    constexpr int K = PAIR ? 2 : 1;  // columns of a head, 4 apart
-    float mt = -INFINITY;
-    for (int w = 0; w < W; ++w)
+  constexpr int K = PAIR ? 2 : 1;               // columns of a head, 4 apart
+  // a warp per head: the maximum over its columns, their factors, the sum of p
+  for (int h = warp; h < p.G; h += W) {
+    const int w = K == 2 ? lane >> 1 : lane, col = h + (K == 2 ? 4 * (lane & 1) : 0);
+    const bool has = w < W;
+    const float mw = has ? sh.m[w][col] : -INFINITY, lw = has ? sh.l[w][col] : 0.f;
+    float mt = mw;
 #pragma unroll
-      for (int k = 0; k < K; ++k) mt = fmaxf(mt, sh.m[w][h + 4 * k]);
-    float o = 0.f, lt = 0.f;
-#pragma unroll 4
+    for (int off = 16; off >= 1; off >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, off));
+    const float f = lw == 0.f ? 0.f : ex2_approx((mw - mt) * kUnit);  // 0: the column saw no key
+    float lt = f * lw;                                                // (a NaN sum stays in)
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) lt += __shfl_xor_sync(0xffffffffu, lt, off);
+    if (has) sh.m[w][col] = f;
+    if (lane == 0) {
+      sh.head_m[h] = mt;
+      sh.head_l[h] = lt;
+    }
+  }
+  __syncthreads();
+  const float* all_o = reinterpret_cast<const float*>(kv4_smem + kKv4Ring);
+  const int slice = p.G * 128 / C;  // of a cluster: a multiple of 16
+  for (int i4 = threadIdx.x; i4 < p.G * 32; i4 += blockDim.x) {
+    const int h = i4 >> 5, d = 4 * (i4 & 31);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int w = 0; w < W; ++w) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const float lw = sh.l[w][h + 4 * k], ow = all_o[w * (S * kKv4TileBytes / 4) + 512 * k + idx];
-        if (lw != 0.f) {  // 0: the column saw no key (a NaN sum stays in)
-          const float f = ex2_approx((sh.m[w][h + 4 * k] - mt) * kUnit);
-          o = fmaf(f, ow, o);
-          lt = fmaf(f, lw, lt);
-        }
+        const float f = sh.m[w][h + 4 * k];
+        const float4 v = *reinterpret_cast<const float4*>(all_o + w * (S * kKv4TileBytes / 4) + (h + 4 * k) * kKv4OStride + d);
+        o.x = fmaf(f, v.x, o.x);
+        o.y = fmaf(f, v.y, o.y);
+        o.z = fmaf(f, v.z, o.z);
+        o.w = fmaf(f, v.w, o.w);
       }
     }
+    const float mt = sh.head_m[h], lt = sh.head_l[h];
     if (C == 1) {
-      p.out[(int64_t)b * p.o_sb + (int64_t)(kvh * p.G + h) * p.o_sh + (idx & 127)] =
-          __float2bfloat16_rn(lt == 0.f ? 0.f : o / lt);
+      kv4_store_out(p.out + (int64_t)b * p.o_sb + (int64_t)(kvh * p.G + h) * p.o_sh + d, o, lt);
     } else if (!clustered) {
       float* rec = p.part + ((int64_t)(kvh * p.G + h) * gridDim.x + blockIdx.x) * kKv4Part;
-      rec[4 + (idx & 127)] = o;
-      if ((idx & 127) == 0) {
-        rec[0] = mt;
-        rec[1] = lt;
-      }
+      *reinterpret_cast<float4*>(rec + 4 + d) = o;
+      if (d == 0) *reinterpret_cast<float2*>(rec) = make_float2(mt, lt);
     } else {
       cooperative_groups::cluster_group cl = cooperative_groups::this_cluster();
-      cl.map_shared_rank(sh.got_o, idx / slice)[rank * slice + idx % slice] = o;
-      if ((idx & 127) < C) {
-        cl.map_shared_rank(&sh.got_m[rank][h], idx & 127)[0] = mt;
-        cl.map_shared_rank(&sh.got_l[rank][h], idx & 127)[0] = lt;
+      *reinterpret_cast<float4*>(cl.map_shared_rank(sh.got_o, 4 * i4 / slice) + rank * slice + 4 * i4 % slice) = o;
+      if ((i4 & 31) < C) {
+        cl.map_shared_rank(&sh.got_m[rank][h], i4 & 31)[0] = mt;
+        cl.map_shared_rank(&sh.got_l[rank][h], i4 & 31)[0] = lt;
       }
     }
   }
@@ -583,7 +611,6 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
   cluster_sync_all();
   for (int i = threadIdx.x; i < slice; i += blockDim.x) {
     const int idx = rank * slice + i, h = idx >> 7;
-    if (idx >= p.G * 128) break;
     float mt = sh.got_m[0][h];
     for (int c = 1; c < C; ++c) mt = fmaxf(mt, sh.got_m[c][h]);
     float o = 0.f, lt = 0.f;

@@ -1404,9 +1404,10 @@ Kv4Shape kv4_shape(int B, int Hkv, int n_keys) {
   } else if (rows * 2 <= sms) {
     s.parts = sms / Hkv;          // one block of 16 warps per SM (16 rows of 131081: 55 us, 12 warps of 3 tiles 57)
   } else {
-    s.warps = 4;                  // many rows: three blocks of 4 warps per SM, and with fewer warps more tiles in flight
-    s.stages = 3;
-    s.parts = 3 * sms / Hkv > 0 ? 3 * sms / Hkv : 1;
+    // many rows: four blocks of 4 warps per SM (512 rows of 2771: 54 us, three blocks of three tiles a warp 69;
+    // 128 ragged rows of 4097: 19.3, two blocks of 8 warps 20.2)
+    s.warps = 4;
+    s.parts = 4 * sms / Hkv > 0 ? 4 * sms / Hkv : 1;
   }
   return s;
 }
