@@ -23,10 +23,9 @@
 //      Each block owns a slice of the row's and hands it to the others;
 //   2. exactly inside that bucket: one pass gives the mass above it and in it,
 //      its smallest and largest logit and the list of its logits (a wrong guess
-//      moves by a bucket); then 8-bit digits of the ordered logit from the
-//      highest bit in which the two differ (none for bf16 logits, whose buckets
-//      hold one or two values), every block on a copy of all lists, so without
-//      a cluster barrier (lists too long for that: over the row again).
+//      moves by a bucket); where the two differ (bf16 logits: hardly ever),
+//      every block narrows them down on a copy of all lists, so without a
+//      cluster barrier (lists too long for that: digits, over the row again).
 // Where no more than 256 logits reach down to the k-th's bucket, they go to one
 // block, which orders them by counting and finishes alone (one row of 151936,
 // k = 50, p = 0.9: 22 -> 14 us).
@@ -444,89 +443,162 @@ struct Smp {
     }
   }
 
-  // Exact selection inside bucket `bk`, whose admitted logits span [lo_key, hi_key] and were listed by the last
-  // look() (`cnt` of them): the key and the number of its ties such that the bucket's elements above the key, and
-  // those ties, are the fewest whose count (BY_MASS: mass) reaches `need`.
-  template <bool BY_MASS>
-  __device__ __forceinline__ void refine(int bk, uint32_t lo_key, uint32_t hi_key, uint32_t cnt, smp_u64 need,
-                                      uint32_t& key, smp_u64& ties) {
-    uint32_t prefix = lo_key, mask = 0xFFFFFFFFu;
-    if (lo_key != hi_key) {
-      const bool listed = cnt <= kSmpAllLists - 1;
-      if (listed) {
-        uint32_t base = 0;
-        for (int c = 0; c < C; ++c) {
-          const uint32_t m = (uint32_t)s.xch[turn ^ 1][c][3];  // as the last reduce() left it
-          const uint32_t* from = remote(s.own[turn ^ 1], c);
-          for (uint32_t i = threadIdx.x; i < m; i += kSmpThreads) s.all[base + i] = from[i];
-          base += m;
-        }
-      }
-      const int top = 31 - __clz(lo_key ^ hi_key);
-      mask = top == 31 ? 0u : ~((2u << top) - 1u);
-      prefix = hi_key & mask;
-      for (int shift = max(top - 7, 0);; shift = max(shift - 8, 0)) {
-        smp_u64* dig = s.dig[parity];
-        parity ^= 1;
-        for (int i = threadIdx.x; i < 256; i += kSmpThreads) dig[i] = 0ull;
-        __syncthreads();
-        if (listed) {
-          for (uint32_t i = threadIdx.x; i < cnt; i += kSmpThreads) {
-            const uint32_t k = s.all[i];
-            if (k != 0u && (k & mask) == prefix)
-              atomicAdd(&dig[(k >> shift) & 255u], BY_MASS ? mass_of_key(k) : 1ull);
-          }
-          __syncthreads();
-        } else {
-          for (int i = w0 + lane; i < w1; i += 32) {
-            const float w = weight(i);
-            if (smp_bucket(w) != bk || w == 0.f) continue;
-            const uint32_t k = smp_key(smp_load(x + i));
-            if ((k & mask) == prefix) atomicAdd(&dig[(k >> shift) & 255u], BY_MASS ? smp_mass(w) : 1ull);
-          }
-          sync();
-        }
-        if (warp == 0) {  // the digits from the highest down, 8 to a lane
-          smp_u64 v[8], sum = 0;
+  // Of the histogram dig[256], digits or bins in order: where the running sum reaches `need`, to s.pick and, less the
+  // sum before it, s.pick_above. By warp 0; C: summed over the cluster's blocks.
+  template <bool ASCENDING>
+  __device__ __forceinline__ void pick_bin(smp_u64* dig, int blocks, smp_u64 need) {
+    smp_u64 v[8], sum = 0;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int dgt = 255 - (lane * 8 + e);
-            v[e] = 0;
-            if (listed) {
-              v[e] = dig[dgt];
-            } else {
-              for (int c = 0; c < C; ++c) v[e] += remote(dig, c)[dgt];
-            }
-            sum += v[e];
-          }
-          smp_u64 before = smp_warp_scan(sum, lane) - sum;
-          if (before < need && need <= before + sum) {
-            int e = 0;
-#pragma unroll
-            for (int q = 0; q < 7; ++q)
-              if (e == q && need > before + v[q]) {
-                before += v[q];
-                ++e;
-              }
-            s.pick = 255 - (lane * 8 + e);
-            s.pick_above = before;
-          }
-        }
-        __syncthreads();
-        const uint32_t dmask = 255u << shift;
-        need -= s.pick_above;
-        prefix = (prefix & ~dmask) | ((uint32_t)s.pick << shift);
-        mask |= dmask;
-        __syncthreads();
-        if (shift == 0) break;
+    for (int e = 0; e < 8; ++e) {
+      const int i = ASCENDING ? lane * 8 + e : 255 - (lane * 8 + e);
+      if (blocks == 1) {
+        v[e] = dig[i];
+      } else {
+        v[e] = 0;
+        for (int c = 0; c < blocks; ++c) v[e] += remote(dig, c)[i];
       }
+      sum += v[e];
     }
-    key = prefix;
+    smp_u64 before = smp_warp_scan(sum, lane) - sum;
+    if (before < need && need <= before + sum) {
+      int e = 0;
+#pragma unroll
+      for (int q = 0; q < 7; ++q)
+        if (e == q && need > before + v[q]) {
+          before += v[q];
+          ++e;
+        }
+      s.pick = ASCENDING ? lane * 8 + e : 255 - (lane * 8 + e);
+      s.pick_above = before;
+    }
+  }
+
+  // Exact selection inside bucket `bk`, whose admitted logits span [lo, hi] and were listed by the last look()
+  // (`cnt` of them): the key and the number of its ties such that the bucket's elements above the key, and those
+  // ties, are the fewest whose count (BY_MASS: mass) reaches `need`.
+  template <bool BY_MASS>
+  __device__ __forceinline__ void refine(int bk, uint32_t lo, uint32_t hi, uint32_t cnt, smp_u64 need, uint32_t& key,
+                                         smp_u64& ties) {
+    if (lo == hi) {
+      key = lo;
+    } else if (cnt < kSmpAllLists) {
+      select_listed<BY_MASS>(lo, hi, cnt, need, key);
+    } else {
+      select_row<BY_MASS>(bk, lo, hi, need, key);
+    }
     ties = need;
     if (BY_MASS) {
-      const smp_u64 w = mass_of_key(prefix);
+      const smp_u64 w = mass_of_key(key);
       ties = w == 0 ? 1ull : max((need + w - 1) / w, 1ull);
     }
+  }
+
+  // On a copy of all blocks' lists, in every block: 256 linear bins of the range of keys narrow it to one bin, until
+  // few enough keys are left to compare each with all. `need` becomes what is still needed at the key.
+  template <bool BY_MASS>
+  __device__ __forceinline__ void select_listed(uint32_t lo, uint32_t hi, uint32_t cnt, smp_u64& need, uint32_t& key) {
+    constexpr uint32_t kHalf = kSmpBuckets / 2;
+    const uint32_t* cur = s.all;
+    {
+      uint32_t base = 0;
+      for (int c = 0; c < C; ++c) {
+        const uint32_t m = (uint32_t)s.xch[turn ^ 1][c][3];  // as the last reduce() left it
+        const uint32_t* from = remote(s.own[turn ^ 1], c);
+        for (uint32_t i = threadIdx.x; i < m; i += kSmpThreads) s.all[base + i] = from[i];
+        base += m;
+      }
+    }
+    smp_u64* dig = s.dig[0];
+    for (int flip = 0;; flip ^= 1) {
+      __syncthreads();
+      if (lo == hi) {
+        key = lo;
+        return;
+      }
+      if (cnt <= kSmpFew) {
+        const uint32_t k = threadIdx.x < cnt ? cur[threadIdx.x] : 0u;
+        const bool in = k >= lo && k <= hi;
+        if (threadIdx.x < cnt) dig[threadIdx.x] = !in ? 0ull : BY_MASS ? mass_of_key(k) : 1ull;
+        __syncthreads();
+        if (warp * 32 < (int)cnt) {
+          smp_u64 above = 0, equal = 0;
+#pragma unroll 8
+          for (uint32_t j = 0; j < cnt; ++j) {
+            const uint32_t kj = cur[j];
+            const smp_u64 m = dig[j];
+            above += kj > k ? m : 0ull;
+            equal += kj == k ? m : 0ull;
+          }
+          if (in && above < need && need <= above + equal) {  // (threads of equal keys write the same)
+            s.pick = (int)k;
+            s.pick_above = above;
+          }
+        }
+        __syncthreads();
+        key = (uint32_t)s.pick;
+        need -= s.pick_above;
+        __syncthreads();
+        return;
+      }
+      const int shift = max(0, 24 - __clz(hi - lo));
+      for (int i = threadIdx.x; i < 256; i += kSmpThreads) dig[i] = 0ull;
+      if (threadIdx.x == 0) s.n_few = 0u;
+      __syncthreads();
+      for (uint32_t i = threadIdx.x; i < cnt; i += kSmpThreads) {
+        const uint32_t k = cur[i];
+        if (k >= lo && k <= hi) atomicAdd(&dig[(hi - k) >> shift], BY_MASS ? mass_of_key(k) : 1ull);
+      }
+      __syncthreads();
+      if (warp == 0) pick_bin<true>(dig, 1, need);
+      __syncthreads();
+      need -= s.pick_above;
+      hi -= (uint32_t)s.pick << shift;
+      lo = max(lo, hi - ((1u << shift) - 1u));
+      // the bin's keys to a list of their own, if they fit
+      uint32_t* kept = s.tot[0] + flip * kHalf;
+      for (uint32_t i = threadIdx.x; i < cnt; i += kSmpThreads) {
+        const uint32_t k = cur[i];
+        if (k >= lo && k <= hi) {
+          const uint32_t at = atomicAdd(&s.n_few, 1u);
+          if (at < kHalf) kept[at] = k;
+        }
+      }
+      __syncthreads();
+      if (s.n_few <= kHalf) {
+        cur = kept;
+        cnt = s.n_few;
+      }
+    }
+  }
+
+  // Over the row itself (lists ran over): 8-bit digits from the highest bit in which lo and hi differ, with a cluster
+  // barrier each. (It sees the whole bucket; above a floor that look() was given its order is the same.)
+  template <bool BY_MASS>
+  __device__ __forceinline__ void select_row(int bk, uint32_t lo, uint32_t hi, smp_u64& need, uint32_t& key) {
+    const int top = 31 - __clz(lo ^ hi);
+    uint32_t mask = top == 31 ? 0u : ~((2u << top) - 1u), prefix = hi & mask;
+    for (int shift = max(top - 7, 0);; shift = max(shift - 8, 0)) {
+      smp_u64* dig = s.dig[parity];
+      parity ^= 1;
+      for (int i = threadIdx.x; i < 256; i += kSmpThreads) dig[i] = 0ull;
+      __syncthreads();
+      for (int i = w0 + lane; i < w1; i += 32) {
+        const float w = weight(i);
+        if (smp_bucket(w) != bk || w == 0.f) continue;
+        const uint32_t k = smp_key(smp_load(x + i));
+        if ((k & mask) == prefix) atomicAdd(&dig[(k >> shift) & 255u], BY_MASS ? smp_mass(w) : 1ull);
+      }
+      sync();
+      if (warp == 0) pick_bin<false>(dig, C, need);
+      __syncthreads();
+      const uint32_t dmask = 255u << shift;
+      need -= s.pick_above;
+      prefix = (prefix & ~dmask) | ((uint32_t)s.pick << shift);
+      mask |= dmask;
+      __syncthreads();
+      if (shift == 0) break;
+    }
+    key = prefix;
   }
 };
 
@@ -725,7 +797,6 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SamplePara
         if (w != 0) ties = min(ties, (left + w - 1) / w);
         listed = false;  // the last look() left the ties out
       } else {
-        // (digit passes over the row see the whole bucket; above the top-k threshold its order is the same)
         c.template refine<true>(bp, lo, hi, cnt, need - above, thr, ties);
       }
     }
