@@ -46,6 +46,7 @@ constexpr int kSmpWarps = kSmpThreads / 32;
 constexpr int kSmpBuckets = 1024;
 constexpr int kSmpList = 1024;      // logits of one bucket that a block can list
 constexpr int kSmpAllLists = 2048;  // and the cluster
+constexpr uint32_t kSmpNoLists = 0xFFFFFFFFu;
 constexpr int kSmpFew = 256;        // logits that one block orders by counting
 constexpr int kSmpMaxCluster = 16;   // above 8: opt-in
 constexpr int kSmpMaxV = 1 << 19;
@@ -238,8 +239,9 @@ struct Smp {
     b = smp_warp_sum(b);
     lo = smp_warp_min(lo);
     hi = smp_warp_max(hi);
-    if (__any_sync(0xffffffffu, cnt > kSmpList)) cnt = kSmpAllLists;  // some block's list ran over
+    const bool over = __any_sync(0xffffffffu, cnt > kSmpList);  // some block's list ran over
     cnt = __reduce_add_sync(0xffffffffu, cnt);
+    if (over) cnt = kSmpNoLists;
   }
 
   // The row's histogram `which` (0: counts, 1: masses) into every block's s.tot: each block's goes to the owners of
@@ -484,7 +486,7 @@ struct Smp {
     } else if (cnt < kSmpAllLists) {
       select_listed<BY_MASS>(lo, hi, cnt, need, key);
     } else {
-      select_row<BY_MASS>(bk, lo, hi, need, key);
+      select_digits<BY_MASS>(bk, lo, hi, cnt != kSmpNoLists, need, key);
     }
     ties = need;
     if (BY_MASS) {
@@ -571,22 +573,33 @@ struct Smp {
     }
   }
 
-  // Over the row itself (lists ran over): 8-bit digits from the highest bit in which lo and hi differ, with a cluster
-  // barrier each. (It sees the whole bucket; above a floor that look() was given its order is the same.)
+  // Where the lists are too long for one block: 8-bit digits from the highest bit in which lo and hi differ, each
+  // block over its own list (or, where a list ran over, over its part of the row: that sees the whole bucket, whose
+  // order above a floor that look() was given is the same), with a cluster barrier each.
   template <bool BY_MASS>
-  __device__ __forceinline__ void select_row(int bk, uint32_t lo, uint32_t hi, smp_u64& need, uint32_t& key) {
+  __device__ __forceinline__ void select_digits(int bk, uint32_t lo, uint32_t hi, bool listed, smp_u64& need,
+                                                uint32_t& key) {
     const int top = 31 - __clz(lo ^ hi);
     uint32_t mask = top == 31 ? 0u : ~((2u << top) - 1u), prefix = hi & mask;
+    const uint32_t* list = s.own[turn ^ 1];
     for (int shift = max(top - 7, 0);; shift = max(shift - 8, 0)) {
       smp_u64* dig = s.dig[parity];
       parity ^= 1;
       for (int i = threadIdx.x; i < 256; i += kSmpThreads) dig[i] = 0ull;
       __syncthreads();
-      for (int i = w0 + lane; i < w1; i += 32) {
-        const float w = weight(i);
-        if (smp_bucket(w) != bk || w == 0.f) continue;
-        const uint32_t k = smp_key(smp_load(x + i));
-        if ((k & mask) == prefix) atomicAdd(&dig[(k >> shift) & 255u], BY_MASS ? smp_mass(w) : 1ull);
+      if (listed) {
+        for (uint32_t i = threadIdx.x; i < s.n_list; i += kSmpThreads) {
+          const uint32_t k = list[i];
+          if (k != 0u && (k & mask) == prefix)
+            atomicAdd(&dig[(k >> shift) & 255u], BY_MASS ? mass_of_key(k) : 1ull);
+        }
+      } else {
+        for (int i = w0 + lane; i < w1; i += 32) {
+          const float w = weight(i);
+          if (smp_bucket(w) != bk || w == 0.f) continue;
+          const uint32_t k = smp_key(smp_load(x + i));
+          if ((k & mask) == prefix) atomicAdd(&dig[(k >> shift) & 255u], BY_MASS ? smp_mass(w) : 1ull);
+        }
       }
       sync();
       if (warp == 0) pick_bin<false>(dig, C, need);
@@ -643,38 +656,38 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SamplePara
 
   // ---- the largest logit; the range goes to shared memory as fp32 (a NaN as it is: it gets no weight below)
   float top = -INFINITY;
+  constexpr int kVec = 16 / sizeof(T);
+  int vec_done = 0;  // elements loaded as vectors
   {
-    constexpr int VEC = 16 / sizeof(T);
-    int done = 0;
     if ((reinterpret_cast<uintptr_t>(c.x) & 15) == 0) {
       const uint4* xv = reinterpret_cast<const uint4*>(c.x);
-      const int nv = n / VEC;
+      const int nv = n / kVec;
 #pragma unroll 4
       for (int i = tid; i < nv; i += kSmpThreads) {
         const uint4 q = ld_nc_v4(xv + i);
         const uint32_t wd[4] = {q.x, q.y, q.z, q.w};
-        float f[VEC];
+        float f[kVec];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          if (VEC == 4) {
+          if (kVec == 4) {
             f[e] = __uint_as_float(wd[e]);
           } else {
-            f[2 * e % VEC] = __uint_as_float(wd[e] << 16);
-            f[(2 * e + 1) % VEC] = __uint_as_float(wd[e] & 0xFFFF0000u);
+            f[2 * e % kVec] = __uint_as_float(wd[e] << 16);
+            f[(2 * e + 1) % kVec] = __uint_as_float(wd[e] & 0xFFFF0000u);
           }
         }
 #pragma unroll
-        for (int e = 0; e < VEC; e += 2) top = fmax3(top, f[e], f[e + 1]);
+        for (int e = 0; e < kVec; e += 2) top = fmax3(top, f[e], f[e + 1]);
         if (HELD) {
 #pragma unroll
-          for (int e = 0; e < VEC / 4; ++e)
-            reinterpret_cast<float4*>(c.sw)[i * (VEC / 4) + e] =
+          for (int e = 0; e < kVec / 4; ++e)
+            reinterpret_cast<float4*>(c.sw)[i * (kVec / 4) + e] =
                 make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
         }
       }
-      done = nv * VEC;
+      vec_done = nv * kVec;
     }
-    for (int i = done + tid; i < n; i += kSmpThreads) {
+    for (int i = vec_done + tid; i < n; i += kSmpThreads) {
       const float v = smp_load(c.x + i);
       if (HELD) c.sw[i] = v;
       top = fmaxf(top, v);
@@ -696,14 +709,17 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SamplePara
   if (c.row.xmax == -INFINITY || top_k == 1u) {
     // nothing to choose from, or the lowest index of the largest logit
     uint32_t first = 0xFFFFFFFFu, none = 0, cnt;
-    for (int i = tid; i < n; i += kSmpThreads)
-      if ((HELD ? c.sw[i] : smp_load(c.x + i)) == c.row.xmax) {
-        first = i0 + i;
-        break;
-      }
+    if (top == c.row.xmax) {  // this thread has seen it: among the elements that it loaded
+      auto seek = [&](int i) {
+        if (first == 0xFFFFFFFFu && smp_load(c.x + i) == c.row.xmax) first = i0 + i;
+      };
+      for (int v = tid; v < vec_done / kVec && first == 0xFFFFFFFFu; v += kSmpThreads)
+        for (int e = 0; e < kVec; ++e) seek(v * kVec + e);
+      for (int i = vec_done + tid; i < n && first == 0xFFFFFFFFu; i += kSmpThreads) seek(i);
+    }
     c.reduce(my, my_ties, first, none, cnt, nullptr);
     if (c.rank == 0 && tid == 0) {
-      p.token[b] = first == 0xFFFFFFFFu ? 0 : first;  // (NaN alone equals nothing)
+      p.token[b] = first;
       if (p.logprob != nullptr) p.logprob[b] = c.row.xmax == -INFINITY ? __uint_as_float(0x7FC00000u) : 0.f;
     }
     return;
