@@ -55,8 +55,13 @@ bool g_attn_attr_set[kMaxDevices] = {};
 bool g_dec_attr_set[kMaxDevices] = {};
 
 int sm_count() {
+  static int cached[kMaxDevices] = {};  // asked once per device: a launch's host time is a few microseconds in all
   int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (cudaGetDevice(&dev) != cudaSuccess) return sms;
+  if (dev >= 0 && dev < kMaxDevices && __atomic_load_n(&cached[dev], __ATOMIC_RELAXED) > 0)
+    return __atomic_load_n(&cached[dev], __ATOMIC_RELAXED);
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && dev >= 0 && dev < kMaxDevices)
+    __atomic_store_n(&cached[dev], sms, __ATOMIC_RELAXED);
   return sms;
 }
 
@@ -1607,13 +1612,14 @@ int tg_sample(const void* logits, int dtype, int64_t row_stride, int B, int V, c
   p.min_p = min_p;
   p.token = token;
   p.logprob = logprob;
+  const int sms = sm_count();
   // blocks of a cluster: as many as half fill the GPU (one row of 151936: 16 blocks 23 us, 8 blocks 30 us), and as
   // many as let two blocks share an SM's memory (64 fp32 rows of 151936: 8 blocks 94 us, 4 blocks 114 us)
   int C = 1;
   auto chunk_of = [&](int c) { return (V + c * tg::kSmpThreads - 1) / (c * tg::kSmpThreads) * tg::kSmpThreads; };
   auto smem_of = [&](int c) { return sizeof(tg::SmpShared) + (size_t)chunk_of(c) * sizeof(float); };
   while (C < tg::kSmpMaxCluster &&
-         (((int64_t)B * C * 2 <= sm_count() && V > C * 4096) || smem_of(C) > (size_t)kSmpMaxSmem / 2 - 1024))
+         (((int64_t)B * C * 2 <= sms && V > C * 4096) || smem_of(C) > (size_t)kSmpMaxSmem / 2 - 1024))
     C *= 2;
   p.chunk = chunk_of(C);
   const bool held = smem_of(C) <= (size_t)kSmpMaxSmem;
