@@ -47,6 +47,7 @@ constexpr int kSmpBuckets = 1024;
 constexpr int kSmpList = 1024;      // logits of one bucket that a block can list
 constexpr int kSmpAllLists = 2048;  // and the cluster
 constexpr uint32_t kSmpNoLists = 0xFFFFFFFFu;
+constexpr int kSmpCompare = 64;     // listed logits that are compared each with all
 constexpr int kSmpFew = 256;        // logits that one block orders by counting
 constexpr int kSmpMaxCluster = 16;   // above 8: opt-in
 constexpr int kSmpMaxV = 1 << 19;
@@ -55,7 +56,7 @@ constexpr double kSmpUnit = 1.0 / 17592186044416.0;  // 2^-44: a mass of 1
 struct SampleParams {
   const void* logits;
   int64_t row_stride;  // elements
-  int V, chunk;        // indices per block, a multiple of kSmpThreads (the last blocks may hold fewer or none)
+  int V, chunk;        // indices per block, a multiple of kSmpThreads below 2^16 (the last blocks may hold fewer or none)
   const float* u;
   const float* temperature;
   const int32_t* top_k;   // nullable
@@ -77,8 +78,8 @@ struct alignas(16) SmpShared {
       smp_u64 few_mass[kSmpFew];
     };
   };
-  uint32_t at[kSmpList];          // where in the block's range the listed logits are
-  smp_u64 dig[2][256];            // digit histograms of a refinement, by pass parity
+  uint16_t at[kSmpList];          // where in the block's range the listed logits are
+  uint32_t dig[2][3][256];        // digit histograms of a refinement, by pass parity: masses in three pieces of 15 bits
   smp_u64 xch[2][kSmpMaxCluster][4];  // what each block of the cluster has sent, by turns
   smp_u64 red[kSmpWarps][4];
   double scan[kSmpWarps];
@@ -342,7 +343,7 @@ struct Smp {
         smp_add_mass(w, ah, al);
       } else if (e == bk && w > 0.f) {
         const uint32_t j = atomicAdd(&s.n_list, 1u);
-        if (j < kSmpList) s.at[j] = i;
+        if (j < kSmpList) s.at[j] = (uint16_t)i;
       }
     }
     __syncthreads();
@@ -368,9 +369,8 @@ struct Smp {
     reduce(above, inside, lo, hi, cnt, nullptr);
   }
 
-  __device__ __forceinline__ smp_u64 mass_of_key(uint32_t key) const {
-    return smp_mass(expf(smp_d(smp_unkey(key), row)));
-  }
+  __device__ __forceinline__ float weight_of_key(uint32_t key) const { return expf(smp_d(smp_unkey(key), row)); }
+  __device__ __forceinline__ smp_u64 mass_of_key(uint32_t key) const { return smp_mass(weight_of_key(key)); }
 
   // The row's token from the elements in buckets up to `bk`, kSmpFew at most, of which the k largest and the rest of
   // the rules are taken: every block sends its own to block 0, and that one compares each with all.
@@ -382,7 +382,7 @@ struct Smp {
 #pragma unroll 4
     for (int i = w0 + lane; i < w1; i += 32) {
       const float w = weight(i);
-      if (smp_bucket(w) <= bk && w > 0.f) s.at[atomicAdd(&s.n_list, 1u)] = i;
+      if (smp_bucket(w) <= bk && w > 0.f) s.at[atomicAdd(&s.n_list, 1u)] = (uint16_t)i;
     }
     __syncthreads();
     const uint32_t own = s.n_list;
@@ -445,19 +445,32 @@ struct Smp {
     }
   }
 
-  // Of the histogram dig[256], digits or bins in order: where the running sum reaches `need`, to s.pick and, less the
+  // Adds a count (of 1) or a mass to bin i of a histogram. Shared memory adds 32 bits natively and 64 only by trying
+  // again, which hurts where many elements are of one bin; 15 bits of 2^16 elements fit 32.
+  template <bool BY_MASS>
+  __device__ __forceinline__ void add_to_bin(uint32_t* dig, uint32_t i, float w) const {
+    if (BY_MASS) {
+      const smp_u64 m = smp_mass(w);
+      atomicAdd(&dig[i], (uint32_t)m & 0x7FFFu);
+      atomicAdd(&dig[256 + i], (uint32_t)(m >> 15) & 0x7FFFu);
+      atomicAdd(&dig[512 + i], (uint32_t)(m >> 30));
+    } else {
+      atomicAdd(&dig[i], 1u);
+    }
+  }
+
+  // Of the histogram dig[3][256], digits or bins in order: where the running sum reaches `need`, to s.pick and, less the
   // sum before it, s.pick_above. By warp 0; C: summed over the cluster's blocks.
   template <bool ASCENDING>
-  __device__ __forceinline__ void pick_bin(smp_u64* dig, int blocks, smp_u64 need) {
+  __device__ __forceinline__ void pick_bin(uint32_t* dig, int blocks, smp_u64 need) {
     smp_u64 v[8], sum = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int i = ASCENDING ? lane * 8 + e : 255 - (lane * 8 + e);
-      if (blocks == 1) {
-        v[e] = dig[i];
-      } else {
-        v[e] = 0;
-        for (int c = 0; c < blocks; ++c) v[e] += remote(dig, c)[i];
+      v[e] = 0;
+      for (int c = 0; c < blocks; ++c) {
+        const uint32_t* from = blocks == 1 ? dig : remote(dig, c);
+        v[e] += from[i] + ((smp_u64)from[256 + i] << 15) + ((smp_u64)from[512 + i] << 30);
       }
       sum += v[e];
     }
@@ -510,24 +523,25 @@ struct Smp {
         base += m;
       }
     }
-    smp_u64* dig = s.dig[0];
+    uint32_t* dig = &s.dig[0][0][0];
+    smp_u64* masses = reinterpret_cast<smp_u64*>(dig);
     for (int flip = 0;; flip ^= 1) {
       __syncthreads();
       if (lo == hi) {
         key = lo;
         return;
       }
-      if (cnt <= kSmpFew) {
+      if (cnt <= kSmpCompare) {
         const uint32_t k = threadIdx.x < cnt ? cur[threadIdx.x] : 0u;
         const bool in = k >= lo && k <= hi;
-        if (threadIdx.x < cnt) dig[threadIdx.x] = !in ? 0ull : BY_MASS ? mass_of_key(k) : 1ull;
+        if (threadIdx.x < cnt) masses[threadIdx.x] = !in ? 0ull : BY_MASS ? mass_of_key(k) : 1ull;
         __syncthreads();
         if (warp * 32 < (int)cnt) {
           smp_u64 above = 0, equal = 0;
 #pragma unroll 8
           for (uint32_t j = 0; j < cnt; ++j) {
             const uint32_t kj = cur[j];
-            const smp_u64 m = dig[j];
+            const smp_u64 m = masses[j];
             above += kj > k ? m : 0ull;
             equal += kj == k ? m : 0ull;
           }
@@ -543,12 +557,12 @@ struct Smp {
         return;
       }
       const int shift = max(0, 24 - __clz(hi - lo));
-      for (int i = threadIdx.x; i < 256; i += kSmpThreads) dig[i] = 0ull;
+      for (int i = threadIdx.x; i < 3 * 256; i += kSmpThreads) dig[i] = 0u;
       if (threadIdx.x == 0) s.n_few = 0u;
       __syncthreads();
       for (uint32_t i = threadIdx.x; i < cnt; i += kSmpThreads) {
         const uint32_t k = cur[i];
-        if (k >= lo && k <= hi) atomicAdd(&dig[(hi - k) >> shift], BY_MASS ? mass_of_key(k) : 1ull);
+        if (k >= lo && k <= hi) add_to_bin<BY_MASS>(dig, (hi - k) >> shift, BY_MASS ? weight_of_key(k) : 0.f);
       }
       __syncthreads();
       if (warp == 0) pick_bin<true>(dig, 1, need);
@@ -583,22 +597,22 @@ struct Smp {
     uint32_t mask = top == 31 ? 0u : ~((2u << top) - 1u), prefix = hi & mask;
     const uint32_t* list = s.own[turn ^ 1];
     for (int shift = max(top - 7, 0);; shift = max(shift - 8, 0)) {
-      smp_u64* dig = s.dig[parity];
+      uint32_t* dig = &s.dig[parity][0][0];
       parity ^= 1;
-      for (int i = threadIdx.x; i < 256; i += kSmpThreads) dig[i] = 0ull;
+      for (int i = threadIdx.x; i < 3 * 256; i += kSmpThreads) dig[i] = 0u;
       __syncthreads();
       if (listed) {
         for (uint32_t i = threadIdx.x; i < s.n_list; i += kSmpThreads) {
           const uint32_t k = list[i];
           if (k != 0u && (k & mask) == prefix)
-            atomicAdd(&dig[(k >> shift) & 255u], BY_MASS ? mass_of_key(k) : 1ull);
+            add_to_bin<BY_MASS>(dig, (k >> shift) & 255u, BY_MASS ? weight_of_key(k) : 0.f);
         }
       } else {
         for (int i = w0 + lane; i < w1; i += 32) {
           const float w = weight(i);
           if (smp_bucket(w) != bk || w == 0.f) continue;
           const uint32_t k = smp_key(smp_load(x + i));
-          if ((k & mask) == prefix) atomicAdd(&dig[(k >> shift) & 255u], BY_MASS ? smp_mass(w) : 1ull);
+          if ((k & mask) == prefix) add_to_bin<BY_MASS>(dig, (k >> shift) & 255u, w);
         }
       }
       sync();
