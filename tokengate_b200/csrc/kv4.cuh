@@ -103,9 +103,9 @@ __device__ __forceinline__ __nv_bfloat162 kv4_minmax8(const uint4 x) {
     mx = __hmax2_nan(mx, a);
     mn = __hmin2_nan(mn, a);
   }
-  const __nv_bfloat16 m = __hmax_nan(__low2bfloat16(mx), __high2bfloat16(mx));
-  const __nv_bfloat16 n = __hmin_nan(__low2bfloat16(mn), __high2bfloat16(mn));
-  return __halves2bfloat162(m, __hneg(n));
+  const uint32_t a = *reinterpret_cast<uint32_t*>(&mx), b = *reinterpret_cast<uint32_t*>(&mn) ^ 0x80008000u;
+  const uint32_t lo = __byte_perm(a, b, 0x5410), hi = __byte_perm(a, b, 0x7632);  // (max, -min) of the even, the odd
+  return __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&lo), *reinterpret_cast<const __nv_bfloat162*>(&hi));
 }
 __device__ __forceinline__ __nv_bfloat162 shfl_xor_bf162(__nv_bfloat162 v, int off) {
   uint32_t u = *reinterpret_cast<uint32_t*>(&v);
@@ -121,12 +121,14 @@ __device__ __forceinline__ __nv_bfloat162 shfl_xor_bf162(__nv_bfloat162 v, int o
 // 32-byte sectors. Consecutive warps take consecutive heads of the same keys
 // (adjacent in the source). Rows outside [start, start + count) are neither
 // read nor written; a word that mixes both is written byte by byte.
-// Bound by instructions before memory, so: the extrema of a lane's 8 rows are
-// reduced and scattered in one exchange (lane c % 8 ends up with row c % 8's,
-// 7 shuffles instead of 24) and a row's step and reciprocal are computed by that
-// lane alone; codes come two at a time (packed fp32). 22 instructions a value
-// (59 us for 32768 keys of 8 heads, 2.9 TB/s) became 8.
-__global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4RowsParams p) {
+// Bound by instructions before memory (41 us under ncu: issue slots 68 % busy,
+// DRAM 42 %), so: the extrema of a lane's 8 rows are reduced and scattered in
+// one exchange (lane c % 8 ends up with row c % 8's, 7 shuffles instead of 24)
+// and a row's step and reciprocal are computed by that lane alone; codes come
+// two at a time (packed fp32). 32768 keys of 8 heads: 59 us before that (22
+// instructions a value), 34.3 us now (13; 172 MB, 5.0 TB/s = 76 % of a copy's
+// rate); four blocks an SM, 37.4 with the three that 65 registers allow.
+__global__ void __launch_bounds__(256, 4) kv4_write_kernel(const Kv4RowsParams p) {
   griddep_wait();
   griddep_launch_dependents();
   const int lane = threadIdx.x & 31, c = lane & 15;
@@ -231,7 +233,9 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4RowsParams p) {
   }
 }
 
-// Read back: the same item and lane mapping, the other way.
+// Read back: the same item and lane mapping, the other way. A nibble becomes a
+// float by a byte permutation under the exponent of 2^23 and one packed
+// subtraction. Bound by memory: 28.7 us for 32768 keys of 8 heads (91 %).
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4RowsParams p) {
   griddep_wait();
   griddep_launch_dependents();
