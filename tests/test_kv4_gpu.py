@@ -247,6 +247,40 @@ def test_attention(cuda, B, Hq, Hkv, n_prefix, n_keys, valid, bias_kind, qs):
     check_attend(cuda, q, k, v, valid, n_prefix, n_keys, bias, q_scale, cap=n_keys + 200, dev_keys=n_keys + 150)
 
 
+@pytest.mark.parametrize("B,Hq,Hkv,n_prefix,n_keys,bias_kind", [
+    (40, 2, 1, 70, 75, "row"),          # blocks shared among more rows than a warp holds at once
+    (70, 6, 3, 40, 40, None),           # more rows than a wave of blocks
+    (33, 4, 4, 260, 260, "head"),
+    (2, 40, 5, 700, 705, "row"),        # eight query heads per KV head, an odd number of them
+    (5, 14, 2, 3000, 3001, "head"),     # seven
+    (1, 3, 1, 20000, 20000, None),
+    (20, 16, 8, 500, 501, None),
+])
+def test_attention_unlike_rows(cuda, B, Hq, Hkv, n_prefix, n_keys, bias_kind):
+    """Rows of every length from none to all, so that blocks are shared unevenly."""
+    g = torch.Generator().manual_seed(n_keys * B)
+    q = torch.randn(B, Hq, 128, generator=g).bfloat16()
+    k, v = rows(g, B, n_keys, Hkv, 128) / 2, rows(g, B, n_keys, Hkv, 128)
+    valid = [(n_prefix * b * b) // max((B - 1) ** 2, 1) for b in range(B)]
+    valid[B // 3] = 0
+    for b in range(B):
+        k[b, valid[b]:n_prefix] = float("nan")
+    bias = None if bias_kind is None else torch.randn(B, Hq if bias_kind == "head" else 1, n_prefix, generator=g)
+    check_attend(cuda, q, k, v, valid, n_prefix, n_keys, bias)
+
+
+def test_attention_without_keys_on_the_device(cuda):
+    """A device-side count of none (or below): zeros, in both ways of merging."""
+    for B, n in ((1, 300), (3, 9000)):
+        c = KV4Cache(B, n, 2, device=cuda)
+        c.data.fill_(0xFF)
+        nv = torch.full((B,), n, dtype=torch.int32, device=cuda)
+        for count in (0, -1, -1000):
+            nk = torch.tensor([count], dtype=torch.int32, device=cuda)
+            out = ops.decode_attention_kv4(torch.ones(B, 4, 128, dtype=torch.bfloat16, device=cuda), c, nv, n, n, n_keys_dev=nk)
+            assert (out == 0).all()
+
+
 def test_attention_masks_of_lowest_value(cuda):
     """-1e9, the type's lowest value and -inf as biases: beside ordinary keys they get no weight, a row
     of the lowest value alone is uniform (as the fp32 sum makes it), a row of -inf alone gives zeros."""

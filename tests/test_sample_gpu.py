@@ -102,6 +102,36 @@ def test_flat_and_peaked(cuda, spread):
         run(cuda, x, u, 0.7, k=500, p=np.array([middle_p(xf[b], 0.7, 500, 250) for b in range(4)], dtype=np.float32))
 
 
+@pytest.mark.parametrize("B,V,spread", [(1, 151936, 0.3), (2, 151936, 0.05), (1, 524288, 1.0), (150, 3000, 0.3), (64, 40000, 0.2)])
+def test_long_and_flat_rows(cuda, B, V, spread):
+    """Boundary buckets of thousands of logits (lists of a block, of all blocks, none), and the longest row."""
+    g = torch.Generator().manual_seed(V + B)
+    for dtype in (torch.bfloat16, torch.float32):
+        x = (torch.randn(B, V, generator=g) * spread).to(dtype)
+        u, xf = torch.rand(B, generator=g).numpy(), x.float().numpy()
+        pick = lambda n: np.array([middle_p(xf[b], 1.0, 0, n) for b in range(B)], dtype=np.float32)  # noqa: E731
+        run(cuda, x, u, 1.0, p=pick(V // 2))
+        run(cuda, x, u, 1.0, k=V // 3)
+        if B == 1:
+            run(cuda, x, u, 1.0, k=V // 3, p=np.array([middle_p(xf[0], 1.0, V // 3, V // 9)], dtype=np.float32), m=0.2)
+
+
+@pytest.mark.parametrize("k", [2, 31, 32, 33, 200, 255, 256, 257, 300])
+def test_few_logits_at_their_limit(cuda, k):
+    """As many logits down to the k-th's bucket as one block orders by counting, one fewer and one more: k
+    isolated logits, the others far below."""
+    g = torch.Generator().manual_seed(k)
+    for V in (5000, 60000):
+        x = torch.full((3, V), -40.0) - torch.rand(3, V, generator=g)
+        for b in range(3):
+            x[b, torch.randperm(V, generator=g)[:k]] = 2 * torch.randn(k, generator=g)
+        u = np.array([0.1, 0.5, 0.95], dtype=np.float32)
+        xf = x.numpy()
+        run(cuda, x, u, 1.0, k=k)
+        run(cuda, x, u, 1.0, k=max(k - 1, 2), p=np.array([middle_p(xf[b], 1.0, max(k - 1, 2), k // 2) for b in range(3)], dtype=np.float32))
+        run(cuda, x, u, 1.0, k=k + 5, m=0.01)
+
+
 def test_ties_go_to_the_lowest_index(cuda):
     x = torch.zeros(6, 5000)
     x[:, 100::700] = 2.0                      # 7 ties at the top

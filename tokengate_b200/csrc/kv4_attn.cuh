@@ -22,7 +22,11 @@
 //       relative to a running maximum that may lag, s to a running power of
 //       two, so neither leaves fp16's range (maximum and power move together,
 //       in a branch that the first tiles take and later ones hardly ever).
-// Scores, maxima, sums and the accumulators are fp32.
+//       So that the rounding weighs code - 8 and not code, which is twice as
+//       large, sum_j p_j v_j is computed as sum (p s) code - 8 sum (p s) +
+//       sum p (low + 8 s), the first two sums of the same rounded p s.
+// Scores, maxima, sums and the accumulators are fp32: finite for keys and values
+// up to 2^100.
 //
 // The cache is read once, at 144 bytes per key: every warp streams its own
 // tiles through a ring of two or three in shared memory (one bulk copy of 4608
@@ -222,7 +226,7 @@ struct Kv4State {
   uint32_t qf[8][2];    // B fragments of q'
   float qs[2][2];       // sum(q') per group and column
   float mul[2];
-  float m[2], l[2], zs[2][2];  // running maximum, sum p, sum p * low per group
+  float m[2], l[2], zs[2][2];  // running maximum, sum p, sum p (low + 8 s) - 8 (p s) per group
   float acc[8][4];             // sum (p s) code, times 2^-24 (rows g) or 2^-20 (rows g + 8)
   float eref, einv;            // the power of two that s is relative to
 };
@@ -336,7 +340,7 @@ __device__ __forceinline__ void kv4_tile(Kv4State& st, const uint8_t* tile, int 
     }
   }
   // ---- p and its sums; p s as B fragments (two key rows to a register)
-  const float off[2] = {kKv4Head - st.m[0], kKv4Head - st.m[1]};
+  const float off[2] = {kKv4Head - st.m[0], kKv4Head - st.m[1]}, eight = -8.f * st.eref;
   uint32_t pf[2][R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
@@ -350,16 +354,19 @@ __device__ __forceinline__ void kv4_tile(Kv4State& st, const uint8_t* tile, int 
     }
 #pragma unroll
     for (int gr = 0; gr < 2; ++gr) {
-      const float z = kv4_low(gr ? vp[r].y : vp[r].x);
-      float u[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float zn = fmaf(p[j], z, st.zs[gr][j]);
-        u[j] = p[j] * sn[r][gr];
-        st.zs[gr][j] = BIAS && p[j] == 0.f ? st.zs[gr][j] : zn;  // a key that the bias masks may hold NaN
-        if (BIAS && p[j] == 0.f) u[j] = 0.f;
+      const uint32_t pm = gr ? vp[r].y : vp[r].x;
+      const float z = fmaf(8.f, kv4_scale(pm), kv4_low(pm));
+      float u[2] = {p[0] * sn[r][gr], p[1] * sn[r][gr]};
+      if (BIAS) {  // a key that the bias masks may hold NaN
+        u[0] = p[0] == 0.f ? 0.f : u[0];
+        u[1] = p[1] == 0.f ? 0.f : u[1];
       }
-      pf[gr][r] = movmatrix_trans(h2_bits(__floats2half2_rn(u[0], u[1])));
+      const __half2 h = __floats2half2_rn(u[0], u[1]);
+      const float2 hf = __half22float2(h);
+      const float z0 = fmaf(hf.x, eight, fmaf(p[0], z, st.zs[gr][0])), z1 = fmaf(hf.y, eight, fmaf(p[1], z, st.zs[gr][1]));
+      st.zs[gr][0] = BIAS && p[0] == 0.f ? st.zs[gr][0] : z0;
+      st.zs[gr][1] = BIAS && p[1] == 0.f ? st.zs[gr][1] : z1;
+      pf[gr][r] = movmatrix_trans(h2_bits(h));
     }
   }
   // ---- P V
@@ -411,7 +418,7 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
   if (clustered) cluster_arrive();
   griddep_wait();
   griddep_launch_dependents();
-  const int n_keys = p.n_keys_dev != nullptr ? min(__ldg(p.n_keys_dev), p.n_keys) : p.n_keys;
+  const int n_keys = p.n_keys_dev != nullptr ? max(min(__ldg(p.n_keys_dev), p.n_keys), 0) : p.n_keys;
   if (p.part != nullptr) {
     int first;
     kv4_share(p, n_keys, lane, [&](int, int f, int c) { return (int)blockIdx.x >= f && (int)blockIdx.x < f + c; }, b,
@@ -643,7 +650,7 @@ __global__ void __launch_bounds__(32 * kKv4CombineWarps) kv4_combine_kernel(cons
   griddep_wait();
   griddep_launch_dependents();
   const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int n_keys = p.n_keys_dev != nullptr ? min(__ldg(p.n_keys_dev), p.n_keys) : p.n_keys;
+  const int n_keys = p.n_keys_dev != nullptr ? max(min(__ldg(p.n_keys_dev), p.n_keys), 0) : p.n_keys;
   int found, first, C;
   kv4_share(p, n_keys, lane, [&](int r, int, int) { return r == b; }, found, first, C);
   if (C == 1) return;  // its one block has written the output

@@ -12,10 +12,10 @@
 // the same decision (V <= 2^19 keeps them in 64 bits).
 //
 // A cluster of C blocks takes a row, each an index range of it, whose weights
-// it computes once and keeps in shared memory (rows too long for that compute
-// them again in each pass). Bound by instructions and by the cluster's
-// barriers, not by memory: the row is read once. No sort: the k-th value (or
-// the value at which the mass reaches p) is found
+// it computes once and keeps in shared memory. Bound by instructions and by
+// latencies (barriers of the cluster and of the block), not by memory: the row
+// is read once. No sort: the k-th value (or the value at which the mass reaches
+// p) is found
 //   1. by a histogram over 1024 buckets of w, 32 to an octave (linear in w's
 //      bits: two instructions, and nearly linear in the logit, so that logits
 //      spread over many buckets and shared-memory atomics seldom collide):
@@ -163,12 +163,12 @@ __device__ __forceinline__ smp_u64 smp_warp_scan(smp_u64 v, int lane) {  // incl
 __device__ __forceinline__ uint32_t smp_warp_max(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
 __device__ __forceinline__ uint32_t smp_warp_min(uint32_t v) { return __reduce_min_sync(0xffffffffu, v); }
 
-// One row's state in a block. HELD: sw holds the weights of the block's range.
-template <typename T, bool HELD>
+// One row's state in a block.
+template <typename T>
 struct Smp {
   SmpShared& s;
   const T* x;   // the block's range of the row
-  float* sw;
+  float* sw;    // the range's weights (at first its logits, as fp32)
   int C, rank, n, w0, w1, lane, warp;  // this warp's indices [w0, w1) of the range, contiguous: index order is warp order
   SmpRow row;
   int turn, parity;
@@ -184,10 +184,6 @@ struct Smp {
   template <typename V>
   __device__ __forceinline__ V* remote(V* p, int r) const {
     return C > 1 ? cooperative_groups::this_cluster().map_shared_rank(p, r) : p;
-  }
-  __device__ __forceinline__ float weight(int i) const {
-    if (HELD) return sw[i];
-    return expf(smp_d(smp_load(x + i), row));
   }
   // To every thread: the sums of a and b, the minimum lo, the maximum hi and the sum of cnt (one value per block)
   // over the cluster; before[2]: a and b of the blocks of lower rank. s.red[w][0 .. 1] keeps a and b of warp w.
@@ -337,7 +333,7 @@ struct Smp {
     __syncthreads();
 #pragma unroll 4
     for (int i = w0 + lane; i < w1; i += 32) {
-      const float w = weight(i);
+      const float w = sw[i];
       const int e = smp_bucket(w);
       if (e < bk) {
         smp_add_mass(w, ah, al);
@@ -351,7 +347,7 @@ struct Smp {
     auto take = [&](int i) {
       const uint32_t k = smp_key(smp_load(x + i));
       if (k <= floor_key) return 0u;
-      smp_add_mass(weight(i), ih, il);
+      smp_add_mass(sw[i], ih, il);
       lo = min(lo, k);
       hi = max(hi, k);
       return k;
@@ -360,7 +356,7 @@ struct Smp {
       for (uint32_t j = threadIdx.x; j < m; j += kSmpThreads) list[j] = take(s.at[j]);
     } else {
       for (int i = w0 + lane; i < w1; i += 32) {
-        const float w = weight(i);
+        const float w = sw[i];
         if (smp_bucket(w) == bk && w > 0.f) take(i);
       }
     }
@@ -381,7 +377,7 @@ struct Smp {
     __syncthreads();
 #pragma unroll 4
     for (int i = w0 + lane; i < w1; i += 32) {
-      const float w = weight(i);
+      const float w = sw[i];
       if (smp_bucket(w) <= bk && w > 0.f) s.at[atomicAdd(&s.n_list, 1u)] = (uint16_t)i;
     }
     __syncthreads();
@@ -609,7 +605,7 @@ struct Smp {
         }
       } else {
         for (int i = w0 + lane; i < w1; i += 32) {
-          const float w = weight(i);
+          const float w = sw[i];
           if (smp_bucket(w) != bk || w == 0.f) continue;
           const uint32_t k = smp_key(smp_load(x + i));
           if ((k & mask) == prefix) add_to_bin<BY_MASS>(dig, (k >> shift) & 255u, w);
@@ -629,7 +625,7 @@ struct Smp {
   }
 };
 
-template <typename T, bool HELD>
+template <typename T>
 __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SampleParams p) {
   extern __shared__ __align__(16) uint8_t smp_dyn[];
   SmpShared& s = *reinterpret_cast<SmpShared*>(smp_dyn);
@@ -637,7 +633,7 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SamplePara
   const int b = blockIdx.y;
   const int i0 = min((int)blockIdx.x * p.chunk, p.V), n = min(p.chunk, p.V - i0);
   const int per = p.chunk / kSmpWarps;
-  Smp<T, HELD> c{s,
+  Smp<T> c{s,
                  static_cast<const T*>(p.logits) + (int64_t)b * p.row_stride + i0,
                  reinterpret_cast<float*>(smp_dyn + sizeof(SmpShared)),
                  (int)gridDim.x,
@@ -692,18 +688,16 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SamplePara
         }
 #pragma unroll
         for (int e = 0; e < kVec; e += 2) top = fmax3(top, f[e], f[e + 1]);
-        if (HELD) {
 #pragma unroll
-          for (int e = 0; e < kVec / 4; ++e)
-            reinterpret_cast<float4*>(c.sw)[i * (kVec / 4) + e] =
-                make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
-        }
+        for (int e = 0; e < kVec / 4; ++e)
+          reinterpret_cast<float4*>(c.sw)[i * (kVec / 4) + e] =
+              make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
       }
       vec_done = nv * kVec;
     }
     for (int i = vec_done + tid; i < n; i += kSmpThreads) {
       const float v = smp_load(c.x + i);
-      if (HELD) c.sw[i] = v;
+      c.sw[i] = v;
       top = fmaxf(top, v);
     }
   }
@@ -745,8 +739,8 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SamplePara
     uint32_t hi = 0, lo = 0, far = 0;
 #pragma unroll 4
     for (int i = c.w0 + lane; i < c.w1; i += 32) {
-      const float w = expf(smp_d(HELD ? c.sw[i] : smp_load(c.x + i), c.row));
-      if (HELD) c.sw[i] = w;
+      const float w = expf(smp_d(c.sw[i], c.row));
+      c.sw[i] = w;
       if (!cut) {
         if (w >= min_p) smp_add_mass(w, hi, lo);
       } else if (w > 0.f) {
@@ -849,7 +843,7 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SamplePara
     const uint32_t* list = s.own[c.turn ^ 1];
     for (uint32_t j = tid; j < s.n_list; j += kSmpThreads) {
       const int i = s.at[j];
-      if (list[j] > thr) atomicAdd(&s.red[i / per][0], smp_mass(c.weight(i)));
+      if (list[j] > thr) atomicAdd(&s.red[i / per][0], smp_mass(c.sw[i]));
       else if (list[j] == thr && ties != 0) atomicAdd(&s.red[i / per][1], 1ull);
     }
     __syncthreads();
@@ -860,7 +854,7 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SamplePara
     uint32_t hi = 0, lo = 0, nt = 0;
 #pragma unroll 2
     for (int i = c.w0 + lane; i < c.w1; i += 32) {
-      const float w = c.weight(i);
+      const float w = c.sw[i];
       const int a = admitted(i, w);
       if (a == 1) smp_add_mass(w, hi, lo);
       if (a == 2) ++nt;
@@ -892,7 +886,7 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SamplePara
       const int r0 = min(c.w0 + lane * run, c.w1), r1 = min(r0 + run, c.w1);
       uint32_t hi = 0, lo = 0, nt = 0;
       for (int i = r0; i < r1; ++i) {
-        const float w = c.weight(i);
+        const float w = c.sw[i];
         const int a = admitted(i, w);
         if (a == 1) smp_add_mass(w, hi, lo);
         if (a == 2) ++nt;
@@ -905,7 +899,7 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SamplePara
       const int j0 = __shfl_sync(0xffffffffu, r0, src), j1 = __shfl_sync(0xffffffffu, r1, src);
       for (int base = j0; base < j1; base += 32) {
         const int i = base + lane;
-        const float w = i < j1 ? c.weight(i) : 0.f;
+        const float w = i < j1 ? c.sw[i] : 0.f;
         const int a = i < j1 ? admitted(i, w) : 0;
         const smp_u64 sm = fm + smp_warp_scan(a == 1 ? smp_mass(w) : 0ull, lane);
         const uint32_t tm = __ballot_sync(0xffffffffu, a == 2);

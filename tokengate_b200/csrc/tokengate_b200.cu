@@ -82,6 +82,17 @@ cudaError_t smem_limit_once(Kern kern, int bytes, bool (&flags)[kMaxDevices], in
   return e;
 }
 
+// The same for a kernel launched as clusters of up to 16 blocks.
+template <typename Kern>
+cudaError_t cluster_limits_once(Kern kern, int bytes, bool (&flags)[kMaxDevices], int dev) {
+  std::lock_guard<std::mutex> lk(g_mu);
+  if (flags[dev]) return cudaSuccess;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) flags[dev] = true;
+  return e;
+}
+
 int current_device(int* dev) {
   cudaError_t e = cudaGetDevice(dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
@@ -1564,9 +1575,7 @@ int tg_decode_attn_kv4(const void* q, int64_t q_sb, int64_t q_sh, const float* q
   auto kern = bias != nullptr ? (pair ? tg::kv4_attn_kernel<true, true> : tg::kv4_attn_kernel<true, false>)
                               : (pair ? tg::kv4_attn_kernel<false, true> : tg::kv4_attn_kernel<false, false>);
   bool(&flags)[kMaxDevices] = g_kv4_attr_set[2 * (bias != nullptr) + pair];
-  cudaError_t e = cudaSuccess;
-  if (!flags[dev]) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e == cudaSuccess) e = smem_limit_once(kern, tg::kv4_attn_smem(tg::kKv4MaxWarps, 2), flags, dev);
+  cudaError_t e = cluster_limits_once(kern, tg::kv4_attn_smem(tg::kKv4MaxWarps, 2), flags, dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(decode_attn_kv4)");
   const dim3 grid((unsigned)(need > 0 ? shape.parts + B : shape.cluster), (unsigned)Hkv, (unsigned)(need > 0 ? 1 : B));
   const dim3 block(32u * shape.warps);
@@ -1583,8 +1592,11 @@ int tg_decode_attn_kv4(const void* q, int64_t q_sb, int64_t q_sh, const float* q
 
 // ---- sampling
 namespace {
-bool g_smp_attr_set[4][kMaxDevices] = {};  // per dtype and whether the weights are held
+bool g_smp_attr_set[2][kMaxDevices] = {};  // per dtype
 constexpr int kSmpMaxSmem = 227 * 1024;
+static_assert(sizeof(tg::SmpShared) + tg::kSmpMaxV / tg::kSmpMaxCluster * sizeof(float) <= kSmpMaxSmem,
+              "the longest row's weights fit the largest cluster");
+static_assert(tg::kSmpMaxV / tg::kSmpMaxCluster <= 65536, "places in a block's range fit 16 bits");
 }  // namespace
 
 int tg_sample(const void* logits, int dtype, int64_t row_stride, int B, int V, const float* u,
@@ -1622,16 +1634,11 @@ int tg_sample(const void* logits, int dtype, int64_t row_stride, int B, int V, c
          (((int64_t)B * C * 2 <= sms && V > C * 4096) || smem_of(C) > (size_t)kSmpMaxSmem / 2 - 1024))
     C *= 2;
   p.chunk = chunk_of(C);
-  const bool held = smem_of(C) <= (size_t)kSmpMaxSmem;
-  auto kern = dtype ? (held ? tg::sample_kernel<__nv_bfloat16, true> : tg::sample_kernel<__nv_bfloat16, false>)
-                    : (held ? tg::sample_kernel<float, true> : tg::sample_kernel<float, false>);
-  bool(&flags)[kMaxDevices] = g_smp_attr_set[2 * dtype + held];
-  cudaError_t e = cudaSuccess;
-  if (!flags[dev]) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  if (e == cudaSuccess) e = smem_limit_once(kern, kSmpMaxSmem, flags, dev);
+  auto kern = dtype ? tg::sample_kernel<__nv_bfloat16> : tg::sample_kernel<float>;
+  cudaError_t e = cluster_limits_once(kern, kSmpMaxSmem, g_smp_attr_set[dtype], dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(sample)");
   e = launch_cluster(kern, dim3((unsigned)C, (unsigned)B), dim3(tg::kSmpThreads),
-                     held ? smem_of(C) : sizeof(tg::SmpShared), static_cast<cudaStream_t>(stream), C, p);
+                     smem_of(C), static_cast<cudaStream_t>(stream), C, p);
   if (e != cudaSuccess) return cuda_fail(e, "sample launch");
   return TG_OK;
 }
