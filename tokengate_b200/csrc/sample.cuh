@@ -19,11 +19,12 @@
 //   1. by a histogram over 1024 buckets of w, 32 to an octave (linear in w's
 //      bits: two instructions, and nearly linear in the logit, so that logits
 //      spread over many buckets and shared-memory atomics seldom collide):
-//      counts for k; for p the top 12 bits of the mantissas, as a guess only.
-//      Each block owns a slice of the row's and hands it to the others;
+//      counts, exact for k; for p the guess that a bucket's logits weigh its
+//      middle each. Each block owns a slice of the row's and hands it to the
+//      others;
 //   2. exactly inside that bucket: one pass gives the mass above it and in it,
-//      its smallest and largest logit and the list of its logits (a wrong guess
-//      moves by a bucket); where the two differ (bf16 logits: hardly ever),
+//      its smallest and largest logit and the list of its logits (after a wrong
+//      guess, the next one from there); where the two differ (bf16 logits: hardly ever),
 //      every block narrows them down on a copy of all lists, so without a
 //      cluster barrier (lists too long for that: digits, over the row again).
 // Where no more than 256 logits reach down to the k-th's bucket, they go to one
@@ -69,10 +70,10 @@ struct SampleParams {
 typedef unsigned long long smp_u64;
 
 struct alignas(16) SmpShared {
-  uint32_t own[2][kSmpBuckets];   // this block's histograms (counts, masses); then lists of a bucket's logits, by turns
-  uint32_t tot[2][kSmpBuckets];   // the row's histograms
+  uint32_t own[2][kSmpBuckets];   // [0]: this block's histogram; then lists of a bucket's logits, by turns
+  uint32_t tot[kSmpBuckets];      // the row's histogram
   union {
-    uint32_t all[kSmpAllLists];   // this block's slices of the row's histograms; then the blocks' lists together
+    uint32_t all[kSmpAllLists];   // this block's slice of the row's histogram; then the blocks' lists together
     struct {                      // or, in block 0, the few logits down to the k-th's bucket
       smp_u64 few_ord[kSmpFew];   // ordered logit above the index's complement: the order of the row, descending
       smp_u64 few_mass[kSmpFew];
@@ -85,7 +86,7 @@ struct alignas(16) SmpShared {
   double scan[kSmpWarps];
   smp_u64 pick_above;
   int pick;
-  uint32_t n_list, n_few;
+  uint32_t n_list, n_few, key_lo, key_hi;
 };
 
 __device__ __forceinline__ uint32_t smp_key(float x) {
@@ -118,6 +119,18 @@ struct SmpRow {
   }
   __device__ __forceinline__ float product(float x) const { return __fmaf_rn(x, rh, __fmul_rn(x, rl)); }
 };
+// The weights of two logits, as exp(smp_d) gives them, of a usual row: two at a
+// time up to the exponentials, whose results for NaN become 0.
+__device__ __forceinline__ float2 smp_weights2(float x, float y, const SmpRow& r) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, h, l, z;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 h, {%4, %4};\n\tmov.b64 l, {%5, %5};\n\tmov.b64 z, {%6, %6};\n\t"
+      "mul.rn.f32x2 l, a, l;\n\tfma.rn.f32x2 a, a, h, l;\n\tadd.rn.f32x2 a, a, z;\n\t"
+      "mov.b64 {%0, %1}, a;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(x), "f"(y), "f"(r.rh), "f"(r.rl), "f"(-r.zmax));
+  return make_float2(fmaxf(expf(d.x), 0.f), fmaxf(expf(d.y), 0.f));
+}
 __device__ __forceinline__ float smp_d(float x, const SmpRow& r) {
   float d;
   if (r.plain) {
@@ -127,23 +140,24 @@ __device__ __forceinline__ float smp_d(float x, const SmpRow& r) {
   }
   return d <= 0.f ? d : -INFINITY;  // NaN: a NaN logit, -inf times 0, or quotients that both overflowed
 }
-__device__ __forceinline__ int smp_bucket(float w) {
-  return min(max((int)(0x3F7FFFFFu - __float_as_uint(w)) >> 18, 0), kSmpBuckets - 1);
+// Bucket e holds the weights in (smp_upper(e + 1), smp_upper(e)], the last one all the positive ones below.
+__device__ __forceinline__ uint32_t smp_bucket(float w) {
+  return min((0x3F800000u - __float_as_uint(w)) >> 18, (uint32_t)kSmpBuckets - 1u);
 }
-// w * 2^44 rounded to an integer, w in [0, 1]: its 22 bits above 2^-22 and the
-// 22 below, each read off the mantissa of 2 + ...
-__device__ __forceinline__ void smp_add_mass(float w, uint32_t& hi, uint32_t& lo) {
-  const float t = __fadd_rz(w, 2.f);
-  const float rest = __fsub_rn(w, __fsub_rn(t, 2.f));
-  hi += __float_as_uint(t) - 0x40000000u;
-  lo += __float_as_uint(__fmaf_rn(rest, 4194304.f, 2.f)) - 0x40000000u;
+__device__ __forceinline__ float smp_upper(int e) {
+  return e >= kSmpBuckets ? 0.f : __uint_as_float(0x3F800000u - ((uint32_t)e << 18));
 }
-__device__ __forceinline__ smp_u64 smp_mass(uint32_t hi, uint32_t lo) { return ((smp_u64)hi << 22) + lo; }
-__device__ __forceinline__ smp_u64 smp_mass(float w) {
-  uint32_t hi = 0, lo = 0;
-  smp_add_mass(w, hi, lo);
-  return smp_mass(hi, lo);
-}
+// A mass: w * 2^44 cut to an integer. A thread sums up to 256 of them in a
+// double that starts at 256, whose last bit is worth 2^-44: the cut is the
+// addition's own, two instructions a weight where integers take six.
+__device__ __forceinline__ smp_u64 smp_mass(float w) { return (smp_u64)__float2ull_rz(w * 17592186044416.f); }
+struct SmpSum {
+  double v = 256.;
+  __device__ __forceinline__ void add(float w) { v = __dadd_rz(v, (double)w); }
+  __device__ __forceinline__ smp_u64 get() const {
+    return (smp_u64)__double_as_longlong(v) & ((1ull << 52) - 1ull);  // v in [256, 512): the mantissa counts
+  }
+};
 
 // sum over the warp: 24-bit pieces (32 of them stay below 2^32), one reduction instruction each
 __device__ __forceinline__ smp_u64 smp_warp_sum(smp_u64 v) {
@@ -180,6 +194,30 @@ struct Smp {
     } else {
       __syncthreads();
     }
+  }
+  // Logits i to i + 3 (i a multiple of 4; -inf past the range)
+  __device__ __forceinline__ float4 logits4(int i) const {
+    constexpr int kBytes = 4 * sizeof(T);
+    if ((reinterpret_cast<uintptr_t>(x) & (kBytes - 1)) == 0 && i + 4 <= n) {
+      if constexpr (sizeof(T) == 4) {
+        return __ldg(reinterpret_cast<const float4*>(x + i));
+      } else {
+        const uint2 q = __ldg(reinterpret_cast<const uint2*>(x + i));
+        return make_float4(__uint_as_float(q.x << 16), __uint_as_float(q.x & 0xFFFF0000u), __uint_as_float(q.y << 16),
+                           __uint_as_float(q.y & 0xFFFF0000u));
+      }
+    }
+    float f[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = i + e < n ? smp_load(x + i + e) : -INFINITY;
+    return make_float4(f[0], f[1], f[2], f[3]);
+  }
+  __device__ __forceinline__ float weight_of(float logit) const { return expf(smp_d(logit, row)); }
+  // f(i, what is held of indices i to i + 3) over this warp's range, each lane every 32nd four
+  template <typename F>
+  __device__ __forceinline__ void each4(F f) const {
+#pragma unroll 2
+    for (int i = w0 + 4 * lane; i < w1; i += 128) f(i, *reinterpret_cast<float4*>(sw + i));
   }
   template <typename V>
   __device__ __forceinline__ V* remote(V* p, int r) const {
@@ -241,40 +279,46 @@ struct Smp {
     if (over) cnt = kSmpNoLists;
   }
 
-  // The row's histogram `which` (0: counts, 1: masses) into every block's s.tot: each block's goes to the owners of
-  // its slices, and from there to all. In two steps, with a cluster barrier after each.
-  __device__ __forceinline__ void merge_to_owner(int which) {
+  // The row's histogram into every block's s.tot: each block's goes to the owners of its slices, and from there to
+  // all. In two steps, with a cluster barrier after each.
+  __device__ __forceinline__ void merge_to_owner() {
     const int slice = kSmpBuckets / C;
     for (int i = threadIdx.x; i < kSmpBuckets; i += kSmpThreads) {
-      const uint32_t v = s.own[which][i];
+      const uint32_t v = s.own[0][i];
       if (C == 1) {
-        s.tot[which][i] = v;
+        s.tot[i] = v;
       } else if (v != 0u) {
-        atomicAdd(remote(s.all, i / slice) + which * (kSmpAllLists / 2) + i % slice, v);
+        atomicAdd(remote(s.all, i / slice) + i % slice, v);
       }
     }
   }
-  __device__ __forceinline__ void merge_to_all(int which) {
+  __device__ __forceinline__ void merge_to_all() {
     const int slice = kSmpBuckets / C;
     for (int i = threadIdx.x; i < kSmpBuckets / 4; i += kSmpThreads) {  // 4 buckets to one block
       const int to = i / (slice / 4), j = i % (slice / 4);
-      *(reinterpret_cast<uint4*>(remote(s.tot[which], to) + rank * slice) + j) =
-          *(reinterpret_cast<const uint4*>(s.all + which * (kSmpAllLists / 2)) + j);
+      *(reinterpret_cast<uint4*>(remote(s.tot, to) + rank * slice) + j) = *(reinterpret_cast<const uint4*>(s.all) + j);
     }
   }
 
-  // First bucket at which the running count / mass reaches `target` (the last if none does), and what is before it.
+  // First bucket at which the running count / mass reaches `target` (the last if none does), but of b0 to b1; what is
+  // before it, and in it.
+  // A bucket's mass is guessed as its count times its middle; the far tail's as next to nothing.
   template <bool BY_MASS>
-  __device__ __forceinline__ int crossing(double target, double& above) {
+  __device__ __forceinline__ int crossing(double target, int b0, int b1, double& above, double& inside) {
     constexpr int E = kSmpBuckets / kSmpThreads;
     const int tid = threadIdx.x;
-    const uint32_t* tot = s.tot[BY_MASS ? 1 : 0];
     double v[E], run = 0.;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int i = E * tid + e;
-      v[e] = (double)tot[i];
-      if (BY_MASS) v[e] *= __longlong_as_double((long long)(1023 - 12 - (i >> 5)) << 52);  // units of [2^-1-o, 2^-o)
+      const uint32_t cnt = s.tot[i];
+      if (BY_MASS) {
+        const float mid = i == kSmpBuckets - 1 ? 1e-20f : __uint_as_float(0x3F800000u - ((uint32_t)i << 18) - (1u << 17));
+        v[e] = (double)cnt * (double)mid;
+        if (i == 0) v[e] += 1. - (double)mid;  // of the first bucket's one is the largest
+      } else {
+        v[e] = (double)cnt;
+      }
       run += v[e];
     }
     const double mine = run;
@@ -307,47 +351,62 @@ struct Smp {
       }
     }
     __syncthreads();
-    const int bk = s.pick;
+    const int bk = min(max(s.pick, b0), b1);
     if (bk / E == tid) {
 #pragma unroll
-      for (int e = 0; e < E; ++e)
+      for (int e = 0; e < E; ++e) {
         if (e < bk % E) before += v[e];
+        if (e == bk % E) s.scan[1] = v[e];
+      }
       s.scan[0] = before;
     }
     __syncthreads();
     above = s.scan[0];
+    inside = s.scan[1];
     __syncthreads();
     return bk;
   }
 
-  // Of the elements in buckets up to `bk` (in `bk` itself only those of a logit above `floor_key`): the mass
-  // above bucket bk, the mass in it, the range of its logits (hi 0: none). Each block lists its logits of the bucket
-  // (0 for those not above floor_key), `cnt` in all.
-  __device__ __forceinline__ void look(int bk, uint32_t floor_key, smp_u64& above, smp_u64& inside, uint32_t& lo,
+  // Notes in s.at which of w, the weights of indices i to i + 3, are in (w_in, w_over], as long as there is room.
+  __device__ __forceinline__ void note(int i, const float (&w)[4], float w_in, float w_over, uint32_t room) {
+    bool in[4];
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m += in[e] = w[e] > w_in && !(w[e] > w_over);
+    if (m) {
+      uint32_t j = atomicAdd(&s.n_list, m);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (in[e] && j < room) s.at[j] = (uint16_t)(i + e);
+        j += in[e];
+      }
+    }
+  }
+
+  // Of the elements in buckets up to `b1` (only those of a logit above `floor_key`, which is below bucket b0 or in b1):
+  // the mass above bucket b0, the mass in b0 to b1, the range of the logits there (hi 0: none). Each block lists its
+  // logits there (0 for those not above floor_key), `cnt` in all.
+  __device__ __forceinline__ void look(int b0, int b1, uint32_t floor_key, smp_u64& above, smp_u64& inside, uint32_t& lo,
                                        uint32_t& hi, uint32_t& cnt) {
-    uint32_t ah = 0, al = 0, ih = 0, il = 0;
+    SmpSum over, in;
+    const float w_over = smp_upper(b0), w_in = smp_upper(b1 + 1);
     uint32_t* list = s.own[turn];
     lo = 0xFFFFFFFFu;
     hi = 0;
     if (threadIdx.x == 0) s.n_list = 0u;
     __syncthreads();
-#pragma unroll 4
-    for (int i = w0 + lane; i < w1; i += 32) {
-      const float w = sw[i];
-      const int e = smp_bucket(w);
-      if (e < bk) {
-        smp_add_mass(w, ah, al);
-      } else if (e == bk && w > 0.f) {
-        const uint32_t j = atomicAdd(&s.n_list, 1u);
-        if (j < kSmpList) s.at[j] = (uint16_t)i;
-      }
-    }
+    each4([&](int i, float4 q) {
+      const float w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) over.add(w[e] > w_over ? w[e] : 0.f);
+      note(i, w, w_in, w_over, kSmpList);
+    });
     __syncthreads();
     const uint32_t m = s.n_list;
     auto take = [&](int i) {
       const uint32_t k = smp_key(smp_load(x + i));
       if (k <= floor_key) return 0u;
-      smp_add_mass(sw[i], ih, il);
+      in.add(sw[i]);
       lo = min(lo, k);
       hi = max(hi, k);
       return k;
@@ -356,16 +415,27 @@ struct Smp {
       for (uint32_t j = threadIdx.x; j < m; j += kSmpThreads) list[j] = take(s.at[j]);
     } else {
       for (int i = w0 + lane; i < w1; i += 32) {
-        const float w = sw[i];
-        if (smp_bucket(w) == bk && w > 0.f) take(i);
+        if (sw[i] > w_in && !(sw[i] > w_over)) take(i);
       }
     }
-    above = smp_mass(ah, al);
-    inside = smp_mass(ih, il);
+    above = over.get();
+    inside = in.get();
     reduce(above, inside, lo, hi, cnt, nullptr);
   }
 
-  __device__ __forceinline__ float weight_of_key(uint32_t key) const { return expf(smp_d(smp_unkey(key), row)); }
+  // The mass of the listed logits above `key` (lists that did not run over).
+  __device__ __forceinline__ void listed_above(uint32_t key, smp_u64& mass) {
+    SmpSum sum;
+    const uint32_t* list = s.own[turn ^ 1];
+    for (uint32_t j = threadIdx.x; j < s.n_list; j += kSmpThreads)
+      if (list[j] > key) sum.add(sw[s.at[j]]);
+    smp_u64 none = 0;
+    uint32_t lo = 0, hi = 0, cnt;
+    mass = sum.get();
+    reduce(mass, none, lo, hi, cnt, nullptr);
+  }
+
+  __device__ __forceinline__ float weight_of_key(uint32_t key) const { return weight_of(smp_unkey(key)); }
   __device__ __forceinline__ smp_u64 mass_of_key(uint32_t key) const { return smp_mass(weight_of_key(key)); }
 
   // The row's token from the elements in buckets up to `bk`, kSmpFew at most, of which the k largest and the rest of
@@ -375,11 +445,11 @@ struct Smp {
     const int tid = threadIdx.x;
     if (tid == 0) s.n_list = 0u;
     __syncthreads();
-#pragma unroll 4
-    for (int i = w0 + lane; i < w1; i += 32) {
-      const float w = sw[i];
-      if (smp_bucket(w) <= bk && w > 0.f) s.at[atomicAdd(&s.n_list, 1u)] = (uint16_t)i;
-    }
+    const float w_in = smp_upper(bk + 1);
+    each4([&](int i, float4 q) {
+      const float w[4] = {q.x, q.y, q.z, q.w};
+      note(i, w, w_in, 1.f, kSmpFew);
+    });
     __syncthreads();
     const uint32_t own = s.n_list;
     if (tid == 0) s.pick = (int)atomicAdd(remote(&s.n_few, 0), own);
@@ -455,19 +525,19 @@ struct Smp {
     }
   }
 
-  // Of the histogram dig[3][256], digits or bins in order: where the running sum reaches `need`, to s.pick and, less the
-  // sum before it, s.pick_above. By warp 0; C: summed over the cluster's blocks.
-  template <bool ASCENDING>
-  __device__ __forceinline__ void pick_bin(uint32_t* dig, int blocks, smp_u64 need) {
+  // A bin's sum of the histogram dig[3][256].
+  __device__ __forceinline__ static smp_u64 bin(const uint32_t* dig, int i) {
+    return dig[i] + ((smp_u64)dig[256 + i] << 15) + ((smp_u64)dig[512 + i] << 30);
+  }
+
+  // Of 256 bins, in order: where the running sum of at(bin) reaches `need`, to s.pick and, less the sum before it,
+  // s.pick_above. By warp 0.
+  template <bool ASCENDING, typename F>
+  __device__ __forceinline__ void pick_bin(F at, smp_u64 need) {
     smp_u64 v[8], sum = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int i = ASCENDING ? lane * 8 + e : 255 - (lane * 8 + e);
-      v[e] = 0;
-      for (int c = 0; c < blocks; ++c) {
-        const uint32_t* from = blocks == 1 ? dig : remote(dig, c);
-        v[e] += from[i] + ((smp_u64)from[256 + i] << 15) + ((smp_u64)from[512 + i] << 30);
-      }
+      v[e] = at(ASCENDING ? lane * 8 + e : 255 - (lane * 8 + e));
       sum += v[e];
     }
     smp_u64 before = smp_warp_scan(sum, lane) - sum;
@@ -484,18 +554,18 @@ struct Smp {
     }
   }
 
-  // Exact selection inside bucket `bk`, whose admitted logits span [lo, hi] and were listed by the last look()
-  // (`cnt` of them): the key and the number of its ties such that the bucket's elements above the key, and those
+  // Exact selection inside buckets b0 to b1, whose admitted logits span [lo, hi] and were listed by the last look()
+  // (`cnt` of them): the key and the number of its ties such that the buckets' elements above the key, and those
   // ties, are the fewest whose count (BY_MASS: mass) reaches `need`.
   template <bool BY_MASS>
-  __device__ __forceinline__ void refine(int bk, uint32_t lo, uint32_t hi, uint32_t cnt, smp_u64 need, uint32_t& key,
+  __device__ __forceinline__ void refine(int b0, int b1, uint32_t lo, uint32_t hi, uint32_t cnt, smp_u64 need, uint32_t& key,
                                          smp_u64& ties) {
     if (lo == hi) {
       key = lo;
     } else if (cnt < kSmpAllLists) {
       select_listed<BY_MASS>(lo, hi, cnt, need, key);
     } else {
-      select_digits<BY_MASS>(bk, lo, hi, cnt != kSmpNoLists, need, key);
+      select_digits<BY_MASS>(b0, b1, lo, hi, cnt != kSmpNoLists, need, key);
     }
     ties = need;
     if (BY_MASS) {
@@ -554,28 +624,43 @@ struct Smp {
       }
       const int shift = max(0, 24 - __clz(hi - lo));
       for (int i = threadIdx.x; i < 3 * 256; i += kSmpThreads) dig[i] = 0u;
-      if (threadIdx.x == 0) s.n_few = 0u;
+      if (threadIdx.x == 0) {
+        s.n_few = 0u;
+        s.key_lo = 0xFFFFFFFFu;
+        s.key_hi = 0u;
+      }
       __syncthreads();
       for (uint32_t i = threadIdx.x; i < cnt; i += kSmpThreads) {
         const uint32_t k = cur[i];
         if (k >= lo && k <= hi) add_to_bin<BY_MASS>(dig, (hi - k) >> shift, BY_MASS ? weight_of_key(k) : 0.f);
       }
       __syncthreads();
-      if (warp == 0) pick_bin<true>(dig, 1, need);
+      if (warp == 0) pick_bin<true>([&](int i) { return bin(dig, i); }, need);
       __syncthreads();
       need -= s.pick_above;
       hi -= (uint32_t)s.pick << shift;
-      lo = max(lo, hi - ((1u << shift) - 1u));
-      // the bin's keys to a list of their own, if they fit
-      uint32_t* kept = s.tot[0] + flip * kHalf;
+      lo = max(lo, hi - ((1u << shift) - 1u));  // (the picked bin: something is in it)
+      // the bin's keys to a list of their own, if they fit, and their range (of bf16 logits they are often alike)
+      uint32_t* kept = s.own[turn] + flip * kHalf;
+      uint32_t k0 = 0xFFFFFFFFu, k1 = 0u;
       for (uint32_t i = threadIdx.x; i < cnt; i += kSmpThreads) {
         const uint32_t k = cur[i];
         if (k >= lo && k <= hi) {
           const uint32_t at = atomicAdd(&s.n_few, 1u);
           if (at < kHalf) kept[at] = k;
+          k0 = min(k0, k);
+          k1 = max(k1, k);
         }
       }
+      k0 = smp_warp_min(k0);
+      k1 = smp_warp_max(k1);
+      if (lane == 0 && k1 != 0u) {
+        atomicMin(&s.key_lo, k0);
+        atomicMax(&s.key_hi, k1);
+      }
       __syncthreads();
+      lo = s.key_lo;
+      hi = s.key_hi;
       if (s.n_few <= kHalf) {
         cur = kept;
         cnt = s.n_few;
@@ -587,7 +672,7 @@ struct Smp {
   // block over its own list (or, where a list ran over, over its part of the row: that sees the whole bucket, whose
   // order above a floor that look() was given is the same), with a cluster barrier each.
   template <bool BY_MASS>
-  __device__ __forceinline__ void select_digits(int bk, uint32_t lo, uint32_t hi, bool listed, smp_u64& need,
+  __device__ __forceinline__ void select_digits(int b0, int b1, uint32_t lo, uint32_t hi, bool listed, smp_u64& need,
                                                 uint32_t& key) {
     const int top = 31 - __clz(lo ^ hi);
     uint32_t mask = top == 31 ? 0u : ~((2u << top) - 1u), prefix = hi & mask;
@@ -606,13 +691,21 @@ struct Smp {
       } else {
         for (int i = w0 + lane; i < w1; i += 32) {
           const float w = sw[i];
-          if (smp_bucket(w) != bk || w == 0.f) continue;
+          if (!(w > smp_upper(b1 + 1)) || w > smp_upper(b0)) continue;
           const uint32_t k = smp_key(smp_load(x + i));
           if ((k & mask) == prefix) add_to_bin<BY_MASS>(dig, (k >> shift) & 255u, w);
         }
       }
       sync();
-      if (warp == 0) pick_bin<false>(dig, C, need);
+      smp_u64* all = reinterpret_cast<smp_u64*>(s.all);
+      if (threadIdx.x < 256) {  // over the cluster's blocks
+        smp_u64 v = 0;
+#pragma unroll 4
+        for (int r = 0; r < C; ++r) v += bin(remote(dig, r), threadIdx.x);
+        all[threadIdx.x] = v;
+      }
+      __syncthreads();
+      if (warp == 0) pick_bin<false>([&](int i) { return all[i]; }, need);
       __syncthreads();
       const uint32_t dmask = 255u << shift;
       need -= s.pick_above;
@@ -661,45 +754,16 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SamplePara
   const bool by_k = top_k > 1u && top_k < (uint32_t)p.V, by_p = top_p < 1.f && top_k > 1u;
 
   for (int i = tid; i < kSmpBuckets; i += kSmpThreads) s.own[0][i] = s.own[1][i] = 0u;
-  for (int i = tid; i < kSmpAllLists; i += kSmpThreads) s.all[i] = 0u;
+  for (int i = tid; i < kSmpBuckets; i += kSmpThreads) s.all[i] = 0u;
   if (tid == 0) s.n_list = s.n_few = 0u;
 
   // ---- the largest logit; the range goes to shared memory as fp32 (a NaN as it is: it gets no weight below)
   float top = -INFINITY;
-  constexpr int kVec = 16 / sizeof(T);
-  int vec_done = 0;  // elements loaded as vectors
-  {
-    if ((reinterpret_cast<uintptr_t>(c.x) & 15) == 0) {
-      const uint4* xv = reinterpret_cast<const uint4*>(c.x);
-      const int nv = n / kVec;
-#pragma unroll 4
-      for (int i = tid; i < nv; i += kSmpThreads) {
-        const uint4 q = ld_nc_v4(xv + i);
-        const uint32_t wd[4] = {q.x, q.y, q.z, q.w};
-        float f[kVec];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (kVec == 4) {
-            f[e] = __uint_as_float(wd[e]);
-          } else {
-            f[2 * e % kVec] = __uint_as_float(wd[e] << 16);
-            f[(2 * e + 1) % kVec] = __uint_as_float(wd[e] & 0xFFFF0000u);
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < kVec; e += 2) top = fmax3(top, f[e], f[e + 1]);
-#pragma unroll
-        for (int e = 0; e < kVec / 4; ++e)
-          reinterpret_cast<float4*>(c.sw)[i * (kVec / 4) + e] =
-              make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
-      }
-      vec_done = nv * kVec;
-    }
-    for (int i = vec_done + tid; i < n; i += kSmpThreads) {
-      const float v = smp_load(c.x + i);
-      c.sw[i] = v;
-      top = fmaxf(top, v);
-    }
+#pragma unroll 8
+  for (int i = c.w0 + 4 * lane; i < c.w1; i += 128) {
+    const float4 q = c.logits4(i);
+    top = fmax3(fmax3(top, q.x, q.y), q.z, q.w);
+    *reinterpret_cast<float4*>(c.sw + i) = q;
   }
   uint32_t best = smp_key(smp_logit(top));
   {
@@ -718,12 +782,9 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SamplePara
     // nothing to choose from, or the lowest index of the largest logit
     uint32_t first = 0xFFFFFFFFu, none = 0, cnt;
     if (top == c.row.xmax) {  // this thread has seen it: among the elements that it loaded
-      auto seek = [&](int i) {
-        if (first == 0xFFFFFFFFu && smp_load(c.x + i) == c.row.xmax) first = i0 + i;
-      };
-      for (int v = tid; v < vec_done / kVec && first == 0xFFFFFFFFu; v += kSmpThreads)
-        for (int e = 0; e < kVec; ++e) seek(v * kVec + e);
-      for (int i = vec_done + tid; i < n && first == 0xFFFFFFFFu; i += kSmpThreads) seek(i);
+      for (int i = c.w0 + 4 * lane; i < c.w1 && first == 0xFFFFFFFFu; i += 128)
+        for (int e = 3; e >= 0; --e)
+          if (i + e < n && smp_load(c.x + i + e) == c.row.xmax) first = i0 + i + e;
     }
     c.reduce(my, my_ties, first, none, cnt, nullptr);
     if (c.rank == 0 && tid == 0) {
@@ -736,64 +797,75 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SamplePara
   // ---- weights, their mass, and the histograms
   const bool cut = by_k || by_p;
   {
-    uint32_t hi = 0, lo = 0, far = 0;
-#pragma unroll 4
-    for (int i = c.w0 + lane; i < c.w1; i += 32) {
-      const float w = expf(smp_d(c.sw[i], c.row));
-      c.sw[i] = w;
-      if (!cut) {
-        if (w >= min_p) smp_add_mass(w, hi, lo);
-      } else if (w > 0.f) {
-        if (!by_k) smp_add_mass(w, hi, lo);
-        const int e = smp_bucket(w);
-        if (e == kSmpBuckets - 1) {
-          ++far;  // the far tail shares the last bucket: counted apart, its mass left out of the guess
-        } else {
-          if (by_k) atomicAdd(&s.own[0][e], 1u);
-          if (by_p)
-            atomicAdd(&s.own[1][e], w == 1.f ? 4096u : ((__float_as_uint(w) & 0x7FFFFFu) | 0x800000u) >> 12);
+    SmpSum sum;
+    uint32_t far = 0;
+    const float w_min = cut ? 0.f : min_p;
+    auto take = [&](const float4 q) {
+      const float w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum.add(w[e] >= w_min ? w[e] : 0.f);
+      if (cut) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t k = smp_bucket(w[e]);
+          if (k < kSmpBuckets - 1) {
+            atomicAdd(&s.own[0][k], 1u);
+          } else {
+            far += w[e] > 0.f;  // the far tail shares the last bucket: counted apart
+          }
         }
       }
+    };
+    if (c.row.plain) {  // logits become weights
+      c.each4([&](int, float4& q) {
+        const float2 a = smp_weights2(q.x, q.y, c.row), b = smp_weights2(q.z, q.w, c.row);
+        q = make_float4(a.x, a.y, b.x, b.y);
+      });
+    } else {
+#pragma unroll 1
+      for (int i = c.w0 + lane; i < ((c.w1 + 3) & ~3); i += 32) c.sw[i] = c.weight_of(c.sw[i]);
+      __syncwarp();
     }
-    my = smp_mass(hi, lo);
+    c.each4([&](int, float4 q) { take(q); });
+    my = sum.get();
     if (cut) {
       far = __reduce_add_sync(0xffffffffu, far);
-      if (lane == 0 && far) {
-        atomicAdd(&s.own[0][kSmpBuckets - 1], far);
-        atomicAdd(&s.own[1][kSmpBuckets - 1], 1u);  // there is something
-      }
+      if (lane == 0 && far) atomicAdd(&s.own[0][kSmpBuckets - 1], far);
     }
   }
   bool listed = min_p == 0.f;
+  float w_listed = 0.f;  // the lower end of the buckets that the last look() listed
   if (cut) {
     smp_u64 total = my, above = 0, inside = 0;
     uint32_t lo = 0, hi = 0, cnt;
-    double above_n;
+    double above_n, in_n;
     __syncthreads();
-    if (by_k) c.merge_to_owner(0);
-    if (by_p) c.merge_to_owner(1);
+    c.merge_to_owner();
     if (c.C > 1) {
       c.sync();
-      if (by_k) c.merge_to_all(0);
-      if (by_p) c.merge_to_all(1);
+      c.merge_to_all();
     }
     c.reduce(total, inside, lo, hi, cnt, nullptr);
     if (by_k) {
-      const int bk = c.template crossing<false>((double)top_k, above_n);
-      if ((uint32_t)above_n + s.tot[0][bk] <= kSmpFew) {  // (the same in every block)
+      const int bk = c.template crossing<false>((double)top_k, 0, kSmpBuckets - 1, above_n, in_n);
+      if ((uint32_t)above_n + s.tot[bk] <= kSmpFew) {  // (the same in every block)
         c.few(p, b, i0, bk, top_k, top_p, min_p, uu);
         return;
       }
-      c.look(bk, 0u, above, inside, lo, hi, cnt);
+      c.look(bk, bk, 0u, above, inside, lo, hi, cnt);
+      w_listed = smp_upper(bk + 1);
       total = above + inside;
       if (hi != 0u) {
         const smp_u64 need = (smp_u64)top_k - (smp_u64)above_n;
-        if (need >= s.tot[0][bk]) {  // the whole bucket, or fewer logits than k
+        if (need >= s.tot[bk]) {  // the whole bucket, or fewer logits than k
           thr = lo - 1u;
         } else {
-          c.template refine<false>(bk, lo, hi, cnt, need, thr, ties);
+          c.template refine<false>(bk, bk, lo, hi, cnt, need, thr, ties);
           if (by_p) {
-            if (lo != hi) c.look(bk, thr, above, inside, lo, hi, cnt); else inside = 0;
+            inside = 0;
+            if (lo != hi) {
+              if (cnt != kSmpNoLists) c.listed_above(thr, inside); else c.look(bk, bk, thr, above, inside, lo, hi, cnt);
+            }
             total = above + inside + ties * c.mass_of_key(thr);
           }
         }
@@ -802,64 +874,91 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SamplePara
     if (by_p) {
       const double goal = (double)top_p * (double)total;
       const smp_u64 need = max((smp_u64)ceil(goal), 1ull);
-      const int bt = thr != 0u ? smp_bucket(expf(smp_d(smp_unkey(thr), c.row))) : kSmpBuckets - 1;
-      int bp = min(c.template crossing<true>(goal * kSmpUnit, above_n), bt);
-      // exact: move the guess until the mass above bucket bp is short of `need` and the mass with it is not
+      const int bt = thr != 0u ? (int)smp_bucket(c.weight_of_key(thr)) : kSmpBuckets - 1;
+      // exact: guess from what a look has found, until the mass above buckets b0 to b1 is short of `need` and the mass
+      // with them is not. Two buckets where the guess is near the edge of one and the lists stay short.
+      int first = 0, last = bt, b0, b1;
+      double at = goal * kSmpUnit;
       for (;;) {
-        c.look(bp, bp == bt ? thr : 0u, above, inside, lo, hi, cnt);
-        if (above >= need && bp > 0) {
-          do --bp; while (bp > 0 && s.tot[1][bp] == 0u);
-        } else if (above + inside < need && bp < bt) {
-          do ++bp; while (bp < bt && s.tot[1][bp] == 0u);
+        b0 = b1 = c.template crossing<true>(at, first, last, above_n, in_n);
+        const double unsure = 3e-4 * at;
+        if (at - above_n < unsure) {
+          if (b0 > first && s.tot[b0 - 1] + s.tot[b0] < kSmpAllLists) --b0;
+        } else if (above_n + in_n - at < unsure) {
+          if (b1 < last && s.tot[b1] + s.tot[b1 + 1] < kSmpAllLists) ++b1;
+        }
+        c.look(b0, b1, b1 == bt ? thr : 0u, above, inside, lo, hi, cnt);
+        if (above >= need && b0 > first) {
+          last = b0 - 1;
+        } else if (above + inside < need && b1 < last) {
+          first = b1 + 1;
         } else {
           break;
         }
+        at = fmax(above_n + ((double)need - (double)above) * kSmpUnit, 1e-30);
       }
+      w_listed = smp_upper(b1 + 1);
       if (above + inside < need) {
         // everything above the top-k threshold is in, and some of its ties
         const smp_u64 w = thr != 0u ? c.mass_of_key(thr) : 0ull, left = need - (above + inside);
         if (w != 0) ties = min(ties, (left + w - 1) / w);
         listed = false;  // the last look() left the ties out
       } else {
-        c.template refine<true>(bp, lo, hi, cnt, need - above, thr, ties);
+        c.template refine<true>(b0, b1, lo, hi, cnt, need - above, thr, ties);
       }
     }
   }
 
   // ---- the kept mass by warp and block
-  const float w_thr = thr != 0u ? expf(smp_d(smp_unkey(thr), c.row)) : 0.f;
-  const int bt = thr != 0u ? smp_bucket(w_thr) : kSmpBuckets;
-  auto admitted = [&](int i, float w) {  // 0: no, 1: above the threshold, 2: a tie
-    if (!(w >= min_p) || w == 0.f) return 0;
-    const int e = smp_bucket(w);
-    if (e != bt) return e < bt ? 1 : 0;
-    const uint32_t k = smp_key(smp_load(c.x + i));
-    return k > thr ? 1 : (k == thr && ties != 0) ? 2 : 0;
-  };
-  if (cut && listed && s.n_list <= kSmpList) {
-    // what the last look() found: s.red[w][0] is the mass that warp w has above the bucket
+  const float w_thr = thr != 0u ? c.weight_of_key(thr) : 0.f;
+  const int bt = thr != 0u ? (int)smp_bucket(w_thr) : kSmpBuckets;
+  // what is kept: weights above w_lo, and as negative ones the ties
+  float w_lo = 0.f;
+  if (!cut) {
+    if (min_p > 0.f) w_lo = __uint_as_float(__float_as_uint(min_p) - 1u);
+  } else if (listed && s.n_list <= kSmpList) {
+    // what the last look() found: s.red[w][0] is the mass that warp w has above the buckets it listed
+    w_lo = w_listed;
     if (lane == 0) s.red[warp][1] = 0ull;
     __syncthreads();
     const uint32_t* list = s.own[c.turn ^ 1];
     for (uint32_t j = tid; j < s.n_list; j += kSmpThreads) {
       const int i = s.at[j];
-      if (list[j] > thr) atomicAdd(&s.red[i / per][0], smp_mass(c.sw[i]));
-      else if (list[j] == thr && ties != 0) atomicAdd(&s.red[i / per][1], 1ull);
+      const float w = c.sw[i];
+      if (list[j] > thr) {
+        atomicAdd(&s.red[i / per][0], smp_mass(w));
+      } else if (list[j] == thr && ties != 0) {
+        atomicAdd(&s.red[i / per][1], 1ull);
+        c.sw[i] = -w;
+      } else {
+        c.sw[i] = 0.f;
+      }
     }
     __syncthreads();
     my = lane == 0 ? s.red[warp][0] : 0ull;
     my_ties = lane == 0 ? s.red[warp][1] : 0ull;
     __syncwarp();
-  } else if (cut) {
-    uint32_t hi = 0, lo = 0, nt = 0;
-#pragma unroll 2
-    for (int i = c.w0 + lane; i < c.w1; i += 32) {
-      const float w = c.sw[i];
-      const int a = admitted(i, w);
-      if (a == 1) smp_add_mass(w, hi, lo);
-      if (a == 2) ++nt;
-    }
-    my = smp_mass(hi, lo);
+  } else {
+    const float w_over = smp_upper(bt), w_in = smp_upper(bt + 1);
+    SmpSum sum;
+    uint32_t nt = 0;
+    c.each4([&](int i, float4& q) {
+      float w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        bool in = w[e] >= min_p && w[e] > w_in, tie = false;
+        if (in && !(w[e] > w_over)) {
+          const uint32_t k = smp_key(smp_load(c.x + i + e));
+          in = k > thr;
+          tie = k == thr && ties != 0;
+        }
+        if (in) sum.add(w[e]);
+        nt += tie;
+        w[e] = in ? w[e] : tie ? -w[e] : 0.f;
+      }
+      q = make_float4(w[0], w[1], w[2], w[3]);
+    });
+    my = sum.get();
     my_ties = nt;
   }
   smp_u64 all_ties = my_ties;
@@ -881,40 +980,55 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SamplePara
     const smp_u64 m0 = __shfl_sync(0xffffffffu, em - wm, warp), t0 = __shfl_sync(0xffffffffu, et - wt, warp);
     const smp_u64 m1 = __shfl_sync(0xffffffffu, em, warp), t1 = __shfl_sync(0xffffffffu, et, warp);
     if (goal >= with_ties(m0, t0) && goal < with_ties(m1, t1)) {
-      // this warp holds the token: its lanes sum a contiguous run each, then all walk the run that holds it
-      const int run = (c.w1 - c.w0 + 31) >> 5;
-      const int r0 = min(c.w0 + lane * run, c.w1), r1 = min(r0 + run, c.w1);
-      uint32_t hi = 0, lo = 0, nt = 0;
-      for (int i = r0; i < r1; ++i) {
-        const float w = c.sw[i];
-        const int a = admitted(i, w);
-        if (a == 1) smp_add_mass(w, hi, lo);
-        if (a == 2) ++nt;
+      // this warp holds the token: steps of 512 indices to the one that passes the goal, of 128, and its lanes' four
+      smp_u64 fm = m0, ft = t0;
+      auto step = [&](int i, SmpSum& sum, uint32_t& nt) {
+        if (i >= c.w1) return;
+        const float4 q = *reinterpret_cast<const float4*>(c.sw + i);
+        const float w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          sum.add(w[e] > w_lo ? w[e] : 0.f);
+          nt += w[e] < 0.f;
+        }
+      };
+      int base = c.w0;
+      for (; base < c.w1; base += 512) {
+        SmpSum sum;
+        uint32_t nt = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) step(base + 128 * e + 4 * lane, sum, nt);
+        const smp_u64 bm = fm + smp_warp_sum(sum.get()), bt = ft + __reduce_add_sync(0xffffffffu, nt);
+        if (with_ties(bm, bt) > goal) break;
+        fm = bm;
+        ft = bt;
       }
-      const smp_u64 rm = smp_mass(hi, lo), rt = nt;
-      const smp_u64 im = m0 + smp_warp_scan(rm, lane), it = t0 + smp_warp_scan(rt, lane);
-      const uint32_t hit = __ballot_sync(0xffffffffu, with_ties(im, it) > goal);
-      const int src = __ffs(hit) - 1;
-      smp_u64 fm = __shfl_sync(0xffffffffu, im - rm, src), ft = __shfl_sync(0xffffffffu, it - rt, src);
-      const int j0 = __shfl_sync(0xffffffffu, r0, src), j1 = __shfl_sync(0xffffffffu, r1, src);
-      for (int base = j0; base < j1; base += 32) {
-        const int i = base + lane;
-        const float w = i < j1 ? c.sw[i] : 0.f;
-        const int a = i < j1 ? admitted(i, w) : 0;
-        const smp_u64 sm = fm + smp_warp_scan(a == 1 ? smp_mass(w) : 0ull, lane);
-        const uint32_t tm = __ballot_sync(0xffffffffu, a == 2);
-        const smp_u64 st = ft + __popc(tm & (0xFFFFFFFFu >> (31 - lane)));
-        const uint32_t found = __ballot_sync(0xffffffffu, with_ties(sm, st) > goal);
-        if (found) {
-          if (lane == __ffs(found) - 1) {
-            p.token[b] = i0 + i;
-            if (p.logprob != nullptr)
-              p.logprob[b] = smp_d(smp_load(c.x + i), c.row) - logf((float)((double)kept * kSmpUnit));
+      for (; base < c.w1; base += 128) {
+        SmpSum sum;
+        uint32_t nt = 0;
+        const int i = base + 4 * lane;
+        step(i, sum, nt);
+        const smp_u64 im = fm + smp_warp_scan(sum.get(), lane), it = ft + smp_warp_scan(nt, lane);
+        const uint32_t hit = __ballot_sync(0xffffffffu, with_ties(im, it) > goal);
+        if (hit) {
+          if (lane == __ffs(hit) - 1) {
+            smp_u64 m = im - sum.get(), t = it - nt;
+            for (int e = 0; e < 4; ++e) {
+              const float w = c.sw[i + e];
+              if (w > w_lo) m += smp_mass(w);
+              t += w < 0.f;
+              if (with_ties(m, t) > goal) {
+                p.token[b] = i0 + i + e;
+                if (p.logprob != nullptr)
+                  p.logprob[b] = smp_d(smp_load(c.x + i + e), c.row) - logf((float)((double)kept * kSmpUnit));
+                break;
+              }
+            }
           }
           break;
         }
-        fm = __shfl_sync(0xffffffffu, sm, 31);
-        ft += __popc(tm);
+        fm = __shfl_sync(0xffffffffu, im, 31);
+        ft = __shfl_sync(0xffffffffu, it, 31);
       }
     }
   }
