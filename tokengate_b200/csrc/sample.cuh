@@ -580,14 +580,14 @@ struct Smp {
   __device__ __forceinline__ void select_listed(uint32_t lo, uint32_t hi, uint32_t cnt, smp_u64& need, uint32_t& key) {
     constexpr uint32_t kHalf = kSmpBuckets / 2;
     const uint32_t* cur = s.all;
-    {
-      uint32_t base = 0;
-      for (int c = 0; c < C; ++c) {
-        const uint32_t m = (uint32_t)s.xch[turn ^ 1][c][3];  // as the last reduce() left it
-        const uint32_t* from = remote(s.own[turn ^ 1], c);
-        for (uint32_t i = threadIdx.x; i < m; i += kSmpThreads) s.all[base + i] = from[i];
-        base += m;
-      }
+    {  // the blocks' lists by a warp or more each, at once
+      const smp_u64(*sent)[4] = s.xch[turn ^ 1];  // as the last reduce() left it
+      const int r = warp % C;
+      const smp_u64 ends = smp_warp_scan(lane < C ? sent[lane][3] : 0ull, lane);
+      const uint32_t m = (uint32_t)sent[r][3], base = (uint32_t)__shfl_sync(0xffffffffu, ends, r) - m;
+      const uint32_t* from = remote(s.own[turn ^ 1], r);
+#pragma unroll 4
+      for (uint32_t i = warp / C * 32 + lane; i < m; i += kSmpWarps / C * 32) s.all[base + i] = from[i];
     }
     uint32_t* dig = &s.dig[0][0][0];
     smp_u64* masses = reinterpret_cast<smp_u64*>(dig);
@@ -743,16 +743,6 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SamplePara
   griddep_wait();
   griddep_launch_dependents();
 
-  float t = p.temperature[b];
-  const bool greedy = !(t > 0.f);
-  if (greedy) t = 1.f;
-  uint32_t top_k = p.top_k != nullptr && p.top_k[b] > 0 ? (uint32_t)p.top_k[b] : 0xFFFFFFFFu;
-  if (greedy) top_k = 1u;
-  const float top_p = p.top_p != nullptr && p.top_p[b] < 1.f ? fmaxf(p.top_p[b], 0.f) : 1.f;
-  const float min_p = p.min_p != nullptr && p.min_p[b] > 0.f ? fminf(p.min_p[b], 1.f) : 0.f;
-  const float uu = p.u[b];
-  const bool by_k = top_k > 1u && top_k < (uint32_t)p.V, by_p = top_p < 1.f && top_k > 1u;
-
   for (int i = tid; i < kSmpBuckets; i += kSmpThreads) s.own[0][i] = s.own[1][i] = 0u;
   for (int i = tid; i < kSmpBuckets; i += kSmpThreads) s.all[i] = 0u;
   if (tid == 0) s.n_list = s.n_few = 0u;
@@ -765,6 +755,16 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SamplePara
     top = fmax3(fmax3(top, q.x, q.y), q.z, q.w);
     *reinterpret_cast<float4*>(c.sw + i) = q;
   }
+  float t = p.temperature[b];
+  const bool greedy = !(t > 0.f);
+  if (greedy) t = 1.f;
+  uint32_t top_k = p.top_k != nullptr && p.top_k[b] > 0 ? (uint32_t)p.top_k[b] : 0xFFFFFFFFu;
+  if (greedy) top_k = 1u;
+  const float top_p = p.top_p != nullptr && p.top_p[b] < 1.f ? fmaxf(p.top_p[b], 0.f) : 1.f;
+  const float min_p = p.min_p != nullptr && p.min_p[b] > 0.f ? fminf(p.min_p[b], 1.f) : 0.f;
+  const float uu = p.u[b];
+  const bool by_k = top_k > 1u && top_k < (uint32_t)p.V, by_p = top_p < 1.f && top_k > 1u;
+
   uint32_t best = smp_key(smp_logit(top));
   {
     smp_u64 z0 = 0, z1 = 0;
