@@ -116,6 +116,21 @@ def test_long_and_flat_rows(cuda, B, V, spread):
             run(cuda, x, u, 1.0, k=V // 3, p=np.array([middle_p(xf[0], 1.0, V // 3, V // 9)], dtype=np.float32), m=0.2)
 
 
+@pytest.mark.parametrize("shift", [0.0, 1e-3, -1e-3])
+@pytest.mark.parametrize("V", [8191, 65528])
+def test_masses_away_from_the_buckets_middles(cuda, V, shift):
+    """Levels of equal mass at the edges of the buckets (powers of two), or just beside them: whatever
+    guesses a bucket's mass from its count is wrong by the same sign everywhere."""
+    levels = int(np.log2(V + 8)) - 3
+    x = np.concatenate([np.full(8 << j, -j * np.log(2) + (shift if j else 0.0)) for j in range(levels)])
+    rng = np.random.default_rng(5)
+    x = torch.tensor(rng.permutation(x)[None], dtype=torch.float32)
+    for k in (0, V // 3):
+        for n in (3, 8, 100, 1000, 3000, V // 4):
+            p = middle_p(x[0].numpy(), 1.0, k, n)
+            run(cuda, x.expand(6, -1).contiguous(), rng.random(6), 1.0, k=k, p=p)
+
+
 @pytest.mark.parametrize("k", [2, 31, 32, 33, 200, 255, 256, 257, 300])
 def test_few_logits_at_their_limit(cuda, k):
     """As many logits down to the k-th's bucket as one block orders by counting, one fewer and one more: k

@@ -31,11 +31,11 @@
 // The cache is read once, at 144 bytes per key: every warp streams its own
 // tiles through a ring of two or three in shared memory (one bulk copy of 4608
 // bytes each, no barrier between warps). 2 rows of 131081 keys, 8 kv heads:
-// 53.7 us, 302 MB = 5.6 TB/s (86 % of a copy's rate), of which 47 are the loop,
+// 54.6 us, 302 MB = 5.5 TB/s (84 % of a copy's rate), of which 47 are the loop,
 // at DRAM's rate, the rest its start, the merges and the second launch. In the
-// L2 cache (one row of 32775: 14.4 us) the loop is bound by instructions, half
-// of them the unpacking (issue slots 58 % busy, the ALU pipe 64 %); a short
-// cache (one row of 2771: 7.0 us) by latencies one after another: the launch,
+// L2 cache (one row of 32775: 14.3 us) the loop is bound by instructions, half
+// of them the unpacking (issue slots 59 % busy, the ALU pipe 63 %); a short
+// cache (one row of 2771: 6.9 us) by latencies one after another: the launch,
 // the counts, the first tile, two barriers.
 #pragma once
 
@@ -217,8 +217,8 @@ __device__ __forceinline__ void kv4_store_out(__nv_bfloat16* at, float4 o, float
 // 8 independent softmaxes, lane (g, t) having columns 2 t and 2 t + 1:
 //   PAIR (up to 4 query heads per kv head): column 4 s + h is head h over the
 //         16-key halves s of the tiles, so no lane works on an empty column
-//         and the two are merged at the end (16 rows of 131081 keys 59.6 ->
-//         56.8 us; 441 instructions a tile under ncu, prologues included);
+//         and the two are merged at the end (2 rows of 131081 keys, 8 kv
+//         heads: 59.6 -> 56.8 us; 461 instructions a tile, prologues included);
 //   else: column h is head h.
 // Without a bias the scores are in log2 units; with one they stay in natural
 // units, where a bias of the type's lowest value does not overflow.

@@ -12,28 +12,32 @@
 // the same decision (V <= 2^19 keeps them in 64 bits).
 //
 // A cluster of C blocks takes a row, each an index range of it, whose weights
-// it computes once and keeps in shared memory. Bound by instructions and by
-// latencies (barriers of the cluster and of the block), not by memory: the row
-// is read once. No sort: the k-th value (or the value at which the mass reaches
-// p) is found
+// it computes once and keeps in shared memory. Bound by latencies (barriers of
+// the cluster and of the block, one after another) and by instructions, not by
+// memory: the row is read once. 64 fp32 rows of 151936, rules of all kinds: 61
+// us, in two rounds of clusters of about 28, of which 4 are the logits' load,
+// 5.5 the weights and the histogram, 3 a look's pass, the rest exchanges (issue
+// slots 43 % busy where an SM works, 78 instructions a logit). No sort: the k-th
+// value (or the value at which the mass reaches p) is found
 //   1. by a histogram over 1024 buckets of w, 32 to an octave (linear in w's
 //      bits: two instructions, and nearly linear in the logit, so that logits
 //      spread over many buckets and shared-memory atomics seldom collide):
 //      counts, exact for k; for p the guess that a bucket's logits weigh its
 //      middle each. Each block owns a slice of the row's and hands it to the
 //      others;
-//   2. exactly inside that bucket: one pass gives the mass above it and in it,
-//      its smallest and largest logit and the list of its logits (after a wrong
-//      guess, the next one from there); where the two differ (bf16 logits: hardly ever),
-//      every block narrows them down on a copy of all lists, so without a
-//      cluster barrier (lists too long for that: digits, over the row again).
+//   2. exactly inside that bucket (or two, where the guess is near an edge):
+//      one pass gives the mass above and in it, its smallest and largest logit
+//      and the list of its logits (after a wrong guess, the next one from
+//      there); where the two differ, every block narrows them down on a copy of
+//      all lists, so without a cluster barrier (lists too long for that: by
+//      digits, with one each).
 // Where no more than 256 logits reach down to the k-th's bucket, they go to one
-// block, which orders them by counting and finishes alone (one row of 151936,
-// k = 50, p = 0.9: 22 -> 14 us).
-// The threshold is a logit and a number of its ties, which go by index. Only
-// elements of the threshold's bucket are looked up in the row again. Blocks
-// write to one another's shared memory and read their own: a remote load costs
-// the reader its latency, and sixteen blocks reading one word queue up.
+// block, which orders them by counting and finishes alone (k = 50, p = 0.9: one
+// row of 151936 18.3 -> 12.5 us, 64 rows 70 -> 43).
+// The threshold is a logit and a number of its ties, which go by index. What is
+// kept is then marked in the weights (ties negative), for the walk to the token.
+// Blocks write to one another's shared memory and read their own: a remote load
+// costs the reader its latency, and sixteen blocks reading one word queue up.
 #pragma once
 
 #include <cooperative_groups.h>

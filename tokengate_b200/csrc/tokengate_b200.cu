@@ -1418,10 +1418,10 @@ Kv4Shape kv4_shape(int B, int Hkv, int n_keys) {
     const int64_t per = (tiles + s.cluster - 1) / s.cluster;
     if (per < s.warps) s.warps = (int)per;
   } else if (rows * 2 <= sms) {
-    s.parts = sms / Hkv;          // one block of 16 warps per SM (16 rows of 131081: 55 us, 12 warps of 3 tiles 57)
+    s.parts = sms / Hkv;          // one block of 16 warps per SM (16 heads' rows of 131081: 55 us, 12 warps of 3 tiles 57)
   } else {
     // many rows: four blocks of 4 warps per SM (512 rows of 2771: 54 us, three blocks of three tiles a warp 69;
-    // 128 ragged rows of 4097: 19.3, two blocks of 8 warps 20.2)
+    // 128 ragged rows of 4097: 18.3 us, two blocks of 8 warps 5 % more)
     s.warps = 4;
     s.parts = 4 * sms / Hkv > 0 ? 4 * sms / Hkv : 1;
   }
@@ -1625,8 +1625,9 @@ int tg_sample(const void* logits, int dtype, int64_t row_stride, int B, int V, c
   p.token = token;
   p.logprob = logprob;
   const int sms = sm_count();
-  // blocks of a cluster: as many as half fill the GPU (one row of 151936: 16 blocks 23 us, 8 blocks 30 us), and as
-  // many as let two blocks share an SM's memory (64 fp32 rows of 151936: 8 blocks 94 us, 4 blocks 114 us)
+  // blocks of a cluster: as many as half fill the GPU (a row of 151936, k = 50: 16 blocks 12.4 us, 8 blocks 15.7, 4
+  // blocks 20.7; 64 rows of 32000: 2 blocks 24.0, 8 blocks 36.9), and as many as let two blocks share an SM's memory
+  // (fp32 rows of 151936: 37 rows 8 blocks 34.9, 4 blocks 36.7, 16 blocks 51; 64 rows 61, 60, 92)
   int C = 1;
   auto chunk_of = [&](int c) { return (V + c * tg::kSmpThreads - 1) / (c * tg::kSmpThreads) * tg::kSmpThreads; };
   auto smem_of = [&](int c) { return sizeof(tg::SmpShared) + (size_t)chunk_of(c) * sizeof(float); };
