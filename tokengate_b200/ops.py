@@ -756,12 +756,12 @@ def kv4_read(cache: KV4Cache, start: int = 0, n: Optional[int] = None, k_out: Op
         raise ValueError(f"slots [{start}, {start + n}) are outside the cache's capacity {c.capacity}")
     H = c.n_kv_heads
     if k_out is None and v_out is None:
-        k_out = c.bf16.new_empty((c.batch, n, H, 128))
+        k_out = c.bf16.new_empty(c.batch, n, H, 128)
         v_out = torch.empty_like(k_out)
         ks = vs = (n * H * 128, H * 128, 128)
     else:
-        k_out = c.bf16.new_empty((c.batch, n, H, 128)) if k_out is None else k_out
-        v_out = c.bf16.new_empty((c.batch, n, H, 128)) if v_out is None else v_out
+        k_out = c.bf16.new_empty(c.batch, n, H, 128) if k_out is None else k_out
+        v_out = c.bf16.new_empty(c.batch, n, H, 128) if v_out is None else v_out
         ks, vs = _kv4_rows("k_out", k_out, c, n), _kv4_rows("v_out", v_out, c, n)
     if n:
         _lib.kv4_read(c.index, c.ptr, c.capacity, c.batch, H, 128, start, n, k_out.data_ptr(), *ks, v_out.data_ptr(),
@@ -769,16 +769,17 @@ def kv4_read(cache: KV4Cache, start: int = 0, n: Optional[int] = None, k_out: Op
     return k_out, v_out
 
 
-def _token_heads(name: str, t: torch.Tensor, B: int, heads: Optional[int], index: int) -> int:
-    """The row stride of a (B, 1, heads, 128) tensor with contiguous heads."""
+def _token_heads(name: str, t: torch.Tensor, B: int, heads: Optional[int], index: int) -> Tuple[int, int]:
+    """The row stride and the heads of a (B, 1, heads, 128) tensor with contiguous heads."""
     _on(name, t, torch.bfloat16, index)
-    if t.dim() != 4 or t.shape[0] != B or t.shape[1] != 1 or t.shape[3] != 128 \
-            or (heads is not None and t.shape[2] != heads):
-        raise ValueError(f"{name} must be ({B}, 1, {'heads' if heads is None else heads}, 128), got {tuple(t.shape)}")
+    shape = t.shape
+    b, one, n, d = shape if len(shape) == 4 else (0, 0, 0, 0)
+    if b != B or one != 1 or d != 128 or (heads is not None and n != heads):
+        raise ValueError(f"{name} must be ({B}, 1, {'heads' if heads is None else heads}, 128), got {tuple(shape)}")
     sb, _, sh, sd = t.stride()
-    if sd != 1 or (sh != 128 and t.shape[2] > 1):
+    if sd != 1 or (sh != 128 and n > 1):
         raise ValueError(f"{name} must have contiguous heads")
-    return sb
+    return sb, n
 
 
 def qk_norm_rope_append_kv4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm_w: torch.Tensor,
@@ -792,15 +793,17 @@ def qk_norm_rope_append_kv4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q
     Returns the finished q, (B, 1, Hq, 128) contiguous (or q_out, which may be q)."""
     c = _kv4(cache)
     B, dev = c.batch, c.index
-    ld_q = _token_heads("q", q, B, None, dev)
-    ld_k, ld_v = _token_heads("k", k, B, c.n_kv_heads, dev), _token_heads("v", v, B, c.n_kv_heads, dev)
+    ld_q, Hq = _token_heads("q", q, B, None, dev)
+    ld_k, _ = _token_heads("k", k, B, c.n_kv_heads, dev)
+    ld_v, _ = _token_heads("v", v, B, c.n_kv_heads, dev)
     row = (B, 1, 128)
     for nm, t in (("cos", cos), ("sin", sin)):
         _on(nm, t, torch.bfloat16, dev)
         if t.shape != row:
             raise ValueError(f"{nm} must be ({B}, 1, 128), got {tuple(t.shape)}")
-    ld_cs, _, cd = cos.stride()
-    if cd != 1 or sin.stride() != cos.stride():
+    cs = cos.stride()
+    ld_cs, _, cd = cs
+    if cd != 1 or sin.stride() != cs:
         raise ValueError("cos and sin must share strides and have a contiguous last dim")
     for nm, t in (("q_norm_w", q_norm_w), ("k_norm_w", k_norm_w)):
         _on(nm, t, torch.bfloat16, dev)
@@ -809,11 +812,10 @@ def qk_norm_rope_append_kv4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q
     _on("slot", slot, torch.int64, dev)
     if slot.numel() != 1:
         raise ValueError("slot must be an int64 (1,) tensor")
-    Hq = q.shape[2]
     if q_out is None:
-        q_out, ld_qo = c.bf16.new_empty((B, 1, Hq, 128)), Hq * 128
+        q_out, ld_qo = c.bf16.new_empty(B, 1, Hq, 128), Hq * 128
     else:
-        ld_qo = _token_heads("q_out", q_out, B, Hq, dev)
+        ld_qo, _ = _token_heads("q_out", q_out, B, Hq, dev)
     _lib.qk_norm_rope_append_kv4(dev, q.data_ptr(), ld_q, Hq, k.data_ptr(), ld_k, c.n_kv_heads, v.data_ptr(), ld_v, B,
                                  q_norm_w.data_ptr(), k_norm_w.data_ptr(), cos.data_ptr(), sin.data_ptr(), ld_cs, 128,
                                  eps, q_out.data_ptr(), ld_qo, c.ptr, c.capacity, slot.data_ptr())
@@ -837,9 +839,10 @@ def decode_attention_kv4(q: torch.Tensor, cache: KV4Cache, n_valid: torch.Tensor
     c = _kv4(cache)
     B, dev = c.batch, c.index
     _on("q", q, torch.bfloat16, dev)
-    if q.dim() != 3 or q.shape[0] != B or q.shape[2] != 128:
-        raise ValueError(f"q must be ({B}, Hq, 128), got {tuple(q.shape)}")
-    Hq = q.shape[1]
+    shape = q.shape
+    b, Hq, d = shape if len(shape) == 3 else (0, 0, 0)
+    if b != B or d != 128:
+        raise ValueError(f"q must be ({B}, Hq, 128), got {tuple(shape)}")
     q_sb, q_sh, q_sd = q.stride()
     if q_sd != 1:
         raise ValueError("q must have a contiguous last dim")
@@ -849,19 +852,18 @@ def decode_attention_kv4(q: torch.Tensor, cache: KV4Cache, n_valid: torch.Tensor
     if n_valid.numel() != B or not n_valid.is_contiguous():
         raise ValueError("n_valid must be a contiguous (B,) int32 tensor")
     if out is None:
-        out, o_sb, o_sh = c.bf16.new_empty((B, Hq, 128)), Hq * 128, 128
+        out, o_sb, o_sh = c.bf16.new_empty(B, Hq, 128), Hq * 128, 128
     else:
         _on("out", out, torch.bfloat16, dev)
-        if out.shape != q.shape or out.stride(2) != 1:
+        if out.shape != shape or out.stride(2) != 1:
             raise ValueError("out must have q's shape with a contiguous last dim")
         o_sb, o_sh = out.stride(0), out.stride(1)
     bias_ptr = qs_ptr = nk_ptr = bsb = bsh = qsb = 0
     if bias is not None:
         _on("bias", bias, torch.float32, dev)
-        shape, strides = (1, 1, *bias.shape)[-3:], (0, 0, *bias.stride())[-3:]
         if bias.dim() > 3:
             raise ValueError(f"bias {tuple(bias.shape)} must broadcast to ({B}, {Hq}, >= {n_prefix})")
-        (b0, b1, b2), (s0, s1, s2) = shape, strides
+        (b0, b1, b2), (s0, s1, s2) = (1, 1, *bias.shape)[-3:], (0, 0, *bias.stride())[-3:]
         if b2 < n_prefix or (s2 != 1 and b2 > 1) or (b0 != 1 and b0 != B) or (b1 != 1 and b1 != Hq):
             raise ValueError(f"bias {tuple(bias.shape)} must broadcast to ({B}, {Hq}, >= {n_prefix}) "
                              "with a contiguous last dim")
@@ -891,7 +893,8 @@ def _per_row(name: str, val, B: int, dtype: torch.dtype, index: int) -> Optional
         return None
     if not isinstance(val, torch.Tensor):
         return torch.full((B,), val, dtype=dtype, device=torch.device("cuda", index))
-    _on(name, val, dtype, index)
+    if val.dtype is not dtype or val.get_device() != index:
+        _on(name, val, dtype, index)
     if val.shape != (B,) or not val.is_contiguous():
         raise ValueError(f"{name} must be a number or a contiguous ({B},) tensor")
     return val
