@@ -440,7 +440,9 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
   const uint8_t* base = p.cache + (int64_t)b * p.c_sb + (int64_t)kvh * p.c_sh;
   const Kv4Span span = kv4_span(nv_raw, p.n_prefix, n_keys);
   const int n = span.n;
-  const int v0 = (int)((int64_t)n * rank / C), v1 = (int)((int64_t)n * (rank + 1) / C);
+  // n / C tiles to a block, one more to the first n % C
+  const int each = (int)((unsigned)n / (unsigned)C), more = n - each * C;
+  const int v0 = rank * each + min(rank, more), v1 = v0 + each + (rank < more);
   const int mine = v1 - v0 > warp ? (v1 - v0 - warp + W - 1) / W : 0;  // this warp's tiles
   auto tile_of = [&](int i) {
     const int v = v0 + warp + i * W;
@@ -454,7 +456,7 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
     for (int i = 0; i < min(mine, S); ++i) fetch(i, i);
 
   // the heads' q', scaled by a power of two
-  for (int h = warp; h < 8; h += W) {
+  for (int h = warp; h < (PAIR ? 4 : 8); h += W) {
     if (h != warp && h < p.G) {
       const int hq = kvh * p.G + h;
       q_raw = kv4_load_q(p.q + (int64_t)b * p.q_sb + (int64_t)hq * p.q_sh, lane);
@@ -647,12 +649,14 @@ constexpr int kKv4CombineWarps = 8;
 __global__ void __launch_bounds__(32 * kKv4CombineWarps) kv4_combine_kernel(const Kv4AttnParams p) {
   __shared__ float s_m[kKv4CombineWarps], s_l[kKv4CombineWarps];
   __shared__ float s_o[kKv4CombineWarps][128];
-  griddep_wait();
-  griddep_launch_dependents();
   const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // The counts before the wait: this grid starts when every block of the attention's has passed its own, so what came
+  // before that is complete, and the attention writes only records and outputs.
   const int n_keys = p.n_keys_dev != nullptr ? max(min(__ldg(p.n_keys_dev), p.n_keys), 0) : p.n_keys;
   int found, first, C;
   kv4_share(p, n_keys, lane, [&](int r, int, int) { return r == b; }, found, first, C);
+  griddep_wait();
+  griddep_launch_dependents();
   if (C == 1) return;  // its one block has written the output
   const float* rec = p.part + ((int64_t)h * (p.parts + p.B) + first) * kKv4Part;
   const float unit = p.bias != nullptr ? kLog2e : 1.f;  // of m
