@@ -73,8 +73,10 @@ __device__ __forceinline__ uint2 kv4_code_bits2(uint32_t pair, float neg_low, fl
   v = __fadd2_rz(__fadd2_rn(v, make_float2(0.5f, 0.5f)), make_float2(8388608.f, 8388608.f));
   return make_uint2(__float_as_uint(v.x), __float_as_uint(v.y));
 }
-constexpr uint32_t kKv4Bias8 = 0u - 0x4B000000u * 0x11111111u;  // minus the biases of 8 codes 4 bits apart
-constexpr uint32_t kKv4Bias4 = 0u - 0x4B000000u * 0x01010101u;  // of 4 codes 8 bits apart
+// the low bytes of four words, a's lowest
+__device__ __forceinline__ uint32_t kv4_low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
 
 // byte of a V key inside its 16-key block's words, and its fragment column t
 __device__ __forceinline__ int kv4_v_byte(int kb) { return ((kb & 1) << 1) | (kb >> 3); }
@@ -147,13 +149,21 @@ __global__ void __launch_bounds__(256, 4) kv4_write_kernel(const Kv4RowsParams p
   uint4 x[8];  // K then V
   bool in[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < 4; ++j) in[j] = (unsigned)(r0 + (j >> 1) + 8 * (j & 1)) < (unsigned)p.count;
+  const bool whole = in[0] && in[1] && in[2] && in[3];
+  auto load = [&](int j) {
     const int dr = (j >> 1) + 8 * (j & 1);
-    in[j] = (unsigned)(r0 + dr) < (unsigned)p.count;
-    x[j] = x[4 + j] = make_uint4(0u, 0u, 0u, 0u);
-    if (in[j]) {
-      x[j] = ld_nc_v4(reinterpret_cast<const uint4*>(kb + dr * p.k_ss));
-      x[4 + j] = ld_nc_v4(reinterpret_cast<const uint4*>(vb + dr * p.v_ss));
+    x[j] = ld_nc_v4(reinterpret_cast<const uint4*>(kb + dr * p.k_ss));
+    x[4 + j] = ld_nc_v4(reinterpret_cast<const uint4*>(vb + dr * p.v_ss));
+  };
+  if (__all_sync(0xffffffffu, whole)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) load(j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[j] = x[4 + j] = make_uint4(0u, 0u, 0u, 0u);
+      if (in[j]) load(j);
     }
   }
   // ---- extrema of the 8 rows: rows split over the lanes as the lanes are merged
@@ -176,47 +186,48 @@ __global__ void __launch_bounds__(256, 4) kv4_write_kernel(const Kv4RowsParams p
       *reinterpret_cast<uint32_t*>(tile + ((c & 4) ? kKv4Vp : kKv4Kp) + row * 8 + (c >> 3) * 4) = own.param;
   }
   float neg_low[8], inv[8];
-  const bool any_bad = __any_sync(0xffffffffu, own.bad);
+  const float own_neg = -own.low;
 #pragma unroll
   for (int r = 0; r < 8; ++r) {
-    const int src = (lane & 24) | r;
-    neg_low[r] = -__shfl_sync(0xffffffffu, own.low, src);
-    inv[r] = __shfl_sync(0xffffffffu, own.inv, src);
-    if (any_bad && __shfl_sync(0xffffffffu, own.bad, src)) x[r] = make_uint4(0u, 0u, 0u, 0u);  // codes of 0
+    neg_low[r] = __shfl_sync(0xffffffffu, own_neg, (lane & 24) | r);
+    inv[r] = __shfl_sync(0xffffffffu, own.inv, (lane & 24) | r);
+  }
+  if (__any_sync(0xffffffffu, own.bad)) {
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      if (__shfl_sync(0xffffffffu, own.bad, (lane & 24) | r)) x[r] = make_uint4(0u, 0u, 0u, 0u);  // codes of 0
   }
   // ---- K: the lane's 8 codes are one word of the row
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
-    uint32_t word = kKv4Bias8;
+    uint32_t two[4];  // a pair's codes in the low byte
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const uint2 n = kv4_code_bits2(w[e], neg_low[j], inv[j]);
-      word += n.x << (8 * e);
-      word += n.y << (8 * e + 4);
+      two[e] = n.x + (n.y << 4);
     }
+    const uint32_t word = kv4_low_bytes(two[0], two[1], two[2], two[3]);
     const int row = row0 + (j >> 1) + 8 * (j & 1);
     if (in[j]) *reinterpret_cast<uint32_t*>(tile + row * 64 + (c & 3) * 16 + (c >> 2) * 4) = word;
   }
   // ---- V: byte j of word g = the code of key j at this lane's dim g
   uint32_t acc[8];
 #pragma unroll
-  for (int g = 0; g < 8; ++g) acc[g] = kKv4Bias4;
+  for (int e = 0; e < 4; ++e) {
+    uint2 n[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint32_t w[4] = {x[4 + j].x, x[4 + j].y, x[4 + j].z, x[4 + j].w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint2 n = kv4_code_bits2(w[e], neg_low[4 + j], inv[4 + j]);
-      acc[2 * e] += n.x << (8 * j);
-      acc[2 * e + 1] += n.y << (8 * j);
+    for (int j = 0; j < 4; ++j) {
+      const uint4 q = x[4 + j];
+      n[j] = kv4_code_bits2(e == 0 ? q.x : e == 1 ? q.y : e == 2 ? q.z : q.w, neg_low[4 + j], inv[4 + j]);
     }
+    acc[2 * e] = kv4_low_bytes(n[0].x, n[1].x, n[2].x, n[3].x);
+    acc[2 * e + 1] = kv4_low_bytes(n[0].y, n[1].y, n[2].y, n[3].y);
   }
   // lanes c (even: low nibbles) and c + 1 (high nibbles) make the 8 words of
   // their 16 dims: the even lane words g = 0..3, the odd one 4..7
   const int odd = c & 1, wd = c >> 1;
   uint8_t* vt = tile + kKv4V + (blk & 1) * 1024 + (wd >> 2) * 512 + t * 16 + (wd & 3) * 4;
-  const bool whole = in[0] && in[1] && in[2] && in[3];
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     const uint32_t give = odd ? acc[g] : acc[4 + g], mine = odd ? acc[4 + g] : acc[g];

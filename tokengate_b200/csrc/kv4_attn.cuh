@@ -31,11 +31,11 @@
 // The cache is read once, at 144 bytes per key: every warp streams its own
 // tiles through a ring of two or three in shared memory (one bulk copy of 4608
 // bytes each, no barrier between warps). 2 rows of 131081 keys, 8 kv heads:
-// 54.6 us, 302 MB = 5.5 TB/s (84 % of a copy's rate), of which 47 are the loop,
+// 53.3 us, 302 MB = 5.7 TB/s (86 % of a copy's rate), of which 47 are the loop,
 // at DRAM's rate, the rest its start, the merges and the second launch. In the
-// L2 cache (one row of 32775: 14.3 us) the loop is bound by instructions, half
+// L2 cache (one row of 32775: 13.6 us) the loop is bound by instructions, half
 // of them the unpacking (issue slots 59 % busy, the ALU pipe 63 %); a short
-// cache (one row of 2771: 6.9 us) by latencies one after another: the launch,
+// cache (one row of 2771: 6.8 us) by latencies one after another: the launch,
 // the counts, the first tile, two barriers.
 #pragma once
 

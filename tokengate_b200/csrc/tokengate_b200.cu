@@ -1421,7 +1421,7 @@ Kv4Shape kv4_shape(int B, int Hkv, int n_keys) {
     s.parts = sms / Hkv;          // one block of 16 warps per SM (16 heads' rows of 131081: 55 us, 12 warps of 3 tiles 57)
   } else {
     // many rows: four blocks of 4 warps per SM (512 rows of 2771: 54 us, three blocks of three tiles a warp 69;
-    // 128 ragged rows of 4097: 18.3 us, two blocks of 8 warps 5 % more)
+    // 128 ragged rows of 4097: 16.8 us, two blocks of 8 warps 5 % more)
     s.warps = 4;
     s.parts = 4 * sms / Hkv > 0 ? 4 * sms / Hkv : 1;
   }
