@@ -123,13 +123,14 @@ __device__ __forceinline__ __nv_bfloat162 shfl_xor_bf162(__nv_bfloat162 v, int o
 // 32-byte sectors. Consecutive warps take consecutive heads of the same keys
 // (adjacent in the source). Rows outside [start, start + count) are neither
 // read nor written; a word that mixes both is written byte by byte.
-// Bound by instructions before memory (41 us under ncu: issue slots 68 % busy,
-// DRAM 42 %), so: the extrema of a lane's 8 rows are reduced and scattered in
-// one exchange (lane c % 8 ends up with row c % 8's, 7 shuffles instead of 24)
-// and a row's step and reciprocal are computed by that lane alone; codes come
-// two at a time (packed fp32). 32768 keys of 8 heads: 59 us before that (22
-// instructions a value), 34.3 us now (13; 172 MB, 5.0 TB/s = 76 % of a copy's
-// rate); four blocks an SM, 37.4 with the three that 65 registers allow.
+// Bound by instructions as much as by memory (35 us under ncu: issue slots 73 %
+// busy, DRAM 49 %), so: the extrema of a lane's 8 rows are reduced and scattered
+// in one exchange (lane c % 8 ends up with row c % 8's, 7 shuffles instead of
+// 24) and a row's step and reciprocal are computed by that lane alone; codes
+// come two at a time (packed fp32) and are gathered by byte permutations. 32768
+// keys of 8 heads: 59 us before that (22 instructions a value), 32.1 us now (12;
+// 172 MB, 5.4 TB/s = 82 % of a copy's rate), of which extrema and steps are a
+// seventh; four blocks an SM (three: 9 % more).
 __global__ void __launch_bounds__(256, 4) kv4_write_kernel(const Kv4RowsParams p) {
   griddep_wait();
   griddep_launch_dependents();
@@ -246,7 +247,7 @@ __global__ void __launch_bounds__(256, 4) kv4_write_kernel(const Kv4RowsParams p
 
 // Read back: the same item and lane mapping, the other way. A nibble becomes a
 // float by a byte permutation under the exponent of 2^23 and one packed
-// subtraction. Bound by memory: 28.7 us for 32768 keys of 8 heads (91 %).
+// subtraction. Bound by memory: 28.8 us for 32768 keys of 8 heads (91 %).
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4RowsParams p) {
   griddep_wait();
   griddep_launch_dependents();
