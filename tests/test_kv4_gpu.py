@@ -269,6 +269,17 @@ def test_attention_unlike_rows(cuda, B, Hq, Hkv, n_prefix, n_keys, bias_kind):
     check_attend(cuda, q, k, v, valid, n_prefix, n_keys, bias)
 
 
+@pytest.mark.parametrize("B,Hkv", [(37, 8), (38, 8), (49, 8), (50, 8), (75, 4), (148, 1), (149, 2)])
+@pytest.mark.parametrize("n", [33, 500])
+def test_attention_of_many_rows(cuda, B, Hkv, n):
+    """Batches about as large as the number of blocks that a KV head has, even and unlike rows."""
+    g = torch.Generator().manual_seed(B)
+    q = torch.randn(B, Hkv, 128, generator=g).bfloat16()
+    k, v = rows(g, B, n, Hkv, 128) / 2, rows(g, B, n, Hkv, 128)
+    check_attend(cuda, q, k, v, [n] * B, n, n)
+    check_attend(cuda, q, k, v, [(7 * b) % (n + 1) for b in range(B)], n, n)
+
+
 def test_attention_without_keys_on_the_device(cuda):
     """A device-side count of none (or below): zeros, in both ways of merging."""
     for B, n in ((1, 300), (3, 9000)):

@@ -1424,6 +1424,10 @@ Kv4Shape kv4_shape(int B, int Hkv, int n_keys) {
     // 128 ragged rows of 4097: 16.8 us, two blocks of 8 warps 5 % more)
     s.warps = 4;
     s.parts = 4 * sms / Hkv > 0 ? 4 * sms / Hkv : 1;
+    // Where that is between one and a half and two to a row, some rows would get one block and some two: three to
+    // each, in two rounds (40 rows of 8200 keys, 8 heads: 114 -> 76 us, of 2771: 50 -> 39, ragged ones 28.0 -> 28.9;
+    // 49 rows of 8200: 116 -> 87). At 64 rows, 1.2 to a row, three were slower (54 -> 59).
+    if (2 * B > s.parts && 3 * B <= 2 * s.parts) s.parts = 3 * B;
   }
   return s;
 }
