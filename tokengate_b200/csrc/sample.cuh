@@ -123,8 +123,10 @@ struct SmpRow {
   }
   __device__ __forceinline__ float product(float x) const { return __fmaf_rn(x, rh, __fmul_rn(x, rl)); }
 };
-// The weights of two logits, as exp(smp_d) gives them, of a usual row: two at a
-// time up to the exponentials, whose results for NaN become 0.
+// exp, held to [0, 1], which the buckets rely on; 0 for NaN
+__device__ __forceinline__ float smp_exp(float d) { return __saturatef(expf(d)); }
+// The weights of two logits, as smp_exp(smp_d) gives them, of a usual row: two at
+// a time up to the exponentials.
 __device__ __forceinline__ float2 smp_weights2(float x, float y, const SmpRow& r) {
   float2 d;
   asm("{\n\t.reg .b64 a, h, l, z;\n\t"
@@ -133,7 +135,7 @@ __device__ __forceinline__ float2 smp_weights2(float x, float y, const SmpRow& r
       "mov.b64 {%0, %1}, a;\n\t}"
       : "=f"(d.x), "=f"(d.y)
       : "f"(x), "f"(y), "f"(r.rh), "f"(r.rl), "f"(-r.zmax));
-  return make_float2(fmaxf(expf(d.x), 0.f), fmaxf(expf(d.y), 0.f));
+  return make_float2(smp_exp(d.x), smp_exp(d.y));
 }
 __device__ __forceinline__ float smp_d(float x, const SmpRow& r) {
   float d;
@@ -216,7 +218,7 @@ struct Smp {
     for (int e = 0; e < 4; ++e) f[e] = i + e < n ? smp_load(x + i + e) : -INFINITY;
     return make_float4(f[0], f[1], f[2], f[3]);
   }
-  __device__ __forceinline__ float weight_of(float logit) const { return expf(smp_d(logit, row)); }
+  __device__ __forceinline__ float weight_of(float logit) const { return smp_exp(smp_d(logit, row)); }
   // f(i, what is held of indices i to i + 3) over this warp's range, each lane every 32nd four
   template <typename F>
   __device__ __forceinline__ void each4(F f) const {
@@ -470,7 +472,7 @@ struct Smp {
     if (tid < m) {
       ord = s.few_ord[tid];
       d = smp_d(smp_unkey((uint32_t)(ord >> 32)), row);
-      w = expf(d);
+      w = smp_exp(d);
       mass = smp_mass(w);
       s.few_mass[tid] = mass;
     }
