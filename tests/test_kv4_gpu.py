@@ -280,6 +280,26 @@ def test_attention_of_many_rows(cuda, B, Hkv, n):
     check_attend(cuda, q, k, v, [(7 * b) % (n + 1) for b in range(B)], n, n)
 
 
+@pytest.mark.parametrize("B,Hq,Hkv", [(1, 4, 4), (3, 16, 2), (40, 8, 8)])
+def test_attention_of_one_key(cuda, B, Hq, Hkv):
+    """A single key's value comes back as the bf16 rounding of something within p s's rounding (2^-11 of code - 8
+    steps) and the cut of the products (2^-14 of a step each, two to a value: 2^-13); other slots masked."""
+    g = torch.Generator().manual_seed(Hq)
+    q = (3 * torch.randn(B, Hq, 128, generator=g)).bfloat16()
+    k, v = rows(g, B, 70, Hkv, 128), rows(g, B, 70, Hkv, 128)
+    c = KV4Cache(B, 70, Hkv, device=cuda)
+    ops.kv4_write(c, k.to(cuda), v.to(cuda))
+    _, exact, zero = quantise(v)
+    groups = v.double().unflatten(-1, (2, 64))
+    step = ((groups.amax(-1, keepdim=True) - groups.amin(-1, keepdim=True)) / 15).expand_as(groups).flatten(-2) * 1.01
+    for j, n_prefix in ((0, 0), (69, 69)):   # the first slot, decoded; the last one behind a masked prompt
+        n_valid = torch.zeros(B, dtype=torch.int32, device=cuda)
+        out = ops.decode_attention_kv4(q.to(cuda), c, n_valid, n_prefix, j + 1).cpu()
+        e, z, s = (t[:, j].repeat_interleave(Hq // Hkv, dim=1) for t in (exact, zero, step))
+        slack = 2 ** -11 * (e - z).abs() + 2 ** -13 * s
+        assert ((out >= (e - slack).bfloat16()) & (out <= (e + slack).bfloat16())).all()
+
+
 def test_attention_without_keys_on_the_device(cuda):
     """A device-side count of none (or below): zeros, in both ways of merging."""
     for B, n in ((1, 300), (3, 9000)):
