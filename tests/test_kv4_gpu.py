@@ -280,6 +280,22 @@ def test_attention_of_many_rows(cuda, B, Hkv, n):
     check_attend(cuda, q, k, v, [(7 * b) % (n + 1) for b in range(B)], n, n)
 
 
+@pytest.mark.parametrize("B", [37, 38, 49, 50])
+def test_attention_of_many_long_rows(cuda, B):
+    """The same where rows are long enough to take several blocks each; every row holds the same keys."""
+    g = torch.Generator().manual_seed(B)
+    n = 2100
+    q = torch.randn(B, 8, 128, generator=g).bfloat16()
+    k, v = rows(g, 1, n, 8, 128) / 2, rows(g, 1, n, 8, 128)
+    c = KV4Cache(B, n, 8, device=cuda)
+    ops.kv4_write(c, k.to(cuda).expand(B, -1, -1, -1), v.to(cuda).expand(B, -1, -1, -1))
+    for valid in ([n] * B, [n * b // (B - 1) for b in range(B)]):
+        out = ops.decode_attention_kv4(q.to(cuda), c, torch.tensor(valid, dtype=torch.int32, device=cuda), n, n).cpu()
+        for b in range(0, B, 3):
+            ref, tol = attend(q[b:b + 1], k, v, [valid[b]], n, n, None, None)
+            assert ((out[b:b + 1].double() - ref).abs() <= tol).all(), b
+
+
 @pytest.mark.parametrize("B,Hq,Hkv", [(1, 4, 4), (3, 16, 2), (40, 8, 8)])
 def test_attention_of_one_key(cuda, B, Hq, Hkv):
     """A single key's value comes back as the bf16 rounding of something within p s's rounding (2^-11 of code - 8

@@ -1425,9 +1425,10 @@ Kv4Shape kv4_shape(int B, int Hkv, int n_keys) {
     s.warps = 4;
     s.parts = 4 * sms / Hkv > 0 ? 4 * sms / Hkv : 1;
     // Where that is between one and a half and two to a row, some rows would get one block and some two: three to
-    // each, in two rounds (40 rows of 8200 keys, 8 heads: 114 -> 76 us, of 2771: 50 -> 39, ragged ones 28.0 -> 28.9;
-    // 49 rows of 8200: 116 -> 87). At 64 rows, 1.2 to a row, three were slower (54 -> 59).
-    if (2 * B > s.parts && 3 * B <= 2 * s.parts) s.parts = 3 * B;
+    // each, in two rounds, if the rows are long (40 rows, 8 heads, of 8200 keys 114 -> 76 us, of 2771 50 -> 39, of
+    // 1500 27 -> 25; of 1000 20.8 -> 21.6, of 100 9.8 -> 14.4; ragged ones of 2771 28.0 -> 28.9; 49 rows of 8200 116
+    // -> 87). At 64 rows, 1.2 to a row, three were slower (54 -> 59).
+    if (tiles > 64 && 2 * B > s.parts && 3 * B <= 2 * s.parts) s.parts = 3 * B;
   }
   return s;
 }
