@@ -193,6 +193,32 @@ def test_hard_logits(cuda):
         assert torch.isnan(l2.cpu()[[3, 8]]).all()
 
 
+@pytest.mark.parametrize("B,V", [(1, 1), (1, 301), (3, 1101), (1, 50257), (2, 50258), (1, 9999), (40, 513)])
+def test_extreme_temperatures_of_odd_rows(cuda, B, V):
+    """Temperatures outside the range in which quotients are products, on rows that do not fill their last four:
+    an infinite one and 1e30 make every token alike, 1e-30 leaves the largest, here exactly 0. Tokens are of the row."""
+    g = torch.Generator().manual_seed(V)
+    u = ((torch.randint(0, V, (B,), generator=g) + 0.5) / V).numpy()
+    u[-1] = (V - 0.5) / V                      # the row's last token
+    for dtype in (torch.bfloat16, torch.float32):
+        x = torch.randn(B, V, generator=g).to(dtype)
+        for t in (float("inf"), 1e30):
+            tok, lp = run(cuda, x, u, t)
+            assert (tok == torch.as_tensor(np.floor(u * V)).long()).all()
+            assert (lp + np.log(V)).abs().max() <= 1e-5
+            run(cuda, x, u, t, k=V // 2 + 1)
+            run(cuda, x, u, t, m=0.5)
+            if V > 8:
+                xf = x.float().numpy()
+                run(cuda, x, u, t, p=np.array([middle_p(xf[b], t, 0, V // 2) for b in range(B)], dtype=np.float32))
+        x = -1 - x.abs()
+        top = torch.randint(0, V, (B,), generator=g)
+        x[torch.arange(B), top] = 0
+        for kw in (dict(), dict(k=5), dict(p=0.9), dict(m=0.2)):
+            tok, lp = run(cuda, x, u, 1e-30, **kw)
+            assert torch.equal(tok, top) and (lp == 0).all(), kw
+
+
 def test_edges_of_the_parameters(cuda):
     g = torch.Generator().manual_seed(12)
     x = torch.randn(3, 3000, generator=g) * 2

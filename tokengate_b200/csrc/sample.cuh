@@ -828,8 +828,12 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SamplePara
         q = make_float4(a.x, a.y, b.x, b.y);
       });
     } else {
+      // The padding up to a four's end goes to zero with the range's last index, by the warp that holds that one: the
+      // warps after it have no range (and would turn it a second time, while others read it).
+      if (c.w0 < c.w1) {
 #pragma unroll 1
-      for (int i = c.w0 + lane; i < ((c.w1 + 3) & ~3); i += 32) c.sw[i] = c.weight_of(c.sw[i]);
+        for (int i = c.w0 + lane; i < ((c.w1 + 3) & ~3); i += 32) c.sw[i] = c.weight_of(c.sw[i]);
+      }
       __syncwarp();
     }
     c.each4([&](int, float4 q) { take(q); });
