@@ -529,12 +529,10 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
     if (h0 + 1 < p.G) bias1 = bp + p.bias_sh;
   }
 
-  bool ok = true;
-  for (int i = 0, s = 0, ph = 0; i < mine; ++i) {
-    if (!mbar_wait(full_s + 8 * s, ph, p.err, ERR_KV4)) {
-      ok = false;
-      break;
-    }
+  int i = 0, s = 0, ph = 0;
+  for (; i < mine; ++i) {
+    // one answer for the warp: lanes that gave up and lanes that did not would wait for one another below
+    if (!__all_sync(0xffffffffu, mbar_wait(full_s + 8 * s, ph, p.err, ERR_KV4))) break;
     const int j0 = tile_of(i) * kKv4Keys;
     const uint8_t* tile = ring + s * kKv4TileBytes;
     if (j0 + kKv4Keys <= n_keys && (j0 + kKv4Keys <= nv || j0 >= p.n_prefix))
@@ -548,8 +546,15 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
       ph ^= 1;
     }
   }
-  if (!ok)  // a copy never came: give those in flight their time before the shared memory goes
-    for (int s = 0; s < S; ++s) mbar_wait(full_s + 8 * s, 0, p.err, ERR_KV4);
+  // a copy never came: it and those behind it get their time, each in its own phase, before the ring is used again
+  for (int k = 0; k < S && i < mine; ++k, ++i) {
+    mbar_wait(full_s + 8 * s, ph, p.err, ERR_KV4);
+    if (++s == S) {
+      s = 0;
+      ph ^= 1;
+    }
+  }
+  __syncwarp();
 
   // ---- merge the warps: their sums into the rings' memory
 #pragma unroll
