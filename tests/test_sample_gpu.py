@@ -219,6 +219,22 @@ def test_extreme_temperatures_of_odd_rows(cuda, B, V):
             assert torch.equal(tok, top) and (lp == 0).all(), kw
 
 
+@pytest.mark.parametrize("V", [300, 700, 1000, 1500, 2047, 9000])
+def test_boundary_among_the_lowest_logits(cuda, V):
+    """A top-k and a top-p that end among logits of the type's lowest value, which an infinite temperature makes
+    as likely as the others: by index, behind all the others."""
+    g = torch.Generator().manual_seed(V)
+    for top in (1.0, 0.99, 0.5000001, 1.5, -0.25):     # keys of any low bits
+        x = torch.full((2, V), torch.finfo(torch.float32).min)
+        for b in range(2):
+            x[b, torch.randperm(V, generator=g)[:V // 3]] = top - torch.rand(V // 3, generator=g)
+            x[b, V // 2 + b] = top
+        u = np.array([0.3, 0.999], dtype=np.float32)
+        run(cuda, x, u, float("inf"), k=V // 2)
+        run(cuda, x, u, float("inf"), p=middle_p(x[0].numpy(), float("inf"), 0, V // 2))
+        run(cuda, x, u, float("inf"), k=V - 3, p=middle_p(x[0].numpy(), float("inf"), V - 3, V // 2))
+
+
 def test_edges_of_the_parameters(cuda):
     g = torch.Generator().manual_seed(12)
     x = torch.randn(3, 3000, generator=g) * 2

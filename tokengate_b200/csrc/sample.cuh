@@ -645,7 +645,7 @@ struct Smp {
       __syncthreads();
       need -= s.pick_above;
       hi -= (uint32_t)s.pick << shift;
-      lo = max(lo, hi - ((1u << shift) - 1u));  // (the picked bin: something is in it)
+      if (hi - lo >= 1u << shift) lo = hi - ((1u << shift) - 1u);  // (the picked bin: something is in it)
       // the bin's keys to a list of their own, if they fit, and their range (of bf16 logits they are often alike)
       uint32_t* kept = s.own[turn] + flip * kHalf;
       uint32_t k0 = 0xFFFFFFFFu, k1 = 0u;
