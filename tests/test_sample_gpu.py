@@ -219,6 +219,20 @@ def test_extreme_temperatures_of_odd_rows(cuda, B, V):
             assert torch.equal(tok, top) and (lp == 0).all(), kw
 
 
+@pytest.mark.parametrize("t", [6e-7, 5e-8, 2e-8, 1e-8, 3e-9, 1e-12, 7e-15, 1e-17])
+def test_small_temperatures_beside_the_lowest_logits(cuda, t):
+    """Logits of the type's lowest value have no weight at any temperature, beside one that is larger than the rest."""
+    g = torch.Generator().manual_seed(20)
+    for dtype in (torch.bfloat16, torch.float32):
+        x = torch.randn(3, 2001, generator=g).clamp(max=3.0).to(dtype)
+        x[:, ::3] = torch.finfo(dtype).min
+        x[1, x[1] > -1] = -1.0
+        x[:, 1000] = torch.tensor([8.0, -1e-3, 1e15]).to(dtype)
+        for kw in (dict(), dict(k=40), dict(p=0.9), dict(m=0.1)):
+            tok, lp = run(cuda, x, np.array([0.0, 0.4, 0.999], dtype=np.float32), t, **kw)
+            assert (tok == 1000).all() and (lp == 0).all(), kw
+
+
 @pytest.mark.parametrize("V", [300, 700, 1000, 1500, 2047, 9000])
 def test_boundary_among_the_lowest_logits(cuda, V):
     """A top-k and a top-p that end among logits of the type's lowest value, which an infinite temperature makes

@@ -108,8 +108,9 @@ __device__ __forceinline__ float smp_load(const __nv_bfloat16* p) { return smp_l
 // J.-M. Muller, "Correctly rounded multiplication by arbitrary precision
 // constants", 2008): x * high + RN(x * low) in one fma is within 2^-47 of the
 // quotient before its rounding, a division's cost without a division. Outside
-// the range in which the low part is a normal number, and for rows whose
-// maximum is huge or infinite, the division itself.
+// the range of T in which the low part is a normal number and below 1 (so that
+// the type's lowest logit times it stays finite, and short of the high part's
+// product), and for rows whose maximum is huge or infinite, the division itself.
 struct SmpRow {
   float xmax, zmax, t, rh, rl;
   bool plain;  // the usual row: a finite maximum, and quotients as products
@@ -118,7 +119,7 @@ struct SmpRow {
     t = tt;
     rh = __frcp_rn(t);
     rl = __fdiv_rn(__fmaf_rn(-t, rh, 1.f), t);
-    plain = t > 8.6736174e-19f && t < 1.1529215e18f && fabsf(x) < 1e18f;  // 2^-60 < T < 2^60
+    plain = t > 9.5367432e-7f && t < 1.1529215e18f && fabsf(x) < 1e18f;  // 2^-20 < T < 2^60
     zmax = plain ? product(x) : __fdiv_rn(x, t);
   }
   __device__ __forceinline__ float product(float x) const { return __fmaf_rn(x, rh, __fmul_rn(x, rl)); }
