@@ -418,6 +418,104 @@ def test_attention_repeats_bit_for_bit(cuda):
     assert all(torch.equal(a, ops.decode_attention_kv4(q, c, nv, 3000, 3000)) for _ in range(5))
 
 
+def _masked(cuda, G, value, at, spoil, n=300):
+    """A batch of two rows whose keys `at` a bias of `value` masks, with their V rows as `spoil` makes them."""
+    g = torch.Generator().manual_seed(G + n)
+    q, k, v = torch.randn(2, 2 * G, 128, generator=g).bfloat16(), rows(g, 2, n, 2, 128) / 2, rows(g, 2, n, 2, 128)
+    bias = torch.randn(2, 1, n, generator=g)
+    bias[..., at] = value
+    c = KV4Cache(2, n, 2, device=cuda)
+    held = v.clone()
+    if isinstance(spoil, float):
+        v[:, at] *= spoil
+    ops.kv4_write(c, k.to(cuda), v.to(cuda))
+    if not isinstance(spoil, float):       # bytes of the two groups' steps and lows (4352: V's parameters in a tile)
+        for j in at:
+            c.data[:, :, j // 32, 4352 + 8 * (j % 32):4360 + 8 * (j % 32)] = torch.tensor(spoil, dtype=torch.uint8, device=cuda)
+    out = ops.decode_attention_kv4(q.to(cuda), c, torch.tensor([n, n], dtype=torch.int32, device=cuda), n, n, bias=bias.to(cuda))
+    ref, tol = attend(q, k, held, [n, n], n, n, bias, None)
+    err = (out.double().cpu() - ref).abs()
+    assert (err <= tol).all(), (err / tol).max()
+
+
+@pytest.mark.parametrize("G", [2, 4, 8])
+@pytest.mark.parametrize("value", [float("-inf"), -1e9, torch.finfo(torch.float32).min])
+@pytest.mark.parametrize("at", [[0], [150], [299], list(range(0, 300, 2)), list(range(100)), list(range(64, 300))])
+def test_attention_masked_keys_weigh_nothing(cuda, G, value, at):
+    """Keys that the bias masks, at either end and between, whatever their V's range: up to bf16's largest, an
+    infinite step, and (behind -inf, where nothing is read as a number) NaN."""
+    for spoil in (1e10, 1e30, 1e37):
+        _masked(cuda, G, value, at, spoil)
+    inf, big, nan = [0x80, 0x7F, 0, 0], [0x7F, 0x7F, 0x7F, 0xFF], [0xC0, 0x7F, 0xC0, 0x7F]
+    _masked(cuda, G, value, at, inf + inf)
+    _masked(cuda, G, value, at, big + inf)
+    if value == -math.inf:
+        _masked(cuda, G, value, at, nan + big)
+
+
+@pytest.mark.parametrize("n,B,Hq,Hkv", [(40, 1, 2, 1), (700, 3, 16, 2), (9000, 1, 4, 2)])
+def test_attention_rubbish_behind_a_bias(cuda, n, B, Hq, Hkv):
+    """Slots that were never written hold random bytes, in K too: a bias of -inf hides them."""
+    g = torch.Generator().manual_seed(n)
+    q, k, v = torch.randn(B, Hq, 128, generator=g).bfloat16(), rows(g, B, n, Hkv, 128) / 2, rows(g, B, n, Hkv, 128)
+    c = KV4Cache(B, n, Hkv, device=cuda)
+    c.data.copy_(torch.randint(0, 256, c.data.shape, generator=g).to(torch.uint8))
+    lo, hi = n // 3, n // 3 + 20
+    ops.kv4_write(c, k[:, lo:hi].to(cuda), v[:, lo:hi].to(cuda), start=lo)
+    bias = torch.full((B, 1, n), float("-inf"))
+    bias[..., lo:hi] = torch.randn(B, 1, 20, generator=g)
+    out = ops.decode_attention_kv4(q.to(cuda), c, torch.full((B,), n, dtype=torch.int32, device=cuda), n, n, bias=bias.to(cuda))
+    ref, tol = attend(q, k[:, lo:hi], v[:, lo:hi], [20] * B, 20, 20, bias[..., lo:hi], None)
+    assert ((out.double().cpu() - ref).abs() <= tol).all()
+
+
+def test_long_cache_of_rubbish(cuda):
+    """5.4 GB of random bytes behind a bias of -inf, and 40 keys."""
+    g = torch.Generator().manual_seed(8)
+    cap = 4_700_032
+    c = KV4Cache(1, cap, 8, device=cuda)
+    c.data.random_(0, 256)
+    q, k, v = torch.randn(1, 16, 128, generator=g).bfloat16(), rows(g, 1, 40, 8, 128), rows(g, 1, 40, 8, 128)
+    for at in (cap - 41, 1_000_003):
+        ops.kv4_write(c, k.to(cuda), v.to(cuda), start=at)
+        bias = torch.full((1, 1, cap), float("-inf"), device=cuda)
+        bias[..., at:at + 40] = 0
+        out = ops.decode_attention_kv4(q.to(cuda), c, torch.tensor([cap], dtype=torch.int32, device=cuda), cap, cap, bias=bias)
+        ref, tol = attend(q, k, v, [40], 40, 40, None, None)
+        assert ((out.double().cpu() - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("G", [1, 4, 8])
+@pytest.mark.parametrize("apart", [1e4, 1e5, 1e6, 1e7, 1e8, 1e10, 1e20])
+def test_attention_groups_of_unlike_steps(cuda, G, apart):
+    """The two groups of a row's values far apart, in either order, few and many keys, with and without a bias."""
+    g = torch.Generator().manual_seed(G)
+    for n in (1, 90, 2100):
+        q, k, v = torch.randn(1, 2 * G, 128, generator=g).bfloat16(), rows(g, 1, n, 2, 128), rows(g, 1, n, 2, 128)
+        bias = torch.randn(1, 2 * G, n, generator=g)
+        for half in (slice(0, 64), slice(64, 128)):
+            w = v.clone()
+            w[..., half] /= apart
+            check_attend(cuda, q, k, w, [n], n, n)
+            check_attend(cuda, q, k, w, [n], n, n, bias)
+
+
+def test_attention_heads_of_unlike_values(cuda):
+    """Keys that hold values 1e8 times the others', of weight in one head of a KV head and of none in the rest; and
+    values that shrink along the cache while the scores grow."""
+    g = torch.Generator().manual_seed(12)
+    for G in (2, 4, 8):
+        n = 400
+        q, k, v = torch.randn(1, 2 * G, 128, generator=g).bfloat16(), rows(g, 1, n, 2, 128) / 2, rows(g, 1, n, 2, 128)
+        v[:, 30] *= 1e8
+        v[:, 390] *= 1e12
+        bias = torch.randn(1, 2 * G, n, generator=g)
+        bias[:, 1::2, 30] = bias[:, 1::2, 390] = -90.0
+        check_attend(cuda, q, k, v, [n], n, n, bias)
+        w = rows(g, 1, n, 2, 128) * torch.logspace(12, 0, n)[None, :, None, None].bfloat16()
+        check_attend(cuda, q, k, w, [n], n, n, torch.linspace(-200, 0, n).repeat(1, 1, 1))
+
+
 # ------------------------------------------------------------------ refusals
 def test_refusals(cuda):
     z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device=cuda)  # noqa: E731

@@ -18,10 +18,14 @@
 //   q': scaled by a power of two per head (largest |q| in [2^12, 2^13)) so that
 //       bf16 fits fp16; exact down to 2^-22 of the largest (the sixteenth that
 //       meets the upper nibbles too), 2^-33 of it below.
-//   p s: fp16 (11 bits), the one rounding of the products' operands; p is
-//       relative to a running maximum that may lag, s to a running power of
-//       two, so neither leaves fp16's range (maximum and power move together,
-//       in a branch that the first tiles take and later ones hardly ever).
+//   p s: fp16 (11 bits), the one rounding of the products' operands. p is
+//       relative to a running maximum that may lag; p s to a power of two of
+//       its head and group that keeps the largest p s seen, not the largest s,
+//       in the upper half of fp16's range, so that a step counts only with the
+//       weight of its key (a masked key's not at all) and no group or head
+//       costs another its bits. Maximum and powers move in two branches that
+//       the first tiles take and later ones hardly ever. A power shrinks with
+//       what was summed when the maximum moves.
 //       So that the rounding weighs code - 8 and not code, which is twice as
 //       large, sum_j p_j v_j is computed as sum (p s) code - 8 sum (p s) +
 //       sum p (low + 8 s), the first two sums of the same rounded p s.
@@ -55,7 +59,7 @@ constexpr int kKv4Stages = 3;          // ring tiles per warp, at most
 constexpr int kKv4MaxWarps = 16;
 constexpr int kKv4MaxCluster = 8;
 constexpr int kKv4OStride = 132;       // of a head's sums in shared memory: the four lanes of a row on different banks
-constexpr float kKv4Head = 4.f;       // p = 2^(4 + ...): small p stay normal in fp16
+constexpr int kKv4Room = 7;            // p s is scaled to [2^7, 2^8) at its largest, 2^15 at most: normal fp16 down to 2^-14
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Kv4AttnParams {
@@ -230,9 +234,18 @@ struct Kv4State {
   uint32_t qf[8][2];    // B fragments of q'
   float qs[2][2];       // sum(q') per group and column
   float mul[2];
-  float m[2], l[2], zs[2][2];  // running maximum, sum p, sum p (low + 8 s) - 8 (p s) per group
-  float acc[8][4];             // sum (p s) code, times 2^-24 (rows g) or 2^-20 (rows g + 8)
-  float eref, einv;            // the power of two that s is relative to
+  float m[2], l[2];           // running maximum, sum p
+  float2 zs[2];               // per column, (group 0, group 1): sum p (low + 8 s) - 8 (p s)
+  float acc[8][4];             // sum (p s) code / e, times 2^-24 (rows g) or 2^-20 (rows g + 8)
+  float2 einv[2];              // likewise 1 / e: e, the power of two that p s is relative to, is 2^-126 to 2^121
+};
+__device__ __forceinline__ float kv4_pow2_inverse(float x) {  // of a power of two from 2^-126 to 2^126
+  return __uint_as_float(0x7F000000u - __float_as_uint(x));
+}
+
+template <bool V>
+struct Kv4Bool {
+  static constexpr bool value = V;
 };
 
 // One tile of 32 keys from shared memory. ALL: every key is attended.
@@ -296,82 +309,126 @@ __device__ __forceinline__ void kv4_tile(Kv4State& st, const uint8_t* tile, int 
       sc[r][j] = !row_ok[r] || (BIAS && bj[r][j] == -INFINITY) ? -INFINITY : v;
     }
   }
-  // ---- move the running maximum / power of two when a score or a step outgrows them
-  float sn[R][2], smax = 0.f, top[2];
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    sn[r][0] = kv4_scale(vp[r].x) * st.einv;
-    sn[r][1] = kv4_scale(vp[r].y) * st.einv;
-    smax = fmax3(smax, sn[r][0], sn[r][1]);
-  }
+  // ---- move the running maximum when a score outgrows it: what was summed shrinks by al, of which the powers of two
+  // take the exponent (rounded up) and the accumulators the rest
+  float top[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     top[j] = fmaxf(sc[0][j], sc[1][j]);
     if (!PAIR) top[j] = fmax3(top[j], sc[R - 2][j], sc[R - 1][j]);
   }
   constexpr float kLag = BIAS ? 4.f : 4.f * kLog2e;
-  const bool grow = top[0] > st.m[0] + kLag || top[1] > st.m[1] + kLag || smax > 16.f;
-  if (__any_sync(0xffffffffu, grow)) {
-    float sraw = 0.f;
-#pragma unroll
-    for (int r = 0; r < R; ++r) sraw = fmax3(sraw, kv4_scale(vp[r].x), kv4_scale(vp[r].y));
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) sraw = fmaxf(sraw, __shfl_xor_sync(0xffffffffu, sraw, off));
-    // a power of two above the largest step, at most 2^126
-    const uint32_t eb = min((__float_as_uint(sraw) >> 23) + 1u, 253u);
-    const float enew = fmaxf(st.eref, __uint_as_float(eb << 23));
-    const float beta = st.eref / enew;
-    st.eref = enew;
-    st.einv = 1.f / enew;
-    float al[2];
+  if (__any_sync(0xffffffffu, top[0] > st.m[0] + kLag || top[1] > st.m[1] + kLag)) {
+    float f[2][2];
+    bool none[2];  // sums that lost all weight are zero, whatever the keys held that a bias has masked
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const float mn = fmaxf(st.m[j], warp_max_rows(top[j]));
-      al[j] = mn == -INFINITY ? 1.f : ex2_approx((st.m[j] - mn) * (BIAS ? kLog2e : 1.f));
+      const float al = mn == -INFINITY ? 1.f : ex2_approx((st.m[j] - mn) * (BIAS ? kLog2e : 1.f));
+      none[j] = BIAS && al == 0.f;
       st.m[j] = mn;
-      st.l[j] *= al[j];
-      st.zs[0][j] *= al[j];
-      st.zs[1][j] *= al[j];
+      st.l[j] *= al;
+      st.zs[j] = none[j] ? make_float2(0.f, 0.f) : make_float2(st.zs[j].x * al, st.zs[j].y * al);
+      const float pow = __uint_as_float((__float_as_uint(al) + 0x007FFFFFu) & 0x7F800000u);
+      auto shrink = [&](float& inv) {
+        const float e = kv4_pow2_inverse(inv);
+        inv = kv4_pow2_inverse(fmaxf(e * pow, 1.17549435e-38f));
+        return al == 0.f ? 0.f : al * (e * inv);
+      };
+      f[0][j] = shrink(st.einv[j].x);
+      f[1][j] = shrink(st.einv[j].y);
     }
 #pragma unroll
     for (int w = 0; w < 8; ++w)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) st.acc[w][e] *= al[e & 1] * beta;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      sn[r][0] = kv4_scale(vp[r].x) * st.einv;
-      sn[r][1] = kv4_scale(vp[r].y) * st.einv;
-    }
+      for (int e = 0; e < 4; ++e) st.acc[w][e] = none[e & 1] ? 0.f : st.acc[w][e] * f[w >> 2][e & 1];
   }
-  // ---- p and its sums; p s as B fragments (two key rows to a register)
-  const float off[2] = {kKv4Head - st.m[0], kKv4Head - st.m[1]}, eight = -8.f * st.eref;
-  uint32_t pf[2][R];
+  // ---- p and its sums; p s / e, a column's two groups at a time
+  float p[R][2], big = 0.f;
+  float2 u[R][2];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    float p[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const float v = sc[r][j];
-      const float e = BIAS ? ex2_approx(fmaf(v - st.m[j], kLog2e, kKv4Head)) : ex2_approx(v + off[j]);
-      p[j] = (BIAS || !ALL) && v == -INFINITY ? 0.f : e;
-      st.l[j] += p[j];
+      const float e = BIAS ? ex2_approx((v - st.m[j]) * kLog2e) : ex2_approx(v - st.m[j]);
+      p[r][j] = (BIAS || !ALL) && v == -INFINITY ? 0.f : e;
+      st.l[j] += p[r][j];
+    }
+  }
+  {
+    float2 sv[R], z[R], odd = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      sv[r] = make_float2(kv4_scale(vp[r].x), kv4_scale(vp[r].y));
+      z[r] = __ffma2_rn(make_float2(8.f, 8.f), sv[r], make_float2(kv4_low(vp[r].x), kv4_low(vp[r].y)));
+      if (BIAS) odd = __ffma2_rn(z[r], make_float2(0.f, 0.f), odd);  // NaN: a step or a low is not finite
+    }
+    auto sums = [&](auto checked) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const bool none = decltype(checked)::value && p[r][j] == 0.f;  // masked: whatever the key holds
+          const float2 pp = make_float2(p[r][j], p[r][j]), nil = make_float2(0.f, 0.f);
+          st.zs[j] = __ffma2_rn(pp, none ? nil : z[r], st.zs[j]);
+          u[r][j] = __fmul2_rn(__fmul2_rn(pp, none ? nil : sv[r]), st.einv[j]);
+          big = fmax3(big, u[r][j].x, u[r][j].y);
+        }
+    };
+    if (BIAS && __any_sync(0xffffffffu, !(odd.x + odd.y == 0.f)))
+      sums(Kv4Bool<true>());
+    else
+      sums(Kv4Bool<false>());
+  }
+  // ---- move the powers of two when a p s outgrows them
+  if (__any_sync(0xffffffffu, big > 32768.f)) {
+    float f[2][2];
+    float2 ps[R];  // once more, from the tile: fewer registers where it does not happen
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float2 m = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const uint2 pm = *reinterpret_cast<const uint2*>(tile + kKv4Vp + (row0 + 8 * r) * 8);
+        const bool none = p[r][j] == 0.f;
+        ps[r] = make_float2(none ? 0.f : p[r][j] * kv4_scale(pm.x), none ? 0.f : p[r][j] * kv4_scale(pm.y));
+        m = make_float2(fmaxf(m.x, ps[r].x), fmaxf(m.y, ps[r].y));
+      }
+      // their exponents, both groups' in a word
+      uint32_t both = __byte_perm(__float_as_uint(m.x), __float_as_uint(m.y), 0x7632);
+#pragma unroll
+      for (int off = 4; off <= 16; off <<= 1) both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, off));
+      auto grow = [&](float& inv, uint32_t exponent) {
+        const float e = kv4_pow2_inverse(inv);
+        inv = kv4_pow2_inverse(fmaxf(e, __uint_as_float((uint32_t)max((int)(exponent & 255u) - kKv4Room, 1) << 23)));
+        return e * inv;
+      };
+      f[0][j] = grow(st.einv[j].x, both >> 7);
+      f[1][j] = grow(st.einv[j].y, both >> 23);
+#pragma unroll
+      for (int r = 0; r < R; ++r) u[r][j] = __fmul2_rn(ps[r], st.einv[j]);
     }
 #pragma unroll
-    for (int gr = 0; gr < 2; ++gr) {
-      const uint32_t pm = gr ? vp[r].y : vp[r].x;
-      const float z = fmaf(8.f, kv4_scale(pm), kv4_low(pm));
-      float u[2] = {p[0] * sn[r][gr], p[1] * sn[r][gr]};
-      if (BIAS) {  // a key that the bias masks may hold NaN
-        u[0] = p[0] == 0.f ? 0.f : u[0];
-        u[1] = p[1] == 0.f ? 0.f : u[1];
-      }
-      const __half2 h = __floats2half2_rn(u[0], u[1]);
-      const float2 hf = __half22float2(h);
-      const float z0 = fmaf(hf.x, eight, fmaf(p[0], z, st.zs[gr][0])), z1 = fmaf(hf.y, eight, fmaf(p[1], z, st.zs[gr][1]));
-      st.zs[gr][0] = BIAS && p[0] == 0.f ? st.zs[gr][0] : z0;
-      st.zs[gr][1] = BIAS && p[1] == 0.f ? st.zs[gr][1] : z1;
-      pf[gr][r] = movmatrix_trans(h2_bits(h));
-    }
+    for (int w = 0; w < 8; ++w)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) st.acc[w][e] *= f[w >> 2][e & 1];
+  }
+  // ---- as fp16, and the sums of these; as B fragments (two key rows to a register)
+  uint32_t pf[2][R];
+  float2 eight[2];  // -8 e
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    eight[j] = make_float2(__uint_as_float(0x00800000u - __float_as_uint(st.einv[j].x)),
+                           __uint_as_float(0x00800000u - __float_as_uint(st.einv[j].y)));
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const __half2 h0 = __floats2half2_rn(u[r][0].x, u[r][1].x), h1 = __floats2half2_rn(u[r][0].y, u[r][1].y);
+    const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
+    st.zs[0] = __ffma2_rn(make_float2(f0.x, f1.x), eight[0], st.zs[0]);
+    st.zs[1] = __ffma2_rn(make_float2(f0.y, f1.y), eight[1], st.zs[1]);
+    pf[0][r] = movmatrix_trans(h2_bits(h0));
+    pf[1][r] = movmatrix_trans(h2_bits(h1));
   }
   // ---- P V
 #pragma unroll
@@ -502,7 +559,9 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
   for (int j = 0; j < 2; ++j) {
     st.mul[j] = sh.mul[h0 + j];
     st.m[j] = -INFINITY;
-    st.l[j] = st.zs[0][j] = st.zs[1][j] = 0.f;
+    st.l[j] = 0.f;
+    st.zs[j] = make_float2(0.f, 0.f);
+    st.einv[j] = make_float2(8.507059173e37f, 8.507059173e37f);  // 2^126
 #pragma unroll
     for (int gr = 0; gr < 2; ++gr) {
       const uint4 x = *reinterpret_cast<const uint4*>(&sh.q[h0 + j][64 * gr + 8 * g]);
@@ -520,8 +579,6 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
   for (int w = 0; w < 8; ++w)
 #pragma unroll
     for (int e = 0; e < 4; ++e) st.acc[w][e] = 0.f;
-  st.eref = 1.17549435e-38f;  // 2^-126
-  st.einv = 8.507059173e37f;
   const float *bias0 = nullptr, *bias1 = nullptr;
   if (BIAS) {
     const float* bp = p.bias + (int64_t)b * p.bias_sb + (int64_t)(kvh * p.G + h0) * p.bias_sh;
@@ -560,8 +617,7 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     st.l[j] = warp_sum_rows(st.l[j]);
-    st.zs[0][j] = warp_sum_rows(st.zs[0][j]);
-    st.zs[1][j] = warp_sum_rows(st.zs[1][j]);
+    st.zs[j] = make_float2(warp_sum_rows(st.zs[j].x), warp_sum_rows(st.zs[j].y));
     if (g == 0) {
       sh.m[warp][2 * t + j] = st.m[j];
       sh.l[warp][2 * t + j] = st.l[j];
@@ -572,9 +628,11 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
 #pragma unroll
   for (int w = 0; w < 8; ++w)
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int e = 0; e < 4; ++e) {
+      const float inv = w < 4 ? st.einv[e & 1].x : st.einv[e & 1].y, z = w < 4 ? st.zs[e & 1].x : st.zs[e & 1].y;
       so[(2 * t + (e & 1)) * kKv4OStride + 16 * w + g + 8 * (e >> 1)] =
-          fmaf(st.acc[w][e] * (e < 2 ? 16777216.f : 1048576.f), st.eref, st.zs[w >> 2][e & 1]);
+          fmaf(st.acc[w][e] * (e < 2 ? 16777216.f : 1048576.f), kv4_pow2_inverse(inv), z);
+    }
   if (clustered) cluster_wait();  // every block has started
   __syncthreads();
   constexpr float kUnit = BIAS ? kLog2e : 1.f;  // of m
@@ -607,6 +665,7 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         const float f = sh.m[w][h + 4 * k];
+        if (BIAS && f == 0.f) continue;  // no weight: whatever the masked keys held
         const float4 v = *reinterpret_cast<const float4*>(all_o + w * (S * kKv4TileBytes / 4) + (h + 4 * k) * kKv4OStride + d);
         o.x = fmaf(f, v.x, o.x);
         o.y = fmaf(f, v.y, o.y);
@@ -641,8 +700,8 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
     for (int c = 0; c < C; ++c) {
       const float lw = sh.got_l[c][h];
       if (lw != 0.f) {
-        const float f = ex2_approx((sh.got_m[c][h] - mt) * kUnit);
-        o = fmaf(f, sh.got_o[c * slice + i], o);
+        const float f = ex2_approx((sh.got_m[c][h] - mt) * kUnit), on = fmaf(f, sh.got_o[c * slice + i], o);
+        o = BIAS && f == 0.f ? o : on;
         lt = fmaf(f, lw, lt);
       }
     }
@@ -668,7 +727,8 @@ __global__ void __launch_bounds__(32 * kKv4CombineWarps) kv4_combine_kernel(cons
   griddep_launch_dependents();
   if (C == 1) return;  // its one block has written the output
   const float* rec = p.part + ((int64_t)h * (p.parts + p.B) + first) * kKv4Part;
-  const float unit = p.bias != nullptr ? kLog2e : 1.f;  // of m
+  const bool masks = p.bias != nullptr;  // sums without weight may hold anything then
+  const float unit = masks ? kLog2e : 1.f;  // of m
   float m = -INFINITY, l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int c0 = warp; c0 < C; c0 += 4 * kKv4CombineWarps) {
@@ -692,11 +752,13 @@ __global__ void __launch_bounds__(32 * kKv4CombineWarps) kv4_combine_kernel(cons
     o.y *= back;
     o.z *= back;
     o.w *= back;
+    if (masks && back == 0.f) o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       if (ml[k].y != 0.f) {  // 0: the block saw no key (a NaN sum stays in)
         const float f = ex2_approx((ml[k].x - m) * unit);
         l = fmaf(f, ml[k].y, l);
+        if (masks && f == 0.f) continue;
         o.x = fmaf(f, v[k].x, o.x);
         o.y = fmaf(f, v[k].y, o.y);
         o.z = fmaf(f, v[k].z, o.z);
@@ -717,8 +779,8 @@ __global__ void __launch_bounds__(32 * kKv4CombineWarps) kv4_combine_kernel(cons
 #pragma unroll
     for (int w = 0; w < kKv4CombineWarps; ++w) {
       if (s_l[w] != 0.f) {
-        const float f = ex2_approx((s_m[w] - mt) * unit);
-        ot = fmaf(f, s_o[w][threadIdx.x], ot);
+        const float f = ex2_approx((s_m[w] - mt) * unit), on = fmaf(f, s_o[w][threadIdx.x], ot);
+        ot = masks && f == 0.f ? ot : on;
         lt = fmaf(f, s_l[w], lt);
       }
     }
