@@ -516,6 +516,19 @@ def test_attention_heads_of_unlike_values(cuda):
         check_attend(cuda, q, k, w, [n], n, n, torch.linspace(-200, 0, n).repeat(1, 1, 1))
 
 
+@pytest.mark.parametrize("G", [2, 8])
+@pytest.mark.parametrize("apart", [1e4, 1e6, 1e8, 1e10])
+def test_attention_groups_of_unlike_queries(cuda, G, apart):
+    """Large keys meet small queries in one group of dims, in the other the reverse: both count in the scores."""
+    g = torch.Generator().manual_seed(G)
+    n = 200
+    for half in (slice(0, 64), slice(64, 128)):
+        q, k, v = torch.randn(1, 2 * G, 128, generator=g).bfloat16(), rows(g, 1, n, 2, 128), rows(g, 1, n, 2, 128)
+        q[..., half] /= apart
+        k[..., half] *= apart
+        check_attend(cuda, q, k, v, [n], n, n)
+
+
 # ------------------------------------------------------------------ refusals
 def test_refusals(cuda):
     z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device=cuda)  # noqa: E731

@@ -15,9 +15,9 @@
 // and the one at bit 4 code * 2^-20: five logic instructions unpack eight codes.
 // The factors 2^-24 and 2^-20 go into q' (K: each nibble meets its own dim) and
 // into the final sums (V: each nibble is a row of the accumulators).
-//   q': scaled by a power of two per head (largest |q| in [2^12, 2^13)) so that
-//       bf16 fits fp16; exact down to 2^-22 of the largest (the sixteenth that
-//       meets the upper nibbles too), 2^-33 of it below.
+//   q': scaled by a power of two per head and group (largest |q| in [2^12, 2^13))
+//       so that bf16 fits fp16; exact down to 2^-22 of the group's largest (the
+//       sixteenth that meets the upper nibbles too), 2^-33 of it below.
 //   p s: fp16 (11 bits), the one rounding of the products' operands. p is
 //       relative to a running maximum that may lag; p s to a power of two of
 //       its head and group that keeps the largest p s seen, not the largest s,
@@ -86,7 +86,7 @@ constexpr int kKv4Part = 4 + 128;  // m, l, 2 pad, O[128]
 
 struct alignas(16) Kv4AttnShared {
   __half q[8][128];
-  float mul[8];
+  float mul[8][2];                                // per group
   float m[kKv4MaxWarps][8], l[kKv4MaxWarps][8];   // of the warps' columns; m becomes their factors of the merge
   float head_m[8], head_l[8];
   float got_o[8 * 128];                           // [rank][slice]: this block's slice of the blocks' sums
@@ -232,8 +232,7 @@ __device__ __forceinline__ void kv4_store_out(__nv_bfloat16* at, float4 o, float
 // units, where a bias of the type's lowest value does not overflow.
 struct Kv4State {
   uint32_t qf[8][2];    // B fragments of q'
-  float qs[2][2];       // sum(q') per group and column
-  float mul[2];
+  float2 qs[2], mul[2];  // per column, (group 0, group 1): sum(q'), and what undoes its power of two
   float m[2], l[2];           // running maximum, sum p
   float2 zs[2];               // per column, (group 0, group 1): sum p (low + 8 s) - 8 (p s)
   float acc[8][4];             // sum (p s) code / e, times 2^-24 (rows g) or 2^-20 (rows g + 8)
@@ -293,18 +292,16 @@ __device__ __forceinline__ void kv4_tile(Kv4State& st, const uint8_t* tile, int 
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const uint2 kp = *reinterpret_cast<const uint2*>(tile + kKv4Kp + (row0 + 8 * r) * 8);
-    const float s0 = kv4_scale(kp.x) * 16777216.f, s1 = kv4_scale(kp.y) * 16777216.f;  // 2^24: the codes' units
-    const float z0 = kv4_low(kp.x), z1 = kv4_low(kp.y);
+    const float2 sk = __fmul2_rn(make_float2(kv4_scale(kp.x), kv4_scale(kp.y)),
+                                 make_float2(16777216.f, 16777216.f));  // 2^24: the codes' units
+    const float2 zk = make_float2(kv4_low(kp.x), kv4_low(kp.y));
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int e = 2 * (r & 1) + j;
       const float c0 = PAIR ? (t < 2 ? c[0][0][e] : c[1][0][e]) : c[r >> 1][0][e];
       const float c1 = PAIR ? (t < 2 ? c[0][1][e] : c[1][1][e]) : c[r >> 1][1][e];
-      float v = z0 * st.qs[0][j];
-      v = fmaf(z1, st.qs[1][j], v);
-      v = fmaf(s0, c0, v);
-      v = fmaf(s1, c1, v);
-      v = BIAS ? fmaf(v, st.mul[j], bj[r][j]) : v * st.mul[j];
+      const float2 d = __ffma2_rn(sk, make_float2(c0, c1), __fmul2_rn(zk, st.qs[j]));
+      const float v = fmaf(d.x, st.mul[j].x, BIAS ? fmaf(d.y, st.mul[j].y, bj[r][j]) : d.y * st.mul[j].y);
       // -inf in the bias is a mask, whatever the key holds
       sc[r][j] = !row_ok[r] || (BIAS && bj[r][j] == -INFINITY) ? -INFINITY : v;
     }
@@ -532,11 +529,11 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
       mx = fmaxf(mx, fabsf(v[e]));
     }
 #pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+    for (int off = 8; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));  // of the group
     // 2^(12 - exponent), inside fp32's normal range on both sides
     const int ex = min(max((int)(__float_as_uint(mx) >> 23) - 127 - 12, -126), 126);
     const float down = __uint_as_float((uint32_t)(127 - ex) << 23);
-    if (lane == 0) sh.mul[h] = __uint_as_float((uint32_t)(127 + ex) << 23) * p.scale * (BIAS ? 1.f : kLog2e);
+    if ((lane & 15) == 0) sh.mul[h][lane >> 4] = __uint_as_float((uint32_t)(127 + ex) << 23) * p.scale * (BIAS ? 1.f : kLog2e);
     const __half2 a = __floats2half2_rn(v[0] * down, v[1] * down), c = __floats2half2_rn(v[2] * down, v[3] * down);
     *reinterpret_cast<uint2*>(&sh.q[h][4 * lane]) = make_uint2(h2_bits(a), h2_bits(c));
   }
@@ -557,7 +554,7 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
   const int h0 = PAIR ? 2 * (t & 1) : 2 * t;  // head of column 2 t
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    st.mul[j] = sh.mul[h0 + j];
+    st.mul[j] = make_float2(sh.mul[h0 + j][0], sh.mul[h0 + j][1]);
     st.m[j] = -INFINITY;
     st.l[j] = 0.f;
     st.zs[j] = make_float2(0.f, 0.f);
@@ -572,7 +569,7 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
         const float2 f = __half22float2(bits_h2(w[e]));
         a += f.x + f.y;
       }
-      st.qs[gr][j] = warp_sum_rows(a);
+      (gr ? st.qs[j].y : st.qs[j].x) = warp_sum_rows(a);
     }
   }
 #pragma unroll
