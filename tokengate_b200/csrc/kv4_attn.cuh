@@ -316,6 +316,8 @@ __device__ __forceinline__ void kv4_tile(Kv4State& st, const uint8_t* tile, int 
   }
   constexpr float kLag = BIAS ? 4.f : 4.f * kLog2e;
   if (__any_sync(0xffffffffu, top[0] > st.m[0] + kLag || top[1] > st.m[1] + kLag)) {
+    // (a warp's first tile rescales nothing: one of the two passes over the accumulators saved where tiles are few)
+    const bool summed = __any_sync(0xffffffffu, st.m[0] > -INFINITY || st.m[1] > -INFINITY);
     float f[2][2];
     bool none[2];  // sums that lost all weight are zero, whatever the keys held that a bias has masked
 #pragma unroll
@@ -335,10 +337,12 @@ __device__ __forceinline__ void kv4_tile(Kv4State& st, const uint8_t* tile, int 
       f[0][j] = shrink(st.einv[j].x);
       f[1][j] = shrink(st.einv[j].y);
     }
+    if (summed) {
 #pragma unroll
-    for (int w = 0; w < 8; ++w)
+      for (int w = 0; w < 8; ++w)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) st.acc[w][e] = none[e & 1] ? 0.f : st.acc[w][e] * f[w >> 2][e & 1];
+        for (int e = 0; e < 4; ++e) st.acc[w][e] = none[e & 1] ? 0.f : st.acc[w][e] * f[w >> 2][e & 1];
+    }
   }
   // ---- p and its sums; p s / e, a column's two groups at a time
   float p[R][2], big = 0.f;
