@@ -30,14 +30,15 @@
 //       large, sum_j p_j v_j is computed as sum (p s) code - 8 sum (p s) +
 //       sum p (low + 8 s), the first two sums of the same rounded p s.
 //   The matrix unit aligns a subnormal's product as if it had fp16's smallest
-//       exponent, so that each step of 16 keys (16 dims) is cut at 2^-24 of
-//       that: 2^-14 of the largest p s (q' s), measured; a tenth of what the
-//       rounding of p s does to a code one step from 8, 2^-18 of a group's range.
+//       exponent, so that each of a step's 16 products is cut at 2^-24 of that:
+//       2^-14 of the largest p s (q' s), measured on one key; of several keys
+//       2^-12.7 of the dominant one's step was the most seen: as much as the
+//       rounding of p s does to a code one step from 8, 2^-16.6 of a group's range.
 // Scores, maxima, sums and the accumulators are fp32: finite for keys and values
 // up to 2^100.
 //
 // The cache is read once, at 144 bytes per key: every warp streams its own
-// tiles through a ring of two or three in shared memory (one bulk copy of 4608
+// tiles through a ring of two in shared memory (one bulk copy of 4608
 // bytes each, no barrier between warps). 2 rows of 131081 keys, 8 kv heads:
 // 53.3 us, 302 MB = 5.7 TB/s (86 % of a copy's rate), of which 47 are the loop,
 // at DRAM's rate, the rest its start, the merges and the second launch. In the
@@ -55,7 +56,7 @@
 namespace tg {
 
 constexpr unsigned int ERR_KV4 = 1u << 15;  // bit of the device error word
-constexpr int kKv4Stages = 3;          // ring tiles per warp, at most
+constexpr int kKv4Stages = 2;          // ring tiles per warp
 constexpr int kKv4MaxWarps = 16;
 constexpr int kKv4MaxCluster = 8;
 constexpr int kKv4OStride = 132;       // of a head's sums in shared memory: the four lanes of a row on different banks
@@ -78,7 +79,7 @@ struct Kv4AttnParams {
   int64_t o_sb, o_sh;
   float* part;           // nullable: records [Hq][parts + B][kKv4Part] instead of a merge in a cluster
   int parts;             // blocks per kv head that fill the GPU, shared among the batch rows
-  int B, G, Hq, stages;
+  int B, G, Hq;
   float scale;
   unsigned int* err;
 };
@@ -94,7 +95,7 @@ struct alignas(16) Kv4AttnShared {
   uint64_t full[kKv4MaxWarps][kKv4Stages];
 };
 constexpr int kKv4Ring = (sizeof(Kv4AttnShared) + 127) / 128 * 128;  // byte offset of the warps' rings
-constexpr int kv4_attn_smem(int warps, int stages) { return kKv4Ring + warps * stages * kKv4TileBytes; }
+constexpr int kv4_attn_smem(int warps) { return kKv4Ring + warps * kKv4Stages * kKv4TileBytes; }
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                               uint32_t b0, uint32_t b1) {
@@ -467,7 +468,7 @@ __global__ void __launch_bounds__(32 * kKv4MaxWarps, 1) kv4_attn_kernel(const Kv
   const int g = lane >> 2, t = lane & 3;
   const int kvh = blockIdx.y;
   int b = blockIdx.z, C = gridDim.x, rank = blockIdx.x;
-  const int S = p.stages;
+  constexpr int S = kKv4Stages;
   uint8_t* ring = kv4_smem + kKv4Ring + warp * S * kKv4TileBytes;
   const uint32_t ring_s = smem_u32(ring), full_s = smem_u32(sh.full[warp]);
   if (lane == 0) {

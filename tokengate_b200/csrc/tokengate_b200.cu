@@ -1406,12 +1406,12 @@ int kv4_rows(const char* what, bool write, const void* k, int64_t k_sb, int64_t 
 // Warps of a block, and the blocks: of a cluster per kv head and row, or (parts
 // > 0) the blocks per kv head that the rows share.
 struct Kv4Shape {
-  int warps, stages, cluster, parts;
+  int warps, cluster, parts;
 };
 Kv4Shape kv4_shape(int B, int Hkv, int n_keys) {
   const int64_t rows = (int64_t)B * Hkv, tiles = kv4_tiles(n_keys);
   const int sms = sm_count();
-  Kv4Shape s = {tg::kKv4MaxWarps, 2, 1, 0};
+  Kv4Shape s = {tg::kKv4MaxWarps, 1, 0};
   if (tiles <= 192 && rows * 2 <= sms) {
     // short caches, where a second launch costs more than idle SMs
     while (s.cluster < 8 && rows * s.cluster * 2 <= sms && tiles > s.cluster) s.cluster *= 2;
@@ -1573,18 +1573,17 @@ int tg_decode_attn_kv4(const void* q, int64_t q_sb, int64_t q_sh, const float* q
   }
   p.part = need > 0 ? static_cast<float*>(workspace) : nullptr;
   p.parts = shape.parts;
-  p.stages = shape.stages;
   p.B = B;
   p.Hq = Hq;
   const bool pair = p.G <= 4;
   auto kern = bias != nullptr ? (pair ? tg::kv4_attn_kernel<true, true> : tg::kv4_attn_kernel<true, false>)
                               : (pair ? tg::kv4_attn_kernel<false, true> : tg::kv4_attn_kernel<false, false>);
   bool(&flags)[kMaxDevices] = g_kv4_attr_set[2 * (bias != nullptr) + pair];
-  cudaError_t e = cluster_limits_once(kern, tg::kv4_attn_smem(tg::kKv4MaxWarps, 2), flags, dev);
+  cudaError_t e = cluster_limits_once(kern, tg::kv4_attn_smem(tg::kKv4MaxWarps), flags, dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(decode_attn_kv4)");
   const dim3 grid((unsigned)(need > 0 ? shape.parts + B : shape.cluster), (unsigned)Hkv, (unsigned)(need > 0 ? 1 : B));
   const dim3 block(32u * shape.warps);
-  e = launch_cluster(kern, grid, block, tg::kv4_attn_smem(shape.warps, shape.stages), static_cast<cudaStream_t>(stream),
+  e = launch_cluster(kern, grid, block, tg::kv4_attn_smem(shape.warps), static_cast<cudaStream_t>(stream),
                      shape.cluster, p);
   if (e != cudaSuccess) return cuda_fail(e, "decode_attn_kv4 launch");
   if (need > 0) {
