@@ -478,8 +478,8 @@ int tg_qk_norm_rope_append_kv4(const void* q, int64_t ld_q, int n_q_heads, const
  * query scale, pad slots and device-side key count. A bias of -inf masks its
  * key whatever the key holds; rows without any key give zeros. 1 to 8 query
  * heads per kv head. workspace: device scratch of
- * tg_decode_attn_kv4_workspace bytes (0: none), 16-byte aligned; calls
- * sharing it must not overlap on the GPU. */
+ * tg_decode_attn_kv4_workspace bytes (0: none; of the current device, as the
+ * call's), 16-byte aligned; calls sharing it must not overlap on the GPU. */
 int tg_decode_attn_kv4(const void* q, int64_t q_sb, int64_t q_sh, const float* q_scale, int64_t qs_sb,
                        const void* cache, int64_t capacity, const float* bias, int64_t bias_sb, int64_t bias_sh,
                        const int32_t* n_valid, int n_prefix, int n_keys, const int32_t* n_keys_dev, void* out,

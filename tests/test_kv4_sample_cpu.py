@@ -106,6 +106,37 @@ def test_packed_calls_are_the_calls():
     assert L.tg_call(3, struct.pack("<23qd", *a), 24, None) == BAD and b"softmax_scale" in L.tg_last_error()
 
 
+def test_workspace_is_asked_of_the_cache_device(monkeypatch):
+    """Devices of different SM counts: each one's own size, whichever is current."""
+    current = [0]
+
+    class On:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.was, current[0] = current[0], self.index
+
+        def __exit__(self, *a):
+            current[0] = self.was
+
+    class Lib:
+        @staticmethod
+        def tg_decode_attn_kv4_workspace(B, Hq, Hkv, n_keys, out):
+            out._obj.value = 1000 + current[0]
+            return 0
+
+    monkeypatch.setattr(torch.cuda, "device", On)
+    monkeypatch.setattr(_lib, "lib", lambda: Lib)
+    ops._kv4_workspace.cache_clear()
+    try:
+        for cur in (0, 1):
+            current[0] = cur
+            assert [ops._kv4_workspace(i, 1, 16, 8, 9000) for i in (0, 1, 0)] == [1000, 1001, 1000]
+    finally:
+        ops._kv4_workspace.cache_clear()
+
+
 def test_no_cpu_path():
     with pytest.raises(ValueError, match="CUDA"):
         KV4Cache(1, 8, 2, device="cpu")

@@ -823,9 +823,11 @@ def qk_norm_rope_append_kv4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q
 
 
 @functools.lru_cache(maxsize=4096)
-def _kv4_workspace(B: int, Hq: int, Hkv: int, n_keys: int) -> int:
+def _kv4_workspace(index: int, B: int, Hq: int, Hkv: int, n_keys: int) -> int:
+    """Of device `index`: the blocks that share the keys go by its SMs."""
     nbytes = ctypes.c_size_t(0)
-    _lib.check(_lib.lib().tg_decode_attn_kv4_workspace(B, Hq, Hkv, n_keys, ctypes.byref(nbytes)))
+    with torch.cuda.device(index):
+        _lib.check(_lib.lib().tg_decode_attn_kv4_workspace(B, Hq, Hkv, n_keys, ctypes.byref(nbytes)))
     return nbytes.value
 
 
@@ -877,7 +879,7 @@ def decode_attention_kv4(q: torch.Tensor, cache: KV4Cache, n_valid: torch.Tensor
     if n_keys_dev is not None:
         _on("n_keys_dev", n_keys_dev, torch.int32, dev)
         nk_ptr = n_keys_dev.data_ptr()
-    ws, ws_ptr, nbytes = None, 0, _kv4_workspace(B, Hq, c.n_kv_heads, n_keys)
+    ws, ws_ptr, nbytes = None, 0, _kv4_workspace(dev, B, Hq, c.n_kv_heads, n_keys)
     if nbytes:
         ws = c.data.new_empty(nbytes)
         ws_ptr = ws.data_ptr()
