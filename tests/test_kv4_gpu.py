@@ -123,6 +123,19 @@ def test_long_cache_offsets(cuda):
     assert ((out.double().cpu() - ref).abs() <= tol).all()
 
 
+def test_a_copied_cache_leaves_the_original_alone(cuda):
+    import copy
+    g = torch.Generator().manual_seed(15)
+    k, v = rows(g, 1, 40, 2, 128), rows(g, 1, 40, 2, 128)
+    c = KV4Cache(1, 40, 2, device=cuda)
+    ops.kv4_write(c, k.to(cuda), v.to(cuda))
+    was = c.data.clone()
+    d = copy.deepcopy(c)
+    ops.kv4_write(d, v.to(cuda), k.to(cuda))
+    assert torch.equal(c.data, was)
+    assert same(ops.kv4_read(d)[0].double().cpu(), quantise(v)[0]) and same(ops.kv4_read(c)[0].double().cpu(), quantise(k)[0])
+
+
 # ------------------------------------------------------------------ append
 @pytest.mark.parametrize("B,Hq,Hkv,slot,cap", [(1, 16, 8, 0, 1), (1, 4, 1, 40, 64), (3, 8, 8, 31, 32), (5, 16, 2, 99, 100),
                                               (64, 32, 8, 17, 40)])

@@ -137,6 +137,20 @@ def test_workspace_is_asked_of_the_cache_device(monkeypatch):
         ops._kv4_workspace.cache_clear()
 
 
+def test_a_copied_cache_is_its_own():
+    """What the calls get of a copied or unpickled cache is its own tensor's address, not the original's."""
+    import copy
+    import pickle
+    c = object.__new__(KV4Cache)
+    c.batch, c.capacity, c.n_kv_heads = 1, 40, 2
+    c.data, c.bf16 = torch.zeros(1, 2, 2, 4608, dtype=torch.uint8), torch.empty(0, dtype=torch.bfloat16)
+    for d in (copy.deepcopy(c), pickle.loads(pickle.dumps(c))):
+        assert d.data.data_ptr() != c.data.data_ptr()
+        assert d.ptr == d.data.data_ptr() and d.index == -1 and (d.batch, d.capacity, d.n_kv_heads) == (1, 40, 2)
+    c.data = torch.zeros(1, 2, 2, 4608, dtype=torch.uint8)
+    assert c.ptr == c.data.data_ptr()
+
+
 def test_no_cpu_path():
     with pytest.raises(ValueError, match="CUDA"):
         KV4Cache(1, 8, 2, device="cpu")

@@ -17,7 +17,7 @@ TILE_BYTES = 4608
 class KV4Cache:
     """`capacity` slots of `batch` rows with `n_kv_heads` KV heads, on a CUDA device."""
 
-    __slots__ = ("data", "batch", "capacity", "n_kv_heads", "ptr", "index", "bf16")
+    __slots__ = ("data", "batch", "capacity", "n_kv_heads", "bf16")
 
     def __init__(self, batch: int, capacity: int, n_kv_heads: int, device="cuda"):
         if batch < 1 or capacity < 1 or n_kv_heads < 1:
@@ -27,8 +27,16 @@ class KV4Cache:
         self.data = torch.empty((self.batch, self.n_kv_heads, tiles, TILE_BYTES), dtype=torch.uint8, device=device)
         if not self.data.is_cuda:
             raise ValueError(f"a KV4Cache lives on a CUDA device (the B200 kernels have no CPU path), got {self.data.device}")
-        self.ptr, self.index = self.data.data_ptr(), self.data.get_device()     # what every call asks for
         self.bf16 = torch.empty(0, dtype=torch.bfloat16, device=self.data.device)   # makes the outputs (new_empty)
+
+    # asked of the tensor at every call (0.1 us): a copied, unpickled or reassigned cache has its data elsewhere
+    @property
+    def ptr(self) -> int:
+        return self.data.data_ptr()
+
+    @property
+    def index(self) -> int:
+        return self.data.get_device()
 
     @property
     def device(self) -> torch.device:
