@@ -151,6 +151,23 @@ def test_a_copied_cache_is_its_own():
     assert c.ptr == c.data.data_ptr()
 
 
+def test_imports_on_a_torch_without_cuda():
+    """The package and the calls' bindings on a torch that lacks the private functions of a CUDA build."""
+    import os
+    import subprocess
+    import sys
+    code = ("import torch\n"
+            "for n in ('_cuda_getDevice', '_cuda_getCurrentRawStream'):\n"
+            "    if hasattr(torch._C, n): delattr(torch._C, n)\n"
+            "import tokengate_b200\n"
+            "from tokengate_b200 import _lib, ops, kv4, decode\n"
+            "_lib._bind_torch()\n"
+            "assert _lib._get_device is torch.cuda.current_device and callable(_lib._raw_stream)\n")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+
+
 def test_no_cpu_path():
     with pytest.raises(ValueError, match="CUDA"):
         KV4Cache(1, 8, 2, device="cpu")

@@ -10,8 +10,6 @@ import os
 import struct
 import threading
 
-import torch
-
 from .build import LIB_PATH
 
 ABI_VERSION = 1
@@ -175,10 +173,18 @@ def check_launch(status: int) -> None:
     check(status)
 
 
-# the current device and a device's current stream, without the Python objects
-# that torch.cuda.current_stream() makes of them (0.2 us instead of 2.5)
-_get_device = torch._C._cuda_getDevice
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_get_device = _raw_stream = None
+
+
+def _bind_torch() -> None:
+    """The current device and a device's current stream, without the Python objects that
+    torch.cuda.current_stream() makes of them (0.2 us instead of 2.5) where this torch has the
+    functions for that. Looked up by the first call: the package imports without them."""
+    global _get_device, _raw_stream
+    import torch
+    _get_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+        lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 class Call:
@@ -193,10 +199,13 @@ class Call:
     def __call__(self, index: int, *args) -> None:
         """Launch on device `index`, on its current stream."""
         global LAUNCH_CALLS
+        if _raw_stream is None:
+            _bind_torch()
         call = _lib.tg_call if _lib is not None else lib().tg_call
         if _get_device() == index:
             status = call(self._entry, self._pack(*args), self._n, _raw_stream(index))
         else:
+            import torch
             with torch.cuda.device(index):
                 status = call(self._entry, self._pack(*args), self._n, _raw_stream(index))
         LAUNCH_CALLS += 1
