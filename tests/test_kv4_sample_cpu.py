@@ -168,6 +168,48 @@ def test_imports_on_a_torch_without_cuda():
     assert r.returncode == 0, r.stderr
 
 
+def _model_of(Hq=16, Hkv=8, head_dim=128, vocab=1000):
+    from types import SimpleNamespace as NS
+    w = torch.empty(vocab, 8, device="meta")
+    cfg = NS(num_attention_heads=Hq, num_key_value_heads=Hkv, head_dim=head_dim, hidden_size=Hq * 128)
+    return NS(config=cfg, parameters=lambda: iter([torch.empty(1)]), lm_head=NS(weight=w), model=NS(layers=[1, 2]))
+
+
+def test_generation_is_refused_before_the_prefill(monkeypatch):
+    """What the 4-bit cache or the sampler does not serve, and settings that do not fit the batch."""
+    from tokengate_b200 import decode
+
+    class Ran(Exception):
+        pass
+
+    def prefill(*a, **k):
+        raise Ran
+
+    monkeypatch.setattr(decode, "prefill_batch_for_decode", prefill)
+
+    def go(model, n=3, **kw):
+        return decode.generate_batch(model, None, [[1, 2, 3]] * 2, [0, 0], [2, 2], 0, 1, n, **kw)
+
+    for kw in (dict(head_dim=64), dict(Hq=18, Hkv=2), dict(Hq=9, Hkv=2), dict(head_dim=None, Hq=16, Hkv=1)):
+        with pytest.raises(ValueError, match="kv_bits=4"):
+            go(_model_of(**kw), kv_bits=4)
+        with pytest.raises(Ran):                       # no decode step, no cache
+            go(_model_of(**kw), n=1, kv_bits=4)
+        with pytest.raises(Ran):
+            go(_model_of(**kw))
+    for kw in (dict(), dict(Hq=8, Hkv=8), dict(Hq=24, Hkv=3), dict(head_dim=None)):
+        with pytest.raises(Ran):
+            go(_model_of(**kw), kv_bits=4)
+    S = decode.Sampling
+    for s in (S(temperature=[1.0, 1.0, 1.0]), S(temperature=None), S(top_p=float("nan")), S(top_k=[5])):
+        with pytest.raises(ValueError):
+            go(_model_of(), sampling=s)
+    with pytest.raises(ValueError, match="vocabular"):
+        go(_model_of(vocab=(1 << 19) + 1), sampling=S())
+    with pytest.raises(Ran):
+        go(_model_of(vocab=1 << 19), sampling=S(temperature=[0.5, 1.0], top_k=3))
+
+
 def test_no_cpu_path():
     with pytest.raises(ValueError, match="CUDA"):
         KV4Cache(1, 8, 2, device="cpu")

@@ -41,7 +41,7 @@ import torch
 import torch.nn.functional as F
 
 from . import ops
-from .kv4 import KV4Cache
+from .kv4 import HEAD_DIM, KV4Cache
 from .layers import fused_weights
 from .prefill import prefill_batch_for_decode
 
@@ -148,6 +148,15 @@ class _DecodeCacheKV4:
             self.width.append(W)
 
 
+def _check_kv4(cfg) -> None:
+    """The heads that the 4-bit cache and its attention serve."""
+    Hq, Hkv = cfg.num_attention_heads, cfg.num_key_value_heads
+    D = getattr(cfg, "head_dim", None) or cfg.hidden_size // Hq
+    if D != HEAD_DIM or Hq % Hkv or Hq // Hkv > 8:
+        raise ValueError(f"kv_bits=4 serves head_dim {HEAD_DIM} and 1 to 8 query heads per KV head, the model has "
+                         f"head_dim {D} and {Hq} query heads on {Hkv} KV heads")
+
+
 @torch.no_grad()
 def generate_batch(model, gate, prompt_ids_list: Sequence, article_starts: Sequence[int],
                    article_ends: Sequence[int], gate_layer: int, max_kept_prefill_tokens,
@@ -174,7 +183,16 @@ def generate_batch(model, gate, prompt_ids_list: Sequence, article_starts: Seque
         raise ValueError("max_new_tokens must be positive")
     if kv_bits not in (4, 16):
         raise ValueError(f"kv_bits={kv_bits}: 16 (bf16) or 4")
+    if kv_bits == 4 and max_new_tokens > 1:
+        _check_kv4(model.config)
     device = next(model.parameters()).device
+    if sampling is not None:     # refused before the prefill, if at all
+        if model.lm_head.weight.shape[0] > ops.SAMPLE_MAX_VOCAB:
+            raise ValueError(f"sampling serves vocabularies of up to {ops.SAMPLE_MAX_VOCAB}, the model's has "
+                             f"{model.lm_head.weight.shape[0]}")
+        draw = sampling.on(len(prompt_ids_list), device)
+        u_all = torch.rand((max_new_tokens, len(prompt_ids_list)), dtype=torch.float32, device=device,
+                           generator=sampling.generator)
     inner = model.model
     n_layers = len(inner.layers)
     st: dict = {}
@@ -188,8 +206,6 @@ def generate_batch(model, gate, prompt_ids_list: Sequence, article_starts: Seque
     B = first.shape[0]
     lps = []
     if sampling is not None:
-        draw = sampling.on(B, device)
-        u_all = torch.rand((max_new_tokens, B), dtype=torch.float32, device=device, generator=sampling.generator)
         tok, lp = ops.sample_tokens(st["logits"], u_all[0], **draw)
         first = tok.view(B, 1)
         lps.append(lp)

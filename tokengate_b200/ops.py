@@ -890,6 +890,9 @@ def decode_attention_kv4(q: torch.Tensor, cache: KV4Cache, n_valid: torch.Tensor
 
 
 # ----------------------------------------------------------------- sampling
+SAMPLE_MAX_VOCAB = 1 << 19     # logits a row that tg_sample serves
+
+
 def _per_row(name: str, val, B: int, dtype: torch.dtype, index: int) -> Optional[torch.Tensor]:
     if val is None:
         return None
