@@ -210,6 +210,20 @@ def test_generation_is_refused_before_the_prefill(monkeypatch):
         go(_model_of(vocab=1 << 19), sampling=S(temperature=[0.5, 1.0], top_k=3))
 
 
+@pytest.mark.parametrize("k", [0.5, 2.7, float("nan"), float("inf"), 2 ** 40, -2 ** 33])
+def test_top_k_is_a_whole_number(k):
+    """Not cut to one: 0.5 would turn the rule off."""
+    from tokengate_b200.decode import Sampling
+    with pytest.raises(ValueError):
+        Sampling(top_k=k).on(1, "cpu")
+    with pytest.raises(ValueError):
+        Sampling(top_k=[3, k]).on(2, "cpu")
+    with pytest.raises(ValueError):
+        ops._per_row("top_k", k, 1, torch.int32, -1)
+    assert Sampling(top_k=[3.0, 7.0]).on(2, "cpu")["top_k"].tolist() == [3, 7]
+    assert Sampling(top_k=-1).on(2, "cpu")["top_k"].dtype == torch.int32
+
+
 def test_no_cpu_path():
     with pytest.raises(ValueError, match="CUDA"):
         KV4Cache(1, 8, 2, device="cpu")

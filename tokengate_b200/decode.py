@@ -83,7 +83,10 @@ class Sampling:
                     raise ValueError("temperature must be a number or one per request")
                 out[name] = None
                 continue
-            t = torch.as_tensor(val, dtype=dtype, device="cpu")
+            t = torch.as_tensor(val, dtype=None if dtype is torch.int32 else dtype, device="cpu")
+            if dtype is torch.int32 and not bool((t == t.to(dtype)).all()):
+                raise ValueError(f"{name} must be whole numbers of 32 bits, got {val}")
+            t = t.to(dtype)
             if t.dim() > 1 or (t.dim() == 1 and t.shape[0] != B):
                 raise ValueError(f"{name}: one value, or one for each of the {B} requests, got shape {tuple(t.shape)}")
             if t.is_floating_point() and bool(torch.isnan(t).any()):

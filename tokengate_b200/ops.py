@@ -897,6 +897,8 @@ def _per_row(name: str, val, B: int, dtype: torch.dtype, index: int) -> Optional
     if val is None:
         return None
     if not isinstance(val, torch.Tensor):
+        if dtype is torch.int32 and (not -2 ** 31 <= val < 2 ** 31 or val != int(val)):
+            raise ValueError(f"{name} must be a whole number of 32 bits, got {val}")
         return torch.full((B,), val, dtype=dtype, device=torch.device("cuda", index))
     if val.dtype is not dtype or val.get_device() != index:
         _on(name, val, dtype, index)
