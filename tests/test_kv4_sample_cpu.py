@@ -224,6 +224,27 @@ def test_top_k_is_a_whole_number(k):
     assert Sampling(top_k=-1).on(2, "cpu")["top_k"].dtype == torch.int32
 
 
+def test_decode_cache_releases_each_layer(monkeypatch):
+    """When a layer is quantised, the bf16 K/V of the layers before it are gone."""
+    import weakref
+    from types import SimpleNamespace as NS
+    from tokengate_b200 import decode
+    fused = [torch.zeros(1, 5, 8, 128, dtype=torch.bfloat16) for _ in range(3)]     # one projection per layer, K/V its views
+    held = [weakref.ref(t) for t in fused]
+    layers = [NS(k_tok=t[:, :, 4:6], v_tok=t[:, :, 6:]) for t in fused]
+    del fused
+    alive = []
+
+    def write(c, k, v):
+        alive.append([i for i, r in enumerate(held) if r() is not None or layers[i].k_tok is not None])
+        assert k.shape == v.shape == (1, 5, 2, 128) and c == (1, 9, 2)
+
+    monkeypatch.setattr(decode, "KV4Cache", lambda B, n, H, device: (B, n, H))
+    monkeypatch.setattr(ops, "kv4_write", write)
+    dc = decode._DecodeCacheKV4(NS(layers=layers), 3, 4)
+    assert alive == [[0, 1, 2], [1, 2], [2]] and dc.width == [5, 5, 5] and len(dc.kv) == 3
+
+
 def test_no_cpu_path():
     with pytest.raises(ValueError, match="CUDA"):
         KV4Cache(1, 8, 2, device="cpu")

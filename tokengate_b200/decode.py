@@ -138,15 +138,17 @@ class _DecodeCache:
 
 
 class _DecodeCacheKV4:
-    """The same in 4 bits: the prefill's prefix quantised to the front, decode tokens appended after it."""
+    """The same in 4 bits: the prefill's prefix quantised to the front, decode tokens appended after it. Each layer's
+    bf16 K/V are released from `cache` once they are written, so that the peak is the prefill's, not both caches."""
 
     def __init__(self, cache, n_layers: int, extra: int):
         self.kv, self.width = [], []
         for i in range(n_layers):
-            k, v = cache.layers[i].k_tok, cache.layers[i].v_tok
-            B, W, Hkv, _ = k.shape
-            c = KV4Cache(B, W + extra, Hkv, device=k.device)
-            ops.kv4_write(c, k, v)
+            layer = cache.layers[i]
+            B, W, Hkv, _ = layer.k_tok.shape
+            c = KV4Cache(B, W + extra, Hkv, device=layer.k_tok.device)
+            ops.kv4_write(c, layer.k_tok, layer.v_tok)
+            layer.k_tok = layer.v_tok = None
             self.kv.append(c)
             self.width.append(W)
 
