@@ -715,9 +715,9 @@ def _kv4(cache: KV4Cache) -> KV4Cache:
     return cache
 
 
-def _kv4_rows(name: str, t: torch.Tensor, c: KV4Cache, n: int) -> Tuple[int, int, int]:
+def _kv4_rows(name: str, t: torch.Tensor, c: KV4Cache, n: int, index: int) -> Tuple[int, int, int]:
     """The batch, slot and head strides of a (B, n, Hkv, 128) tensor."""
-    _on(name, t, torch.bfloat16, c.index)
+    _on(name, t, torch.bfloat16, index)
     if t.shape != (c.batch, n, c.n_kv_heads, 128):
         raise ValueError(f"{name} must be ({c.batch}, {n}, {c.n_kv_heads}, 128), got {tuple(t.shape)}")
     sb, ss, sh, sd = t.stride()
@@ -737,12 +737,14 @@ def kv4_write(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, start: int = 0)
     if not isinstance(k, torch.Tensor) or k.dim() != 4:
         raise ValueError("k must be a 4-D (B, S, Hkv, 128) tensor")
     S = k.shape[1]
-    ks, vs = _kv4_rows("k", k, c, S), _kv4_rows("v", v, c, S)
+    data = c.data
+    dev = data.get_device()
+    ks, vs = _kv4_rows("k", k, c, S, dev), _kv4_rows("v", v, c, S, dev)
     if start < 0 or start + S > c.capacity:
         raise ValueError(f"slots [{start}, {start + S}) are outside the cache's capacity {c.capacity}")
     if S:
-        _lib.kv4_write(c.index, k.data_ptr(), *ks, v.data_ptr(), *vs, c.batch, c.n_kv_heads, 128, start, S, c.ptr,
-                       c.capacity)
+        _lib.kv4_write(dev, k.data_ptr(), *ks, v.data_ptr(), *vs, c.batch, c.n_kv_heads, 128, start, S,
+                       data.data_ptr(), c.capacity)
 
 
 def kv4_read(cache: KV4Cache, start: int = 0, n: Optional[int] = None, k_out: Optional[torch.Tensor] = None,
@@ -754,7 +756,8 @@ def kv4_read(cache: KV4Cache, start: int = 0, n: Optional[int] = None, k_out: Op
     n = c.capacity - start if n is None else n
     if start < 0 or n < 0 or start + n > c.capacity:
         raise ValueError(f"slots [{start}, {start + n}) are outside the cache's capacity {c.capacity}")
-    H = c.n_kv_heads
+    H, data = c.n_kv_heads, c.data
+    dev = data.get_device()
     if k_out is None and v_out is None:
         k_out = c.bf16.new_empty(c.batch, n, H, 128)
         v_out = torch.empty_like(k_out)
@@ -762,10 +765,10 @@ def kv4_read(cache: KV4Cache, start: int = 0, n: Optional[int] = None, k_out: Op
     else:
         k_out = c.bf16.new_empty(c.batch, n, H, 128) if k_out is None else k_out
         v_out = c.bf16.new_empty(c.batch, n, H, 128) if v_out is None else v_out
-        ks, vs = _kv4_rows("k_out", k_out, c, n), _kv4_rows("v_out", v_out, c, n)
+        ks, vs = _kv4_rows("k_out", k_out, c, n, dev), _kv4_rows("v_out", v_out, c, n, dev)
     if n:
-        _lib.kv4_read(c.index, c.ptr, c.capacity, c.batch, H, 128, start, n, k_out.data_ptr(), *ks, v_out.data_ptr(),
-                      *vs)
+        _lib.kv4_read(dev, data.data_ptr(), c.capacity, c.batch, H, 128, start, n, k_out.data_ptr(), *ks,
+                      v_out.data_ptr(), *vs)
     return k_out, v_out
 
 
@@ -792,7 +795,8 @@ def qk_norm_rope_append_kv4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q
     rotated in fp32 with one rounding to bf16; k and v are quantised into the slot and left unchanged.
     Returns the finished q, (B, 1, Hq, 128) contiguous (or q_out, which may be q)."""
     c = _kv4(cache)
-    B, dev = c.batch, c.index
+    B, data = c.batch, c.data
+    dev = data.get_device()
     ld_q, Hq = _token_heads("q", q, B, None, dev)
     ld_k, _ = _token_heads("k", k, B, c.n_kv_heads, dev)
     ld_v, _ = _token_heads("v", v, B, c.n_kv_heads, dev)
@@ -818,7 +822,7 @@ def qk_norm_rope_append_kv4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q
         ld_qo, _ = _token_heads("q_out", q_out, B, Hq, dev)
     _lib.qk_norm_rope_append_kv4(dev, q.data_ptr(), ld_q, Hq, k.data_ptr(), ld_k, c.n_kv_heads, v.data_ptr(), ld_v, B,
                                  q_norm_w.data_ptr(), k_norm_w.data_ptr(), cos.data_ptr(), sin.data_ptr(), ld_cs, 128,
-                                 eps, q_out.data_ptr(), ld_qo, c.ptr, c.capacity, slot.data_ptr())
+                                 eps, q_out.data_ptr(), ld_qo, data.data_ptr(), c.capacity, slot.data_ptr())
     return q_out
 
 
@@ -839,7 +843,8 @@ def decode_attention_kv4(q: torch.Tensor, cache: KV4Cache, n_valid: torch.Tensor
     the place of k and v. q: (B, Hq, 128) bf16, Hq / Hkv from 1 to 8. A bias of -inf masks its key
     whatever the key holds; a row without any key gives zeros. Returns (B, Hq, 128) bf16."""
     c = _kv4(cache)
-    B, dev = c.batch, c.index
+    B, data = c.batch, c.data
+    dev = data.get_device()
     _on("q", q, torch.bfloat16, dev)
     shape = q.shape
     b, Hq, d = shape if len(shape) == 3 else (0, 0, 0)
@@ -881,9 +886,9 @@ def decode_attention_kv4(q: torch.Tensor, cache: KV4Cache, n_valid: torch.Tensor
         nk_ptr = n_keys_dev.data_ptr()
     ws, ws_ptr, nbytes = None, 0, _kv4_workspace(dev, B, Hq, c.n_kv_heads, n_keys)
     if nbytes:
-        ws = c.data.new_empty(nbytes)
+        ws = data.new_empty(nbytes)
         ws_ptr = ws.data_ptr()
-    _lib.decode_attn_kv4(dev, q.data_ptr(), q_sb, q_sh, qs_ptr, qsb, c.ptr, c.capacity, bias_ptr, bsb, bsh,
+    _lib.decode_attn_kv4(dev, q.data_ptr(), q_sb, q_sh, qs_ptr, qsb, data.data_ptr(), c.capacity, bias_ptr, bsb, bsh,
                          n_valid.data_ptr(), n_prefix, n_keys, nk_ptr, out.data_ptr(), o_sb, o_sh, ws_ptr, nbytes, B,
                          Hq, c.n_kv_heads, 128, 128 ** -0.5 if softmax_scale is None else softmax_scale)
     return out
