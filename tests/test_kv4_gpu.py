@@ -187,6 +187,27 @@ def test_append(cuda, B, Hq, Hkv, slot, cap):
     assert r is q2 and torch.equal(q2, out) and torch.equal(c.data, was)
 
 
+def test_append_of_one_row_takes_any_row_stride(cuda):
+    """Strides of dims of one are not used, whatever a view left there; those of more rows must be alike."""
+    g = torch.Generator().manual_seed(16)
+    q, k, v = rows(g, 1, 1, 4, 128).to(cuda), rows(g, 1, 1, 2, 128).to(cuda), rows(g, 1, 1, 2, 128).to(cuda)
+    w = rows(g, 128).to(cuda)
+    cos, sin = (torch.randn(1, 1, 128, generator=g).bfloat16().to(cuda) for _ in range(2))
+    sl = torch.tensor([3], dtype=torch.int64, device=cuda)
+    a, b = KV4Cache(1, 9, 2, device=cuda), KV4Cache(1, 9, 2, device=cuda)
+    a.data.zero_()
+    b.data.zero_()
+    want = ops.qk_norm_rope_append_kv4(q, k, v, w, w, cos, sin, 1e-6, a, sl)
+    odd = lambda t: t.as_strided(t.shape, (0, 3) + t.stride()[2:])  # noqa: E731
+    got = ops.qk_norm_rope_append_kv4(odd(q), odd(k), v.as_strided(v.shape, (5, 1, 128, 1)), w, w, odd(cos), sin, 1e-6, b, sl)
+    assert torch.equal(got, want) and torch.equal(a.data, b.data)
+    two = torch.zeros(2, 1, 4, 128, dtype=torch.bfloat16, device=cuda)
+    c2 = KV4Cache(2, 9, 2, device=cuda)
+    cs = torch.zeros(2, 1, 128, dtype=torch.bfloat16, device=cuda)
+    with pytest.raises(ValueError, match="strides"):
+        ops.qk_norm_rope_append_kv4(two, two[:, :, :2], two[:, :, 2:], w, w, cs, cs[:1].expand(2, -1, -1), 1e-6, c2, sl)
+
+
 # ------------------------------------------------------------------ attention
 def attend(q, k, v, n_valid, n_prefix, n_keys, bias, q_scale):
     """float64 (output, tolerance) of the definition over the values that the cache stands for."""

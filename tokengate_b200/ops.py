@@ -782,7 +782,7 @@ def _token_heads(name: str, t: torch.Tensor, B: int, heads: Optional[int], index
     sb, _, sh, sd = t.stride()
     if sd != 1 or (sh != 128 and n > 1):
         raise ValueError(f"{name} must have contiguous heads")
-    return sb, n
+    return sb if B > 1 else n * 128, n          # the stride of a dim of one is not used
 
 
 def qk_norm_rope_append_kv4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm_w: torch.Tensor,
@@ -805,10 +805,11 @@ def qk_norm_rope_append_kv4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q
         _on(nm, t, torch.bfloat16, dev)
         if t.shape != row:
             raise ValueError(f"{nm} must be ({B}, 1, 128), got {tuple(t.shape)}")
-    cs = cos.stride()
-    ld_cs, _, cd = cs
-    if cd != 1 or sin.stride() != cs:
+    (ld_cs, _, cd), (ld_sn, _, sd) = cos.stride(), sin.stride()
+    if cd != 1 or sd != 1 or (ld_cs != ld_sn and B > 1):
         raise ValueError("cos and sin must share strides and have a contiguous last dim")
+    if B == 1:
+        ld_cs = 128
     for nm, t in (("q_norm_w", q_norm_w), ("k_norm_w", k_norm_w)):
         _on(nm, t, torch.bfloat16, dev)
         if t.shape != (128,) or not t.is_contiguous():
