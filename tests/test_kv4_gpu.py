@@ -611,3 +611,13 @@ def test_refusals(cuda):
         ops.qk_norm_rope_append_kv4(a[0], z(1, 1, 4, 128), *a[2:], sl)
     with pytest.raises(ValueError):
         ops.qk_norm_rope_append_kv4(z(1, 2, 4, 128), *a[1:], sl)
+
+
+def test_a_device_count_of_no_element_is_refused(cuda):
+    """An empty tensor has no address, which would read as no count at all."""
+    c = KV4Cache(1, 10, 2, device=cuda)
+    nv = torch.tensor([5], dtype=torch.int32, device=cuda)
+    q = torch.zeros(1, 4, 128, dtype=torch.bfloat16, device=cuda)
+    for bad in (nv[:0], nv.expand(2)):
+        with pytest.raises(ValueError, match="n_keys_dev"):
+            ops.decode_attention_kv4(q, c, nv, 5, 5, n_keys_dev=bad)

@@ -884,6 +884,8 @@ def decode_attention_kv4(q: torch.Tensor, cache: KV4Cache, n_valid: torch.Tensor
         qs_ptr, qsb = q_scale.data_ptr(), q_scale.stride(0)
     if n_keys_dev is not None:
         _on("n_keys_dev", n_keys_dev, torch.int32, dev)
+        if n_keys_dev.numel() != 1:
+            raise ValueError("n_keys_dev must be an int32 (1,) tensor")
         nk_ptr = n_keys_dev.data_ptr()
     ws, ws_ptr, nbytes = None, 0, _kv4_workspace(dev, B, Hq, c.n_kv_heads, n_keys)
     if nbytes:
