@@ -435,8 +435,12 @@ int tg_decode_attn_noalloc(const void* q, int64_t q_sb, int64_t q_sh,
  * The 4-bit KV cache: K and V rows of head_dim 128 as 4-bit codes above a
  * bf16 low, with a bf16 step, per group of 64 consecutive dims:
  *   low   = min(x), scale = bf16((max/2 - min/2) / 7.5)  (0 below 2^-100)
- *   code  = floor((x - low) / scale + 1/2), 0..15         (0 where scale is 0)
+ *   code  = floor((x - low) * inv + 1/2), 0..15           (0 where scale is 0)
+ *           inv = (1 / scale) * (1 + 2^-22)
  *   value = bf16(low + code * scale)
+ * in fp32, each operation rounded by itself. inv is 2^-22 high so that exact
+ * halves go up whatever the reciprocal's own rounding; an x that is less than
+ * 2^-21 of itself short of a half goes up too.
  * A group with a NaN or an infinity, or with max - min past fp32's largest,
  * reads back as NaN. 144 bytes per (slot, kv head) instead of 512. One buffer of tg_kv4_cache_bytes bytes, 16-byte
  * aligned, holds K and V of one layer, (B, Hkv, capacity rounded up to 32

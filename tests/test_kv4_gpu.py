@@ -13,6 +13,7 @@ of 128 products, 2^-22 from the exponential).
 """
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -102,6 +103,30 @@ def test_hard_rows(cuda):
     want = quantise(x)[0]
     assert torch.isnan(want[0, 5, 0, :64]).all() and not torch.isnan(want[0, 5, 0, 64:]).any()
     assert same(gk.double().cpu(), want) and same(gv.double().cpu(), want)
+
+
+def test_codes_next_to_halves(cuda):
+    """The definition's own fp32 operations, bit for bit, on values at and beside half steps: halves go up, and so
+    does what the reciprocal (2^-22 high) lifts to one."""
+    f = np.float32
+    tiny = [0.0] + [s * 10.0 ** -e for e in range(2, 9) for s in (1, -1, 3, -3)]
+    x = torch.zeros(1, 12, 1, 128, dtype=torch.bfloat16)
+    for r in range(12):
+        low, step = -0.5 - r, [1.0, 0.75, 2.0, 0.3125][r % 4]
+        for h in (0, 64):
+            v = [low, low + 15 * step] + [low + (c + 0.5) * step for c in range(15)] + tiny + [t + low + 0.5 * step for t in tiny[:18]]
+            x[0, r, 0, h:h + 64] = torch.tensor(v[:64]).clamp(low, low + 15 * step).bfloat16()
+    c = KV4Cache(1, 12, 1, device=cuda)
+    ops.kv4_write(c, x.to(cuda), x.to(cuda))
+    gk, gv = ops.kv4_read(c)
+    g = x.float().numpy().reshape(24, 64)
+    low, high = g.min(1, keepdims=True), g.max(1, keepdims=True)
+    scale = torch.from_numpy(((high * f(0.5) - low * f(0.5)) / f(7.5)).astype(f)).bfloat16().float().numpy()
+    inv = ((f(1) / scale) * f(1 + 2.0 ** -22)).astype(f)
+    code = np.floor(((g - low).astype(f) * inv).astype(f) + f(0.5)).astype(f)
+    assert code.min() == 0 and code.max() == 15
+    want = torch.from_numpy((low + code * scale).astype(f)).bfloat16().reshape(1, 12, 1, 128)
+    assert torch.equal(gk.cpu(), want) and torch.equal(gv.cpu(), want)
 
 
 def test_long_cache_offsets(cuda):

@@ -731,8 +731,8 @@ def kv4_write(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, start: int = 0)
 
     Any strides with a contiguous last dim, multiples of 8 elements (the K/V views of a fused
     projection, say). Per group of 64 dims: low = min, scale = bf16((max - min) / 15), code =
-    floor((x - low) / scale + 1/2); a group with a NaN or an infinity (or a range past fp32's
-    largest) reads back as NaN."""
+    floor((x - low) * inv + 1/2) with inv = (1 / scale) * (1 + 2^-22), in fp32 (halves go up); a group
+    with a NaN or an infinity (or a range past fp32's largest) reads back as NaN."""
     c = _kv4(cache)
     if not isinstance(k, torch.Tensor) or k.dim() != 4:
         raise ValueError("k must be a 4-D (B, S, Hkv, 128) tensor")
