@@ -96,6 +96,24 @@ def test_kv4_decode_is_the_decode_over_its_values(cuda, monkeypatch, e2e, prune)
     assert err <= 0.15 and cos >= 0.998, (err, cos)
 
 
+def test_what_four_bits_cost_a_generation(cuda):
+    """Logits of a bf16 and of a 4-bit decode cache on the tiny model: an attention output over some 100 to 300 keys
+    moves by about a tenth (test_what_four_bits_cost), in each of at most four layers, and is a part of the residual
+    stream: within 0.4 of the logits' size, cosine above 0.92."""
+    model, gate = _model(cuda, False)
+    prompts, starts, ends = _prompts(33)
+    forced = torch.randint(0, 1000, (2, 8), generator=torch.Generator().manual_seed(6))
+    lg = {}
+    for bits in (16, 4):
+        lg[bits] = []
+        generate_batch(model, gate, prompts, starts, ends, 1, 30, 9, forced_tokens=forced, logits_out=lg[bits], kv_bits=bits)
+    a, b = torch.stack(lg[16]).double(), torch.stack(lg[4]).double()
+    rel = ((a - b).norm() / a.norm()).item()
+    cos = torch.nn.functional.cosine_similarity(a.flatten(), b.flatten(), dim=0).item()
+    print(f"logits: relative difference {rel:.4f}, cosine {cos:.5f}")
+    assert 0 < rel <= 0.4 and cos >= 0.92 and len(model.model.layers) <= 4
+
+
 def test_sampled_tokens_follow_the_logits(cuda):
     """Every drawn token is the definition's for its step's logits and uniform number, eager and as a graph;
     one seed gives one text, greedy settings give the greedy text."""

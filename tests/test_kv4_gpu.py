@@ -233,6 +233,23 @@ def test_append_of_one_row_takes_any_row_stride(cuda):
         ops.qk_norm_rope_append_kv4(two, two[:, :, :2], two[:, :, 2:], w, w, cs, cs[:1].expand(2, -1, -1), 1e-6, c2, sl)
 
 
+@pytest.mark.parametrize("B,Hkv,slot", [(1, 1, 0), (3, 2, 37), (64, 8, 95)])
+def test_append_is_the_bulk_write_of_its_key(cuda, B, Hkv, slot):
+    """The slot's bytes are those of a bulk write of the same bf16 key, which the q heads give: the same rows through
+    the same arithmetic, handed out."""
+    g = torch.Generator().manual_seed(B)
+    k, v = rows(g, B, 1, Hkv, 128).to(cuda), rows(g, B, 1, Hkv, 128).to(cuda)
+    w = (1 + 0.3 * torch.randn(128, generator=g)).bfloat16().to(cuda)
+    ang = torch.randn(B, 1, 64, generator=g) * 50
+    cos, sin = (torch.cat([f(ang)] * 2, -1).bfloat16().to(cuda) for f in (torch.cos, torch.sin))
+    a, b = KV4Cache(B, 96, Hkv, device=cuda), KV4Cache(B, 96, Hkv, device=cuda)
+    a.data.fill_(0x3C)
+    b.data.fill_(0x3C)
+    key = ops.qk_norm_rope_append_kv4(k, k, v, w, w, cos, sin, 1e-6, a, torch.tensor([slot], dtype=torch.int64, device=cuda))
+    ops.kv4_write(b, key, v, start=slot)
+    assert torch.equal(a.data, b.data)
+
+
 # ------------------------------------------------------------------ attention
 def attend(q, k, v, n_valid, n_prefix, n_keys, bias, q_scale):
     """float64 (output, tolerance) of the definition over the values that the cache stands for."""
@@ -436,6 +453,31 @@ def test_attention_growing_scores(cuda):
     bias = torch.linspace(0, 40, 700).repeat(1, 1, 1)
     check_attend(cuda, q, k, v, [700], 700, 700, bias)
     check_attend(cuda, q, k, v, [700], 700, 700, -bias)
+
+
+@pytest.mark.parametrize("n", [100, 2771, 32768])
+def test_what_four_bits_cost(cuda, n):
+    """Against attention over the bf16 rows. With errors of a value uniform over its step (variance step^2 / 12), of a
+    score s_j = scale * sqrt(sum q^2 step_k^2 / 12), the output's variance is sum_j p_j^2 (step_v^2 / 12 + s_j^2 (v_j -
+    out)^2), to first order. The errors' mean square over 2048 outputs is within 1.5^2 of that, and not far below."""
+    g = torch.Generator().manual_seed(n)
+    Hq, Hkv = 16, 8
+    q, k, v = torch.randn(1, Hq, 128, generator=g).bfloat16(), rows(g, 1, n, Hkv, 128), rows(g, 1, n, Hkv, 128)
+    c = KV4Cache(1, n, Hkv, device=cuda)
+    ops.kv4_write(c, k.to(cuda), v.to(cuda))
+    out = ops.decode_attention_kv4(q.to(cuda), c, torch.tensor([n], dtype=torch.int32, device=cuda), n, n)[0].double()
+    kd, vd, qd = k[0].double().to(cuda), v[0].double().to(cuda), q[0].double().to(cuda)
+    step = lambda x: ((x.unflatten(-1, (2, 64)).amax(-1) - x.unflatten(-1, (2, 64)).amin(-1)) / 15).repeat_interleave(64, -1)  # noqa: E731
+    want, var = torch.zeros_like(out), torch.zeros_like(out)
+    for h in range(Hq):
+        kh, vh = kd[:, h // 2], vd[:, h // 2]
+        p = torch.softmax(kh @ qd[h] * 128 ** -0.5, 0)
+        want[h] = p @ vh
+        s2 = (step(kh) ** 2 / 12) @ qd[h] ** 2 / 128
+        var[h] = (p ** 2) @ (step(vh) ** 2 / 12 + s2[:, None] * (vh - want[h]) ** 2)
+    got, guess, size = (((out - want) ** 2).mean().sqrt().item(), var.mean().sqrt().item(), (want ** 2).mean().sqrt().item())
+    print(f"{n} keys: relative error {got / size:.4f}, expected {guess / size:.4f}")
+    assert 0.5 * guess <= got <= 1.5 * guess + 2 ** -9 * size
 
 
 def test_attention_strides_stream_and_graph(cuda):
