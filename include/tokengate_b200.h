@@ -480,7 +480,10 @@ int tg_qk_norm_rope_append_kv4(const void* q, int64_t ld_q, int n_q_heads, const
 /* tg_decode_attn_ex over a 4-bit cache of `capacity` slots: the same
  * operation on the values that the cache stands for, with the same bias,
  * query scale, pad slots and device-side key count. A bias of -inf masks its
- * key whatever the key holds; rows without any key give zeros. 1 to 8 query
+ * key whatever the key holds (-1e9 or the type's lowest value, beside keys of
+ * ordinary scores, whatever its V holds); rows without any key give zeros.
+ * Scores, weights and sums are fp32; a weight times its key's step is rounded to
+ * 11 bits relative to the largest such product of its head and group. 1 to 8 query
  * heads per kv head. workspace: device scratch of
  * tg_decode_attn_kv4_workspace bytes (0: none; of the current device, as the
  * call's), 16-byte aligned; calls sharing it must not overlap on the GPU. */
@@ -504,8 +507,10 @@ int tg_decode_attn_kv4_workspace(int B, int Hq, int Hkv, int n_keys, size_t* byt
  * temperature T <= 0 (or NaN): the largest logit, lowest index on ties
  * (logprob 0). top_k (nullable) <= 0, top_p (nullable) >= 1 and min_p
  * (nullable) <= 0 are off; at least the largest logit is always kept. u in
- * [0, 1]. A row of -inf or NaN alone gives token 0 and logprob NaN. Masses
- * are summed exactly, so results do not depend on any order of summing.
+ * [0, 1]. A row of -inf or NaN alone gives token 0 and logprob NaN. Weights are
+ * fp32, each cut to a multiple of 2^-44 (below that it has no mass), and the cut
+ * ones summed exactly, so results do not depend on any order of summing.
+ * row_stride is at least V where B > 1.
  * The reference decodes greedily (tokengate/e2e_gate/decode/gate_decode.py:
  * 87-260); no counterpart there. B == 0 returns TG_OK.
  */

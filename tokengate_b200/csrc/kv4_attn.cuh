@@ -40,11 +40,11 @@
 // The cache is read once, at 144 bytes per key: every warp streams its own
 // tiles through a ring of two in shared memory (one bulk copy of 4608
 // bytes each, no barrier between warps). 2 rows of 131081 keys, 8 kv heads:
-// 53.3 us, 302 MB = 5.7 TB/s (86 % of a copy's rate), of which 47 are the loop,
+// 53.1 us, 302 MB = 5.7 TB/s (87 % of a copy's rate), of which 47 are the loop,
 // at DRAM's rate, the rest its start, the merges and the second launch. In the
-// L2 cache (one row of 32775: 13.6 us) the loop is bound by instructions, half
-// of them the unpacking (issue slots 59 % busy, the ALU pipe 63 %); a short
-// cache (one row of 2771: 6.8 us) by latencies one after another: the launch,
+// L2 cache (one row of 32775: 13.7 us) the loop is bound by instructions, half
+// of them the unpacking (issue slots 57 % busy, the ALU pipe 65 %); a short
+// cache (one row of 2771: 6.6 us) by latencies one after another: the launch,
 // the counts, the first tile, two barriers.
 #pragma once
 
@@ -227,7 +227,8 @@ __device__ __forceinline__ void kv4_store_out(__nv_bfloat16* at, float4 o, float
 //   PAIR (up to 4 query heads per kv head): column 4 s + h is head h over the
 //         16-key halves s of the tiles, so no lane works on an empty column
 //         and the two are merged at the end (2 rows of 131081 keys, 8 kv
-//         heads: 59.6 -> 56.8 us; 461 instructions a tile, prologues included);
+//         heads: 59.6 -> 56.8 us when it came; 444 instructions a tile now,
+//         prologues included);
 //   else: column h is head h.
 // Without a bias the scores are in log2 units; with one they stay in natural
 // units, where a bias of the type's lowest value does not overflow.

@@ -842,7 +842,8 @@ def decode_attention_kv4(q: torch.Tensor, cache: KV4Cache, n_valid: torch.Tensor
                          n_keys_dev: Optional[torch.Tensor] = None) -> torch.Tensor:
     """decode_attention over a 4-bit cache (tg_decode_attn_kv4): the same arguments, with the cache in
     the place of k and v. q: (B, Hq, 128) bf16, Hq / Hkv from 1 to 8. A bias of -inf masks its key
-    whatever the key holds; a row without any key gives zeros. Returns (B, Hq, 128) bf16."""
+    whatever the key holds; a row without any key gives zeros. Scores, weights and sums are fp32, a
+    weight times its key's step is rounded to 11 bits. Returns (B, Hq, 128) bf16."""
     c = _kv4(cache)
     B, data = c.batch, c.data
     dev = data.get_device()
@@ -925,7 +926,8 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     None or <= 0, top_p None or >= 1 and min_p None or <= 0 are off. Order: temperature, the top_k
     largest, of these the shortest prefix with mass >= top_p, of these those at least min_p times as
     likely as the largest; ties go to the lower index. The token is the first, by index, at which the
-    running kept mass passes u times the whole. A NaN logit counts as -inf; a row of nothing else
+    running kept mass passes u times the whole (weights cut to multiples of 2^-44 of the largest). A
+    NaN logit counts as -inf; a row of nothing else
     gives token 0 and logprob NaN. Returns (token int64 (B,), logprob fp32 (B,)), logprob under the
     distribution sampled from. token / logprob: written instead of new tensors."""
     if not isinstance(logits, torch.Tensor) or (logits.dtype is not torch.float32 and logits.dtype is not torch.bfloat16):
